@@ -155,3 +155,51 @@ def sample(logits: int, V: int, B: int, idx: int, val: int = 0, temperature: flo
            seed: int = 0, step_dev: int = 0, step_add: int = 0) -> None:
     """Temperature / top-k / top-p sampling over f32 logits [B][V] (deterministic; see bkSample)."""
     _check(cu().bkSample(logits, V, B, temperature, top_k, top_p, seed, step_dev, step_add, idx, val))
+
+
+def paged_attn_scratch_bytes(B: int, T: int, Hq: int, Hkv: int, HD: int, prefix_rows: int) -> int:
+    return int(R.load_library().bkPagedAttnScratchBytes(B, T, Hq, Hkv, HD, prefix_rows))
+
+
+def paged_attn_args(**kw) -> R.bkPagedAttnArgs:
+    """The arguments of ``paged_attn``; keyword names are the fields of bkPagedAttnArgs (``len`` may stand for ``lens``).
+    A decode loop whose buffers stay makes them once."""
+    a = R.bkPagedAttnArgs()
+    if "len" in kw:
+        kw["lens"] = kw.pop("len")
+    for k, v in kw.items():
+        if not hasattr(a, k):
+            raise TypeError(f"paged_attn_args: bkPagedAttnArgs has no field {k!r}")
+        setattr(a, k, v)
+    return a
+
+
+def paged_attn(args: R.bkPagedAttnArgs) -> None:
+    """Append the new rows and attend over pages; the rows that all sequences share are computed once for all."""
+    _check(cu().bkPagedAttn(C.byref(args)))
+
+
+def lora_scratch_bytes(K: int, B: int, rank: int, n_segs: int) -> int:
+    return int(R.load_library().bkLoraScratchBytes(K, B, rank, n_segs))
+
+
+def lora_seg(A: int, Bm: int, n_rows: int, out: int, base: int = 0, *, bf16: bool = False, ld_out: int | None = None,
+             col_off: int = 0) -> R.bkLoraSeg:
+    return R.bkLoraSeg(A=A, Bm=Bm, base=base, out=out, n_rows=n_rows, dtype=R.BK_DTYPE_BF16 if bf16 else R.BK_DTYPE_F32,
+                       ld_out=n_rows + col_off if ld_out is None else ld_out, col_off=col_off)
+
+
+def lora_args(x: int, K: int, B: int, rank: int, n_adapters: int, ids: int, segs: Sequence[R.bkLoraSeg], scratch: int, scratch_bytes: int,
+              scale: int = 0, weights_are_settled: bool = False) -> R.bkLoraArgs:
+    if not 1 <= len(segs) <= 4:
+        raise ValueError(f"lora_args: {len(segs)} segments (1 to 4)")
+    a = R.bkLoraArgs(K=K, B=B, n_segs=len(segs), rank=rank, n_adapters=n_adapters, weights_are_settled=int(weights_are_settled), x=x, ids=ids,
+                     scale=scale, scratch=scratch, scratch_bytes=scratch_bytes)
+    for i, s in enumerate(segs):
+        a.segs[i] = s
+    return a
+
+
+def lora(args: R.bkLoraArgs) -> None:
+    """Low-rank adapters, one per column, added to a shared projection's output (call it after ``gemv``)."""
+    _check(cu().bkLora(C.byref(args)))

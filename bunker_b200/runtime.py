@@ -69,6 +69,28 @@ class bkAttnArgs(C.Structure):
                 ("cache_is_settled", C.c_int32), ("out_q8_layout", C.c_int32), ("out_q8", C.c_uint64)]
 
 
+class bkPages(C.Structure):
+    _fields_ = [(n, C.c_uint64) for n in ("base", "plane_bytes", "ref", "table", "lens", "scratch", "scratch_bytes")] + \
+               [(n, C.c_int32) for n in ("n_planes", "n_pages", "heads", "page_rows", "row_bytes", "n_seqs", "max_pages", "reserved")]
+
+
+class bkPagedAttnArgs(C.Structure):
+    _fields_ = [(n, C.c_uint64) for n in ("qg", "k", "v", "gate", "q_norm_w", "k_norm_w", "cos_t", "sin_t", "k_pages", "v_pages", "table",
+                                           "lens", "n_new", "out", "scratch", "scratch_bytes")] + \
+               [(n, C.c_int32) for n in ("B", "T", "Hq", "Hkv", "HD", "rot_half", "n_pages", "page_rows", "max_pages", "prefix_rows",
+                                          "max_len", "fused_norm_rope")] + [("scale", C.c_float), ("eps", C.c_float)]
+
+
+class bkLoraSeg(C.Structure):
+    _fields_ = [("A", C.c_uint64), ("Bm", C.c_uint64), ("base", C.c_uint64), ("out", C.c_uint64), ("n_rows", C.c_int32), ("dtype", C.c_int32),
+                ("ld_out", C.c_int32), ("col_off", C.c_int32)]
+
+
+class bkLoraArgs(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("K", "B", "n_segs", "rank", "n_adapters", "weights_are_settled")] + \
+               [(n, C.c_uint64) for n in ("x", "ids", "scale", "scratch", "scratch_bytes")] + [("segs", bkLoraSeg * 4)]
+
+
 class bkModelConfig(C.Structure):
     _fields_ = [(n, C.c_int32) for n in ("hidden", "n_layers", "full_attn_interval", "vocab", "gdn_k_heads",
                                           "gdn_v_heads", "attn_q_heads", "attn_kv_heads", "head_dim", "rot_dim",
@@ -134,6 +156,16 @@ SIGNATURES = {
     "bkArgmaxScratchBytes": (_U64, [_I32]),
     "bkArgmaxStatic": (_I32, [_U64, _I32, _I32, _U64, _U64]),
     "bkSample": (_I32, [_U64, _I32, _I32, _F32, _I32, _F32, _U64, _U64, C.c_uint32, _U64, _U64]),
+    "bkPagesScratchBytes": (_U64, [_I32, _I32]),
+    "bkPagesCopy": (_I32, [C.POINTER(bkPages), C.POINTER(bkPages), _U64, _U64, _I32]),
+    "bkPagesFork": (_I32, [C.POINTER(bkPages), _U64, _U64, _I32, _U64]),
+    "bkPagesGrow": (_I32, [C.POINTER(bkPages), _U64, _U64, _I32, _U64]),
+    "bkPagesFree": (_I32, [C.POINTER(bkPages), _U64, _I32]),
+    "bkPagesCompact": (_I32, [C.POINTER(bkPages), _U64, _U64, _U64, _U64]),
+    "bkPagedAttn": (_I32, [C.POINTER(bkPagedAttnArgs)]),
+    "bkPagedAttnScratchBytes": (_U64, [_I32, _I32, _I32, _I32, _I32, _I32]),
+    "bkLora": (_I32, [C.POINTER(bkLoraArgs)]),
+    "bkLoraScratchBytes": (_U64, [_I32, _I32, _I32, _I32]),
     "bkLaunch": (_I32, [_I32, _PU64, _I32]),
     "bkCommCreate": (_I32, [_I32, _I32, _U64, _PU64]),
     "bkCommExportHandle": (_I32, [_U64, C.POINTER(C.c_uint8)]),

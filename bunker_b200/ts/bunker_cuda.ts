@@ -68,6 +68,16 @@ const SYMBOLS = {
   bkArgmaxScratchBytes: { args: ["i32"], returns: "u64" },
   bkArgmaxStatic: { args: ["u64", "i32", "i32", "u64", "u64"], returns: "i32" },
   bkSample: { args: ["u64", "i32", "i32", "f32", "i32", "f32", "u64", "u64", "u32", "u64", "u64"], returns: "i32" },
+  bkPagesScratchBytes: { args: ["i32", "i32"], returns: "u64" },
+  bkPagesCopy: { args: ["ptr", "ptr", "u64", "u64", "i32"], returns: "i32" },
+  bkPagesFork: { args: ["ptr", "u64", "u64", "i32", "u64"], returns: "i32" },
+  bkPagesGrow: { args: ["ptr", "u64", "u64", "i32", "u64"], returns: "i32" },
+  bkPagesFree: { args: ["ptr", "u64", "i32"], returns: "i32" },
+  bkPagesCompact: { args: ["ptr", "u64", "u64", "u64", "u64"], returns: "i32" },
+  bkPagedAttn: { args: ["ptr"], returns: "i32" },
+  bkPagedAttnScratchBytes: { args: ["i32", "i32", "i32", "i32", "i32", "i32"], returns: "u64" },
+  bkLora: { args: ["ptr"], returns: "i32" },
+  bkLoraScratchBytes: { args: ["i32", "i32", "i32", "i32"], returns: "u64" },
   bkModelCreate: { args: ["ptr", "ptr"], returns: "i32" },
   bkModelSetTensor: { args: ["u64", "ptr", "u64", "u64"], returns: "i32" },
   bkModelSetComm: { args: ["u64", "u64"], returns: "i32" },

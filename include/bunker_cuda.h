@@ -262,6 +262,109 @@ BK_API int32_t bkArgmaxStatic(uint64_t logits, int32_t V, int32_t B, uint64_t id
 BK_API int32_t bkSample(uint64_t logits, int32_t V, int32_t B, float temperature, int32_t top_k, float top_p, uint64_t seed,
                         uint64_t step_dev, uint32_t step_add, uint64_t idx, uint64_t val);
 
+/* ---- serving many requests: a cache in pages, attention behind a shared prefix, adapters --------------------
+ * No counterpart in the reference, whose cache is one contiguous 128-row buffer (src/emitters.ts:202).  All of it is enqueued on the
+ * library stream like every other op; page tables, lengths, reference counts and request lists stay on the device, so nothing here
+ * waits for the GPU. */
+
+/* A pool of pages.  Plane i holds page p at base + i*plane_bytes + p*(heads*page_rows*row_bytes); a page is [heads][page_rows][row_bytes],
+ * a plane is, for instance, the keys or the values of one layer.  A sequence's row j lies in page table[s][j / page_rows], at row
+ * j % page_rows.  ref counts the table entries that hold a page; a page is free when it is 0.  lens, table and ref are changed by
+ * the calls below only; a host starts with lens 0 and ref 0.  Requests travel as device lists of at most 1024 entries; an
+ * entry that cannot be served changes nothing and gets ok = 0.  A sequence named twice in one list counts once, at its first entry. */
+#define BK_PAGES_MAX_LIST 1024
+typedef struct bkPages {
+  uint64_t base;         /* 16-byte aligned */
+  uint64_t plane_bytes;  /* multiple of 16, at least a plane's size */
+  uint64_t ref;          /* int32 [n_pages] */
+  uint64_t table;        /* int32 [n_seqs][max_pages] */
+  uint64_t lens;         /* int32 [n_seqs]: rows held */
+  uint64_t scratch;      /* bkPagesScratchBytes(n_pages, n_seqs) bytes, 16-byte aligned; contents need not survive a call */
+  uint64_t scratch_bytes;
+  int32_t n_planes, n_pages, heads, page_rows, row_bytes; /* row_bytes: multiple of 16 */
+  int32_t n_seqs, max_pages;
+  int32_t reserved;
+} bkPages;
+BK_API uint64_t bkPagesScratchBytes(int32_t n_pages, int32_t n_seqs);
+/* n pages of `from` into pages of `to` (may be the same pool), all planes: page dst[i] = page src[i].  The pools agree in planes and
+ * page shape.  Pairs with a page outside its pool are skipped.  No page may be in dst twice, nor, in one pool, in both lists. */
+BK_API int32_t bkPagesCopy(const bkPages* from, const bkPages* to, uint64_t src, uint64_t dst, int32_t n);
+/* Sequence dst[i], which must be empty, becomes what src[i] is at the start of the call: whole pages are shared, the filled rows of a
+ * partial last page are copied into a fresh page, so that both can go on on their own.  Fresh pages are the lowest-numbered free ones, in
+ * list order.  ok[i] (int32; 0 to skip): 1, or 0 where a sequence is out of range, dst[i] is not empty or is src[i], or the pages run out
+ * (a fork that needs none is always served; one that needs a page is served if the needs of the valid forks up to it fit). */
+BK_API int32_t bkPagesFork(const bkPages* pool, uint64_t src, uint64_t dst, int32_t n, uint64_t ok);
+/* Room for add[i] >= 0 more rows of sequence seqs[i]: fresh pages where its last page does not hold them, lens += add.  What is in the new
+ * rows is whatever was there.  Same rules for fresh pages and ok. */
+BK_API int32_t bkPagesGrow(const bkPages* pool, uint64_t seqs, uint64_t add, int32_t n, uint64_t ok);
+/* The sequences give up their pages: ref - 1, table entries -1, lens 0.  Out-of-range entries are skipped. */
+BK_API int32_t bkPagesFree(const bkPages* pool, uint64_t seqs, int32_t n);
+/* Moves the n_used pages in use to the front of the pool: those at n_used and behind, ascending, go to the free ones below n_used,
+ * ascending; the rest stay.  table_out [n_seqs][max_pages] and ref_out [n_pages] get the tables of the new places (they may be the
+ * pool's own; an entry that names no page in use becomes -1), map [n_pages] the new place of each page or -1, used (int32) n_used. */
+BK_API int32_t bkPagesCompact(const bkPages* pool, uint64_t table_out, uint64_t ref_out, uint64_t map, uint64_t used);
+
+/* Attention of B sequences with up to T new tokens each over pages of keys and values, [n_pages][Hkv][page_rows][HD] bf16 (one plane
+ * each of a bkPages pool).  Token t of sequence b is row t*B + b of every input and output; it stands at row lens[b] - n_new[b] + t of its
+ * sequence and attends to the rows up to its own.  A token t >= n_new[b], or at a row outside [0, max_len), is not there: its out is 0.
+ * The first prefix_rows rows are the same for all sequences: their whole pages are read through sequence 0's table, once for all.
+ *   fused_norm_rope = 1: qg bf16 [T*B][Hq][2*HD] = q | gate; q and k get their head RMSNorm (times 1 + w) and the partial rotary at the
+ *     token's row, in f32 with one rounding to bf16; k and v [T*B][Hkv][HD] are stored into the pages; out = attention * sigmoid(gate).
+ *   fused_norm_rope = 0: qg holds ready q [T*B][Hq][HD]; k, v (ready, or both 0 where the pages have them) are stored as they are;
+ *     gate bf16 [T*B][Hq][HD], or 0 for none.
+ * out bf16 [T*B][Hq*HD].  Rows of a page past a sequence's end are never part of a result, whatever they hold.  Nothing is stored
+ * through a table entry that names no page, and rows whose page is missing count as not there. */
+typedef struct bkPagedAttnArgs {
+  uint64_t qg, k, v, gate;
+  uint64_t q_norm_w, k_norm_w, cos_t, sin_t; /* bf16 [HD]; f32 [max_len][rot_half] */
+  uint64_t k_pages, v_pages;
+  uint64_t table;        /* int32 [B][max_pages] */
+  uint64_t lens;         /* int32 [B]: rows of each sequence, its new ones among them */
+  uint64_t n_new;        /* int32 [B], 0..T; 0 = every sequence has T */
+  uint64_t out;
+  uint64_t scratch;      /* bkPagedAttnScratchBytes() bytes, 16-byte aligned; contents need not survive a call */
+  uint64_t scratch_bytes;
+  int32_t B, T, Hq, Hkv, HD; /* HD 128 or 256; Hq / Hkv 1..16 */
+  int32_t rot_half;
+  int32_t n_pages, page_rows, max_pages; /* page_rows: a power of two, 16..1024 */
+  int32_t prefix_rows;
+  int32_t max_len;       /* upper bound of lens[] */
+  int32_t fused_norm_rope;
+  float scale, eps;
+} bkPagedAttnArgs;
+BK_API int32_t bkPagedAttn(const bkPagedAttnArgs* args);
+BK_API uint64_t bkPagedAttnScratchBytes(int32_t B, int32_t T, int32_t Hq, int32_t Hkv, int32_t HD, int32_t prefix_rows);
+
+/* Low-rank adapters of many requests beside a shared projection: for every segment
+ *   out[b] = base[b] + scale[a] * Bm[a] (A[a] x[b]),   a = ids[b];   out[b] = base[b] where a is outside [0, n_adapters).
+ * Sums and A x in f32, one rounding at the end.  Call it after the projection (bkGemvQ4K) that wrote base. */
+typedef struct bkLoraSeg {
+  uint64_t A;            /* bf16 [n_adapters][rank][K] */
+  uint64_t Bm;           /* bf16 [n_adapters][n_rows][rank] */
+  uint64_t base;         /* [B][ld_out] of dtype, may be out; 0 = zeros */
+  uint64_t out;          /* [B][ld_out] */
+  int32_t n_rows;
+  int32_t dtype;         /* BK_DTYPE_F32 or BK_DTYPE_BF16: of base and out */
+  int32_t ld_out;        /* elements between rows of base and out */
+  int32_t col_off;       /* column of base and out that belongs to row 0 of this segment */
+} bkLoraSeg;
+typedef struct bkLoraArgs {
+  int32_t K;             /* multiple of 8 */
+  int32_t B;             /* 1..64 */
+  int32_t n_segs;        /* 1..4 row segments that share x */
+  int32_t rank;          /* multiple of 8, 8..128 */
+  int32_t n_adapters;
+  int32_t weights_are_settled; /* 1: A and Bm were NOT written by launches that may still run, so they may be read before those end */
+  uint64_t x;            /* bf16 [B][K] */
+  uint64_t ids;          /* int32 [B] */
+  uint64_t scale;        /* f32 [n_adapters]; 0 = all 1 */
+  uint64_t scratch;      /* bkLoraScratchBytes() bytes, 16-byte aligned; contents need not survive a call */
+  uint64_t scratch_bytes;
+  bkLoraSeg segs[4];
+} bkLoraArgs;
+BK_API int32_t bkLora(const bkLoraArgs* args);
+BK_API uint64_t bkLoraScratchBytes(int32_t K, int32_t B, int32_t rank, int32_t n_segs);
+
 /* ---- whole decode step: replaces buildModelGraph + compileStep + runGraphDecode
  *      (src/model.ts:46-204, src/runner.ts:94-162) --------------------------------
  * One call per token; the CUDA graph lives inside the library because replaying a graph
