@@ -158,7 +158,7 @@ def sample(logits: int, V: int, B: int, idx: int, val: int = 0, temperature: flo
 
 
 def paged_attn_scratch_bytes(B: int, T: int, Hq: int, Hkv: int, HD: int, prefix_rows: int) -> int:
-    return int(R.load_library().bkPagedAttnScratchBytes(B, T, Hq, Hkv, HD, prefix_rows))
+    return int(cu().bkPagedAttnScratchBytes(B, T, Hq, Hkv, HD, prefix_rows))
 
 
 def paged_attn_args(**kw) -> R.bkPagedAttnArgs:

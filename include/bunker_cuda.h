@@ -313,7 +313,7 @@ BK_API int32_t bkPagesCompact(const bkPages* pool, uint64_t table_out, uint64_t 
  *   fused_norm_rope = 0: qg holds ready q [T*B][Hq][HD]; k, v (ready, or both 0 where the pages have them) are stored as they are;
  *     gate bf16 [T*B][Hq][HD], or 0 for none.
  * out bf16 [T*B][Hq*HD].  Rows of a page past a sequence's end are never part of a result, whatever they hold.  Nothing is stored
- * through a table entry that names no page, and rows whose page is missing count as not there. */
+ * through a table entry that names no page; read, such an entry is rows of zeros (the calls above leave none among a sequence's rows). */
 typedef struct bkPagedAttnArgs {
   uint64_t qg, k, v, gate;
   uint64_t q_norm_w, k_norm_w, cos_t, sin_t; /* bf16 [HD]; f32 [max_len][rot_half] */
@@ -333,6 +333,7 @@ typedef struct bkPagedAttnArgs {
   float scale, eps;
 } bkPagedAttnArgs;
 BK_API int32_t bkPagedAttn(const bkPagedAttnArgs* args);
+/* (after bkInit: it depends on the number of SMs) */
 BK_API uint64_t bkPagedAttnScratchBytes(int32_t B, int32_t T, int32_t Hq, int32_t Hkv, int32_t HD, int32_t prefix_rows);
 
 /* Low-rank adapters of many requests beside a shared projection: for every segment
