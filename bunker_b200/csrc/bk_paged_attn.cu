@@ -54,7 +54,7 @@ struct Layout {                 // of the scratch buffer, and the numbers of job
   int n_p, n_s;                 // jobs over common keys, over a sequence's own
   int rows_s;                   // rows of a partial result of the latter
   int ctas;
-  size_t q, starts, ml_p, ml_s, o_p, o_s, bytes;   // byte offsets
+  size_t q, jobs, pieces, ml_p, ml_s, o_p, o_s, bytes;   // byte offsets
 };
 
 __host__ __device__ inline size_t round16(size_t n) { return (n + 15) / 16 * 16; }
@@ -71,14 +71,16 @@ inline Layout make_layout(int B, int T, int Hq, int Hkv, int HD, int prefix_rows
   L.ctas = ctas;
   size_t at = round16((size_t)B * T * Hq * HD * 2);
   L.q = 0;
-  L.starts = at;
-  at += round16((size_t)(L.n_p + L.n_s + 1) * 8);
+  L.jobs = at;
+  at += (size_t)(L.n_p + L.n_s + 1) * 16;
+  L.pieces = at;
+  at += round16((size_t)(ctas + 2) * 8);
   // partial results: a job and a CTA that has a piece of it meet in slot job + CTA, which no other pair has
   const size_t slots_p = L.n_p ? L.n_p + ctas : 0, slots_s = L.n_s + ctas;
   L.ml_p = at;
-  at += round16(slots_p * kRows * 8);
+  at += slots_p * kRows * 16;
   L.ml_s = at;
-  at += round16(slots_s * L.rows_s * 8);
+  at += slots_s * L.rows_s * 16;
   L.o_p = at;
   at += slots_p * kRows * HD * 4;
   L.o_s = at;
@@ -96,9 +98,9 @@ struct TileParams {
   CUtensorMap k_map, v_map;
 };
 
-// job j: its KV head, row tile, sequence (-1: all) and the end of its keys
+// job j: its KV head, row tile, sequence (-1: all) and where its keys begin
 struct Job {
-  int seq, kvh, mt, key0, key1;
+  int seq, kvh, mt, key0;
 };
 BK_DEVINL Job job_of(const PagedParams& p, const Layout& L, int j) {
   Job q;
@@ -107,7 +109,6 @@ BK_DEVINL Job job_of(const PagedParams& p, const Layout& L, int j) {
     q.kvh = j / L.mt_p;
     q.mt = j - q.kvh * L.mt_p;
     q.key0 = 0;
-    q.key1 = L.P;
     return q;
   }
   const int i = j - L.n_p, bk = i / L.mt_s;
@@ -115,58 +116,92 @@ BK_DEVINL Job job_of(const PagedParams& p, const Layout& L, int j) {
   q.seq = bk / p.Hkv;
   q.kvh = bk - q.seq * p.Hkv;
   q.key0 = L.P;
-  // the last of the tile's tokens that is there
-  const int G = p.Hq / p.Hkv, n = p.n_new ? min(p.n_new[q.seq], p.T) : p.T, last = min(n, (min(p.T * G, (q.mt + 1) * kRows) - 1) / G + 1) - 1;
-  q.key1 = L.P;
-  for (int t = last; t >= 0 && t >= q.mt * kRows / G; t--) {   // (one turn but for tokens past max_len)
-    const int at = row_of(p, q.seq, t);
-    if (at >= 0) {
-      q.key1 = max(L.P, at + 1);
-      break;
-    }
-  }
   return q;
 }
-BK_DEVINL int tiles_of(const Job& q) { return (q.key1 - q.key0 + kTile - 1) / kTile; }
-
-// starts[j]: where job j begins on the line; one CTA of 128 threads
-BK_DEVINL void plan_jobs(const PagedParams& p, const Layout& L, long long* starts) {
-  __shared__ long long warp_s[4];
-  const int n = L.n_p + L.n_s, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  long long base = 0;
-  for (int j0 = 0; j0 < n; j0 += 128) {
-    const int j = j0 + (int)threadIdx.x;
-    long long units = 0;
-    if (j < n) {
-      const int tiles = tiles_of(job_of(p, L, j));
-      units = tiles ? tiles + kOverhead : 0;
-    }
-    long long v = units;
-#pragma unroll
-    for (int off = 1; off < 32; off <<= 1) {
-      const long long o = __shfl_up_sync(0xffffffffu, v, off);
-      if (lane >= off) v += o;
-    }
-    if (lane == 31) warp_s[warp] = v;
-    __syncthreads();
-    long long before = base;
-    for (int w = 0; w < 4; w++) {
-      if (w < warp) before += warp_s[w];
-      base += warp_s[w];
-    }
-    if (j < n) starts[j] = before + v - units;
-    __syncthreads();
+// the end of its keys: behind the row of the last of the tile's tokens that is there
+BK_DEVINL int keys_end(const PagedParams& p, const Layout& L, const Job& q) {
+  if (q.seq < 0) return L.P;
+  const int G = p.Hq / p.Hkv, n = p.n_new ? min(p.n_new[q.seq], p.T) : p.T, last = min(n, (min(p.T * G, (q.mt + 1) * kRows) - 1) / G + 1) - 1;
+  for (int t = last; t >= 0 && t >= q.mt * kRows / G; t--) {   // (one turn but for tokens past max_len)
+    const int at = row_of(p, q.seq, t);
+    if (at >= 0) return max(L.P, at + 1);
   }
-  if (threadIdx.x == 0) starts[n] = base;
+  return L.P;
 }
 
-// CTA c of the line's C pieces: units [bound(c), bound(c + 1))
-BK_DEVINL long long bound_of(long long units, int c, int C) { return units * c / C; }
-BK_DEVINL int cta_at(long long units, long long x, int C) { return (int)(((x + 1) * C - 1) / units); }
-// the tiles of a job that starts at s and has n tiles which lie in units [u0, u1)
-BK_DEVINL void piece_of(long long s, int n, long long u0, long long u1, int* t0, int* t1) {
-  *t0 = (int)max(0ll, min((long long)n, u0 - s - kOverhead));
-  *t1 = (int)max(0ll, min((long long)n, u1 - s - kOverhead));
+// What the first launch leaves for the others.  jobs[j] = {start on the line, end of the keys, first and last CTA that may have a piece of it};
+// pieces[c] = {start of CTA c's piece of the line, first job in it}; pieces[ctas + 1].x = the number of CTAs that get one.
+BK_DEVINL int4* jobs_of(const Layout& L, uint8_t* scratch) { return reinterpret_cast<int4*>(scratch + L.jobs); }
+BK_DEVINL int2* pieces_of(const Layout& L, uint8_t* scratch) { return reinterpret_cast<int2*>(scratch + L.pieces); }
+BK_DEVINL int tiles_of(const Layout& L, int j, int key1) { return (key1 - (j < L.n_p ? 0 : L.P) + kTile - 1) / kTile; }
+// the tiles of a job that starts at s and has n tiles which lie in units [u0, u1): [t0, t1)
+BK_DEVINL void piece_of(int s, int n, int u0, int u1, int* t0, int* t1) {
+  *t0 = max(0, min(n, u0 - s - kOverhead));
+  *t1 = max(0, min(n, u1 - s - kOverhead));
+}
+
+// one CTA of 128 threads
+BK_DEVINL void plan_jobs(const PagedParams& p, const Layout& L, uint8_t* scratch) {
+  __shared__ int warp_s[4][2];
+  int4* jobs = jobs_of(L, scratch);
+  int2* pieces = pieces_of(L, scratch);
+  const int n = L.n_p + L.n_s, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int base = 0, tiles_all = 0;
+  for (int j0 = 0; j0 < n; j0 += 128) {
+    const int j = j0 + (int)threadIdx.x;
+    int tiles = 0, end = 0;
+    if (j < n) {
+      end = keys_end(p, L, job_of(p, L, j));
+      tiles = tiles_of(L, j, end);
+    }
+    const int units = tiles ? tiles + kOverhead : 0;
+    int v = units;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const int o = __shfl_up_sync(0xffffffffu, v, off);
+      if (lane >= off) v += o;
+    }
+    const int sum = __reduce_add_sync(0xffffffffu, tiles);
+    if (lane == 31) {
+      warp_s[warp][0] = v;
+      warp_s[warp][1] = sum;
+    }
+    __syncthreads();
+    int before = base;
+    for (int w = 0; w < 4; w++) {
+      if (w < warp) before += warp_s[w][0];
+      base += warp_s[w][0];
+      tiles_all += warp_s[w][1];
+    }
+    if (j < n) jobs[j] = make_int4(before + v - units, end, 0, 0);
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) jobs[n] = make_int4(base, 0, 0, 0);
+  __syncthreads();   // jobs[].x is there for all
+  const int C = max(1, min(L.ctas, tiles_all)), units = base;   // every CTA has a tile to do
+  auto bound = [&](int c) { return (int)((long long)units * c / C); };
+  for (int c = threadIdx.x; c <= C; c += 128) {
+    const int u = bound(c);
+    int lo = 0, hi = n;   // the last job that starts at u or before
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (jobs[mid].x <= u) lo = mid;
+      else hi = mid;
+    }
+    pieces[c] = make_int2(u, lo);
+  }
+  if (threadIdx.x == 0) pieces[L.ctas + 1] = make_int2(C, 0);
+  for (int j = threadIdx.x; j < n; j += 128) {
+    const int s = jobs[j].x, s1 = jobs[j + 1].x;
+    auto cta_at = [&](int x) { return (int)((((long long)x + 1) * C - 1) / units); };   // the CTA that has unit x
+    if (s1 > s) {
+      jobs[j].z = cta_at(s);
+      jobs[j].w = cta_at(s1 - 1);
+    } else {
+      jobs[j].z = 0;
+      jobs[j].w = -1;
+    }
+  }
 }
 
 // row i of a job's tile -> token row e and query head of its group; false past the last
@@ -193,7 +228,7 @@ __global__ void __launch_bounds__(128) paged_prepare_kernel(const PagedParams p,
   bk_pdl_trigger();
   bk_pdl_wait();
   if (blockIdx.x == gridDim.x - 1) {
-    plan_jobs(p, L, reinterpret_cast<long long*>(scratch + L.starts));
+    plan_jobs(p, L, scratch);
     return;
   }
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -330,7 +365,7 @@ struct TileCfg {
   static constexpr int kSmem = kStages * kStage + 1024;
   static constexpr int kO = 0, kQ = HD, kS = HD + HD / 2;     // tensor memory: output, queries, two buffers of scores (then probabilities)
 };
-constexpr int kTileThreads = 192;   // warps 0-3: a row each lane; 4: copies; 5: MMAs
+constexpr int kCopyWarp = 8, kMmaWarp = 9, kTileThreads = 320;   // warps 0-3 and 4-7: a row each lane, even and odd tiles
 
 // S = Q K^T and O += P V on the tensor cores.  Q (operand A), S, P and O live in tensor memory, a row per lane; K and V tiles of 64 rows come
 // through a ring in shared memory.  P = 2^(S c - m) with the running maximum m of the row; it overwrites its S as two bf16 matrices, the
@@ -343,7 +378,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
   const Layout& L = P.L;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-  __shared__ __align__(8) uint64_t full[C::kStages], empty[C::kStages], q_full, s_full[2], p_full[2], o_full;
+  __shared__ __align__(8) uint64_t full[C::kStages], empty[C::kStages], q_full, s_full[2], p_full[2], o_full[2], m_full[2][4];
+  __shared__ float m_s[2][kRows];
   __shared__ uint32_t tmem_slot;
   __shared__ int dead_s;
   volatile int* dead = &dead_s;
@@ -355,16 +391,17 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
       mbar_init(smem_u32(full + i), 1);
       mbar_init(smem_u32(empty + i), 1);
     }
-    mbar_init(smem_u32(&q_full), 128);
+    mbar_init(smem_u32(&q_full), 256);
     for (int i = 0; i < 2; i++) {
       mbar_init(smem_u32(s_full + i), 1);
       mbar_init(smem_u32(p_full + i), 128);
+      mbar_init(smem_u32(o_full + i), 1);
+      for (int w = 0; w < 4; w++) mbar_init(smem_u32(&m_full[i][w]), 1);
     }
-    mbar_init(smem_u32(&o_full), 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
-  if (warp == 5) {
+  if (warp == kMmaWarp) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(512u) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
@@ -374,23 +411,37 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(&tmem_slot);
   bk_pdl_wait();
 
-  const long long* starts = reinterpret_cast<const long long*>(P.scratch + L.starts);
-  const int n_jobs = L.n_p + L.n_s, cta = blockIdx.x;
-  const long long units = __ldcg(starts + n_jobs), u0 = bound_of(units, cta, L.ctas), u1 = bound_of(units, cta + 1, L.ctas);
-  // the first job that ends behind u0
-  int j = 0;
-  {
-    int lo = 0, hi = n_jobs;   // starts[lo] <= u0 < starts[hi]
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (__ldcg(starts + mid) <= u0) lo = mid;
-      else hi = mid;
-    }
-    j = lo;
+  const int4* jobs = jobs_of(L, P.scratch);
+  const int2* pieces = pieces_of(L, P.scratch);
+  const int n_jobs = L.n_p + L.n_s, cta = blockIdx.x, n_ctas = __ldcg(&pieces[L.ctas + 1].x);
+  int j = 0, u0 = 0, u1 = 0;
+  if (cta < n_ctas) {
+    const int2 from = __ldcg(pieces + cta);
+    u0 = from.x;
+    j = from.y;
+    u1 = __ldcg(&pieces[cta + 1].x);
   }
+  // the next piece of a job, from job j on
+  struct Piece {
+    Job q;
+    int key1, t0, t1;
+  };
+  auto next_piece = [&](Piece* x) {
+    for (; j < n_jobs; j++) {
+      const int4 job = __ldcg(jobs + j);
+      if (job.x >= u1) return false;
+      piece_of(job.x, tiles_of(L, j, job.y), u0, u1, &x->t0, &x->t1);
+      if (x->t0 >= x->t1) continue;
+      x->q = job_of(p, L, j);
+      x->key1 = job.y;
+      return true;
+    }
+    return false;
+  };
+  Piece x;
 
   if (u1 > u0) {
-    if (warp == 4) {
+    if (warp == kCopyWarp) {
       // ================= copies: lane (chunk, block) takes box_rows rows x 64 dims =================
       asm volatile("fence.proxy.async;" ::: "memory");   // rows that an earlier kernel stored
       constexpr int kBlocks = HD / 64;
@@ -400,17 +451,13 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
       const uint32_t box_at = block * (kTile * 128) + chunk * P.box_rows * 128;
       int stage = 0;
       uint32_t parity = 1;
-      for (; j < n_jobs; j++) {
-        const long long s = __ldcg(starts + j);
-        if (s >= u1) break;
-        const Job q = job_of(p, L, j);
-        int t0, t1;
-        piece_of(s, tiles_of(q), u0, u1, &t0, &t1);
-        if (t0 >= t1) continue;
+      for (; next_piece(&x); j++) {
+        const Job q = x.q;
+        const int t0 = x.t0, t1 = x.t1, key1 = x.key1;
         const int* table = p.table + (size_t)max(q.seq, 0) * p.max_pages;
         auto row_of_tile = [&](int i) {   // row of the map that this lane's box of tile i starts at
           const int key = q.key0 + i * kTile + chunk * P.box_rows;
-          if (lane >= n_box || i >= t1 || key >= q.key1 || key / p.page_rows >= p.max_pages) return no_row;
+          if (lane >= n_box || i >= t1 || key >= key1 || key / p.page_rows >= p.max_pages) return no_row;
           const int page = __ldg(table + key / p.page_rows);
           return page >= 0 && page < p.n_pages ? (page * p.Hkv + q.kvh) * p.page_rows + key % p.page_rows : no_row;
         };
@@ -445,7 +492,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
           }
         }
       }
-    } else if (warp == 5) {
+    } else if (warp == kMmaWarp) {
       // ================= MMAs =================
       constexpr uint32_t kShapeS = mma_shape(kTile, false), kShapeO = mma_shape(HD, true);
       int stage = 0, tile = 0, pieces = 0;   // tile: counted over all pieces
@@ -456,12 +503,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
           parity ^= 1u;
         }
       };
-      for (; j < n_jobs; j++) {
-        const long long s = __ldcg(starts + j);
-        if (s >= u1) break;
-        int t0, t1;
-        piece_of(s, tiles_of(job_of(p, L, j)), u0, u1, &t0, &t1);
-        if (t0 >= t1) continue;
+      for (; next_piece(&x); j++) {
+        const int t0 = x.t0, t1 = x.t1;
         bar_wait_warp(smem_u32(&q_full), pieces & 1, P.status, dead);
         tc_after();
         for (int i = t0; i <= t1; i++) {
@@ -493,7 +536,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
                   tc_mma(tmem + C::kO, tmem + C::kS + (prev & 1) * kTile + half * 32 + ks * 8, smem_desc(v_at + ks * 2048, kTile * 128, 1024), kShapeO,
                          i - 1 > t0 || half > 0 || ks > 0);
               tc_commit(smem_u32(empty + stage));
-              tc_commit(smem_u32(&o_full));
+              tc_commit(smem_u32(o_full + (prev & 1)));
             }
             __syncwarp();
             next_stage();
@@ -502,34 +545,41 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
         pieces++;
       }
     } else {
-      // ================= rows: thread <-> row of the tile =================
-      const int i_row = threadIdx.x;
-      const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16);
+      // ================= rows: thread <-> row of the tile; two groups of four warps take turns at the tiles =================
+      // The row's maximum goes from tile to tile, so from group to group, as soon as the tile's scores have been looked at; the rest of a
+      // tile's work runs beside the next one's.
+      const int group = warp >> 2, quarter = warp & 3, i_row = threadIdx.x & 127;
+      const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16), s_at = lanes + C::kS + group * kTile;
       const float c = __fmul_rn(p.scale, 1.44269504088896341f);   // scores in powers of two
       int tile = 0, stream = 0;   // counted over all pieces
-      for (; j < n_jobs; j++) {
-        const long long s0 = __ldcg(starts + j);
-        if (s0 >= u1) break;
-        const Job q = job_of(p, L, j);
-        int t0, t1;
-        piece_of(s0, tiles_of(q), u0, u1, &t0, &t1);
-        if (t0 >= t1) continue;
-        const int n = t1 - t0;
-        int b, t, g, limit = 0;
+      // A wait tells a phase from the next one only, so nobody may be two phases off.  Scores of a tile that are there mean that the output of
+      // the tile two before is, so with a barrier for even and one for odd tiles the waits below are within one.
+      auto wait_output = [&](int t) {
+        bar_wait_warp(smem_u32(o_full + (t & 1)), (t >> 1) & 1, P.status, dead);
+        tc_after();
+      };
+      auto other_maximum = [&](int t) {   // of this row after tile t, which the other group has
+        bar_wait_warp(smem_u32(&m_full[group ^ 1][quarter]), (t >> 1) & 1, P.status, dead);
+        return *reinterpret_cast<volatile float*>(&m_s[group ^ 1][i_row]);
+      };
+      for (; next_piece(&x); j++) {
+        const Job q = x.q;
+        const int t0 = x.t0, n = x.t1 - t0, key1 = x.key1;
+        int b, t, g, limit = 0x7fffffff;   // (lanes without a row: never masked, never read)
         const bool mine = row_at(p, q, i_row, &b, &t, &g);
-        if (mine) limit = min(row_of(p, b, t) + 1, q.key1);
+        if (mine) limit = min(row_of(p, b, t) + 1, key1);
         __syncwarp();
         const bool warp_on = __any_sync(0xffffffffu, mine);
-        {   // queries into tensor memory (the MMAs that read the ones before have completed: their scores were there)
+        {   // queries into tensor memory, half of the dims a group (the MMAs that read the ones before have completed: their output was there)
           const uint16_t* src = p.q + ((size_t)(t * p.B + b) * p.Hq + q.kvh * (p.Hq / p.Hkv) + g) * HD;
           tc_after();
           if (warp_on) {
 #pragma unroll
-            for (int d = 0; d < HD / 64; d++) {
+            for (int d = group * (HD / 128); d < (group + 1) * (HD / 128); d++) {
               uint32_t v[32];
 #pragma unroll
               for (int e = 0; e < 8; e++) {
-                const uint4 w = limit > 0 ? __ldcg(reinterpret_cast<const uint4*>(src + d * 64 + e * 8)) : make_uint4(0, 0, 0, 0);
+                const uint4 w = mine && limit > 0 ? __ldcg(reinterpret_cast<const uint4*>(src + d * 64 + e * 8)) : make_uint4(0, 0, 0, 0);
                 v[4 * e] = w.x; v[4 * e + 1] = w.y; v[4 * e + 2] = w.z; v[4 * e + 3] = w.w;
               }
               tmem_st32(lanes + C::kQ + d * 32, v);
@@ -539,97 +589,98 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
           tc_before();
           bar_arrive(smem_u32(&q_full));
         }
-        float m = -INFINITY, l = 0.0f;
+        float m = -INFINITY, l = 0.0f;   // the maximum that this group used last, and its part of the row sum
         for (int i = 0; i < n; i++, tile++) {
-          const int key0 = q.key0 + (t0 + i) * kTile, there = min(kTile, q.key1 - key0);
-          const uint32_t s_at = lanes + C::kS + (tile & 1) * kTile;
-          bar_wait_warp(smem_u32(s_full + (tile & 1)), (tile >> 1) & 1, P.status, dead);
+          if ((tile & 1) != group) continue;
+          const int tile_key = q.key0 + (t0 + i) * kTile, there = min(kTile, key1 - tile_key);
+          bar_wait_warp(smem_u32(s_full + group), (tile >> 1) & 1, P.status, dead);
           tc_after();
           if (there < kTile) {   // values past the end count as zeros, whatever the page holds there
             const int v_pos = stream + stream_v(i, n), v_stage = v_pos % C::kStages;
             bar_wait_warp(smem_u32(full + v_stage), (v_pos / C::kStages) & 1, P.status, dead);
             uint8_t* v_at = ring + (size_t)v_stage * C::kStage;
-            for (int x = threadIdx.x; x < (kTile - there) * (HD / 8); x += 128) {
-              const int row = there + x / (HD / 8), piece = x % (HD / 8);
+            for (int y = i_row; y < (kTile - there) * (HD / 8); y += 128) {
+              const int row = there + y / (HD / 8), piece = y % (HD / 8);
               *reinterpret_cast<uint4*>(v_at + (piece >> 3) * (kTile * 128) + row * 128 + (piece & 7) * 16) = make_uint4(0, 0, 0, 0);
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
           }
           if (warp_on) {
-            float s[64];
-            {
-              uint32_t v[64];
-              tmem_ld64(s_at, v);
+            uint32_t s[64];
+            tmem_ld64(s_at, s);
+            if (!__all_sync(0xffffffffu, tile_key + kTile <= limit)) {
 #pragma unroll
-              for (int x = 0; x < 64; x++) s[x] = __uint_as_float(v[x]);
+              for (int y = 0; y < 64; y++) s[y] = tile_key + y < limit ? s[y] : 0xff800000u;
             }
-            if (!__all_sync(0xffffffffu, key0 + kTile <= limit)) {
+            float mx = __uint_as_float(s[0]);
 #pragma unroll
-              for (int x = 0; x < 64; x++) s[x] = key0 + x < limit ? s[x] : -INFINITY;
-            }
-            float mx = s[0];
-#pragma unroll
-            for (int x = 1; x < 64; x++) mx = fmaxf(mx, s[x]);
+            for (int y = 1; y < 64; y++) mx = fmaxf(mx, __uint_as_float(s[y]));
             mx = __fmul_rn(mx, c);
-            const bool move = mx > __fadd_rn(m, 8.0f);
-            if (__any_sync(0xffffffffu, move)) {
-              const float to = move ? mx : m;
-              const float f = m == to || m == -INFINITY ? 1.0f : exp2_approx(__fsub_rn(m, to));
-              const bool rescale = move && m != -INFINITY;
-              m = to;
-              l = __fmul_rn(l, f);
-              if (__any_sync(0xffffffffu, rescale)) {
-                bar_wait_warp(smem_u32(&o_full), (tile - 1) & 1, P.status, dead);   // tile i - 1 has been added to the output
-                tc_after();
+            const float m0 = i > 0 ? other_maximum(tile - 1) : -INFINITY;
+            const bool move = mx > __fadd_rn(m0, 8.0f);
+            const float m1 = move ? mx : m0;
+            m_s[group][i_row] = m1;
+            __syncwarp();
+            if (lane == 0) bar_arrive(smem_u32(&m_full[group][quarter]));
+            if (__any_sync(0xffffffffu, move && m0 != -INFINITY)) {   // the output so far is rescaled
+              const float f = move && m0 != -INFINITY ? exp2_approx(__fsub_rn(m0, m1)) : 1.0f;
+              wait_output(tile - 1);
 #pragma unroll 1
-                for (int d = 0; d < HD / 32; d++) {
-                  uint32_t o[32];
-                  tmem_ld32(lanes + C::kO + d * 32, o);
+              for (int d = 0; d < HD / 32; d++) {
+                uint32_t o[32];
+                tmem_ld32(lanes + C::kO + d * 32, o);
 #pragma unroll
-                  for (int x = 0; x < 32; x++) o[x] = __float_as_uint(__fmul_rn(__uint_as_float(o[x]), f));
-                  tmem_st32(lanes + C::kO + d * 32, o);
-                }
+                for (int y = 0; y < 32; y++) o[y] = __float_as_uint(__fmul_rn(__uint_as_float(o[y]), f));
+                tmem_st32(lanes + C::kO + d * 32, o);
               }
             }
+            if (m != m1 && m != -INFINITY) l = __fmul_rn(l, exp2_approx(__fsub_rn(m, m1)));
+            m = m1;
             const float base = m == -INFINITY ? 0.0f : m;
-            uint32_t hi[32], lo[32];
             float2 sum = make_float2(0.0f, 0.0f);
+            uint32_t lo[32];
 #pragma unroll
-            for (int x = 0; x < 32; x++) {
-              const float2 y = bk_fma2(make_float2(s[2 * x], s[2 * x + 1]), make_float2(c, c), make_float2(-base, -base));
-              const float2 e = make_float2(exp2_approx(y.x), exp2_approx(y.y));
+            for (int y = 0; y < 32; y++) {
+              const float2 z = bk_fma2(make_float2(__uint_as_float(s[2 * y]), __uint_as_float(s[2 * y + 1])), make_float2(c, c), make_float2(-base, -base));
+              const float2 e = make_float2(exp2_approx(z.x), exp2_approx(z.y));
               sum = bk_add2(sum, e);
-              hi[x] = bk_f32x2_to_bf16x2(e.x, e.y);
-              lo[x] = bk_f32x2_to_bf16x2(__fsub_rn(e.x, __uint_as_float(hi[x] << 16)), __fsub_rn(e.y, __uint_as_float(hi[x] & 0xffff0000u)));
+              s[y] = bk_f32x2_to_bf16x2(e.x, e.y);
+              lo[y] = bk_f32x2_to_bf16x2(__fsub_rn(e.x, __uint_as_float(s[y] << 16)), __fsub_rn(e.y, __uint_as_float(s[y] & 0xffff0000u)));
             }
             l = __fadd_rn(l, __fadd_rn(sum.x, sum.y));
-            tmem_st32(s_at, hi);
+            tmem_st32(s_at, s);
             tmem_st32(s_at + 32, lo);
             tmem_wait_st();
-          }
+          } else if (lane == 0) bar_arrive(smem_u32(&m_full[group][quarter]));
           tc_before();
-          bar_arrive(smem_u32(p_full + (tile & 1)));
+          bar_arrive(smem_u32(p_full + group));
         }
         stream += 2 * n;
-        // the piece's part of the result
-        if (n > 1) bar_wait_warp(smem_u32(&o_full), (tile - 2) & 1, P.status, dead);   // (a wait must not be two phases ahead)
-        bar_wait_warp(smem_u32(&o_full), (tile - 1) & 1, P.status, dead);
-        tc_after();
+        // the piece's part of the result: row sums relative to the last maximum, half of the dims a group
+        if (((tile - 1) & 1) != group) {
+          const float m1 = other_maximum(tile - 1);   // (of a warp without rows: whatever it is)
+          if (m != m1 && m != -INFINITY) l = __fmul_rn(l, exp2_approx(__fsub_rn(m, m1)));
+          m = m1;
+        }
+        wait_output(tile - 1);
         if (warp_on) {
           const bool common = q.seq < 0;
           const size_t slot = common ? (size_t)(j + cta) * kRows : (size_t)(j - L.n_p + cta) * L.rows_s;
-          float2* ml = reinterpret_cast<float2*>(P.scratch + (common ? L.ml_p : L.ml_s)) + slot + i_row;
+          float* ml = reinterpret_cast<float*>(P.scratch + (common ? L.ml_p : L.ml_s)) + (slot + i_row) * 4;
           float* o_to = reinterpret_cast<float*>(P.scratch + (common ? L.o_p : L.o_s)) + (slot + i_row) * HD;
-          if (mine) *ml = make_float2(m, l);
+          if (mine) {
+            if (group == 0) ml[0] = m;
+            ml[1 + group] = l;
+          }
           __syncwarp();
 #pragma unroll 1
-          for (int d = 0; d < HD / 32; d++) {
+          for (int d = group * (HD / 64); d < (group + 1) * (HD / 64); d++) {
             uint32_t o[32];
             tmem_ld32(lanes + C::kO + d * 32, o);
             if (mine) {
 #pragma unroll
-              for (int x = 0; x < 32; x += 4) *reinterpret_cast<uint4*>(o_to + d * 32 + x) = make_uint4(o[x], o[x + 1], o[x + 2], o[x + 3]);
+              for (int y = 0; y < 32; y += 4) *reinterpret_cast<uint4*>(o_to + d * 32 + y) = make_uint4(o[y], o[y + 1], o[y + 2], o[y + 3]);
             }
             __syncwarp();
           }
@@ -641,56 +692,101 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
   tc_before();
   __syncthreads();
   tc_after();
-  if (warp == 5) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+  if (warp == kMmaWarp) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
 }
 
-// One CTA per (token row, query head): out = sum of the pieces' results, the common keys' first, each in the order of the line.
+// One CTA per (token row, query head): the pieces' results, the common keys' first, each in the order of the line.  Four quarters of the
+// pieces at a time, a thread four dims of each.
+constexpr int kMaxPieces = 512;   // of a row: two jobs, at most one piece a CTA
 template <int HD>
-__global__ void __launch_bounds__(HD / 4) paged_merge_kernel(const PagedParams p, const Layout L, const uint8_t* scratch) {
+__global__ void __launch_bounds__(HD) paged_merge_kernel(const PagedParams p, const Layout L, uint8_t* scratch) {
+  __shared__ float w_s[kMaxPieces];
+  __shared__ float red_s[HD / 32];
+  __shared__ __align__(16) float4 o_s[3][HD / 4];
   bk_pdl_trigger();
+  const int h = blockIdx.y, e = blockIdx.x, t = e / p.B, b = e - t * p.B, G = p.Hq / p.Hkv, kvh = h / G, g = h - kvh * G, tid = threadIdx.x;
+  const int rp = (b * p.T + t) * G + g, rs = t * G + g;
+  const int jp = kvh * L.mt_p + rp / kRows, js = (b * p.Hkv + kvh) * L.mt_s + rs / kRows;   // within their kind
   bk_pdl_wait();
-  const int h = blockIdx.y, e = blockIdx.x, t = e / p.B, b = e - t * p.B, G = p.Hq / p.Hkv, kvh = h / G, g = h - kvh * G;
-  const long long* starts = reinterpret_cast<const long long*>(scratch + L.starts);
-  const long long units = __ldcg(starts + L.n_p + L.n_s);
+  const int4* jobs = jobs_of(L, scratch);
+  const int2* pieces = pieces_of(L, scratch);
   const bool here = row_of(p, b, t) >= 0;
-  float m = -INFINITY, l = 0.0f;
-  float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  for (int part = 0; part < 2 && here; part++) {
-    const bool common = part == 0;
-    if (common && L.n_p == 0) continue;
-    const int r = common ? (b * p.T + t) * G + g : t * G + g, mt = r / kRows, row = r - mt * kRows;
-    const int j = common ? kvh * L.mt_p + mt : (b * p.Hkv + kvh) * L.mt_s + mt;   // within its kind
-    const int job = common ? j : L.n_p + j;
-    const long long s = __ldcg(starts + job), s_end = __ldcg(starts + job + 1);
-    if (s == s_end) continue;
-    const int tiles = (int)(s_end - s) - kOverhead, c1 = cta_at(units, s_end - 1, L.ctas);
-    const int rows = common ? kRows : L.rows_s;
-    const float2* ml = reinterpret_cast<const float2*>(scratch + (common ? L.ml_p : L.ml_s));
-    const float* os = reinterpret_cast<const float*>(scratch + (common ? L.o_p : L.o_s));
-    for (int c = cta_at(units, s, L.ctas); c <= c1; c++) {
+  const uint16_t* gate = p.fused ? p.qg + ((size_t)e * p.Hq + h) * 2 * HD + HD : p.gate ? p.gate + ((size_t)e * p.Hq + h) * HD : nullptr;
+  uint2 gv = make_uint2(0, 0);
+  if (gate && tid < HD / 4) gv = *reinterpret_cast<const uint2*>(gate + tid * 4);
+  const int4 none = make_int4(0, 0, 0, -1);
+  const int4 qp = here && L.n_p ? __ldcg(jobs + jp) : none, qs = here ? __ldcg(jobs + L.n_p + js) : none;
+  const int np = qp.w - qp.z + 1, n = np + qs.w - qs.z + 1;
+  auto row_of_piece = [&](int i) {   // in the partial results of its kind
+    return i < np ? (size_t)(jp + qp.z + i) * kRows + rp % kRows : (size_t)(js + qs.z + i - np) * L.rows_s + rs % kRows;
+  };
+  // weights: w_i = 2^(m_i - M), and the sum of w_i l_i
+  float m[kMaxPieces / HD], l[kMaxPieces / HD], M = -INFINITY, sum = 0.0f;
+#pragma unroll
+  for (int k = 0; k < kMaxPieces / HD; k++) {
+    const int i = tid + k * HD;
+    m[k] = -INFINITY;
+    l[k] = 0.0f;
+    if (i < n) {
+      const bool common = i < np;
+      const int4 q = common ? qp : qs;
+      const int cta = common ? qp.z + i : qs.z + i - np;
       int t0, t1;
-      piece_of(s, tiles, bound_of(units, c, L.ctas), bound_of(units, c + 1, L.ctas), &t0, &t1);
-      if (t0 >= t1) continue;
-      const size_t at = (size_t)(j + c) * rows + row;
-      const float2 x = __ldcg(ml + at);
-      if (x.x == -INFINITY) continue;
-      const float4 v = __ldcg(reinterpret_cast<const float4*>(os + at * HD) + threadIdx.x);
-      const float mn = fmaxf(m, x.x), f = exp2_approx(__fsub_rn(m, mn)), w = exp2_approx(__fsub_rn(x.x, mn));   // (m = -inf: f = 0)
-      l = fmaf(l, f, __fmul_rn(w, x.y));
-      o.x = fmaf(o.x, f, __fmul_rn(w, v.x)); o.y = fmaf(o.y, f, __fmul_rn(w, v.y));
-      o.z = fmaf(o.z, f, __fmul_rn(w, v.z)); o.w = fmaf(o.w, f, __fmul_rn(w, v.w));
-      m = mn;
+      piece_of(q.x, tiles_of(L, common ? jp : L.n_p + js, q.y), __ldcg(&pieces[cta].x), __ldcg(&pieces[cta + 1].x), &t0, &t1);
+      if (t0 < t1) {
+        const float4 v = __ldcg(reinterpret_cast<const float4*>(scratch + (common ? L.ml_p : L.ml_s)) + row_of_piece(i));
+        m[k] = v.x;
+        l[k] = __fadd_rn(v.y, v.z);
+      }
     }
+    M = fmaxf(M, m[k]);
+  }
+  M = bk_warp_max(M);
+  if ((tid & 31) == 0) red_s[tid >> 5] = M;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < HD / 32; w++) M = fmaxf(M, red_s[w]);
+#pragma unroll
+  for (int k = 0; k < kMaxPieces / HD; k++) {
+    const int i = tid + k * HD;
+    const float w = m[k] == -INFINITY ? 0.0f : exp2_approx(__fsub_rn(m[k], M));
+    if (i < n) w_s[i] = w;
+    sum = fmaf(w, l[k], sum);
+  }
+  sum = bk_warp_sum(sum);
+  __syncthreads();
+  if ((tid & 31) == 0) red_s[tid >> 5] = sum;
+  __syncthreads();
+  sum = 0.0f;
+#pragma unroll
+  for (int w = 0; w < HD / 32; w++) sum = __fadd_rn(sum, red_s[w]);
+
+  const int slice = tid / (HD / 4), col = tid % (HD / 4);
+  float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+  for (int i = slice; i < n; i += 4) {
+    const float w = w_s[i];
+    if (w == 0.0f) continue;   // (nothing there, perhaps not even written)
+    const float4 v = __ldcg(reinterpret_cast<const float4*>(scratch + (i < np ? L.o_p : L.o_s)) + row_of_piece(i) * (HD / 4) + col);
+    o.x = fmaf(w, v.x, o.x); o.y = fmaf(w, v.y, o.y); o.z = fmaf(w, v.z, o.z); o.w = fmaf(w, v.w, o.w);
+  }
+  if (slice) o_s[slice - 1][col] = o;
+  __syncthreads();
+  if (slice) return;
+#pragma unroll
+  for (int k = 0; k < 3; k++) {
+    const float4 v = o_s[k][col];
+    o.x = __fadd_rn(o.x, v.x); o.y = __fadd_rn(o.y, v.y); o.z = __fadd_rn(o.z, v.z); o.w = __fadd_rn(o.w, v.w);
   }
   float y[4] = {o.x, o.y, o.z, o.w};
-  const bool any = m != -INFINITY;
-  const uint16_t* gate = p.fused ? p.qg + ((size_t)e * p.Hq + h) * 2 * HD + HD : p.gate ? p.gate + ((size_t)e * p.Hq + h) * HD : nullptr;
+  const uint32_t gw[2] = {gv.x, gv.y};
+  const bool any = M != -INFINITY;
 #pragma unroll
   for (int i = 0; i < 4; i++) {
-    y[i] = any ? __fdiv_rn(y[i], l) : 0.0f;
-    if (gate && any) y[i] = __fmul_rn(y[i], bk_sigmoidf(bk_bf16_to_f32(gate[threadIdx.x * 4 + i])));
+    y[i] = any ? __fdiv_rn(y[i], sum) : 0.0f;
+    if (gate && any) y[i] = __fmul_rn(y[i], bk_sigmoidf(__uint_as_float(i & 1 ? gw[i >> 1] & 0xffff0000u : gw[i >> 1] << 16)));
   }
-  *reinterpret_cast<uint2*>(p.out + ((size_t)e * p.Hq + h) * HD + threadIdx.x * 4) = make_uint2(bk_f32x2_to_bf16x2(y[0], y[1]), bk_f32x2_to_bf16x2(y[2], y[3]));
+  *reinterpret_cast<uint2*>(p.out + ((size_t)e * p.Hq + h) * HD + col * 4) = make_uint2(bk_f32x2_to_bf16x2(y[0], y[1]), bk_f32x2_to_bf16x2(y[2], y[3]));
 }
 
 template <int HD>
@@ -715,7 +811,7 @@ int32_t launch_paged(const PagedParams& p, const Layout& L, uint64_t scratch) {
   }
   BK_CUDA(bk_launch_pdl(paged_tile_kernel<HD>, dim3(L.ctas), dim3(kTileThreads), TileCfg<HD>::kSmem, P));
   BK_CHECK_LAUNCH();
-  BK_CUDA(bk_launch_pdl(paged_merge_kernel<HD>, dim3(p.T * p.B, p.Hq), dim3(HD / 4), 0, p, L, P.scratch));
+  BK_CUDA(bk_launch_pdl(paged_merge_kernel<HD>, dim3(p.T * p.B, p.Hq), dim3(HD), 0, p, L, P.scratch));
   BK_CHECK_LAUNCH();
   return BK_OK;
 }
@@ -762,6 +858,8 @@ int32_t bkPagedAttn(const bkPagedAttnArgs* args) {
   p.B = a.B; p.T = a.T; p.Hq = a.Hq; p.Hkv = a.Hkv; p.rot_half = a.rot_half; p.n_pages = a.n_pages; p.page_rows = a.page_rows; p.max_pages = a.max_pages;
   p.max_rows = (int)std::min<long long>(a.max_len, (long long)a.max_pages * a.page_rows); p.fused = a.fused_norm_rope != 0; p.scale = a.scale; p.eps = a.eps;
   const Layout L = make_layout(a.B, a.T, a.Hq, a.Hkv, a.HD, a.prefix_rows, a.page_rows, bk_ctx().sm_count);
+  BK_ARG((long long)(L.n_p + L.n_s) * ((long long)p.max_rows / kTile + 1 + kOverhead) < (1ll << 31) && 2 * L.ctas <= kMaxPieces, "bkPagedAttn: B=%d T=%d Hkv=%d with %d rows a sequence: too much for one call", a.B,
+         a.T, a.Hkv, p.max_rows);
   return a.HD == 256 ? launch_paged<256>(p, L, a.scratch) : launch_paged<128>(p, L, a.scratch);
 }
 
