@@ -17,7 +17,7 @@ struct PagedParams {
   uint16_t *k_pages, *v_pages;
   const int *table, *lens, *n_new;
   uint16_t* out;
-  uint16_t* q;        // ready q [T*B][Hq][HD]: qg, or the scratch buffer
+  uint16_t* q;        // ready q [Hkv][B][T][Hq / Hkv][HD] in the scratch buffer: the rows of a job lie together
   int B, T, Hq, Hkv, rot_half, n_pages, page_rows, max_pages, max_rows, fused;   // max_rows: what a sequence can have
   float scale, eps;
 };
@@ -74,7 +74,7 @@ inline Layout make_layout(int B, int T, int Hq, int Hkv, int HD, int prefix_rows
   L.jobs = at;
   at += (size_t)(L.n_p + L.n_s + 1) * 16;
   L.pieces = at;
-  at += round16((size_t)(ctas + 2) * 8);
+  at += (size_t)ctas * 32;
   // partial results: a job and a CTA that has a piece of it meet in slot job + CTA, which no other pair has
   const size_t slots_p = L.n_p ? L.n_p + ctas : 0, slots_s = L.n_s + ctas;
   L.ml_p = at;
@@ -95,7 +95,8 @@ struct TileParams {
   uint8_t* scratch;
   int* status;
   int box_rows;   // rows of a page that one copy takes: min(page_rows, kTile)
-  CUtensorMap k_map, v_map;
+  int q_rows[2];  // rows of queries that a job takes: over a sequence's own keys, over the common ones
+  CUtensorMap k_map, v_map, q_map[2];
 };
 
 // job j: its KV head, row tile, sequence (-1: all) and where its keys begin
@@ -129,10 +130,10 @@ BK_DEVINL int keys_end(const PagedParams& p, const Layout& L, const Job& q) {
   return L.P;
 }
 
-// What the first launch leaves for the others.  jobs[j] = {start on the line, end of the keys, first and last CTA that may have a piece of it};
-// pieces[c] = {start of CTA c's piece of the line, first job in it}; pieces[ctas + 1].x = the number of CTAs that get one.
+// What the first launch leaves for the others.  jobs[j] = {start on the line, end of the keys, first and last CTA that have a piece of it};
+// pieces[2c] = {start and end of CTA c's piece of the line, first job in it, -}, pieces[2c + 1] = that job.
 BK_DEVINL int4* jobs_of(const Layout& L, uint8_t* scratch) { return reinterpret_cast<int4*>(scratch + L.jobs); }
-BK_DEVINL int2* pieces_of(const Layout& L, uint8_t* scratch) { return reinterpret_cast<int2*>(scratch + L.pieces); }
+BK_DEVINL int4* pieces_of(const Layout& L, uint8_t* scratch) { return reinterpret_cast<int4*>(scratch + L.pieces); }
 BK_DEVINL int tiles_of(const Layout& L, int j, int key1) { return (key1 - (j < L.n_p ? 0 : L.P) + kTile - 1) / kTile; }
 // the tiles of a job that starts at s and has n tiles which lie in units [u0, u1): [t0, t1)
 BK_DEVINL void piece_of(int s, int n, int u0, int u1, int* t0, int* t1) {
@@ -144,7 +145,7 @@ BK_DEVINL void piece_of(int s, int n, int u0, int u1, int* t0, int* t1) {
 BK_DEVINL void plan_jobs(const PagedParams& p, const Layout& L, uint8_t* scratch) {
   __shared__ int warp_s[4][2];
   int4* jobs = jobs_of(L, scratch);
-  int2* pieces = pieces_of(L, scratch);
+  int4* pieces = pieces_of(L, scratch);
   const int n = L.n_p + L.n_s, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int base = 0, tiles_all = 0;
   for (int j0 = 0; j0 < n; j0 += 128) {
@@ -180,22 +181,22 @@ BK_DEVINL void plan_jobs(const PagedParams& p, const Layout& L, uint8_t* scratch
   __syncthreads();   // jobs[].x is there for all
   const int C = max(1, min(L.ctas, tiles_all)), units = base;   // every CTA has a tile to do
   auto bound = [&](int c) { return (int)((long long)units * c / C); };
-  for (int c = threadIdx.x; c <= C; c += 128) {
-    const int u = bound(c);
-    int lo = 0, hi = n;   // the last job that starts at u or before
+  for (int c = threadIdx.x; c < L.ctas; c += 128) {
+    const int u0 = c < C ? bound(c) : 0, u1 = c < C ? bound(c + 1) : 0;
+    int lo = 0, hi = n;   // the last job that starts at u0 or before
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
-      if (jobs[mid].x <= u) lo = mid;
+      if (jobs[mid].x <= u0) lo = mid;
       else hi = mid;
     }
-    pieces[c] = make_int2(u, lo);
+    pieces[2 * c] = make_int4(u0, u1, lo, 0);
+    pieces[2 * c + 1] = jobs[lo];
   }
-  if (threadIdx.x == 0) pieces[L.ctas + 1] = make_int2(C, 0);
   for (int j = threadIdx.x; j < n; j += 128) {
     const int s = jobs[j].x, s1 = jobs[j + 1].x;
     auto cta_at = [&](int x) { return (int)((((long long)x + 1) * C - 1) / units); };   // the CTA that has unit x
     if (s1 > s) {
-      jobs[j].z = cta_at(s);
+      jobs[j].z = cta_at(s + kOverhead);
       jobs[j].w = cta_at(s1 - 1);
     } else {
       jobs[j].z = 0;
@@ -232,16 +233,16 @@ __global__ void __launch_bounds__(128) paged_prepare_kernel(const PagedParams p,
     return;
   }
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int heads = (p.fused ? p.Hq : 0) + (p.k ? p.Hkv : 0);
+  const int heads = p.Hq + (p.k ? p.Hkv : 0);
   const int item = blockIdx.x * 4 + warp;
   if (item >= p.T * p.B * heads) return;
   const int e = item / heads, h = item - e * heads, t = e / p.B, b = e - t * p.B;
   const int at = row_of(p, b, t);
   if (at < 0) return;
-  const bool is_q = p.fused && h < p.Hq;
-  const int kvh = h - (p.fused ? p.Hq : 0);
-  const uint16_t* src = is_q ? p.qg + ((size_t)e * p.Hq + h) * 2 * HD : p.k + ((size_t)e * p.Hkv + kvh) * HD;
-  uint16_t* dst = p.q + ((size_t)e * p.Hq + h) * HD;
+  const bool is_q = h < p.Hq;
+  const int kvh = h - p.Hq, G = p.Hq / p.Hkv;
+  const uint16_t* src = is_q ? p.qg + ((size_t)e * p.Hq + h) * (p.fused ? 2 : 1) * HD : p.k + ((size_t)e * p.Hkv + kvh) * HD;
+  uint16_t* dst = p.q + (((size_t)(h / G) * p.B + b) * p.T + t) * G * HD + (size_t)(h % G) * HD;
   if (!is_q) {
     const int page = p.table[(size_t)b * p.max_pages + at / p.page_rows];
     if (page < 0 || page >= p.n_pages) return;
@@ -361,14 +362,16 @@ BK_DEVINL int stream_v(int i, int n) { return i < n - 1 ? 2 * i + 2 : 2 * n - 1;
 template <int HD>
 struct TileCfg {
   static constexpr int kStage = kTile * HD * 2;               // bytes of 64 keys or values
-  static constexpr int kStages = HD == 256 ? 6 : 12;
-  static constexpr int kSmem = kStages * kStage + 1024;
+  static constexpr int kStages = HD == 256 ? 5 : 12;
+  static constexpr int kQuery = kRows * HD * 2;               // bytes of the queries
+  static constexpr int kSmem = kQuery + kStages * kStage + 1024;
   static constexpr int kO = 0, kQ = HD, kS = HD + HD / 2;     // tensor memory: output, queries, two buffers of scores (then probabilities)
 };
-constexpr int kCopyWarp = 8, kMmaWarp = 9, kTileThreads = 320;   // warps 0-3 and 4-7: a row each lane, even and odd tiles
+constexpr int kCopyWarp = 8, kMmaWarp = 9, kQueryWarp = 10, kTileThreads = 352;   // warps 0-3 and 4-7: a row each lane, even and odd tiles
 
-// S = Q K^T and O += P V on the tensor cores.  Q (operand A), S, P and O live in tensor memory, a row per lane; K and V tiles of 64 rows come
-// through a ring in shared memory.  P = 2^(S c - m) with the running maximum m of the row; it overwrites its S as two bf16 matrices, the
+// S = Q K^T and O += P V on the tensor cores.  Q, S, P and O live in tensor memory, a row per lane (with Q in shared memory its reads, 64 KB a step,
+// make a step 500 cycles longer: K, V twice and what TMA writes take three quarters of that bandwidth); a ring of K and V tiles of 64 rows in shared
+// memory, by TMA.  Q comes by TMA too, ahead of its turn, and is moved by the lanes that own the rows.  P = 2^(S c - m) with the running maximum m of the row; it overwrites its S as two bf16 matrices, the
 // rounded values and what rounding left (16 bits of the value; with 8 the result's error against exact arithmetic is 1.7 times that of its own rounding).
 // m is only moved when a score passes it by more than 2^8, since O must be rescaled then.  Row sums are in f32, by the lane that owns the row.
 template <int HD>
@@ -377,8 +380,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
   const PagedParams& p = P.g;
   const Layout& L = P.L;
   extern __shared__ uint8_t smem_raw[];
-  uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-  __shared__ __align__(8) uint64_t full[C::kStages], empty[C::kStages], q_full, s_full[2], p_full[2], o_full[2], m_full[2][4];
+  uint8_t* q_s = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);   // [HD / 64][kRows][64]
+  uint8_t* ring = q_s + C::kQuery;                                                                                // stages [HD / 64][kTile][64]
+  __shared__ __align__(8) uint64_t full[C::kStages], empty[C::kStages], q_here, q_empty, q_full, s_full[2], p_full[2], o_full[2], m_full[2][4];
   __shared__ float m_s[2][kRows];
   __shared__ uint32_t tmem_slot;
   __shared__ int dead_s;
@@ -391,7 +395,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
       mbar_init(smem_u32(full + i), 1);
       mbar_init(smem_u32(empty + i), 1);
     }
-    mbar_init(smem_u32(&q_full), 256);
+    mbar_init(smem_u32(&q_here), 1);
+    mbar_init(smem_u32(&q_empty), 8);
+    mbar_init(smem_u32(&q_full), 8);
     for (int i = 0; i < 2; i++) {
       mbar_init(smem_u32(s_full + i), 1);
       mbar_init(smem_u32(p_full + i), 128);
@@ -405,6 +411,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(512u) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
+  if (warp == kCopyWarp && lane < 4)
+    asm volatile("prefetch.tensormap [%0];" ::"l"(lane == 0 ? &P.k_map : lane == 1 ? &P.v_map : P.q_map + (lane - 2)) : "memory");
   tc_before();
   __syncthreads();
   tc_after();
@@ -412,15 +420,10 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
   bk_pdl_wait();
 
   const int4* jobs = jobs_of(L, P.scratch);
-  const int2* pieces = pieces_of(L, P.scratch);
-  const int n_jobs = L.n_p + L.n_s, cta = blockIdx.x, n_ctas = __ldcg(&pieces[L.ctas + 1].x);
-  int j = 0, u0 = 0, u1 = 0;
-  if (cta < n_ctas) {
-    const int2 from = __ldcg(pieces + cta);
-    u0 = from.x;
-    j = from.y;
-    u1 = __ldcg(&pieces[cta + 1].x);
-  }
+  const int cta = blockIdx.x, n_jobs = L.n_p + L.n_s;
+  const int4 line = __ldcg(pieces_of(L, P.scratch) + 2 * cta), first_job = __ldcg(pieces_of(L, P.scratch) + 2 * cta + 1);
+  const int u0 = line.x, u1 = line.y;
+  int j = line.z;
   // the next piece of a job, from job j on
   struct Piece {
     Job q;
@@ -428,7 +431,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
   };
   auto next_piece = [&](Piece* x) {
     for (; j < n_jobs; j++) {
-      const int4 job = __ldcg(jobs + j);
+      const int4 job = j == line.z ? first_job : __ldcg(jobs + j);
       if (job.x >= u1) return false;
       piece_of(job.x, tiles_of(L, j, job.y), u0, u1, &x->t0, &x->t1);
       if (x->t0 >= x->t1) continue;
@@ -544,6 +547,20 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
         }
         pieces++;
       }
+    } else if (warp == kQueryWarp) {
+      // ================= queries of a piece, as soon as those before have moved on =================
+      asm volatile("fence.proxy.async;" ::: "memory");   // rows that the kernel before stored
+      uint32_t parity = 1;
+      for (; next_piece(&x); j++) {
+        const bool common = x.q.seq < 0;
+        const CUtensorMap* map = P.q_map + common;
+        const int rows = P.q_rows[common], row = common ? x.q.kvh * p.B * p.T * (p.Hq / p.Hkv) : (x.q.kvh * p.B + x.q.seq) * p.T * (p.Hq / p.Hkv);
+        bar_wait_warp(smem_u32(&q_empty), parity, P.status, dead);
+        if (lane == 0) mbar_expect_tx(smem_u32(&q_here), rows * HD * 2);
+        __syncwarp();
+        if (lane < HD / 64) tma_load(smem_u32(q_s) + lane * (kRows * 128), map, lane * 64, row + x.q.mt * kRows, smem_u32(&q_here));
+        parity ^= 1u;
+      }
     } else {
       // ================= rows: thread <-> row of the tile; two groups of four warps take turns at the tiles =================
       // The row's maximum goes from tile to tile, so from group to group, as soon as the tile's scores have been looked at; the rest of a
@@ -551,7 +568,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
       const int group = warp >> 2, quarter = warp & 3, i_row = threadIdx.x & 127;
       const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16), s_at = lanes + C::kS + group * kTile;
       const float c = __fmul_rn(p.scale, 1.44269504088896341f);   // scores in powers of two
-      int tile = 0, stream = 0;   // counted over all pieces
+      int tile = 0, stream = 0, pieces = 0;   // counted over all pieces
       // A wait tells a phase from the next one only, so nobody may be two phases off.  Scores of a tile that are there mean that the output of
       // the tile two before is, so with a barrier for even and one for odd tiles the waits below are within one.
       auto wait_output = [&](int t) {
@@ -562,7 +579,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
         bar_wait_warp(smem_u32(&m_full[group ^ 1][quarter]), (t >> 1) & 1, P.status, dead);
         return *reinterpret_cast<volatile float*>(&m_s[group ^ 1][i_row]);
       };
-      for (; next_piece(&x); j++) {
+      for (; next_piece(&x); j++, pieces++) {
         const Job q = x.q;
         const int t0 = x.t0, n = x.t1 - t0, key1 = x.key1;
         int b, t, g, limit = 0x7fffffff;   // (lanes without a row: never masked, never read)
@@ -570,24 +587,27 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
         if (mine) limit = min(row_of(p, b, t) + 1, key1);
         __syncwarp();
         const bool warp_on = __any_sync(0xffffffffu, mine);
-        {   // queries into tensor memory, half of the dims a group (the MMAs that read the ones before have completed: their output was there)
-          const uint16_t* src = p.q + ((size_t)(t * p.B + b) * p.Hq + q.kvh * (p.Hq / p.Hkv) + g) * HD;
-          tc_after();
-          if (warp_on) {
+        // queries into tensor memory, half of the dims a group (the MMAs that read the ones before have completed: their output was there)
+        bar_wait_warp(smem_u32(&q_here), pieces & 1, P.status, dead);
+        tc_after();
+        if (warp_on) {
 #pragma unroll
-            for (int d = group * (HD / 128); d < (group + 1) * (HD / 128); d++) {
-              uint32_t v[32];
+          for (int d = group * (HD / 128); d < (group + 1) * (HD / 128); d++) {
+            uint32_t v[32];
 #pragma unroll
-              for (int e = 0; e < 8; e++) {
-                const uint4 w = mine && limit > 0 ? __ldcg(reinterpret_cast<const uint4*>(src + d * 64 + e * 8)) : make_uint4(0, 0, 0, 0);
-                v[4 * e] = w.x; v[4 * e + 1] = w.y; v[4 * e + 2] = w.z; v[4 * e + 3] = w.w;
-              }
-              tmem_st32(lanes + C::kQ + d * 32, v);
+            for (int y = 0; y < 8; y++) {
+              const uint4 w = *reinterpret_cast<const uint4*>(q_s + d * (kRows * 128) + i_row * 128 + ((y ^ (i_row & 7)) << 4));   // (as TMA swizzles them)
+              v[4 * y] = w.x; v[4 * y + 1] = w.y; v[4 * y + 2] = w.z; v[4 * y + 3] = w.w;
             }
-            tmem_wait_st();
+            tmem_st32(lanes + C::kQ + d * 32, v);
           }
-          tc_before();
+          tmem_wait_st();
+        }
+        tc_before();
+        __syncwarp();
+        if (lane == 0) {
           bar_arrive(smem_u32(&q_full));
+          bar_arrive(smem_u32(&q_empty));   // (in this order: the next queries' turn comes after all of these)
         }
         float m = -INFINITY, l = 0.0f;   // the maximum that this group used last, and its part of the row sum
         for (int i = 0; i < n; i++, tile++) {
@@ -618,7 +638,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
             for (int y = 1; y < 64; y++) mx = fmaxf(mx, __uint_as_float(s[y]));
             mx = __fmul_rn(mx, c);
             const float m0 = i > 0 ? other_maximum(tile - 1) : -INFINITY;
-            const bool move = mx > __fadd_rn(m0, 8.0f);
+            const bool move = mine && mx > __fadd_rn(m0, 8.0f);
             const float m1 = move ? mx : m0;
             m_s[group][i_row] = m1;
             __syncwarp();
@@ -668,7 +688,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
           const bool common = q.seq < 0;
           const size_t slot = common ? (size_t)(j + cta) * kRows : (size_t)(j - L.n_p + cta) * L.rows_s;
           float* ml = reinterpret_cast<float*>(P.scratch + (common ? L.ml_p : L.ml_s)) + (slot + i_row) * 4;
-          float* o_to = reinterpret_cast<float*>(P.scratch + (common ? L.o_p : L.o_s)) + (slot + i_row) * HD;
+          const int rows = common ? kRows : L.rows_s;
+          uint4* o_to = reinterpret_cast<uint4*>(P.scratch + (common ? L.o_p : L.o_s)) + slot * (HD / 4) + i_row;   // [HD / 4][rows] x 4 dims: lanes side by side
           if (mine) {
             if (group == 0) ml[0] = m;
             ml[1 + group] = l;
@@ -680,7 +701,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
             tmem_ld32(lanes + C::kO + d * 32, o);
             if (mine) {
 #pragma unroll
-              for (int y = 0; y < 32; y += 4) *reinterpret_cast<uint4*>(o_to + d * 32 + y) = make_uint4(o[y], o[y + 1], o[y + 2], o[y + 3]);
+              for (int y = 0; y < 32; y += 4) o_to[(size_t)(d * 8 + y / 4) * rows] = make_uint4(o[y], o[y + 1], o[y + 2], o[y + 3]);
             }
             __syncwarp();
           }
@@ -695,98 +716,85 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
   if (warp == kMmaWarp) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
 }
 
-// One CTA per (token row, query head): the pieces' results, the common keys' first, each in the order of the line.  Four quarters of the
-// pieces at a time, a thread four dims of each.
-constexpr int kMaxPieces = 512;   // of a row: two jobs, at most one piece a CTA
+// The pieces' results of a token row and KV head together: a CTA takes 64 dims of the group's heads, whose rows lie side by side in the
+// partial results; a thread 4 dims of one head, from every kSlices-th piece.  The common keys' pieces first, each kind in the order of the line.
+constexpr int kSlices = 4;
 template <int HD>
-__global__ void __launch_bounds__(HD) paged_merge_kernel(const PagedParams p, const Layout L, uint8_t* scratch) {
-  __shared__ float w_s[kMaxPieces];
-  __shared__ float red_s[HD / 32];
-  __shared__ __align__(16) float4 o_s[3][HD / 4];
+__global__ void __launch_bounds__(1024) paged_merge_kernel(const PagedParams p, const Layout L, uint8_t* scratch) {
+  __shared__ __align__(16) float4 o_s[kSlices - 1][16 * 16];
+  __shared__ float2 ml_s[kSlices][16];
   bk_pdl_trigger();
-  const int h = blockIdx.y, e = blockIdx.x, t = e / p.B, b = e - t * p.B, G = p.Hq / p.Hkv, kvh = h / G, g = h - kvh * G, tid = threadIdx.x;
+  const int G = p.Hq / p.Hkv, e = blockIdx.x, kvh = blockIdx.y / (HD / 64), d0 = blockIdx.y % (HD / 64) * 16, t = e / p.B, b = e - t * p.B;
+  const int g = threadIdx.x % G, d = threadIdx.x / G % 16, slice = threadIdx.x / (G * 16);
   const int rp = (b * p.T + t) * G + g, rs = t * G + g;
   const int jp = kvh * L.mt_p + rp / kRows, js = (b * p.Hkv + kvh) * L.mt_s + rs / kRows;   // within their kind
+  const uint16_t* gate = p.fused ? p.qg + ((size_t)e * p.Hq + kvh * G + g) * 2 * HD + HD : p.gate ? p.gate + ((size_t)e * p.Hq + kvh * G + g) * HD : nullptr;
   bk_pdl_wait();
   const int4* jobs = jobs_of(L, scratch);
-  const int2* pieces = pieces_of(L, scratch);
+  int4 qp = make_int4(0, 0, 0, -1), qs = __ldcg(jobs + L.n_p + js);
+  if (L.n_p) qp = __ldcg(jobs + jp);
   const bool here = row_of(p, b, t) >= 0;
-  const uint16_t* gate = p.fused ? p.qg + ((size_t)e * p.Hq + h) * 2 * HD + HD : p.gate ? p.gate + ((size_t)e * p.Hq + h) * HD : nullptr;
   uint2 gv = make_uint2(0, 0);
-  if (gate && tid < HD / 4) gv = *reinterpret_cast<const uint2*>(gate + tid * 4);
-  const int4 none = make_int4(0, 0, 0, -1);
-  const int4 qp = here && L.n_p ? __ldcg(jobs + jp) : none, qs = here ? __ldcg(jobs + L.n_p + js) : none;
-  const int np = qp.w - qp.z + 1, n = np + qs.w - qs.z + 1;
-  auto row_of_piece = [&](int i) {   // in the partial results of its kind
-    return i < np ? (size_t)(jp + qp.z + i) * kRows + rp % kRows : (size_t)(js + qs.z + i - np) * L.rows_s + rs % kRows;
-  };
-  // weights: w_i = 2^(m_i - M), and the sum of w_i l_i
-  float m[kMaxPieces / HD], l[kMaxPieces / HD], M = -INFINITY, sum = 0.0f;
+  if (gate && slice == 0) gv = *reinterpret_cast<const uint2*>(gate + (d0 + d) * 4);
+  const int np = here ? qp.w - qp.z + 1 : 0, n = here ? np + qs.w - qs.z + 1 : 0;
+  float m = -INFINITY, l = 0.0f;
+  float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  constexpr int U = 4;   // pieces requested together
+  for (int i0 = slice; i0 < n; i0 += kSlices * U) {
+    float4 v[U], x[U];
 #pragma unroll
-  for (int k = 0; k < kMaxPieces / HD; k++) {
-    const int i = tid + k * HD;
-    m[k] = -INFINITY;
-    l[k] = 0.0f;
-    if (i < n) {
-      const bool common = i < np;
-      const int4 q = common ? qp : qs;
-      const int cta = common ? qp.z + i : qs.z + i - np;
-      int t0, t1;
-      piece_of(q.x, tiles_of(L, common ? jp : L.n_p + js, q.y), __ldcg(&pieces[cta].x), __ldcg(&pieces[cta + 1].x), &t0, &t1);
-      if (t0 < t1) {
-        const float4 v = __ldcg(reinterpret_cast<const float4*>(scratch + (common ? L.ml_p : L.ml_s)) + row_of_piece(i));
-        m[k] = v.x;
-        l[k] = __fadd_rn(v.y, v.z);
+    for (int k = 0; k < U; k++) {
+      const int i = i0 + k * kSlices;
+      x[k] = make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
+      if (i < n) {
+        const bool common = i < np;
+        const size_t slot = common ? (size_t)(jp + qp.z + i) : (size_t)(js + qs.z + i - np);
+        const int rows = common ? kRows : L.rows_s, row = (common ? rp : rs) % kRows;
+        x[k] = __ldcg(reinterpret_cast<const float4*>(scratch + (common ? L.ml_p : L.ml_s)) + slot * rows + row);
+        v[k] = __ldcg(reinterpret_cast<const float4*>(scratch + (common ? L.o_p : L.o_s)) + (slot * (HD / 4) + d0 + d) * rows + row);
       }
     }
-    M = fmaxf(M, m[k]);
-  }
-  M = bk_warp_max(M);
-  if ((tid & 31) == 0) red_s[tid >> 5] = M;
-  __syncthreads();
+    float mn = m;
 #pragma unroll
-  for (int w = 0; w < HD / 32; w++) M = fmaxf(M, red_s[w]);
+    for (int k = 0; k < U; k++) mn = fmaxf(mn, x[k].x);
+    if (mn == -INFINITY) continue;
+    const float f = exp2_approx(__fsub_rn(m, mn));   // (m = -inf: 0)
+    l = __fmul_rn(l, f);
+    o.x = __fmul_rn(o.x, f); o.y = __fmul_rn(o.y, f); o.z = __fmul_rn(o.z, f); o.w = __fmul_rn(o.w, f);
+    m = mn;
 #pragma unroll
-  for (int k = 0; k < kMaxPieces / HD; k++) {
-    const int i = tid + k * HD;
-    const float w = m[k] == -INFINITY ? 0.0f : exp2_approx(__fsub_rn(m[k], M));
-    if (i < n) w_s[i] = w;
-    sum = fmaf(w, l[k], sum);
+    for (int k = 0; k < U; k++)
+      if (x[k].x != -INFINITY) {
+        const float w = exp2_approx(__fsub_rn(x[k].x, m));
+        l = fmaf(w, __fadd_rn(x[k].y, x[k].z), l);
+        o.x = fmaf(w, v[k].x, o.x); o.y = fmaf(w, v[k].y, o.y); o.z = fmaf(w, v[k].z, o.z); o.w = fmaf(w, v[k].w, o.w);
+      }
   }
-  sum = bk_warp_sum(sum);
-  __syncthreads();
-  if ((tid & 31) == 0) red_s[tid >> 5] = sum;
-  __syncthreads();
-  sum = 0.0f;
-#pragma unroll
-  for (int w = 0; w < HD / 32; w++) sum = __fadd_rn(sum, red_s[w]);
-
-  const int slice = tid / (HD / 4), col = tid % (HD / 4);
-  float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
-  for (int i = slice; i < n; i += 4) {
-    const float w = w_s[i];
-    if (w == 0.0f) continue;   // (nothing there, perhaps not even written)
-    const float4 v = __ldcg(reinterpret_cast<const float4*>(scratch + (i < np ? L.o_p : L.o_s)) + row_of_piece(i) * (HD / 4) + col);
-    o.x = fmaf(w, v.x, o.x); o.y = fmaf(w, v.y, o.y); o.z = fmaf(w, v.z, o.z); o.w = fmaf(w, v.w, o.w);
-  }
-  if (slice) o_s[slice - 1][col] = o;
+  if (slice) o_s[slice - 1][d * 16 + g] = o;
+  if (d == 0) ml_s[slice][g] = make_float2(m, l);
   __syncthreads();
   if (slice) return;
+  float M = -INFINITY;
 #pragma unroll
-  for (int k = 0; k < 3; k++) {
-    const float4 v = o_s[k][col];
-    o.x = __fadd_rn(o.x, v.x); o.y = __fadd_rn(o.y, v.y); o.z = __fadd_rn(o.z, v.z); o.w = __fadd_rn(o.w, v.w);
-  }
-  float y[4] = {o.x, o.y, o.z, o.w};
-  const uint32_t gw[2] = {gv.x, gv.y};
-  const bool any = M != -INFINITY;
+  for (int k = 0; k < kSlices; k++) M = fmaxf(M, ml_s[k][g].x);
+  float sum = 0.0f, y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  if (M != -INFINITY) {
 #pragma unroll
-  for (int i = 0; i < 4; i++) {
-    y[i] = any ? __fdiv_rn(y[i], sum) : 0.0f;
-    if (gate && any) y[i] = __fmul_rn(y[i], bk_sigmoidf(__uint_as_float(i & 1 ? gw[i >> 1] & 0xffff0000u : gw[i >> 1] << 16)));
+    for (int k = 0; k < kSlices; k++) {
+      const float2 x = ml_s[k][g];
+      const float w = exp2_approx(__fsub_rn(x.x, M));
+      const float4 v = k ? o_s[k - 1][d * 16 + g] : o;
+      sum = fmaf(w, x.y, sum);
+      y[0] = fmaf(w, v.x, y[0]); y[1] = fmaf(w, v.y, y[1]); y[2] = fmaf(w, v.z, y[2]); y[3] = fmaf(w, v.w, y[3]);
+    }
+    const uint32_t gw[2] = {gv.x, gv.y};
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      y[i] = __fdiv_rn(y[i], sum);
+      if (gate) y[i] = __fmul_rn(y[i], bk_sigmoidf(__uint_as_float(i & 1 ? gw[i >> 1] & 0xffff0000u : gw[i >> 1] << 16)));
+    }
   }
-  *reinterpret_cast<uint2*>(p.out + ((size_t)e * p.Hq + h) * HD + col * 4) = make_uint2(bk_f32x2_to_bf16x2(y[0], y[1]), bk_f32x2_to_bf16x2(y[2], y[3]));
+  *reinterpret_cast<uint2*>(p.out + ((size_t)e * p.Hq + kvh * G + g) * HD + (d0 + d) * 4) = make_uint2(bk_f32x2_to_bf16x2(y[0], y[1]), bk_f32x2_to_bf16x2(y[2], y[3]));
 }
 
 template <int HD>
@@ -801,7 +809,13 @@ int32_t launch_paged(const PagedParams& p, const Layout& L, uint64_t scratch) {
   if (!bk_encode_map_2d(&P.k_map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, (uint64_t)(uintptr_t)p.k_pages, HD, rows, HD * 2, 64, P.box_rows, CU_TENSOR_MAP_SWIZZLE_128B) ||
       !bk_encode_map_2d(&P.v_map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, (uint64_t)(uintptr_t)p.v_pages, HD, rows, HD * 2, 64, P.box_rows, CU_TENSOR_MAP_SWIZZLE_128B))
     return bk_fail(BK_ERR_UNSUPPORTED, "bkPagedAttn: the driver refuses a tensor map of %llu rows of %d values", (unsigned long long)rows, HD);
-  const int heads = (p.fused ? p.Hq : 0) + (p.k ? p.Hkv : 0);
+  const uint64_t q_rows = (uint64_t)p.B * p.T * p.Hq;
+  for (int common = 0; common < 2; common++) {   // whole groups of 8 rows; rows of another job are read and not used
+    P.q_rows[common] = std::min(kRows, ((common ? p.B : 1) * p.T * (p.Hq / p.Hkv) + 7) / 8 * 8);
+    if (!bk_encode_map_2d(&P.q_map[common], CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, scratch + L.q, HD, q_rows, HD * 2, 64, P.q_rows[common], CU_TENSOR_MAP_SWIZZLE_128B))
+      return bk_fail(BK_ERR_UNSUPPORTED, "bkPagedAttn: the driver refuses a tensor map of %llu rows of %d queries", (unsigned long long)q_rows, HD);
+  }
+  const int heads = p.Hq + (p.k ? p.Hkv : 0);
   BK_CUDA(bk_launch_pdl(paged_prepare_kernel<HD>, dim3((p.T * p.B * heads + 3) / 4 + 1), dim3(128), 0, p, L, P.scratch));
   BK_CHECK_LAUNCH();
   static bool configured = false;
@@ -811,7 +825,7 @@ int32_t launch_paged(const PagedParams& p, const Layout& L, uint64_t scratch) {
   }
   BK_CUDA(bk_launch_pdl(paged_tile_kernel<HD>, dim3(L.ctas), dim3(kTileThreads), TileCfg<HD>::kSmem, P));
   BK_CHECK_LAUNCH();
-  BK_CUDA(bk_launch_pdl(paged_merge_kernel<HD>, dim3(p.T * p.B, p.Hq), dim3(HD), 0, p, L, P.scratch));
+  BK_CUDA(bk_launch_pdl(paged_merge_kernel<HD>, dim3(p.T * p.B, p.Hkv * (HD / 64)), dim3(p.Hq / p.Hkv * 16 * kSlices), 0, p, L, P.scratch));
   BK_CHECK_LAUNCH();
   return BK_OK;
 }
@@ -854,11 +868,11 @@ int32_t bkPagedAttn(const bkPagedAttnArgs* args) {
   p.q_norm_w = bk_ptr<uint16_t>(a.q_norm_w); p.k_norm_w = bk_ptr<uint16_t>(a.k_norm_w); p.cos_t = bk_ptr<float>(a.cos_t); p.sin_t = bk_ptr<float>(a.sin_t);
   p.k_pages = bk_ptr<uint16_t>(a.k_pages); p.v_pages = bk_ptr<uint16_t>(a.v_pages);
   p.table = bk_ptr<int>(a.table); p.lens = bk_ptr<int>(a.lens); p.n_new = bk_ptr<int>(a.n_new); p.out = bk_ptr<uint16_t>(a.out);
-  p.q = a.fused_norm_rope ? bk_ptr<uint16_t>(a.scratch) : bk_ptr<uint16_t>(a.qg);
+  p.q = bk_ptr<uint16_t>(a.scratch);
   p.B = a.B; p.T = a.T; p.Hq = a.Hq; p.Hkv = a.Hkv; p.rot_half = a.rot_half; p.n_pages = a.n_pages; p.page_rows = a.page_rows; p.max_pages = a.max_pages;
   p.max_rows = (int)std::min<long long>(a.max_len, (long long)a.max_pages * a.page_rows); p.fused = a.fused_norm_rope != 0; p.scale = a.scale; p.eps = a.eps;
   const Layout L = make_layout(a.B, a.T, a.Hq, a.Hkv, a.HD, a.prefix_rows, a.page_rows, bk_ctx().sm_count);
-  BK_ARG((long long)(L.n_p + L.n_s) * ((long long)p.max_rows / kTile + 1 + kOverhead) < (1ll << 31) && 2 * L.ctas <= kMaxPieces, "bkPagedAttn: B=%d T=%d Hkv=%d with %d rows a sequence: too much for one call", a.B,
+  BK_ARG((long long)(L.n_p + L.n_s) * ((long long)p.max_rows / kTile + 1 + kOverhead) < (1ll << 31), "bkPagedAttn: B=%d T=%d Hkv=%d with %d rows a sequence: too much for one call", a.B,
          a.T, a.Hkv, p.max_rows);
   return a.HD == 256 ? launch_paged<256>(p, L, a.scratch) : launch_paged<128>(p, L, a.scratch);
 }
