@@ -141,67 +141,79 @@ BK_DEVINL void piece_of(int s, int n, int u0, int u1, int* t0, int* t1) {
   *t1 = max(0, min(n, u1 - s - kOverhead));
 }
 
-// one CTA of 128 threads
+// one CTA
+constexpr int kPrepThreads = 256, kPlanned = 1024;   // jobs whose starts fit in shared memory
 BK_DEVINL void plan_jobs(const PagedParams& p, const Layout& L, uint8_t* scratch) {
-  __shared__ int warp_s[4][2];
+  __shared__ int warp_s[kPrepThreads / 32][2], starts_s[kPlanned + 1], bounds_s[kPrepThreads + 1];
   int4* jobs = jobs_of(L, scratch);
   int4* pieces = pieces_of(L, scratch);
   const int n = L.n_p + L.n_s, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int base = 0, tiles_all = 0;
-  for (int j0 = 0; j0 < n; j0 += 128) {
-    const int j = j0 + (int)threadIdx.x;
-    int tiles = 0, end = 0;
-    if (j < n) {
-      end = keys_end(p, L, job_of(p, L, j));
-      tiles = tiles_of(L, j, end);
-    }
-    const int units = tiles ? tiles + kOverhead : 0;
-    int v = units;
-#pragma unroll
-    for (int off = 1; off < 32; off <<= 1) {
-      const int o = __shfl_up_sync(0xffffffffu, v, off);
-      if (lane >= off) v += o;
-    }
-    const int sum = __reduce_add_sync(0xffffffffu, tiles);
-    if (lane == 31) {
-      warp_s[warp][0] = v;
-      warp_s[warp][1] = sum;
-    }
-    __syncthreads();
-    int before = base;
-    for (int w = 0; w < 4; w++) {
-      if (w < warp) before += warp_s[w][0];
-      base += warp_s[w][0];
-      tiles_all += warp_s[w][1];
-    }
-    if (j < n) jobs[j] = make_int4(before + v - units, end, 0, 0);
-    __syncthreads();
+  const bool in_smem = n <= kPlanned;
+  // a thread has `per` jobs in a row
+  const int per = (n + kPrepThreads - 1) / kPrepThreads, j0 = threadIdx.x * per, j1 = min(n, j0 + per);
+  int mine = 0, tiles_mine = 0;
+  for (int j = j0; j < j1; j++) {
+    const int end = keys_end(p, L, job_of(p, L, j)), tiles = tiles_of(L, j, end);
+    jobs[j] = make_int4(mine, end, 0, -1);   // .x: within the thread, for now
+    mine += tiles ? tiles + kOverhead : 0;
+    tiles_mine += tiles;
   }
-  if (threadIdx.x == 0) jobs[n] = make_int4(base, 0, 0, 0);
-  __syncthreads();   // jobs[].x is there for all
-  const int C = max(1, min(L.ctas, tiles_all)), units = base;   // every CTA has a tile to do
-  auto bound = [&](int c) { return (int)((long long)units * c / C); };
-  for (int c = threadIdx.x; c < L.ctas; c += 128) {
-    const int u0 = c < C ? bound(c) : 0, u1 = c < C ? bound(c + 1) : 0;
+  int v = mine;
+#pragma unroll
+  for (int off = 1; off < 32; off <<= 1) {
+    const int o = __shfl_up_sync(0xffffffffu, v, off);
+    if (lane >= off) v += o;
+  }
+  const int sum = __reduce_add_sync(0xffffffffu, tiles_mine);
+  if (lane == 31) {
+    warp_s[warp][0] = v;
+    warp_s[warp][1] = sum;
+  }
+  __syncthreads();
+  int before = v - mine, units = 0, tiles_all = 0;
+#pragma unroll
+  for (int w = 0; w < kPrepThreads / 32; w++) {
+    if (w < warp) before += warp_s[w][0];
+    units += warp_s[w][0];
+    tiles_all += warp_s[w][1];
+  }
+  for (int j = j0; j < j1; j++) {
+    const int s = jobs[j].x + before;
+    jobs[j].x = s;
+    if (in_smem) starts_s[j] = s;
+  }
+  if (threadIdx.x == 0) {
+    jobs[n] = make_int4(units, 0, 0, -1);
+    if (in_smem) starts_s[n] = units;
+  }
+  const int C = max(1, min(min(L.ctas, kPrepThreads), tiles_all));   // every CTA has a tile to do
+  // (a quotient that is no whole number is at least 1 / C away from one, so the double below it is too)
+  for (int c = threadIdx.x; c <= C; c += kPrepThreads) bounds_s[c] = (int)((double)units * c / C);
+  __syncthreads();
+  auto start = [&](int j) { return in_smem ? starts_s[j] : jobs[j].x; };
+  for (int c = threadIdx.x; c < L.ctas; c += kPrepThreads) {
+    const int u0 = c < C ? bounds_s[c] : 0, u1 = c < C ? bounds_s[c + 1] : 0;
     int lo = 0, hi = n;   // the last job that starts at u0 or before
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
-      if (jobs[mid].x <= u0) lo = mid;
+      if (start(mid) <= u0) lo = mid;
       else hi = mid;
     }
     pieces[2 * c] = make_int4(u0, u1, lo, 0);
     pieces[2 * c + 1] = jobs[lo];
   }
-  for (int j = threadIdx.x; j < n; j += 128) {
-    const int s = jobs[j].x, s1 = jobs[j + 1].x;
-    auto cta_at = [&](int x) { return (int)((((long long)x + 1) * C - 1) / units); };   // the CTA that has unit x
-    if (s1 > s) {
-      jobs[j].z = cta_at(s + kOverhead);
-      jobs[j].w = cta_at(s1 - 1);
-    } else {
-      jobs[j].z = 0;
-      jobs[j].w = -1;
+  auto cta_at = [&](int unit) {   // the CTA that has it
+    int lo = 0, hi = C;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (bounds_s[mid] <= unit) lo = mid;
+      else hi = mid;
     }
+    return lo;
+  };
+  for (int j = threadIdx.x; j < n; j += kPrepThreads) {
+    const int s = start(j), s1 = start(j + 1);
+    if (s1 > s) *reinterpret_cast<int2*>(&jobs[j].z) = make_int2(cta_at(s + kOverhead), cta_at(s1 - 1));
   }
 }
 
@@ -221,20 +233,20 @@ BK_DEVINL bool row_at(const PagedParams& p, const Job& q, int i, int* b, int* t,
   return r < p.B * p.T * G;
 }
 
-// One warp per (token row, head): q heads to the scratch buffer, k and v heads into their page.  The last CTA lays out the work of the next launch.
+// One warp per (token row, head): q heads to the scratch buffer, k and v heads into their page.  The first CTA lays out the work of the next launch.
 template <int HD>
-__global__ void __launch_bounds__(128) paged_prepare_kernel(const PagedParams p, const Layout L, uint8_t* scratch) {
+__global__ void __launch_bounds__(kPrepThreads) paged_prepare_kernel(const PagedParams p, const Layout L, uint8_t* scratch) {
   constexpr int PER = HD / 32;
-  __shared__ float y_s[4][HD];
+  __shared__ float y_s[kPrepThreads / 32][HD];
   bk_pdl_trigger();
   bk_pdl_wait();
-  if (blockIdx.x == gridDim.x - 1) {
+  if (blockIdx.x == 0) {   // (first: it takes longest)
     plan_jobs(p, L, scratch);
     return;
   }
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int heads = p.Hq + (p.k ? p.Hkv : 0);
-  const int item = blockIdx.x * 4 + warp;
+  const int item = (blockIdx.x - 1) * (kPrepThreads / 32) + warp;
   if (item >= p.T * p.B * heads) return;
   const int e = item / heads, h = item - e * heads, t = e / p.B, b = e - t * p.B;
   const int at = row_of(p, b, t);
@@ -497,54 +509,60 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
       }
     } else if (warp == kMmaWarp) {
       // ================= MMAs =================
+      // Scores of tile i, then the output of tile i - 1.  What the second half of a batch does not need is waited for ahead of it, while the
+      // first half runs: a wait takes 100 cycles or more even where there is nothing to wait for, and four of them a step with the tensor
+      // cores idle made it 2,200 cycles instead of 1,7xx.
       constexpr uint32_t kShapeS = mma_shape(kTile, false), kShapeO = mma_shape(HD, true);
-      int stage = 0, tile = 0, pieces = 0;   // tile: counted over all pieces
-      uint32_t parity = 0;
-      auto next_stage = [&]() {
-        if (++stage == C::kStages) {
-          stage = 0;
-          parity ^= 1u;
-        }
-      };
+      int tile = 0, pieces = 0, pos = 0;   // tile, pos: counted over all pieces, pos in the stream
+      auto stage_at = [&](int at) { return smem_u32(ring + (size_t)(at % C::kStages) * C::kStage); };
+      auto wait_full = [&](int at) { bar_wait_warp(smem_u32(full + at % C::kStages), (at / C::kStages) & 1, P.status, dead); };
       for (; next_piece(&x); j++) {
-        const int t0 = x.t0, t1 = x.t1;
+        const int n = x.t1 - x.t0;
+        wait_full(pos);
         bar_wait_warp(smem_u32(&q_full), pieces & 1, P.status, dead);
         tc_after();
-        for (int i = t0; i <= t1; i++) {
-          if (i < t1) {   // scores of tile i; the probabilities that this buffer held have been multiplied: MMAs run in order
-            bar_wait_warp(smem_u32(full + stage), parity, P.status, dead);
-            const uint32_t k_at = smem_u32(ring + (size_t)stage * C::kStage);
+        for (int i = 0; i <= n; i++) {
+          const int k_pos = pos + (i ? 2 * i - 1 : 0), v_pos = i ? pos + stream_v(i - 1, n) : 0, prev = tile + i - 1;
+          auto scores = [&](int half) {   // (the probabilities that this buffer held have been multiplied: MMAs run in order)
+            const uint32_t k_at = stage_at(k_pos), d = tmem + C::kS + ((tile + i) & 1) * kTile;
             if (elect_lane()) {
 #pragma unroll
-              for (int ks = 0; ks < HD / 16; ks++)
-                tc_mma(tmem + C::kS + (tile & 1) * kTile, tmem + C::kQ + ks * 8, smem_desc(k_at + (ks >> 2) * (kTile * 128) + (ks & 3) * 32, 16, 1024), kShapeS, ks > 0);
-              tc_commit(smem_u32(empty + stage));
-              tc_commit(smem_u32(s_full + (tile & 1)));
+              for (int y = 0; y < HD / 32; y++) {
+                const int ks = half * (HD / 32) + y;
+                tc_mma(d, tmem + C::kQ + ks * 8, smem_desc(k_at + (ks >> 2) * (kTile * 128) + (ks & 3) * 32, 16, 1024), kShapeS, ks > 0);
+              }
+              if (half) {
+                tc_commit(smem_u32(empty + k_pos % C::kStages));
+                tc_commit(smem_u32(s_full + ((tile + i) & 1)));
+              }
             }
             __syncwarp();
-            next_stage();
-            tile++;
-          }
-          if (i > t0) {   // output of tile i - 1
-            const int prev = i < t1 ? tile - 2 : tile - 1;
+          };
+          auto output = [&](int half) {   // the rounded probabilities, then what rounding left
+            const uint32_t v_at = stage_at(v_pos), p_at = tmem + C::kS + (prev & 1) * kTile + half * 32;
+            if (elect_lane()) {
+#pragma unroll
+              for (int ks = 0; ks < kTile / 16; ks++) tc_mma(tmem + C::kO, p_at + ks * 8, smem_desc(v_at + ks * 2048, kTile * 128, 1024), kShapeO, i > 1 || half > 0 || ks > 0);
+              if (half) {
+                tc_commit(smem_u32(empty + v_pos % C::kStages));
+                tc_commit(smem_u32(o_full + (prev & 1)));
+              }
+            }
+            __syncwarp();
+          };
+          if (i < n) scores(0);
+          if (i > 0) {
             bar_wait_warp(smem_u32(p_full + (prev & 1)), (prev >> 1) & 1, P.status, dead);
-            bar_wait_warp(smem_u32(full + stage), parity, P.status, dead);
+            wait_full(v_pos);
             tc_after();
-            const uint32_t v_at = smem_u32(ring + (size_t)stage * C::kStage);
-            if (elect_lane()) {
-#pragma unroll
-              for (int half = 0; half < 2; half++)
-#pragma unroll
-                for (int ks = 0; ks < kTile / 16; ks++)
-                  tc_mma(tmem + C::kO, tmem + C::kS + (prev & 1) * kTile + half * 32 + ks * 8, smem_desc(v_at + ks * 2048, kTile * 128, 1024), kShapeO,
-                         i - 1 > t0 || half > 0 || ks > 0);
-              tc_commit(smem_u32(empty + stage));
-              tc_commit(smem_u32(o_full + (prev & 1)));
-            }
-            __syncwarp();
-            next_stage();
           }
+          if (i < n) scores(1);
+          if (i > 0) output(0);
+          if (i + 1 < n) wait_full(pos + 2 * i + 1);
+          if (i > 0) output(1);
         }
+        tile += n;
+        pos += 2 * n;
         pieces++;
       }
     } else if (warp == kQueryWarp) {
@@ -718,10 +736,11 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
 
 // The pieces' results of a token row and KV head together: a CTA takes 64 dims of the group's heads, whose rows lie side by side in the
 // partial results; a thread 4 dims of one head, from every kSlices-th piece.  The common keys' pieces first, each kind in the order of the line.
-constexpr int kSlices = 4;
-template <int HD>
-__global__ void __launch_bounds__(1024) paged_merge_kernel(const PagedParams p, const Layout L, uint8_t* scratch) {
-  __shared__ __align__(16) float4 o_s[kSlices - 1][16 * 16];
+// Bound: latency, of a chain of loads.  Few CTAs have many pieces to a row, which four slices take together; many CTAs hide one another's
+// latency better when they are small.
+template <int HD, int kSlices>
+__global__ void __launch_bounds__(256 * kSlices) paged_merge_kernel(const PagedParams p, const Layout L, uint8_t* scratch) {
+  __shared__ __align__(16) float4 o_s[kSlices > 1 ? kSlices - 1 : 1][16 * 16];
   __shared__ float2 ml_s[kSlices][16];
   bk_pdl_trigger();
   const int G = p.Hq / p.Hkv, e = blockIdx.x, kvh = blockIdx.y / (HD / 64), d0 = blockIdx.y % (HD / 64) * 16, t = e / p.B, b = e - t * p.B;
@@ -739,7 +758,7 @@ __global__ void __launch_bounds__(1024) paged_merge_kernel(const PagedParams p, 
   const int np = here ? qp.w - qp.z + 1 : 0, n = here ? np + qs.w - qs.z + 1 : 0;
   float m = -INFINITY, l = 0.0f;
   float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  constexpr int U = 4;   // pieces requested together
+  constexpr int U = kSlices == 1 ? 6 : 4;   // pieces requested together
   for (int i0 = slice; i0 < n; i0 += kSlices * U) {
     float4 v[U], x[U];
 #pragma unroll
@@ -816,7 +835,7 @@ int32_t launch_paged(const PagedParams& p, const Layout& L, uint64_t scratch) {
       return bk_fail(BK_ERR_UNSUPPORTED, "bkPagedAttn: the driver refuses a tensor map of %llu rows of %d queries", (unsigned long long)q_rows, HD);
   }
   const int heads = p.Hq + (p.k ? p.Hkv : 0);
-  BK_CUDA(bk_launch_pdl(paged_prepare_kernel<HD>, dim3((p.T * p.B * heads + 3) / 4 + 1), dim3(128), 0, p, L, P.scratch));
+  BK_CUDA(bk_launch_pdl(paged_prepare_kernel<HD>, dim3((p.T * p.B * heads + kPrepThreads / 32 - 1) / (kPrepThreads / 32) + 1), dim3(kPrepThreads), 0, p, L, P.scratch));
   BK_CHECK_LAUNCH();
   static bool configured = false;
   if (!configured) {
@@ -825,7 +844,9 @@ int32_t launch_paged(const PagedParams& p, const Layout& L, uint64_t scratch) {
   }
   BK_CUDA(bk_launch_pdl(paged_tile_kernel<HD>, dim3(L.ctas), dim3(kTileThreads), TileCfg<HD>::kSmem, P));
   BK_CHECK_LAUNCH();
-  BK_CUDA(bk_launch_pdl(paged_merge_kernel<HD>, dim3(p.T * p.B, p.Hkv * (HD / 64)), dim3(p.Hq / p.Hkv * 16 * kSlices), 0, p, L, P.scratch));
+  const dim3 merge(p.T * p.B, p.Hkv * (HD / 64));
+  if ((long long)merge.x * merge.y <= 2 * bk_ctx().sm_count) BK_CUDA(bk_launch_pdl(paged_merge_kernel<HD, 4>, merge, dim3(p.Hq / p.Hkv * 64), 0, p, L, P.scratch));
+  else BK_CUDA(bk_launch_pdl(paged_merge_kernel<HD, 1>, merge, dim3(p.Hq / p.Hkv * 16), 0, p, L, P.scratch));
   BK_CHECK_LAUNCH();
   return BK_OK;
 }
