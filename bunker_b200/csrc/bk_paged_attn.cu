@@ -41,9 +41,11 @@ BK_DEVINL void load_bf16(const uint16_t* src, float (&y)[PER]) {
 
 // ---- who does what -----------------------------------------------------------------
 // A job is a tile of up to 128 rows (token, query head) of one KV head and the keys they attend to: the common keys [0, P) once for the
-// rows of all sequences, then for each sequence its own keys [P, end).  The work, in tiles of 64 keys and kOverhead more for each job, is
-// laid out in one line and cut into equal pieces, one per CTA, so that a long prefix and many short sequences keep every SM busy until the
-// end.  The line is made on the device (lengths are there), by one CTA of the first launch.
+// rows of all sequences, then for each sequence its own keys [P, end).  The jobs, in tiles of 64 keys and kOverhead more for each job, are laid
+// out in one line and cut into equal pieces, one per CTA, so that a long prefix and many short sequences keep every SM busy until the end.  The
+// line is made on the device (lengths are there), by one CTA of the first launch.  (With the same cuts for all row tiles of a KV head, which then read
+// the same keys at the same time, and the line for the rest, most CTAs have two pieces: 32 sequences behind 8,192 rows 30.5 -> 36.2 us, 64
+// behind 32,768 rows 105.2 -> 102.2.)
 constexpr int kTile = 64;       // keys of a step
 constexpr int kRows = 128;      // rows of a job: the lanes of tensor memory
 constexpr int kOverhead = 2;    // what a job's start and end cost, in steps
@@ -130,8 +132,8 @@ BK_DEVINL int keys_end(const PagedParams& p, const Layout& L, const Job& q) {
   return L.P;
 }
 
-// What the first launch leaves for the others.  jobs[j] = {start on the line, end of the keys, first and last CTA that have a piece of it};
-// pieces[2c] = {start and end of CTA c's piece of the line, first job in it, -}, pieces[2c + 1] = that job.
+// What the first launch leaves for the others.  jobs[j] = {start on the line, end of the keys, slot of its first partial result, their number};
+// pieces[2c] = {start and end of CTA c's piece of the line, first job in it, -}, pieces[2c + 1] = that job's .x and .y.
 BK_DEVINL int4* jobs_of(const Layout& L, uint8_t* scratch) { return reinterpret_cast<int4*>(scratch + L.jobs); }
 BK_DEVINL int4* pieces_of(const Layout& L, uint8_t* scratch) { return reinterpret_cast<int4*>(scratch + L.pieces); }
 BK_DEVINL int tiles_of(const Layout& L, int j, int key1) { return (key1 - (j < L.n_p ? 0 : L.P) + kTile - 1) / kTile; }
@@ -154,7 +156,7 @@ BK_DEVINL void plan_jobs(const PagedParams& p, const Layout& L, uint8_t* scratch
   int mine = 0, tiles_mine = 0;
   for (int j = j0; j < j1; j++) {
     const int end = keys_end(p, L, job_of(p, L, j)), tiles = tiles_of(L, j, end);
-    jobs[j] = make_int4(mine, end, 0, -1);   // .x: within the thread, for now
+    *reinterpret_cast<int2*>(jobs + j) = make_int2(mine, end);   // .x: within the thread, for now
     mine += tiles ? tiles + kOverhead : 0;
     tiles_mine += tiles;
   }
@@ -183,7 +185,7 @@ BK_DEVINL void plan_jobs(const PagedParams& p, const Layout& L, uint8_t* scratch
     if (in_smem) starts_s[j] = s;
   }
   if (threadIdx.x == 0) {
-    jobs[n] = make_int4(units, 0, 0, -1);
+    jobs[n].x = units;
     if (in_smem) starts_s[n] = units;
   }
   const int C = max(1, min(min(L.ctas, kPrepThreads), tiles_all));   // every CTA has a tile to do
@@ -200,7 +202,7 @@ BK_DEVINL void plan_jobs(const PagedParams& p, const Layout& L, uint8_t* scratch
       else hi = mid;
     }
     pieces[2 * c] = make_int4(u0, u1, lo, 0);
-    pieces[2 * c + 1] = jobs[lo];
+    pieces[2 * c + 1] = make_int4(start(lo), jobs[lo].y, 0, 0);
   }
   auto cta_at = [&](int unit) {   // the CTA that has it
     int lo = 0, hi = C;
@@ -212,8 +214,8 @@ BK_DEVINL void plan_jobs(const PagedParams& p, const Layout& L, uint8_t* scratch
     return lo;
   };
   for (int j = threadIdx.x; j < n; j += kPrepThreads) {
-    const int s = start(j), s1 = start(j + 1);
-    if (s1 > s) *reinterpret_cast<int2*>(&jobs[j].z) = make_int2(cta_at(s + kOverhead), cta_at(s1 - 1));
+    const int s = start(j), s1 = start(j + 1), first = cta_at(s + kOverhead);
+    *reinterpret_cast<int2*>(&jobs[j].z) = s1 > s ? make_int2((j < L.n_p ? j : j - L.n_p) + first, cta_at(s1 - 1) - first + 1) : make_int2(0, 0);
   }
 }
 
@@ -295,21 +297,12 @@ __global__ void __launch_bounds__(kPrepThreads) paged_prepare_kernel(const Paged
     F(v[o + 23]), F(v[o + 24]), F(v[o + 25]), F(v[o + 26]), F(v[o + 27]), F(v[o + 28]), F(v[o + 29]), F(v[o + 30]), F(v[o + 31])
 #define BK_OUT(x) "=r"(x)
 #define BK_IN(x) "r"(x)
-// 32 or 64 columns of the calling lane's row.  The wait is part of it, so that no use of a register can come before.
+// 32 or 16 columns of the calling lane's row.  The wait is part of it, so that no use of a register can come before.
 BK_DEVINL void tmem_ld32(uint32_t at, uint32_t* v) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, "
       "%23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n\ttcgen05.wait::ld.sync.aligned;"
       : BK_R32(BK_OUT, v, 0)
-      : "r"(at)
-      : "memory");
-}
-BK_DEVINL void tmem_ld64(uint32_t at, uint32_t* v) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x64.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, "
-      "%23, %24, %25, %26, %27, %28, %29, %30, %31, %32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, %48, %49, %50, %51, %52, "
-      "%53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63}, [%64];\n\ttcgen05.wait::ld.sync.aligned;"
-      : BK_R32(BK_OUT, v, 0), BK_R32(BK_OUT, v, 32)
       : "r"(at)
       : "memory");
 }
@@ -320,6 +313,11 @@ BK_DEVINL void tmem_st32(uint32_t at, const uint32_t* v) {
       BK_R32(BK_IN, v, 0)
       : "memory");
 }
+BK_DEVINL void tmem_st16(uint32_t at, const uint32_t* v) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(at), "r"(v[0]), "r"(v[1]), "r"(v[2]),
+               "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+               : "memory");
+}
 BK_DEVINL void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 BK_DEVINL void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 BK_DEVINL void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -327,9 +325,10 @@ BK_DEVINL void tc_commit(uint32_t bar) {   // arrives when every MMA issued so f
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
 // D (+)= A * B, M = 128, K = 16; A in tensor memory
-BK_DEVINL void tc_mma(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool acc) {
+template <bool ACC>
+BK_DEVINL void tc_mma(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc) {
   asm volatile("{\n\t.reg .pred pz;\n\tsetp.ne.b32 pz, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, pz;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc),
-               "r"(acc ? 1u : 0u)
+               "n"(ACC ? 1 : 0)
                : "memory");
 }
 // Operand B in shared memory, rows of 128 bytes swizzled in groups of 8 (1,024 bytes).  K-major (keys): group_stride between groups of 8 keys.
@@ -362,6 +361,11 @@ BK_DEVINL void tma_load(uint32_t dst, const CUtensorMap* map, int x, int y, uint
   asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar)
                : "memory");
 }
+BK_DEVINL float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
 BK_DEVINL float exp2_approx(float x) {   // 2^x to 2 ulp or so; 2^-inf = 0
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -371,15 +375,22 @@ BK_DEVINL float exp2_approx(float x) {   // 2^x to 2 ulp or so; 2^-inf = 0
 // positions in the stream of a piece's tiles: K0, K1, V0, K2, V1, ..., V(n-1)
 BK_DEVINL int stream_v(int i, int n) { return i < n - 1 ? 2 * i + 2 : 2 * n - 1; }
 
+template <int kStages>
+struct TileShared {   // behind the tiles
+  uint64_t full[kStages], empty[kStages], q_here, q_empty, q_full, s_full[2], p_full[2], o_full[2];
+  float m_s[2][2][kRows];   // [tile & 1][half of the keys]: largest score
+  uint32_t tmem_slot;
+  int dead;
+};
 template <int HD>
 struct TileCfg {
   static constexpr int kStage = kTile * HD * 2;               // bytes of 64 keys or values
   static constexpr int kStages = HD == 256 ? 5 : 12;
   static constexpr int kQuery = kRows * HD * 2;               // bytes of the queries
-  static constexpr int kSmem = kQuery + kStages * kStage + 1024;
+  static constexpr int kSmem = kQuery + kStages * kStage + (int)sizeof(TileShared<kStages>);
   static constexpr int kO = 0, kQ = HD, kS = HD + HD / 2;     // tensor memory: output, queries, two buffers of scores (then probabilities)
 };
-constexpr int kCopyWarp = 8, kMmaWarp = 9, kQueryWarp = 10, kTileThreads = 352;   // warps 0-3 and 4-7: a row each lane, even and odd tiles
+constexpr int kCopyWarp = 8, kMmaWarp = 9, kQueryWarp = 10, kTileThreads = 352;   // warps 0-3 and 4-7: a row each lane, halves of a tile's keys
 
 // S = Q K^T and O += P V on the tensor cores.  Q, S, P and O live in tensor memory, a row per lane (with Q in shared memory its reads, 64 KB a step,
 // make a step 500 cycles longer: K, V twice and what TMA writes take three quarters of that bandwidth); a ring of K and V tiles of 64 rows in shared
@@ -391,13 +402,14 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
   using C = TileCfg<HD>;
   const PagedParams& p = P.g;
   const Layout& L = P.L;
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* q_s = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);   // [HD / 64][kRows][64]
-  uint8_t* ring = q_s + C::kQuery;                                                                                // stages [HD / 64][kTile][64]
-  __shared__ __align__(8) uint64_t full[C::kStages], empty[C::kStages], q_here, q_empty, q_full, s_full[2], p_full[2], o_full[2], m_full[2][4];
-  __shared__ float m_s[2][kRows];
-  __shared__ uint32_t tmem_slot;
-  __shared__ int dead_s;
+  extern __shared__ __align__(1024) uint8_t q_s[];   // queries [HD / 64][kRows][64], then the ring: stages [HD / 64][kTile][64]
+  uint8_t* ring = q_s + C::kQuery;
+  TileShared<C::kStages>& sh = *reinterpret_cast<TileShared<C::kStages>*>(ring + C::kStages * C::kStage);
+  uint64_t *full = sh.full, *empty = sh.empty, *s_full = sh.s_full, *p_full = sh.p_full, *o_full = sh.o_full;
+  uint64_t &q_here = sh.q_here, &q_empty = sh.q_empty, &q_full = sh.q_full;
+  auto& m_s = sh.m_s;
+  uint32_t& tmem_slot = sh.tmem_slot;
+  int& dead_s = sh.dead;
   volatile int* dead = &dead_s;
   bk_pdl_trigger();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -412,9 +424,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
     mbar_init(smem_u32(&q_full), 8);
     for (int i = 0; i < 2; i++) {
       mbar_init(smem_u32(s_full + i), 1);
-      mbar_init(smem_u32(p_full + i), 128);
+      mbar_init(smem_u32(p_full + i), 8);
       mbar_init(smem_u32(o_full + i), 1);
-      for (int w = 0; w < 4; w++) mbar_init(smem_u32(&m_full[i][w]), 1);
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -433,29 +444,32 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
 
   const int4* jobs = jobs_of(L, P.scratch);
   const int cta = blockIdx.x, n_jobs = L.n_p + L.n_s;
-  const int4 line = __ldcg(pieces_of(L, P.scratch) + 2 * cta), first_job = __ldcg(pieces_of(L, P.scratch) + 2 * cta + 1);
+  const int4 line = __ldcg(pieces_of(L, P.scratch) + 2 * cta), first = __ldcg(pieces_of(L, P.scratch) + 2 * cta + 1);
   const int u0 = line.x, u1 = line.y;
-  int j = line.z;
-  // the next piece of a job, from job j on
+  int j = line.z - 1;
+  // the next piece of a job, from job j + 1 on
   struct Piece {
     Job q;
     int key1, t0, t1;
+    size_t slot;   // of its partial result, among its kind's
   };
   auto next_piece = [&](Piece* x) {
-    for (; j < n_jobs; j++) {
-      const int4 job = j == line.z ? first_job : __ldcg(jobs + j);
+    while (++j < n_jobs) {
+      int2 job = make_int2(first.x, first.y);   // start, end of the keys
+      if (j != line.z) job = __ldcg(reinterpret_cast<const int2*>(jobs + j));
       if (job.x >= u1) return false;
       piece_of(job.x, tiles_of(L, j, job.y), u0, u1, &x->t0, &x->t1);
       if (x->t0 >= x->t1) continue;
       x->q = job_of(p, L, j);
       x->key1 = job.y;
+      x->slot = (j < L.n_p ? j : j - L.n_p) + cta;
       return true;
     }
     return false;
   };
   Piece x;
 
-  if (u1 > u0) {
+  {
     if (warp == kCopyWarp) {
       // ================= copies: lane (chunk, block) takes box_rows rows x 64 dims =================
       asm volatile("fence.proxy.async;" ::: "memory");   // rows that an earlier kernel stored
@@ -466,7 +480,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
       const uint32_t box_at = block * (kTile * 128) + chunk * P.box_rows * 128;
       int stage = 0;
       uint32_t parity = 1;
-      for (; next_piece(&x); j++) {
+      while (next_piece(&x)) {
         const Job q = x.q;
         const int t0 = x.t0, t1 = x.t1, key1 = x.key1;
         const int* table = p.table + (size_t)max(q.seq, 0) * p.max_pages;
@@ -510,66 +524,90 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
     } else if (warp == kMmaWarp) {
       // ================= MMAs =================
       // Scores of tile i, then the output of tile i - 1.  What the second half of a batch does not need is waited for ahead of it, while the
-      // first half runs: a wait takes 100 cycles or more even where there is nothing to wait for, and four of them a step with the tensor
-      // cores idle made it 2,200 cycles instead of 1,7xx.
+      // first half runs.  Bound: the MMAs (1,600 cycles a step: 16 of 128 x 64 and 8 of 128 x 256) and, while little is queued, what this warp does
+      // between them, so addresses are counted up, not made from positions.
       constexpr uint32_t kShapeS = mma_shape(kTile, false), kShapeO = mma_shape(HD, true);
-      int tile = 0, pieces = 0, pos = 0;   // tile, pos: counted over all pieces, pos in the stream
-      auto stage_at = [&](int at) { return smem_u32(ring + (size_t)(at % C::kStages) * C::kStage); };
-      auto wait_full = [&](int at) { bar_wait_warp(smem_u32(full + at % C::kStages), (at / C::kStages) & 1, P.status, dead); };
-      for (; next_piece(&x); j++) {
-        const int n = x.t1 - x.t0;
-        wait_full(pos);
-        bar_wait_warp(smem_u32(&q_full), pieces & 1, P.status, dead);
-        tc_after();
-        for (int i = 0; i <= n; i++) {
-          const int k_pos = pos + (i ? 2 * i - 1 : 0), v_pos = i ? pos + stream_v(i - 1, n) : 0, prev = tile + i - 1;
-          auto scores = [&](int half) {   // (the probabilities that this buffer held have been multiplied: MMAs run in order)
-            const uint32_t k_at = stage_at(k_pos), d = tmem + C::kS + ((tile + i) & 1) * kTile;
-            if (elect_lane()) {
-#pragma unroll
-              for (int y = 0; y < HD / 32; y++) {
-                const int ks = half * (HD / 32) + y;
-                tc_mma(d, tmem + C::kQ + ks * 8, smem_desc(k_at + (ks >> 2) * (kTile * 128) + (ks & 3) * 32, 16, 1024), kShapeS, ks > 0);
-              }
-              if (half) {
-                tc_commit(smem_u32(empty + k_pos % C::kStages));
-                tc_commit(smem_u32(s_full + ((tile + i) & 1)));
-              }
-            }
-            __syncwarp();
-          };
-          auto output = [&](int half) {   // the rounded probabilities, then what rounding left
-            const uint32_t v_at = stage_at(v_pos), p_at = tmem + C::kS + (prev & 1) * kTile + half * 32;
-            if (elect_lane()) {
-#pragma unroll
-              for (int ks = 0; ks < kTile / 16; ks++) tc_mma(tmem + C::kO, p_at + ks * 8, smem_desc(v_at + ks * 2048, kTile * 128, 1024), kShapeO, i > 1 || half > 0 || ks > 0);
-              if (half) {
-                tc_commit(smem_u32(empty + v_pos % C::kStages));
-                tc_commit(smem_u32(o_full + (prev & 1)));
-              }
-            }
-            __syncwarp();
-          };
-          if (i < n) scores(0);
-          if (i > 0) {
-            bar_wait_warp(smem_u32(p_full + (prev & 1)), (prev >> 1) & 1, P.status, dead);
-            wait_full(v_pos);
-            tc_after();
-          }
-          if (i < n) scores(1);
-          if (i > 0) output(0);
-          if (i + 1 < n) wait_full(pos + 2 * i + 1);
-          if (i > 0) output(1);
+      const uint64_t k_desc0 = smem_desc(smem_u32(ring), 16, 1024), v_desc0 = smem_desc(smem_u32(ring), kTile * 128, 1024);
+      const uint32_t full0 = smem_u32(full), empty0 = smem_u32(empty), s_full0 = smem_u32(s_full), p_full0 = smem_u32(p_full), o_full0 = smem_u32(o_full);
+      int stage = 0, tile = 0, pieces = 0;   // tile: counted over all pieces
+      uint32_t parity = 0;
+      auto next_stage = [&]() {
+        if (++stage == C::kStages) {
+          stage = 0;
+          parity ^= 1u;
         }
+      };
+      auto wait = [&](uint32_t bar, uint32_t par) { bar_wait_warp(bar, par, P.status, dead); };
+      auto scores = [&](int half, uint64_t desc, int t) {   // (the probabilities that this buffer held have been multiplied: MMAs run in order)
+        const uint32_t d = tmem + C::kS + (t & 1) * kTile;
+#pragma unroll
+        for (int y = 0; y < HD / 32; y++) {
+          const int ks = half * (HD / 32) + y;
+          const uint64_t at = desc + ((ks >> 2) * (kTile * 128) + (ks & 3) * 32) / 16;
+          if (ks == 0) tc_mma<false>(d, tmem + C::kQ + ks * 8, at, kShapeS);
+          else tc_mma<true>(d, tmem + C::kQ + ks * 8, at, kShapeS);
+        }
+      };
+      auto output = [&](int half, uint64_t desc, int t, bool first) {   // the rounded probabilities, then what rounding left
+        const uint32_t p_at = tmem + C::kS + (t & 1) * kTile + half * 32;
+#pragma unroll
+        for (int ks = 0; ks < kTile / 16; ks++) {
+          if (ks == 0 && half == 0 && first) tc_mma<false>(tmem + C::kO, p_at, desc, kShapeO);
+          else tc_mma<true>(tmem + C::kO, p_at + ks * 8, desc + ks * (2048 / 16), kShapeO);
+        }
+      };
+      while (next_piece(&x)) {
+        const int n = x.t1 - x.t0;
+        wait(full0 + stage * 8, parity);
+        wait(smem_u32(&q_full), pieces & 1);
+        tc_after();
+        // the first tile's scores
+        if (elect_lane()) {
+          scores(0, k_desc0 + stage * (C::kStage / 16), tile);
+          scores(1, k_desc0 + stage * (C::kStage / 16), tile);
+          tc_commit(empty0 + stage * 8);
+          tc_commit(s_full0 + (tile & 1) * 8);
+        }
+        next_stage();
+        if (n > 1) wait(full0 + stage * 8, parity);
+        for (int i = 1; i <= n; i++) {
+          const int t = tile + i - 1;   // whose output is added
+          const uint32_t k_bar = empty0 + stage * 8;
+          const uint64_t k_desc = k_desc0 + stage * (C::kStage / 16);
+          if (i < n) {
+            if (elect_lane()) scores(0, k_desc, t + 1);
+            next_stage();
+          }
+          const uint64_t v_desc = v_desc0 + stage * (C::kStage / 16);
+          const uint32_t v_bar = empty0 + stage * 8;
+          wait(p_full0 + (t & 1) * 8, (t >> 1) & 1);
+          wait(full0 + stage * 8, parity);
+          tc_after();
+          next_stage();
+          if (elect_lane()) {
+            if (i < n) {
+              scores(1, k_desc, t + 1);
+              tc_commit(k_bar);
+              tc_commit(s_full0 + ((t + 1) & 1) * 8);
+            }
+            output(0, v_desc, t, i == 1);
+          }
+          if (i + 1 < n) wait(full0 + stage * 8, parity);
+          if (elect_lane()) {
+            output(1, v_desc, t, false);
+            tc_commit(v_bar);
+            tc_commit(o_full0 + (t & 1) * 8);
+          }
+        }
+        __syncwarp();
         tile += n;
-        pos += 2 * n;
         pieces++;
       }
     } else if (warp == kQueryWarp) {
       // ================= queries of a piece, as soon as those before have moved on =================
       asm volatile("fence.proxy.async;" ::: "memory");   // rows that the kernel before stored
       uint32_t parity = 1;
-      for (; next_piece(&x); j++) {
+      while (next_piece(&x)) {
         const bool common = x.q.seq < 0;
         const CUtensorMap* map = P.q_map + common;
         const int rows = P.q_rows[common], row = common ? x.q.kvh * p.B * p.T * (p.Hq / p.Hkv) : (x.q.kvh * p.B + x.q.seq) * p.T * (p.Hq / p.Hkv);
@@ -580,11 +618,11 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
         parity ^= 1u;
       }
     } else {
-      // ================= rows: thread <-> row of the tile; two groups of four warps take turns at the tiles =================
-      // The row's maximum goes from tile to tile, so from group to group, as soon as the tile's scores have been looked at; the rest of a
-      // tile's work runs beside the next one's.
+      // ================= rows: thread <-> row of the tile; two groups of four warps have 32 keys of it each =================
+      // (A group a tile, taking turns, made the way from a tile's scores to its probabilities twice as long, and with two buffers of scores the
+      // MMAs waited for it.)
       const int group = warp >> 2, quarter = warp & 3, i_row = threadIdx.x & 127;
-      const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16), s_at = lanes + C::kS + group * kTile;
+      const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
       const float c = __fmul_rn(p.scale, 1.44269504088896341f);   // scores in powers of two
       int tile = 0, stream = 0, pieces = 0;   // counted over all pieces
       // A wait tells a phase from the next one only, so nobody may be two phases off.  Scores of a tile that are there mean that the output of
@@ -593,11 +631,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
         bar_wait_warp(smem_u32(o_full + (t & 1)), (t >> 1) & 1, P.status, dead);
         tc_after();
       };
-      auto other_maximum = [&](int t) {   // of this row after tile t, which the other group has
-        bar_wait_warp(smem_u32(&m_full[group ^ 1][quarter]), (t >> 1) & 1, P.status, dead);
-        return *reinterpret_cast<volatile float*>(&m_s[group ^ 1][i_row]);
-      };
-      for (; next_piece(&x); j++, pieces++) {
+      for (; next_piece(&x); pieces++) {
         const Job q = x.q;
         const int t0 = x.t0, n = x.t1 - t0, key1 = x.key1;
         int b, t, g, limit = 0x7fffffff;   // (lanes without a row: never masked, never read)
@@ -627,17 +661,17 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
           bar_arrive(smem_u32(&q_full));
           bar_arrive(smem_u32(&q_empty));   // (in this order: the next queries' turn comes after all of these)
         }
-        float m = -INFINITY, l = 0.0f;   // the maximum that this group used last, and its part of the row sum
+        float m = -INFINITY, l = 0.0f;   // the maximum, and this group's part of the row sum
         for (int i = 0; i < n; i++, tile++) {
-          if ((tile & 1) != group) continue;
-          const int tile_key = q.key0 + (t0 + i) * kTile, there = min(kTile, key1 - tile_key);
-          bar_wait_warp(smem_u32(s_full + group), (tile >> 1) & 1, P.status, dead);
+          const int tile_key = q.key0 + (t0 + i) * kTile, there = min(kTile, key1 - tile_key), key = tile_key + group * 32;
+          const uint32_t s_at = lanes + C::kS + (tile & 1) * kTile;
+          bar_wait_warp(smem_u32(s_full + (tile & 1)), (tile >> 1) & 1, P.status, dead);
           tc_after();
           if (there < kTile) {   // values past the end count as zeros, whatever the page holds there
             const int v_pos = stream + stream_v(i, n), v_stage = v_pos % C::kStages;
             bar_wait_warp(smem_u32(full + v_stage), (v_pos / C::kStages) & 1, P.status, dead);
             uint8_t* v_at = ring + (size_t)v_stage * C::kStage;
-            for (int y = i_row; y < (kTile - there) * (HD / 8); y += 128) {
+            for (int y = threadIdx.x; y < (kTile - there) * (HD / 8); y += 256) {
               const int row = there + y / (HD / 8), piece = y % (HD / 8);
               *reinterpret_cast<uint4*>(v_at + (piece >> 3) * (kTile * 128) + row * 128 + (piece & 7) * 16) = make_uint4(0, 0, 0, 0);
             }
@@ -645,68 +679,73 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
             __syncwarp();
           }
           if (warp_on) {
-            uint32_t s[64];
-            tmem_ld64(s_at, s);
-            if (!__all_sync(0xffffffffu, tile_key + kTile <= limit)) {
+            uint32_t s[32];
+            tmem_ld32(s_at + group * 32, s);
+            if (!__all_sync(0xffffffffu, key + 32 <= limit)) {
 #pragma unroll
-              for (int y = 0; y < 64; y++) s[y] = tile_key + y < limit ? s[y] : 0xff800000u;
+              for (int y = 0; y < 32; y++) s[y] = key + y < limit ? s[y] : 0xff800000u;
             }
-            float mx = __uint_as_float(s[0]);
+            float top[4];   // four chains: one alone is 32 results of the instruction before
 #pragma unroll
-            for (int y = 1; y < 64; y++) mx = fmaxf(mx, __uint_as_float(s[y]));
-            mx = __fmul_rn(mx, c);
-            const float m0 = i > 0 ? other_maximum(tile - 1) : -INFINITY;
-            const bool move = mine && mx > __fadd_rn(m0, 8.0f);
-            const float m1 = move ? mx : m0;
-            m_s[group][i_row] = m1;
-            __syncwarp();
-            if (lane == 0) bar_arrive(smem_u32(&m_full[group][quarter]));
-            if (__any_sync(0xffffffffu, move && m0 != -INFINITY)) {   // the output so far is rescaled
-              const float f = move && m0 != -INFINITY ? exp2_approx(__fsub_rn(m0, m1)) : 1.0f;
-              wait_output(tile - 1);
+            for (int y = 0; y < 4; y++) top[y] = max3(__uint_as_float(s[2 * y]), __uint_as_float(s[2 * y + 1]), __uint_as_float(s[2 * y + 8]));
+#pragma unroll
+            for (int y = 0; y < 4; y++) top[y] = max3(top[y], __uint_as_float(s[2 * y + 9]), __uint_as_float(s[2 * y + 16]));
+#pragma unroll
+            for (int y = 0; y < 4; y++) top[y] = max3(top[y], __uint_as_float(s[2 * y + 17]), __uint_as_float(s[2 * y + 24]));
+#pragma unroll
+            for (int y = 0; y < 4; y++) top[y] = fmaxf(top[y], __uint_as_float(s[2 * y + 25]));
+            float mx = fmaxf(max3(top[0], top[1], top[2]), top[3]);
+            m_s[tile & 1][group][i_row] = mx;
+            asm volatile("bar.sync %0, 64;" ::"r"(1 + quarter) : "memory");   // (both halves have been read, too: probabilities may go over them)
+            mx = __fmul_rn(fmaxf(mx, m_s[tile & 1][group ^ 1][i_row]), c);
+            const bool move = mine && mx > __fadd_rn(m, 8.0f);
+            if (__any_sync(0xffffffffu, move)) {
+              const bool rescale = move && m != -INFINITY;
+              const float f = rescale ? exp2_approx(__fsub_rn(m, mx)) : 1.0f;
+              l = __fmul_rn(l, f);
+              if (move) m = mx;
+              if (__any_sync(0xffffffffu, rescale)) {   // the output so far, half of the dims a group
+                wait_output(tile - 1);
 #pragma unroll 1
-              for (int d = 0; d < HD / 32; d++) {
-                uint32_t o[32];
-                tmem_ld32(lanes + C::kO + d * 32, o);
+                for (int d = group * (HD / 64); d < (group + 1) * (HD / 64); d++) {
+                  uint32_t o[32];
+                  tmem_ld32(lanes + C::kO + d * 32, o);
 #pragma unroll
-                for (int y = 0; y < 32; y++) o[y] = __float_as_uint(__fmul_rn(__uint_as_float(o[y]), f));
-                tmem_st32(lanes + C::kO + d * 32, o);
+                  for (int y = 0; y < 32; y++) o[y] = __float_as_uint(__fmul_rn(__uint_as_float(o[y]), f));
+                  tmem_st32(lanes + C::kO + d * 32, o);
+                }
               }
             }
-            if (m != m1 && m != -INFINITY) l = __fmul_rn(l, exp2_approx(__fsub_rn(m, m1)));
-            m = m1;
             const float base = m == -INFINITY ? 0.0f : m;
-            float2 sum = make_float2(0.0f, 0.0f);
-            uint32_t lo[32];
+            float2 sum[2];
+            uint32_t lo[16];
 #pragma unroll
-            for (int y = 0; y < 32; y++) {
+            for (int y = 0; y < 16; y++) {
               const float2 z = bk_fma2(make_float2(__uint_as_float(s[2 * y]), __uint_as_float(s[2 * y + 1])), make_float2(c, c), make_float2(-base, -base));
               const float2 e = make_float2(exp2_approx(z.x), exp2_approx(z.y));
-              sum = bk_add2(sum, e);
+              sum[y & 1] = y < 2 ? e : bk_add2(sum[y & 1], e);
               s[y] = bk_f32x2_to_bf16x2(e.x, e.y);
-              lo[y] = bk_f32x2_to_bf16x2(__fsub_rn(e.x, __uint_as_float(s[y] << 16)), __fsub_rn(e.y, __uint_as_float(s[y] & 0xffff0000u)));
+              const float2 left = bk_fma2(make_float2(__uint_as_float(s[y] << 16), __uint_as_float(s[y] & 0xffff0000u)), make_float2(-1.0f, -1.0f), e);
+              lo[y] = bk_f32x2_to_bf16x2(left.x, left.y);
             }
-            l = __fadd_rn(l, __fadd_rn(sum.x, sum.y));
-            tmem_st32(s_at, s);
-            tmem_st32(s_at + 32, lo);
+            const float2 all = bk_add2(sum[0], sum[1]);
+            l = __fadd_rn(l, __fadd_rn(all.x, all.y));
+            tmem_st16(s_at + group * 16, s);
+            tmem_st16(s_at + 32 + group * 16, lo);
             tmem_wait_st();
-          } else if (lane == 0) bar_arrive(smem_u32(&m_full[group][quarter]));
+          }
           tc_before();
-          bar_arrive(smem_u32(p_full + group));
+          __syncwarp();
+          if (lane == 0) bar_arrive(smem_u32(p_full + (tile & 1)));
         }
         stream += 2 * n;
-        // the piece's part of the result: row sums relative to the last maximum, half of the dims a group
-        if (((tile - 1) & 1) != group) {
-          const float m1 = other_maximum(tile - 1);   // (of a warp without rows: whatever it is)
-          if (m != m1 && m != -INFINITY) l = __fmul_rn(l, exp2_approx(__fsub_rn(m, m1)));
-          m = m1;
-        }
+        // the piece's part of the result, half of the dims a group
         wait_output(tile - 1);
         if (warp_on) {
           const bool common = q.seq < 0;
-          const size_t slot = common ? (size_t)(j + cta) * kRows : (size_t)(j - L.n_p + cta) * L.rows_s;
-          float* ml = reinterpret_cast<float*>(P.scratch + (common ? L.ml_p : L.ml_s)) + (slot + i_row) * 4;
           const int rows = common ? kRows : L.rows_s;
+          const size_t slot = x.slot * rows;
+          float* ml = reinterpret_cast<float*>(P.scratch + (common ? L.ml_p : L.ml_s)) + (slot + i_row) * 4;
           uint4* o_to = reinterpret_cast<uint4*>(P.scratch + (common ? L.o_p : L.o_s)) + slot * (HD / 4) + i_row;   // [HD / 4][rows] x 4 dims: lanes side by side
           if (mine) {
             if (group == 0) ml[0] = m;
@@ -750,12 +789,12 @@ __global__ void __launch_bounds__(256 * kSlices) paged_merge_kernel(const PagedP
   const uint16_t* gate = p.fused ? p.qg + ((size_t)e * p.Hq + kvh * G + g) * 2 * HD + HD : p.gate ? p.gate + ((size_t)e * p.Hq + kvh * G + g) * HD : nullptr;
   bk_pdl_wait();
   const int4* jobs = jobs_of(L, scratch);
-  int4 qp = make_int4(0, 0, 0, -1), qs = __ldcg(jobs + L.n_p + js);
-  if (L.n_p) qp = __ldcg(jobs + jp);
+  const int2 qs = __ldcg(reinterpret_cast<const int2*>(&jobs[L.n_p + js].z));   // first slot, number
+  const int2 qp = L.n_p ? __ldcg(reinterpret_cast<const int2*>(&jobs[jp].z)) : make_int2(0, 0);
   const bool here = row_of(p, b, t) >= 0;
   uint2 gv = make_uint2(0, 0);
   if (gate && slice == 0) gv = *reinterpret_cast<const uint2*>(gate + (d0 + d) * 4);
-  const int np = here ? qp.w - qp.z + 1 : 0, n = here ? np + qs.w - qs.z + 1 : 0;
+  const int np = here ? qp.y : 0, n = here ? np + qs.y : 0;
   float m = -INFINITY, l = 0.0f;
   float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   constexpr int U = kSlices == 1 ? 6 : 4;   // pieces requested together
@@ -767,7 +806,7 @@ __global__ void __launch_bounds__(256 * kSlices) paged_merge_kernel(const PagedP
       x[k] = make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
       if (i < n) {
         const bool common = i < np;
-        const size_t slot = common ? (size_t)(jp + qp.z + i) : (size_t)(js + qs.z + i - np);
+        const size_t slot = common ? qp.x + i : qs.x + i - np;
         const int rows = common ? kRows : L.rows_s, row = (common ? rp : rs) % kRows;
         x[k] = __ldcg(reinterpret_cast<const float4*>(scratch + (common ? L.ml_p : L.ml_s)) + slot * rows + row);
         v[k] = __ldcg(reinterpret_cast<const float4*>(scratch + (common ? L.o_p : L.o_s)) + (slot * (HD / 4) + d0 + d) * rows + row);
