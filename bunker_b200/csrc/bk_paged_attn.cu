@@ -42,13 +42,14 @@ BK_DEVINL void load_bf16(const uint16_t* src, float (&y)[PER]) {
 // ---- who does what -----------------------------------------------------------------
 // A job is a tile of up to 128 rows (token, query head) of one KV head and the keys they attend to: the common keys [0, P) once for the
 // rows of all sequences, then for each sequence its own keys [P, end).  The jobs, in tiles of 64 keys and kOverhead more for each job, are laid
-// out in one line and cut into equal pieces, one per CTA, so that a long prefix and many short sequences keep every SM busy until the end.  The
-// line is made on the device (lengths are there), by one CTA of the first launch.  (With the same cuts for all row tiles of a KV head, which then read
-// the same keys at the same time, and the line for the rest, most CTAs have two pieces: 32 sequences behind 8,192 rows 30.5 -> 36.2 us, 64
-// behind 32,768 rows 105.2 -> 102.2.)
+// out in one line and cut into equal pieces, one per CTA, so that a long prefix and many short sequences keep every SM busy until the end.
+// Where common keys have several row tiles, all of those are cut at the same keys, one range a CTA, and the line is for the other CTAs: the row tiles
+// of a KV head then read the same keys at the same time, once from memory (in one line they read them at times that hang on the cuts: 64
+// sequences, 24 heads on 4, 32,768 common rows 100 to 118 us by the overhead that the line counts with, so @T1@).
+// The plan is made on the device (lengths are there), by one CTA of the first launch.
 constexpr int kTile = 64;       // keys of a step
 constexpr int kRows = 128;      // rows of a job: the lanes of tensor memory
-constexpr int kOverhead = 2;    // what a job's start and end cost, in steps
+constexpr int kOverhead = 3;    // what a job's start and end cost, in steps
 
 struct Layout {                 // of the scratch buffer, and the numbers of jobs
   int P;                        // common keys: whole pages
@@ -77,7 +78,7 @@ inline Layout make_layout(int B, int T, int Hq, int Hkv, int HD, int prefix_rows
   at += (size_t)(L.n_p + L.n_s + 1) * 16;
   L.pieces = at;
   at += (size_t)ctas * 32;
-  // partial results: a job and a CTA that has a piece of it meet in slot job + CTA, which no other pair has
+  // partial results: on the line a job and a CTA that has a piece of it meet in slot job + CTA, which no other pair has; off it the slot is the CTA
   const size_t slots_p = L.n_p ? L.n_p + ctas : 0, slots_s = L.n_s + ctas;
   L.ml_p = at;
   at += slots_p * kRows * 16;
@@ -132,8 +133,9 @@ BK_DEVINL int keys_end(const PagedParams& p, const Layout& L, const Job& q) {
   return L.P;
 }
 
-// What the first launch leaves for the others.  jobs[j] = {start on the line, end of the keys, slot of its first partial result, their number};
-// pieces[2c] = {start and end of CTA c's piece of the line, first job in it, -}, pieces[2c + 1] = that job's .x and .y.
+// What the first launch leaves for the others.  jobs[j] = {start on the line, end of the keys, slot of its first partial result, their number and
+// (<< 16) the distance of their slots}; pieces[2c] = {start and end of CTA c's piece of the line, first job in it, job over common keys or -1},
+// pieces[2c + 1] = {.x and .y of the first job in the line, the range of tiles over common keys}.
 BK_DEVINL int4* jobs_of(const Layout& L, uint8_t* scratch) { return reinterpret_cast<int4*>(scratch + L.jobs); }
 BK_DEVINL int4* pieces_of(const Layout& L, uint8_t* scratch) { return reinterpret_cast<int4*>(scratch + L.pieces); }
 BK_DEVINL int tiles_of(const Layout& L, int j, int key1) { return (key1 - (j < L.n_p ? 0 : L.P) + kTile - 1) / kTile; }
@@ -150,15 +152,18 @@ BK_DEVINL void plan_jobs(const PagedParams& p, const Layout& L, uint8_t* scratch
   int4* jobs = jobs_of(L, scratch);
   int4* pieces = pieces_of(L, scratch);
   const int n = L.n_p + L.n_s, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const bool in_smem = n <= kPlanned;
+  const int tiles_p = (L.P + kTile - 1) / kTile, all_ctas = min(L.ctas, kPrepThreads);
+  const bool in_smem = n <= kPlanned, apart = L.mt_p > 1 && L.n_p > 0 && L.n_p <= all_ctas / 2 && L.n_p * tiles_p >= all_ctas;   // common keys apart from the line
   // a thread has `per` jobs in a row
   const int per = (n + kPrepThreads - 1) / kPrepThreads, j0 = threadIdx.x * per, j1 = min(n, j0 + per);
   int mine = 0, tiles_mine = 0;
   for (int j = j0; j < j1; j++) {
     const int end = keys_end(p, L, job_of(p, L, j)), tiles = tiles_of(L, j, end);
     *reinterpret_cast<int2*>(jobs + j) = make_int2(mine, end);   // .x: within the thread, for now
-    mine += tiles ? tiles + kOverhead : 0;
-    tiles_mine += tiles;
+    if (!apart || j >= L.n_p) {
+      mine += tiles ? tiles + kOverhead : 0;
+      tiles_mine += tiles;
+    }
   }
   int v = mine;
 #pragma unroll
@@ -188,9 +193,20 @@ BK_DEVINL void plan_jobs(const PagedParams& p, const Layout& L, uint8_t* scratch
     jobs[n].x = units;
     if (in_smem) starts_s[n] = units;
   }
-  const int C = max(1, min(min(L.ctas, kPrepThreads), tiles_all));   // every CTA has a tile to do
+  // ranges of a job over common keys: so many that the longest range and the line's pieces come out equal, as far as whole numbers let them
+  int ranges = 0;
+  if (apart) {
+    unsigned int best = 0xffffffffu;
+    for (int r = lane + 1; r <= min(all_ctas / L.n_p, tiles_p); r += 32) {
+      const int others = all_ctas - L.n_p * r;
+      const float cost = fmaxf((float)((tiles_p + r - 1) / r), units ? others ? (float)units / others : 4e6f : 0.0f);
+      best = min(best, (unsigned int)fminf(cost * 4.0f, 4e6f) << 8 | r);   // (r below 256)
+    }
+    ranges = __reduce_min_sync(0xffffffffu, best) & 255;
+  }
+  const int c0 = L.n_p * ranges, C = max(c0 + 1, min(all_ctas, c0 + tiles_all));   // the line's CTAs: from c0 on, and every one of them has a tile to do
   // (a quotient that is no whole number is at least 1 / C away from one, so the double below it is too)
-  for (int c = threadIdx.x; c <= C; c += kPrepThreads) bounds_s[c] = (int)((double)units * c / C);
+  for (int c = threadIdx.x; c <= C; c += kPrepThreads) bounds_s[c] = c <= c0 ? 0 : (int)((double)units * (c - c0) / (C - c0));
   __syncthreads();
   auto start = [&](int j) { return in_smem ? starts_s[j] : jobs[j].x; };
   for (int c = threadIdx.x; c < L.ctas; c += kPrepThreads) {
@@ -201,11 +217,13 @@ BK_DEVINL void plan_jobs(const PagedParams& p, const Layout& L, uint8_t* scratch
       if (start(mid) <= u0) lo = mid;
       else hi = mid;
     }
-    pieces[2 * c] = make_int4(u0, u1, lo, 0);
-    pieces[2 * c + 1] = make_int4(start(lo), jobs[lo].y, 0, 0);
+    // CTA c < c0: range r of job (KV head, row tile), the row tiles next to one another
+    const int group = c / L.mt_p, r = apart ? group % ranges : 0;
+    pieces[2 * c] = make_int4(u0, u1, lo, c < c0 ? group / ranges * L.mt_p + c % L.mt_p : -1);
+    pieces[2 * c + 1] = make_int4(start(lo), jobs[lo].y, c < c0 ? tiles_p * r / ranges : 0, c < c0 ? tiles_p * (r + 1) / ranges : 0);
   }
   auto cta_at = [&](int unit) {   // the CTA that has it
-    int lo = 0, hi = C;
+    int lo = c0, hi = C;
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
       if (bounds_s[mid] <= unit) lo = mid;
@@ -215,7 +233,9 @@ BK_DEVINL void plan_jobs(const PagedParams& p, const Layout& L, uint8_t* scratch
   };
   for (int j = threadIdx.x; j < n; j += kPrepThreads) {
     const int s = start(j), s1 = start(j + 1), first = cta_at(s + kOverhead);
-    *reinterpret_cast<int2*>(&jobs[j].z) = s1 > s ? make_int2((j < L.n_p ? j : j - L.n_p) + first, cta_at(s1 - 1) - first + 1) : make_int2(0, 0);
+    *reinterpret_cast<int2*>(&jobs[j].z) = apart && j < L.n_p ? make_int2(j / L.mt_p * ranges * L.mt_p + j % L.mt_p, ranges | L.mt_p << 16)
+                                           : s1 > s          ? make_int2((j < L.n_p ? j : j - L.n_p) + first, (cta_at(s1 - 1) - first + 1) | 1 << 16)
+                                                             : make_int2(0, 0);
   }
 }
 
@@ -447,13 +467,25 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
   const int4 line = __ldcg(pieces_of(L, P.scratch) + 2 * cta), first = __ldcg(pieces_of(L, P.scratch) + 2 * cta + 1);
   const int u0 = line.x, u1 = line.y;
   int j = line.z - 1;
-  // the next piece of a job, from job j + 1 on
+  // the next piece: a range of common keys, then the line's jobs from j + 1 on
   struct Piece {
     Job q;
     int key1, t0, t1;
     size_t slot;   // of its partial result, among its kind's
   };
+  bool began = false;
   auto next_piece = [&](Piece* x) {
+    if (!began) {
+      began = true;
+      if (line.w >= 0) {
+        x->q = job_of(p, L, line.w);
+        x->key1 = L.P;
+        x->t0 = first.z;
+        x->t1 = first.w;
+        x->slot = cta;
+        return true;
+      }
+    }
     while (++j < n_jobs) {
       int2 job = make_int2(first.x, first.y);   // start, end of the keys
       if (j != line.z) job = __ldcg(reinterpret_cast<const int2*>(jobs + j));
@@ -789,12 +821,12 @@ __global__ void __launch_bounds__(256 * kSlices) paged_merge_kernel(const PagedP
   const uint16_t* gate = p.fused ? p.qg + ((size_t)e * p.Hq + kvh * G + g) * 2 * HD + HD : p.gate ? p.gate + ((size_t)e * p.Hq + kvh * G + g) * HD : nullptr;
   bk_pdl_wait();
   const int4* jobs = jobs_of(L, scratch);
-  const int2 qs = __ldcg(reinterpret_cast<const int2*>(&jobs[L.n_p + js].z));   // first slot, number
+  const int2 qs = __ldcg(reinterpret_cast<const int2*>(&jobs[L.n_p + js].z));   // first slot; number and distance
   const int2 qp = L.n_p ? __ldcg(reinterpret_cast<const int2*>(&jobs[jp].z)) : make_int2(0, 0);
   const bool here = row_of(p, b, t) >= 0;
   uint2 gv = make_uint2(0, 0);
   if (gate && slice == 0) gv = *reinterpret_cast<const uint2*>(gate + (d0 + d) * 4);
-  const int np = here ? qp.y : 0, n = here ? np + qs.y : 0;
+  const int np = here ? qp.y & 0xffff : 0, n = here ? np + (qs.y & 0xffff) : 0;
   float m = -INFINITY, l = 0.0f;
   float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   constexpr int U = kSlices == 1 ? 6 : 4;   // pieces requested together
@@ -806,7 +838,7 @@ __global__ void __launch_bounds__(256 * kSlices) paged_merge_kernel(const PagedP
       x[k] = make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
       if (i < n) {
         const bool common = i < np;
-        const size_t slot = common ? qp.x + i : qs.x + i - np;
+        const size_t slot = common ? qp.x + i * (qp.y >> 16) : qs.x + i - np;
         const int rows = common ? kRows : L.rows_s, row = (common ? rp : rs) % kRows;
         x[k] = __ldcg(reinterpret_cast<const float4*>(scratch + (common ? L.ml_p : L.ml_s)) + slot * rows + row);
         v[k] = __ldcg(reinterpret_cast<const float4*>(scratch + (common ? L.o_p : L.o_s)) + (slot * (HD / 4) + d0 + d) * rows + row);
