@@ -190,10 +190,10 @@ def lora_seg(A: int, Bm: int, n_rows: int, out: int, base: int = 0, *, bf16: boo
 
 
 def lora_args(x: int, K: int, B: int, rank: int, n_adapters: int, ids: int, segs: Sequence[R.bkLoraSeg], scratch: int, scratch_bytes: int,
-              scale: int = 0, weights_are_settled: bool = False) -> R.bkLoraArgs:
+              scale: int = 0) -> R.bkLoraArgs:
     if not 1 <= len(segs) <= 4:
         raise ValueError(f"lora_args: {len(segs)} segments (1 to 4)")
-    a = R.bkLoraArgs(K=K, B=B, n_segs=len(segs), rank=rank, n_adapters=n_adapters, weights_are_settled=int(weights_are_settled), x=x, ids=ids,
+    a = R.bkLoraArgs(K=K, B=B, n_segs=len(segs), rank=rank, n_adapters=n_adapters, x=x, ids=ids,
                      scale=scale, scratch=scratch, scratch_bytes=scratch_bytes)
     for i, s in enumerate(segs):
         a.segs[i] = s

@@ -87,7 +87,7 @@ class bkLoraSeg(C.Structure):
 
 
 class bkLoraArgs(C.Structure):
-    _fields_ = [(n, C.c_int32) for n in ("K", "B", "n_segs", "rank", "n_adapters", "weights_are_settled")] + \
+    _fields_ = [(n, C.c_int32) for n in ("K", "B", "n_segs", "rank", "n_adapters", "reserved")] + \
                [(n, C.c_uint64) for n in ("x", "ids", "scale", "scratch", "scratch_bytes")] + [("segs", bkLoraSeg * 4)]
 
 

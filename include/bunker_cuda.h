@@ -355,7 +355,7 @@ typedef struct bkLoraArgs {
   int32_t n_segs;        /* 1..4 row segments that share x */
   int32_t rank;          /* multiple of 8, 8..128 */
   int32_t n_adapters;
-  int32_t weights_are_settled; /* 1: A and Bm were NOT written by launches that may still run, so they may be read before those end */
+  int32_t reserved;
   uint64_t x;            /* bf16 [B][K] */
   uint64_t ids;          /* int32 [B] */
   uint64_t scale;        /* f32 [n_adapters]; 0 = all 1 */
