@@ -164,7 +164,7 @@ BK_DEVINL void load_weights(const LoraSeg& s, const uint16_t* from, int rank, in
 }
 // grid (M * p.per tiles of rows, column)
 template <int P, int M>
-__global__ void __launch_bounds__(kThreads) lora_expand_kernel(const __grid_constant__ LoraParams p) {
+__global__ void __launch_bounds__(kThreads, P <= 4 ? 4 : 1) lora_expand_kernel(const __grid_constant__ LoraParams p) {
   extern __shared__ __align__(16) float u_s[];   // [columns of the adapter][8 P]
   bk_pdl_trigger();
   bk_pdl_wait();

@@ -23,7 +23,8 @@ struct Pool {
   int n_planes, n_pages, heads, page_rows, row_bytes, n_seqs, max_pages;
 };
 
-BK_DEVINL int pages_of(long long rows, int page_rows) { return (int)((rows + page_rows - 1) / page_rows); }
+// rows below 2^31
+BK_DEVINL int pages_of(unsigned int rows, int page_rows) { return (int)((rows + (unsigned int)page_rows - 1) / (unsigned int)page_rows); }
 
 // inclusive sum over the block
 BK_DEVINL long long block_scan(long long v, long long* warp_sums) {
@@ -50,12 +51,17 @@ BK_DEVINL long long block_scan(long long v, long long* warp_sums) {
   return v;
 }
 
-// whether entry i of a list names a sequence that an earlier entry has not named
-BK_DEVINL bool first_entry(const int* list, int i) {
+// Whether entry i of a list of n names a sequence that an earlier entry has not named.  Every thread looks at as many entries, four a load and
+// without a way out of the loop: one that ends early, an entry a load, took 11 us of a call with 64 entries.
+BK_DEVINL bool first_entry(const int* list, int n, int i) {
   const int s = list[i];
-  for (int j = 0; j < i; j++)
-    if (list[j] == s) return false;
-  return true;
+  bool again = false;
+#pragma unroll 4
+  for (int j = 0; j < n; j += 4) {   // (entries behind the list are -1)
+    const int4 v = *reinterpret_cast<const int4*>(list + j);
+    again |= (v.x == s && j < i) | (v.y == s && j + 1 < i) | (v.z == s && j + 2 < i) | (v.w == s && j + 3 < i);
+  }
+  return !again;
 }
 
 // The lowest-numbered free pages, at most `want`, in ascending order into fresh[]; returns how many there are.  All threads call.
@@ -92,7 +98,8 @@ struct ForkPlan {   // of one fork, in the scratch buffer
 // One CTA: which forks are served, and the fresh page of each.
 __global__ void __launch_bounds__(kPlanThreads) pages_fork_plan_kernel(const Pool p, const int* src, const int* dst, int n, int* ok, ForkPlan* plan, int* fresh) {
   __shared__ long long warp_sums[32];
-  __shared__ int dst_s[kPlanThreads], total_s;
+  __shared__ __align__(16) int dst_s[kPlanThreads];
+  __shared__ int total_s;
   __shared__ long long want_s;
   bk_pdl_trigger();
   bk_pdl_wait();
@@ -101,9 +108,9 @@ __global__ void __launch_bounds__(kPlanThreads) pages_fork_plan_kernel(const Poo
   dst_s[i] = d;
   __syncthreads();
   int rows = -1;
-  if (i < n && s >= 0 && s < p.n_seqs && d >= 0 && d < p.n_seqs && s != d && p.lens[d] == 0 && first_entry(dst_s, i)) {
-    rows = p.lens[s];
-    if (rows > (long long)p.max_pages * p.page_rows) rows = -1;
+  if (i < n && s >= 0 && s < p.n_seqs && d >= 0 && d < p.n_seqs && s != d) {
+    const int held = __ldcg(p.lens + s), there = __ldcg(p.lens + d);
+    if (first_entry(dst_s, n, i) && there == 0 && held <= p.max_pages * p.page_rows) rows = held;
   }
   const int need = rows > 0 && rows % p.page_rows ? 1 : 0;
   const long long upto = block_scan(need, warp_sums);
@@ -169,7 +176,8 @@ __global__ void __launch_bounds__(kCopyThreads) pages_fork_kernel(const Pool p, 
 // One CTA: room for more rows.
 __global__ void __launch_bounds__(kPlanThreads) pages_grow_kernel(const Pool p, const int* seqs, const int* add, int n, int* ok, int* fresh) {
   __shared__ long long warp_sums[32], upto_s[kPlanThreads];
-  __shared__ int list_s[kPlanThreads], need_s[kPlanThreads], before_s[kPlanThreads], total_s;
+  __shared__ __align__(16) int list_s[kPlanThreads];
+  __shared__ int need_s[kPlanThreads], before_s[kPlanThreads], total_s;
   __shared__ long long want_s;
   bk_pdl_trigger();
   bk_pdl_wait();
@@ -180,11 +188,11 @@ __global__ void __launch_bounds__(kPlanThreads) pages_grow_kernel(const Pool p, 
   __syncthreads();
   long long rows = -1;
   int len = 0, need = 0;
-  if (i < n && s >= 0 && s < p.n_seqs && more >= 0 && first_entry(list_s, i)) {
-    len = p.lens[s];
+  if (i < n && s >= 0 && s < p.n_seqs && more >= 0) {
+    len = __ldcg(p.lens + s);
     rows = (long long)len + more;
-    if (len < 0 || rows > (long long)p.max_pages * p.page_rows) rows = -1;
-    else need = pages_of(rows, p.page_rows) - pages_of(len, p.page_rows);
+    if (!first_entry(list_s, n, i) || len < 0 || rows > p.max_pages * p.page_rows) rows = -1;
+    else need = pages_of((unsigned int)rows, p.page_rows) - pages_of(len, p.page_rows);
   }
   const long long upto = block_scan(need, warp_sums);
   if (i == kPlanThreads - 1) want_s = upto;
@@ -192,7 +200,7 @@ __global__ void __launch_bounds__(kPlanThreads) pages_grow_kernel(const Pool p, 
   const int have = find_free(p, min(want_s, (long long)p.n_pages), fresh, warp_sums, &total_s);
   const bool served = rows >= 0 && (need == 0 || upto <= have);
   need_s[i] = served ? need : 0;
-  before_s[i] = pages_of(len, p.page_rows);
+  before_s[i] = len > 0 ? pages_of(len, p.page_rows) : 0;
   upto_s[i] = upto;
   if (served) p.lens[s] = (int)rows;
   if (i < n && ok) ok[i] = served;
