@@ -2,7 +2,11 @@
 //
 // No counterpart in the reference.  Two launches: u = A x, split over K so that few requests fill the GPU too, then out = base + s Bm u.
 // A CTA takes all columns of one adapter (it belongs to the first of them), so an adapter's weights are read once whatever the number
-// of requests that share it.  Sums in f32; the parts of K are added in ascending order, so results do not depend on the launch.
+// of requests that share it.  Both products are m16n8k16 MMAs on fragments that lanes load from memory as they lie: the order of the
+// contraction's index is free as long as both operands have the same, so a lane takes 8 or 16 consecutive bytes of a row.  (With one row of weights
+// a thread, or a few lanes, and FMAs, unpacking and reducing were 200 instructions for 32 rows and a column.)  x and the weights are
+// bf16, exact; u goes in as three bf16 matrices, what is left of its 24 bits after each rounding in the next.  Sums in f32, the parts of K added
+// in ascending order: results do not depend on the launch.
 #include <string.h>
 
 #include <algorithm>
@@ -19,14 +23,14 @@ struct LoraSeg {
   const uint16_t *A, *Bm;
   const void* base;
   void* out;
-  int n_rows, f32, ld_out, col_off, tile0;   // tile0: first CTA of the segment in the expanding launch
+  int n_rows, f32, ld_out, col_off, u_seg, tile0;   // u_seg: its number in u; tile0: its first CTA in the expanding launch
 };
 struct LoraParams {
   const uint16_t* x;
   const int* ids;
   const float* scale;
   float* u;   // [part of K][segment][column][rank]
-  int K, B, n_segs, rank, n_adapters, parts, chunk, per;
+  int K, B, n_segs, rank, n_adapters, parts, chunk, per, u_segs;   // u_segs: segments that u has
   LoraSeg segs[4];
 };
 
@@ -42,249 +46,287 @@ BK_DEVINL unsigned long long columns_of(const LoraParams& p, int b, int* adapter
   return there && __ffsll(same) - 1 == b ? same : 0;
 }
 
-BK_DEVINL void unpack8(uint4 v, float (&y)[8]) {
-  y[0] = __uint_as_float(v.x << 16); y[1] = __uint_as_float(v.x & 0xffff0000u);
-  y[2] = __uint_as_float(v.y << 16); y[3] = __uint_as_float(v.y & 0xffff0000u);
-  y[4] = __uint_as_float(v.z << 16); y[5] = __uint_as_float(v.z & 0xffff0000u);
-  y[6] = __uint_as_float(v.w << 16); y[7] = __uint_as_float(v.w & 0xffff0000u);
+// D += A B; a: rows lane/4 and +8, two pairs of the contraction's index; b: column lane/4, the same pairs; d: rows lane/4 and +8, columns 2(lane mod 4), +1
+BK_DEVINL void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-constexpr int kChunk = 2048;   // of K, at most: what a CTA keeps of x, for kCols columns
-constexpr int kCols = 4;
+constexpr int kWarps = kThreads / 32;
 
-// 1,024 values of two rows of A, 4 KB a warp
-BK_DEVINL void load_rows(const uint16_t* row0, const uint16_t* row1, int kb, int len, uint4 (&w)[2][4]) {
-#pragma unroll
-  for (int i = 0; i < 4; i++) {
-    const int k = kb + i * 256 + (threadIdx.x & 31) * 8;
-    w[0][i] = k < len ? __ldg(reinterpret_cast<const uint4*>(row0 + k)) : make_uint4(0, 0, 0, 0);
-    w[1][i] = k < len ? __ldg(reinterpret_cast<const uint4*>(row1 + k)) : make_uint4(0, 0, 0, 0);
-  }
-}
-// u of C columns (n of them are there): two rows of A a warp at a time, the first of them in w already, x from shared memory
-template <int C>
-BK_DEVINL void shrink_rows(const LoraParams& p, const uint16_t* A, const uint16_t* x_s, int k0, int len, int seg, int part, const int* cols, int n, uint4 (&w)[2][4]) {
-  const int lane = threadIdx.x & 31;
-  for (int r = threadIdx.x >> 5; r < p.rank; r += 2 * kThreads / 32) {
-    const bool two = r + kThreads / 32 < p.rank;
-    const uint16_t* row0 = A + (size_t)r * p.K + k0;
-    const uint16_t* row1 = two ? row0 + (size_t)(kThreads / 32) * p.K : row0;
-    float acc[2][C];
-#pragma unroll
-    for (int c = 0; c < C; c++) acc[0][c] = acc[1][c] = 0.0f;
-    for (int kb = 0; kb < len; kb += 1024) {
-      if (kb || r != (threadIdx.x >> 5)) load_rows(row0, row1, kb, len, w);
-#pragma unroll
-      for (int i = 0; i < 4; i++) {
-        const int k = kb + i * 256 + lane * 8;
-        if (k < len) {
-          float w0[8], w1[8];
-          unpack8(w[0][i], w0);
-          unpack8(w[1][i], w1);
-#pragma unroll
-          for (int c = 0; c < C; c++) {
-            float x[8];
-            unpack8(*reinterpret_cast<const uint4*>(x_s + c * kChunk + k), x);
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-              acc[0][c] = fmaf(w0[e], x[e], acc[0][c]);
-              acc[1][c] = fmaf(w1[e], x[e], acc[1][c]);
-            }
-          }
-        }
-      }
-    }
-#pragma unroll
-    for (int c = 0; c < C; c++) {
-      const float y0 = bk_warp_sum(acc[0][c]), y1 = bk_warp_sum(acc[1][c]);
-      if (lane == 0 && c < n) {
-        float* u = p.u + (((size_t)part * p.n_segs + seg) * p.B + cols[c]) * p.rank + r;
-        u[0] = y0;
-        if (two) u[kThreads / 32] = y1;
-      }
-    }
-  }
+// The adapter's columns as a list; whole CTA, one barrier
+BK_DEVINL void list_columns(unsigned long long cols, int* list) {
+  if (threadIdx.x < 64 && (cols >> threadIdx.x & 1)) list[__popcll(cols & ((1ull << threadIdx.x) - 1))] = threadIdx.x;
+  __syncthreads();
 }
 
-// grid (part of K, column, segment).  Bound: latency, of ids, then of the first rows of A (requested before x is staged).
+// grid (part of K, column, segment).  A warp takes every eighth 32 of the CTA's K: MT tiles of 16 rows of A and up to 8 columns of x.  Bound: memory,
+// and for few requests the latency of ids, then of the weights.
+template <int MT>
 __global__ void __launch_bounds__(kThreads) lora_shrink_kernel(const __grid_constant__ LoraParams p) {
-  __shared__ __align__(16) uint16_t x_s[kCols * kChunk];
+  constexpr int U = MT <= 2 ? 4 : MT <= 4 ? 2 : 1;   // of 32 values of K requested together: up to 8 KB of weights a warp
+  __shared__ int list[kMaxB];
+  __shared__ float part_s[kWarps][MT * 16][8];
   bk_pdl_trigger();
   bk_pdl_wait();
   int a;
-  unsigned long long left = columns_of(p, blockIdx.y, &a);
-  if (!left) return;
-  const uint16_t* A = p.segs[blockIdx.z].A + (size_t)a * p.rank * p.K;
-  const int k0 = blockIdx.x * p.chunk, len = min(p.K - k0, p.chunk), r0 = threadIdx.x >> 5;
-  uint4 w[2][4];
-  bool first = true;
-  while (left) {
-    const uint16_t* row0 = A + (size_t)r0 * p.K + k0;   // (rank is at least the number of warps)
-    load_rows(row0, r0 + kThreads / 32 < p.rank ? row0 + (size_t)(kThreads / 32) * p.K : row0, 0, len, w);
-    int cols[kCols], m = 0;
+  const unsigned long long cols = columns_of(p, blockIdx.y, &a);
+  if (!cols) return;
+  list_columns(cols, list);
+  const int n = __popcll(cols), lane = threadIdx.x & 31, warp = threadIdx.x >> 5, q = lane >> 2, j = lane & 3;
+  const int k0 = blockIdx.x * p.chunk, k1 = min(p.K, k0 + p.chunk);
+  const uint16_t* A = p.segs[blockIdx.z].A + ((size_t)a * p.rank + q) * p.K + j * 8;
+  const uint4 zero = make_uint4(0, 0, 0, 0);
+  for (int c0 = 0; c0 < n; c0 += 8) {
+    const uint16_t* x = p.x + (size_t)list[min(c0 + q, n - 1)] * p.K + j * 8;
+    const bool col = c0 + q < n;
+    float d[MT][4];
 #pragma unroll
-    for (int c = 0; c < kCols; c++) {   // (a column that is not there is a copy of the last one that is: what it gives is not used)
-      if (left) {
-        cols[c] = __ffsll(left) - 1;
-        left &= left - 1;
-        m++;
-      } else cols[c] = cols[c ? c - 1 : 0];
+    for (int t = 0; t < MT; t++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) d[t][e] = 0.0f;
+    for (int kb = k0 + warp * 32; kb < k1; kb += kWarps * 32 * U) {
+      uint4 w[U][MT][2], v[U];
+#pragma unroll
+      for (int u = 0; u < U; u++) {
+        const int k = kb + u * kWarps * 32;
+        const bool in = k + j * 8 < k1;   // (K and the parts are multiples of 8)
+        v[u] = in && col ? __ldg(reinterpret_cast<const uint4*>(x + k)) : zero;
+#pragma unroll
+        for (int t = 0; t < MT; t++)
+#pragma unroll
+          for (int h = 0; h < 2; h++) w[u][t][h] = in && t * 16 + h * 8 < p.rank ? __ldg(reinterpret_cast<const uint4*>(A + (size_t)(t * 16 + h * 8) * p.K + k)) : zero;
+      }
+#pragma unroll
+      for (int u = 0; u < U; u++)
+#pragma unroll
+        for (int t = 0; t < MT; t++) {
+          mma_bf16(d[t], w[u][t][0].x, w[u][t][1].x, w[u][t][0].y, w[u][t][1].y, v[u].x, v[u].y);
+          mma_bf16(d[t], w[u][t][0].z, w[u][t][1].z, w[u][t][0].w, w[u][t][1].w, v[u].z, v[u].w);
+        }
     }
-    if (!first) __syncthreads();
-    first = false;
+    if (c0) __syncthreads();   // the sums before have been taken
 #pragma unroll
-    for (int c = 0; c < kCols; c++)
-      if (c < m || m > 1)
-        for (int k = threadIdx.x * 8; k < len; k += kThreads * 8) *reinterpret_cast<uint4*>(x_s + c * kChunk + k) = *reinterpret_cast<const uint4*>(p.x + (size_t)cols[c] * p.K + k0 + k);
+    for (int t = 0; t < MT; t++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) part_s[warp][t * 16 + (e >> 1) * 8 + q][2 * j + (e & 1)] = d[t][e];
     __syncthreads();
-    if (m == 1) shrink_rows<1>(p, A, x_s, k0, len, blockIdx.z, blockIdx.x, cols, m, w);
-    else shrink_rows<kCols>(p, A, x_s, k0, len, blockIdx.z, blockIdx.x, cols, m, w);
-  }
-}
-
-BK_DEVINL float load_base(const LoraSeg& s, size_t at) {
-  return !s.base ? 0.0f : s.f32 ? reinterpret_cast<const float*>(s.base)[at] : bk_bf16_to_f32(reinterpret_cast<const uint16_t*>(s.base)[at]);
-}
-BK_DEVINL void store_out(const LoraSeg& s, size_t at, float v) {
-  if (s.f32) reinterpret_cast<float*>(s.out)[at] = v;
-  else reinterpret_cast<uint16_t*>(s.out)[at] = bk_f32_to_bf16(v);
-}
-
-// P lanes read a row of Bm (16 bytes each, rank <= 8 P), so that a warp's loads are whole lines; P loads a lane are 32 rows of a warp, a CTA's 256 are
-// a tile.  The sums of the P lanes of a row are halved out so that every lane ends up with one row.  A CTA takes p.per times M tiles; the next M are
-// requested before these are multiplied.
-template <int P>
-BK_DEVINL void load_weights(const LoraSeg& s, const uint16_t* from, int rank, int row, uint4* w) {
-  const int lane = threadIdx.x & 31;
+    for (int i = threadIdx.x; i < p.rank * 8; i += kThreads) {
+      const int r = i >> 3, c = c0 + (i & 7);
+      float y = 0.0f;
 #pragma unroll
-  for (int i = 0; i < P; i++) {
-    const int r = row + i * (32 / P) + lane / P;
-    w[i] = r < s.n_rows && lane % P * 8 < rank ? __ldg(reinterpret_cast<const uint4*>(from + (size_t)r * rank)) : make_uint4(0, 0, 0, 0);
+      for (int w = 0; w < kWarps; w++) y = __fadd_rn(y, part_s[w][r][i & 7]);
+      if (c < n) p.u[(((size_t)blockIdx.x * p.n_segs + blockIdx.z) * p.B + list[c]) * p.rank + r] = y;
+    }
   }
 }
-// grid (M * p.per tiles of rows, column)
-template <int P, int M>
-__global__ void __launch_bounds__(kThreads, P <= 4 ? 4 : 1) lora_expand_kernel(const __grid_constant__ LoraParams p) {
-  extern __shared__ __align__(16) float u_s[];   // [columns of the adapter][8 P]
+
+// u as three bf16 values; one that is not finite stays whole in the first
+BK_DEVINL void split3(float u, uint16_t (&o)[3]) {
+  o[0] = bk_f32_to_bf16(u);
+  const float r = isfinite(u) ? __fsub_rn(u, bk_bf16_to_f32(o[0])) : 0.0f;
+  const bool sound = isfinite(r);   // (rounding may pass the largest f32)
+  o[1] = sound ? bk_f32_to_bf16(r) : 0;
+  o[2] = sound ? bk_f32_to_bf16(__fsub_rn(r, bk_bf16_to_f32(o[1]))) : 0;
+}
+
+// grid (p.per tiles of 256 rows, column).  A warp has 32 rows of a tile, KS steps of 16 of the rank; the next tile's weights are requested before
+// these are multiplied.  WIDE (rank a multiple of 32): a lane's 16 bytes are two steps of a row.  Bound: memory.
+template <bool F32>
+BK_DEVINL float load_as(const uint8_t* at) { return F32 ? *reinterpret_cast<const float*>(at) : bk_bf16_to_f32(*reinterpret_cast<const uint16_t*>(at)); }
+template <bool F32>
+BK_DEVINL void store_as(uint8_t* at, float v) {
+  if (F32) *reinterpret_cast<float*>(at) = v;
+  else *reinterpret_cast<uint16_t*>(at) = bk_f32_to_bf16(v);
+}
+template <int KS, bool WIDE, bool F32>
+__global__ void __launch_bounds__(kThreads, KS <= 2 ? 3 : KS <= 4 ? 2 : 1) lora_expand_kernel(const __grid_constant__ LoraParams p) {
+  constexpr int R = KS * 16, SZ = F32 ? 4 : 2;
+  extern __shared__ __align__(16) uint16_t u_s[];   // [3][columns of the adapter][R]
+  __shared__ int list[kMaxB];
   bk_pdl_trigger();
   bk_pdl_wait();
   int seg = 0;
   while (seg + 1 < p.n_segs && (int)blockIdx.x >= p.segs[seg + 1].tile0) seg++;
   const LoraSeg& s = p.segs[seg];
-  const int lane = threadIdx.x & 31, b = blockIdx.y, piece = lane % P;
-  const int row0 = ((int)blockIdx.x - s.tile0) * (p.per * M * kThreads) + (threadIdx.x >> 5) * 32, row_end = min(s.n_rows, row0 + p.per * M * kThreads);   // of this warp: 32 rows of every tile
+  const int lane = threadIdx.x & 31, q = lane >> 2, j = lane & 3, b = blockIdx.y;
+  const int row0 = ((int)blockIdx.x - s.tile0) * (p.per * kThreads) + (threadIdx.x >> 5) * 32, row_end = min(s.n_rows, row0 + p.per * kThreads);   // of this warp
   int a;
-  unsigned long long cols = columns_of(p, b, &a);
+  const unsigned long long cols = columns_of(p, b, &a);
+  const uint8_t* const base0 = reinterpret_cast<const uint8_t*>(s.base);   // (0: zeros)
+  uint8_t* const out0 = reinterpret_cast<uint8_t*>(s.out);
+  const int n_rows = s.n_rows, rank = p.rank, ld = s.ld_out, col_off = s.col_off;
   if (a < 0) {   // no adapter
-    if (s.base == s.out) return;
+    if (base0 == out0) return;
     for (int row = row0 + lane; row < row_end; row += kThreads) {
-      const size_t at = (size_t)b * s.ld_out + s.col_off + row;
-      store_out(s, at, load_base(s, at));
+      const size_t at = ((size_t)b * ld + col_off + row) * SZ;
+      store_as<F32>(out0 + at, base0 ? load_as<F32>(base0 + at) : 0.0f);
     }
     return;
   }
   if (!cols) return;
+  const int n = __popcll(cols);
   // weights first: what is needed beside them is small and near
-  const uint16_t* from = s.Bm + (size_t)a * s.n_rows * p.rank + piece * 8;
-  const size_t first_col = (size_t)b * s.ld_out + s.col_off;
-  // the row that this lane ends up with of each 32: the halving leaves the first half of the loads to the lanes whose first bit of `piece` is 0
-  int turn = 0;
-#pragma unroll
-  for (int bit = 1; bit < P; bit <<= 1) turn = turn << 1 | ((piece / bit) & 1);
-  const int my_row = turn * (32 / P) + lane / P;
-  uint4 w[M][P];
-  float base[M];
+  const uint16_t* from = s.Bm + ((size_t)a * n_rows + q) * rank;
+  uint2 w[4][KS];
   auto request = [&](int row) {
 #pragma unroll
-    for (int m = 0; m < M; m++) {
-      load_weights<P>(s, from, p.rank, row + m * kThreads, w[m]);
-      base[m] = row + m * kThreads + my_row < s.n_rows ? load_base(s, first_col + row + m * kThreads + my_row) : 0.0f;
+    for (int i = 0; i < 4; i++) {
+      const uint16_t* at = from + (size_t)(row + i * 8) * rank;
+      const bool in = row + i * 8 + q < n_rows;
+      if (WIDE) {
+#pragma unroll
+        for (int k = 0; k < KS; k += 2) {
+          const uint4 v = in ? __ldg(reinterpret_cast<const uint4*>(at + k * 16 + j * 8)) : make_uint4(0, 0, 0, 0);
+          w[i][k] = make_uint2(v.x, v.y);
+          w[i][k + 1 < KS ? k + 1 : k] = make_uint2(v.z, v.w);
+        }
+      } else {
+#pragma unroll
+        for (int k = 0; k < KS; k++) w[i][k] = in && k * 16 + j * 4 < rank ? __ldg(reinterpret_cast<const uint2*>(at + k * 16 + j * 4)) : make_uint2(0, 0);
+      }
     }
   };
   request(row0);
-  const float scale = p.scale ? __ldg(p.scale + a) : 1.0f;
-  const int n = __popcll(cols);
-  {
-    unsigned long long rest = cols;
-    for (int c = 0; c < n; c++, rest &= rest - 1) {
-      const int col = __ffsll(rest) - 1;
-      for (int r = threadIdx.x; r < 8 * P; r += kThreads) {   // (rows of 8 P, zeros behind the rank)
-        float y = 0.0f;
-        if (r < p.rank)
-#pragma unroll 4
-          for (int part = 0; part < p.parts; part++) y = __fadd_rn(y, __ldcg(p.u + (((size_t)part * p.n_segs + seg) * p.B + col) * p.rank + r));
-        u_s[c * 8 * P + r] = __fmul_rn(scale, y);
+  list_columns(cols, list);
+  // this lane's two of eight columns, at row q; base a tile ahead where these are all
+  size_t col[2];
+  bool has[2];
+  auto columns_at = [&](int c0) {
+#pragma unroll
+    for (int e = 0; e < 2; e++) {
+      has[e] = c0 + 2 * j + e < n;
+      col[e] = ((size_t)(has[e] ? list[c0 + 2 * j + e] : 0) * ld + col_off + q) * SZ;
+    }
+  };
+  columns_at(0);
+  float base[2][4];
+  auto request_base = [&](int row) {
+#pragma unroll
+    for (int e = 0; e < 2; e++) {
+#pragma unroll
+      for (int i = 0; i < 4; i++) base[e][i] = 0.0f;
+      if (has[e] && base0) {
+        const uint8_t* at = base0 + col[e] + (size_t)row * SZ;
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+          if (row + i * 8 + q < n_rows) base[e][i] = load_as<F32>(at + i * 8 * SZ);
       }
     }
+  };
+  request_base(row0);
+  const float scale = p.scale ? __ldg(p.scale + a) : 1.0f;
+  for (int i = threadIdx.x; i < n * R; i += kThreads) {   // (zeros behind the rank)
+    const int c = i / R, r = i % R;
+    float y = 0.0f;
+    if (r < rank) {
+      const float* u = p.u + ((size_t)s.u_seg * p.B + list[c]) * rank + r;
+#pragma unroll 4
+      for (int part = 0; part < p.parts; part++) y = __fadd_rn(y, __ldcg(u + (size_t)part * p.u_segs * p.B * rank));
+    }
+    uint16_t o[3];
+    split3(__fmul_rn(scale, y), o);
+#pragma unroll
+    for (int t = 0; t < 3; t++) u_s[(size_t)t * n * R + i] = o[t];
   }
   __syncthreads();
-#pragma unroll 1
-  for (int row = row0; row < row_end; row += M * kThreads) {
-    uint4 now[M][P];
-    float base_now[M];
+  uint2 u[3][KS];   // operand B of eight columns
+  auto columns_from = [&](int c0) {
 #pragma unroll
-    for (int m = 0; m < M; m++) {
-      base_now[m] = base[m];
+    for (int t = 0; t < 3; t++)
 #pragma unroll
-      for (int i = 0; i < P; i++) now[m][i] = w[m][i];
-    }
-    if (row + M * kThreads < row_end) request(row + M * kThreads);
-    unsigned long long rest = cols;
-#pragma unroll 1
-    for (int c = 0; c < n; c++, rest &= rest - 1) {
-      float u[8];
-      *reinterpret_cast<float4*>(u) = *reinterpret_cast<const float4*>(u_s + c * 8 * P + piece * 8);
-      *reinterpret_cast<float4*>(u + 4) = *reinterpret_cast<const float4*>(u_s + c * 8 * P + piece * 8 + 4);
-      const size_t col = (size_t)(__ffsll(rest) - 1) * s.ld_out + s.col_off;
-#pragma unroll
-      for (int m = 0; m < M; m++) {
-        float y[P];
-#pragma unroll
-        for (int i = 0; i < P; i++) {
-          float v[8];
-          unpack8(now[m][i], v);
-          y[i] = __fmul_rn(v[0], u[0]);
-#pragma unroll
-          for (int e = 1; e < 8; e++) y[i] = fmaf(v[e], u[e], y[i]);
-        }
-        // the lanes of a row: a lane keeps the half of its sums that its bit of `piece` says and gets the partner's
-#pragma unroll
-        for (int half = P / 2, bit = 1; half >= 1; half >>= 1, bit <<= 1) {
-          const bool upper = piece & bit;
-#pragma unroll
-          for (int i = 0; i < half; i++) {
-            const float send = upper ? y[i] : y[i + half], keep = upper ? y[i + half] : y[i];
-            y[i] = __fadd_rn(keep, __shfl_xor_sync(0xffffffffu, send, bit));
-          }
-        }
-        const int r = row + m * kThreads + my_row;
-        if (r < s.n_rows) store_out(s, col + r, __fadd_rn(c == 0 ? base_now[m] : load_base(s, col + r), y[0]));
+      for (int k = 0; k < KS; k++) {
+        const int r = WIDE ? (k >> 1) * 32 + j * 8 + (k & 1) * 4 : k * 16 + j * 4;
+        u[t][k] = c0 + q < n ? *reinterpret_cast<const uint2*>(u_s + ((size_t)t * n + c0 + q) * R + r) : make_uint2(0, 0);
       }
+  };
+  columns_from(0);
+#pragma unroll 1
+  for (int row = row0; row < row_end; row += kThreads) {
+#pragma unroll 1
+    for (int c0 = 0; c0 < n; c0 += 8) {
+      if (n > 8) {
+        columns_from(c0);
+        columns_at(c0);
+        request_base(row);
+      }
+      float d[2][4];
+#pragma unroll
+      for (int t = 0; t < 2; t++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) d[t][e] = 0.0f;
+#pragma unroll
+      for (int part = 2; part >= 0; part--)   // the smallest first
+#pragma unroll
+        for (int k = 0; k < KS; k++)
+#pragma unroll
+          for (int t = 0; t < 2; t++) mma_bf16(d[t], w[2 * t][k].x, w[2 * t + 1][k].x, w[2 * t][k].y, w[2 * t + 1][k].y, u[part][k].x, u[part][k].y);
+      float now[2][4];
+#pragma unroll
+      for (int e = 0; e < 2; e++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) now[e][i] = __fadd_rn(base[e][i], d[i >> 1][(i & 1) * 2 + e]);
+      if (c0 + 8 >= n && row + kThreads < row_end) {   // (the last use of these weights)
+        request(row + kThreads);
+        if (n <= 8) request_base(row + kThreads);
+      }
+#pragma unroll
+      for (int e = 0; e < 2; e++)
+        if (has[e]) {
+          uint8_t* at = out0 + col[e] + (size_t)row * SZ;
+#pragma unroll
+          for (int i = 0; i < 4; i++)
+            if (row + i * 8 + q < n_rows) store_as<F32>(at + i * 8 * SZ, now[e][i]);
+        }
     }
   }
 }
 
-template <int P, int M>
-int32_t launch_expand_as(LoraParams& p, int per) {
+// A CTA takes one tile where there are few, else as many as leave eight CTAs an SM.
+template <int KS, bool WIDE, bool F32>
+int32_t launch_expand_as(LoraParams& p) {
+  long long tiles = 0;
+  for (int i = 0; i < p.n_segs; i++) tiles += (p.segs[i].n_rows + kThreads - 1) / kThreads;
+  p.per = (int)std::max(1ll, std::min(16ll, tiles * std::min(p.B, p.n_adapters) / (8 * bk_ctx().sm_count)));
   int ctas = 0;
-  p.per = per;
   for (int i = 0; i < p.n_segs; i++) {
     p.segs[i].tile0 = ctas;
-    ctas += (p.segs[i].n_rows + per * M * kThreads - 1) / (per * M * kThreads);
+    ctas += (p.segs[i].n_rows + p.per * kThreads - 1) / (p.per * kThreads);
   }
-  BK_CUDA(bk_launch_pdl(lora_expand_kernel<P, M>, dim3(ctas, p.B), dim3(kThreads), (size_t)p.B * 8 * P * 4, p));
+  const size_t smem = (size_t)3 * p.B * KS * 16 * 2;
+  static bool configured = false;
+  if (!configured) {
+    BK_CUDA(cudaFuncSetAttribute(lora_expand_kernel<KS, WIDE, F32>, cudaFuncAttributeMaxDynamicSharedMemorySize, 3 * kMaxB * KS * 16 * 2));
+    configured = true;
+  }
+  BK_CUDA(bk_launch_pdl(lora_expand_kernel<KS, WIDE, F32>, dim3(ctas, p.B), dim3(kThreads), smem, p));
   BK_CHECK_LAUNCH();
   return BK_OK;
 }
-// A CTA takes one tile where there are few, else as many as leave eight CTAs an SM.
-template <int P>
-int32_t launch_expand(LoraParams& p) {
-  long long tiles = 0;
-  for (int i = 0; i < p.n_segs; i++) tiles += (p.segs[i].n_rows + kThreads - 1) / kThreads;
-  const long long each = tiles * std::min(p.B, p.n_adapters) / (8 * bk_ctx().sm_count);
-  constexpr int M = P >= 4 ? 1 : 4 / P;
-  if (each < M) return launch_expand_as<P, 1>(p, 1);
-  return launch_expand_as<P, M>(p, (int)std::min(16ll, each / M));
+// The segments of one type at a time: a launch for each that there is.
+template <int KS, bool WIDE>
+int32_t launch_expand(const LoraParams& all) {
+  for (int f32 = 0; f32 < 2; f32++) {
+    LoraParams p = all;
+    int n = 0;
+    for (int i = 0; i < all.n_segs; i++)
+      if (all.segs[i].f32 == f32) {
+        p.segs[n] = all.segs[i];
+        p.segs[n++].u_seg = i;
+      }
+    p.n_segs = n;
+    if (n == 0) continue;
+    const int32_t rc = f32 ? launch_expand_as<KS, WIDE, true>(p) : launch_expand_as<KS, WIDE, false>(p);
+    if (rc) return rc;
+  }
+  return BK_OK;
+}
+template <int MT>
+int32_t launch_shrink(LoraParams& p) {
+  BK_CUDA(bk_launch_pdl(lora_shrink_kernel<MT>, dim3(p.parts, p.B, p.n_segs), dim3(kThreads), 0, p));
+  BK_CHECK_LAUNCH();
+  return BK_OK;
 }
 
 }  // namespace
@@ -311,7 +353,7 @@ int32_t bkLora(const bkLoraArgs* args) {
   LoraParams p;
   memset(&p, 0, sizeof(p));
   p.x = bk_ptr<uint16_t>(a.x); p.ids = bk_ptr<int>(a.ids); p.scale = bk_ptr<float>(a.scale); p.u = bk_ptr<float>(a.scratch);
-  p.K = a.K; p.B = a.B; p.n_segs = a.n_segs; p.rank = a.rank; p.n_adapters = a.n_adapters;
+  p.K = a.K; p.B = a.B; p.n_segs = p.u_segs = a.n_segs; p.rank = a.rank; p.n_adapters = a.n_adapters;
   for (int i = 0; i < a.n_segs; i++) {
     const bkLoraSeg& s = a.segs[i];
     BK_ARG(s.n_rows > 0 && s.n_rows < (1 << 30) && s.col_off >= 0 && (long long)s.col_off + s.n_rows <= s.ld_out, "bkLora: segment %d: n_rows=%d col_off=%d ld_out=%d", i, s.n_rows, s.col_off,
@@ -319,17 +361,20 @@ int32_t bkLora(const bkLoraArgs* args) {
     BK_ARG(s.dtype == BK_DTYPE_F32 || s.dtype == BK_DTYPE_BF16, "bkLora: segment %d: dtype %d", i, s.dtype);
     const uint64_t mask = s.dtype == BK_DTYPE_F32 ? 3 : 1;
     BK_ARG(s.A && s.Bm && s.out && ((s.A | s.Bm) & 15) == 0 && ((s.base | s.out) & mask) == 0, "bkLora: segment %d: A and Bm must be 16-byte aligned, out non-null, base and out aligned to their type", i);
-    p.segs[i] = LoraSeg{bk_ptr<uint16_t>(s.A), bk_ptr<uint16_t>(s.Bm), bk_ptr<void>(s.base), bk_ptr<void>(s.out), s.n_rows, s.dtype == BK_DTYPE_F32, s.ld_out, s.col_off, 0};
+    p.segs[i] = LoraSeg{bk_ptr<uint16_t>(s.A), bk_ptr<uint16_t>(s.Bm), bk_ptr<void>(s.base), bk_ptr<void>(s.out), s.n_rows, s.dtype == BK_DTYPE_F32, s.ld_out, s.col_off, i, 0};
   }
-  // Parts of K, multiples of 256: about four CTAs an SM, but no more than 512 partial rows of u for an expanding CTA to add up, and x in its place.
-  const int units = (a.K + 255) / 256, least = (units + kChunk / 256 - 1) / (kChunk / 256);
-  int parts = std::max(1, std::min(units, 4 * bk_ctx().sm_count / (a.n_segs * std::min(a.B, a.n_adapters))));
-  parts = std::max(least, std::min(parts, std::max(1, 512 / a.B)));
+  // Parts of K, multiples of 256 (32 a warp): about four CTAs an SM, no more than 16 for the expanding launch to add up.
+  const int units = (a.K + 255) / 256;
+  const int parts = std::max(1, std::min({units, 16, 4 * bk_ctx().sm_count / (a.n_segs * std::min(a.B, a.n_adapters))}));
   p.chunk = (units + parts - 1) / parts * 256;
   p.parts = (a.K + p.chunk - 1) / p.chunk;
-  BK_CUDA(bk_launch_pdl(lora_shrink_kernel, dim3(p.parts, a.B, a.n_segs), dim3(kThreads), 0, p));
-  BK_CHECK_LAUNCH();
-  return a.rank <= 8 ? launch_expand<1>(p) : a.rank <= 16 ? launch_expand<2>(p) : a.rank <= 32 ? launch_expand<4>(p) : a.rank <= 64 ? launch_expand<8>(p) : launch_expand<16>(p);
+  const int32_t rc = a.rank <= 16 ? launch_shrink<1>(p) : a.rank <= 32 ? launch_shrink<2>(p) : a.rank <= 64 ? launch_shrink<4>(p) : launch_shrink<8>(p);
+  if (rc) return rc;
+  const bool wide = a.rank % 32 == 0;
+  return a.rank <= 16   ? launch_expand<1, false>(p)
+         : a.rank <= 32 ? (wide ? launch_expand<2, true>(p) : launch_expand<2, false>(p))
+         : a.rank <= 64 ? (wide ? launch_expand<4, true>(p) : launch_expand<4, false>(p))
+                        : (wide ? a.rank == 96 ? launch_expand<6, true>(p) : launch_expand<8, true>(p) : launch_expand<8, false>(p));
 }
 
 }  // extern "C"
