@@ -674,19 +674,21 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
         // queries into tensor memory, half of the dims a group (the MMAs that read the ones before have completed: their output was there)
         bar_wait_warp(smem_u32(&q_here), pieces & 1, P.status, dead);
         tc_after();
-        if (warp_on) {
+        // Lanes without a row get zeros: their scores are then zeros, which read as probabilities are zeros too, and zeros cost the tensor
+        // cores less power than what was there.
 #pragma unroll
-          for (int d = group * (HD / 128); d < (group + 1) * (HD / 128); d++) {
-            uint32_t v[32];
+        for (int d = group * (HD / 128); d < (group + 1) * (HD / 128); d++) {
+          uint32_t v[32];
 #pragma unroll
-            for (int y = 0; y < 8; y++) {
-              const uint4 w = *reinterpret_cast<const uint4*>(q_s + d * (kRows * 128) + i_row * 128 + ((y ^ (i_row & 7)) << 4));   // (as TMA swizzles them)
-              v[4 * y] = w.x; v[4 * y + 1] = w.y; v[4 * y + 2] = w.z; v[4 * y + 3] = w.w;
-            }
-            tmem_st32(lanes + C::kQ + d * 32, v);
+          for (int y = 0; y < 8; y++) {
+            uint4 w = make_uint4(0, 0, 0, 0);
+            if (mine) w = *reinterpret_cast<const uint4*>(q_s + d * (kRows * 128) + i_row * 128 + ((y ^ (i_row & 7)) << 4));   // (as TMA swizzles them)
+            v[4 * y] = w.x; v[4 * y + 1] = w.y; v[4 * y + 2] = w.z; v[4 * y + 3] = w.w;
           }
-          tmem_wait_st();
+          __syncwarp();
+          tmem_st32(lanes + C::kQ + d * 32, v);
         }
+        tmem_wait_st();
         tc_before();
         __syncwarp();
         if (lane == 0) {
