@@ -147,23 +147,35 @@ BK_DEVINL void piece_of(int s, int n, int u0, int u1, int* t0, int* t1) {
 
 // one CTA
 constexpr int kPrepThreads = 256, kPlanned = 1024;   // jobs whose starts fit in shared memory
+// SMEM: no more than kPlanned jobs, whose lines are worked on in shared memory; otherwise in the records themselves.  What it takes is on every
+// call's way: a chain of loads from L2 costs 0.6 us a link.
+template <bool SMEM>
 BK_DEVINL void plan_jobs(const PagedParams& p, const Layout& L, uint8_t* scratch) {
-  __shared__ int warp_s[kPrepThreads / 32][2], starts_s[kPlanned + 1], bounds_s[kPrepThreads + 1];
+  __shared__ int warp_s[kPrepThreads / 32][2], starts_s[SMEM ? kPlanned + 1 : 1], ends_s[SMEM ? kPlanned : 1], bounds_s[kPrepThreads + 1];
   int4* jobs = jobs_of(L, scratch);
   int4* pieces = pieces_of(L, scratch);
   const int n = L.n_p + L.n_s, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int tiles_p = (L.P + kTile - 1) / kTile, all_ctas = min(L.ctas, kPrepThreads);
-  const bool in_smem = n <= kPlanned, apart = L.mt_p > 1 && L.n_p > 0 && L.n_p <= all_ctas / 2 && L.n_p * tiles_p >= all_ctas;   // common keys apart from the line
+  const bool apart = L.mt_p > 1 && L.n_p > 0 && L.n_p <= all_ctas / 2 && L.n_p * tiles_p >= all_ctas;   // common keys apart from the line
+  if (SMEM) {
+    for (int j = threadIdx.x; j < n; j += kPrepThreads) ends_s[j] = keys_end(p, L, job_of(p, L, j));
+    __syncthreads();
+  }
+  auto units_of = [&](int j, int end, int* tiles) {
+    *tiles = apart && j < L.n_p ? 0 : tiles_of(L, j, end);
+    return *tiles ? *tiles + kOverhead : 0;
+  };
   // a thread has `per` jobs in a row
   const int per = (n + kPrepThreads - 1) / kPrepThreads, j0 = threadIdx.x * per, j1 = min(n, j0 + per);
   int mine = 0, tiles_mine = 0;
   for (int j = j0; j < j1; j++) {
-    const int end = keys_end(p, L, job_of(p, L, j)), tiles = tiles_of(L, j, end);
-    *reinterpret_cast<int2*>(jobs + j) = make_int2(mine, end);   // .x: within the thread, for now
-    if (!apart || j >= L.n_p) {
-      mine += tiles ? tiles + kOverhead : 0;
-      tiles_mine += tiles;
-    }
+    const int end = SMEM ? ends_s[j] : keys_end(p, L, job_of(p, L, j));
+    int tiles;
+    const int units = units_of(j, end, &tiles);
+    if (SMEM) starts_s[j] = mine;
+    else *reinterpret_cast<int2*>(jobs + j) = make_int2(mine, end);   // .x: within the thread, for now
+    mine += units;
+    tiles_mine += tiles;
   }
   int v = mine;
 #pragma unroll
@@ -185,13 +197,12 @@ BK_DEVINL void plan_jobs(const PagedParams& p, const Layout& L, uint8_t* scratch
     tiles_all += warp_s[w][1];
   }
   for (int j = j0; j < j1; j++) {
-    const int s = jobs[j].x + before;
-    jobs[j].x = s;
-    if (in_smem) starts_s[j] = s;
+    if (SMEM) starts_s[j] += before;
+    else jobs[j].x += before;
   }
   if (threadIdx.x == 0) {
-    jobs[n].x = units;
-    if (in_smem) starts_s[n] = units;
+    if (SMEM) starts_s[n] = units;
+    else jobs[n].x = units;
   }
   // ranges of a job over common keys: so many that the longest range and the line's pieces come out equal, as far as whole numbers let them
   int ranges = 0;
@@ -199,16 +210,19 @@ BK_DEVINL void plan_jobs(const PagedParams& p, const Layout& L, uint8_t* scratch
     unsigned int best = 0xffffffffu;
     for (int r = lane + 1; r <= min(all_ctas / L.n_p, tiles_p); r += 32) {
       const int others = all_ctas - L.n_p * r;
-      const float cost = fmaxf((float)((tiles_p + r - 1) / r), units ? others ? (float)units / others : 4e6f : 0.0f);
+      const float cost = fmaxf((float)((tiles_p + r - 1) / r), units ? others ? __fdividef((float)units, (float)others) : 4e6f : 0.0f);
       best = min(best, (unsigned int)fminf(cost * 4.0f, 4e6f) << 8 | r);   // (r below 256)
     }
     ranges = __reduce_min_sync(0xffffffffu, best) & 255;
   }
   const int c0 = L.n_p * ranges, C = max(c0 + 1, min(all_ctas, c0 + tiles_all));   // the line's CTAs: from c0 on, and every one of them has a tile to do
-  // (a quotient that is no whole number is at least 1 / C away from one, so the double below it is too)
-  for (int c = threadIdx.x; c <= C; c += kPrepThreads) bounds_s[c] = c <= c0 ? 0 : (int)((double)units * (c - c0) / (C - c0));
+  for (int c = threadIdx.x; c <= C; c += kPrepThreads) {
+    // (a quotient that is no whole number is at least 1 / C away from one, so the double below it is too)
+    const int share = units < (1 << 23) ? (int)((unsigned int)units * (unsigned int)max(0, c - c0) / (unsigned int)(C - c0)) : (int)((double)units * (c - c0) / (C - c0));
+    bounds_s[c] = c <= c0 ? 0 : share;
+  }
   __syncthreads();
-  auto start = [&](int j) { return in_smem ? starts_s[j] : jobs[j].x; };
+  auto start = [&](int j) { return SMEM ? starts_s[j] : jobs[j].x; };
   for (int c = threadIdx.x; c < L.ctas; c += kPrepThreads) {
     const int u0 = c < C ? bounds_s[c] : 0, u1 = c < C ? bounds_s[c + 1] : 0;
     int lo = 0, hi = n;   // the last job that starts at u0 or before
@@ -218,9 +232,15 @@ BK_DEVINL void plan_jobs(const PagedParams& p, const Layout& L, uint8_t* scratch
       else hi = mid;
     }
     // CTA c < c0: range r of job (KV head, row tile), the row tiles next to one another
-    const int group = c / L.mt_p, r = apart ? group % ranges : 0;
-    pieces[2 * c] = make_int4(u0, u1, lo, c < c0 ? group / ranges * L.mt_p + c % L.mt_p : -1);
-    pieces[2 * c + 1] = make_int4(start(lo), jobs[lo].y, c < c0 ? tiles_p * r / ranges : 0, c < c0 ? tiles_p * (r + 1) / ranges : 0);
+    int job = -1, t0 = 0, t1 = 0;
+    if (c < c0) {
+      const int group = c / L.mt_p, kvh = group / ranges, r = group - kvh * ranges;
+      job = kvh * L.mt_p + c - group * L.mt_p;
+      t0 = tiles_p * r / ranges;
+      t1 = tiles_p * (r + 1) / ranges;
+    }
+    pieces[2 * c] = make_int4(u0, u1, lo, job);
+    pieces[2 * c + 1] = make_int4(start(lo), SMEM ? ends_s[lo] : jobs[lo].y, t0, t1);
   }
   auto cta_at = [&](int unit) {   // the CTA that has it
     int lo = c0, hi = C;
@@ -232,11 +252,19 @@ BK_DEVINL void plan_jobs(const PagedParams& p, const Layout& L, uint8_t* scratch
     return lo;
   };
   for (int j = threadIdx.x; j < n; j += kPrepThreads) {
-    const int s = start(j), s1 = start(j + 1), first = cta_at(s + kOverhead);
-    *reinterpret_cast<int2*>(&jobs[j].z) = apart && j < L.n_p ? make_int2(j / L.mt_p * ranges * L.mt_p + j % L.mt_p, ranges | L.mt_p << 16)
-                                           : s1 > s          ? make_int2((j < L.n_p ? j : j - L.n_p) + first, (cta_at(s1 - 1) - first + 1) | 1 << 16)
-                                                             : make_int2(0, 0);
+    const int s = start(j), s1 = start(j + 1);
+    int2 slots = make_int2(0, 0);
+    if (apart && j < L.n_p) {
+      const int kvh = j / L.mt_p;
+      slots = make_int2(kvh * ranges * L.mt_p + j - kvh * L.mt_p, ranges | L.mt_p << 16);
+    } else if (s1 > s) {
+      const int first = cta_at(s + kOverhead);
+      slots = make_int2((j < L.n_p ? j : j - L.n_p) + first, (cta_at(s1 - 1) - first + 1) | 1 << 16);
+    }
+    if (SMEM) jobs[j] = make_int4(s, ends_s[j], slots.x, slots.y);
+    else *reinterpret_cast<int2*>(&jobs[j].z) = slots;
   }
+  if (SMEM && threadIdx.x == 0) jobs[n] = make_int4(units, 0, 0, 0);
 }
 
 // row i of a job's tile -> token row e and query head of its group; false past the last
@@ -263,7 +291,8 @@ __global__ void __launch_bounds__(kPrepThreads) paged_prepare_kernel(const Paged
   bk_pdl_trigger();
   bk_pdl_wait();
   if (blockIdx.x == 0) {   // (first: it takes longest)
-    plan_jobs(p, L, scratch);
+    if (L.n_p + L.n_s <= kPlanned) plan_jobs<true>(p, L, scratch);
+    else plan_jobs<false>(p, L, scratch);
     return;
   }
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -271,33 +300,41 @@ __global__ void __launch_bounds__(kPrepThreads) paged_prepare_kernel(const Paged
   const int item = (blockIdx.x - 1) * (kPrepThreads / 32) + warp;
   if (item >= p.T * p.B * heads) return;
   const int e = item / heads, h = item - e * heads, t = e / p.B, b = e - t * p.B;
-  const int at = row_of(p, b, t);
-  if (at < 0) return;
   const bool is_q = h < p.Hq;
   const int kvh = h - p.Hq, G = p.Hq / p.Hkv;
+  // what does not wait for the token's row first
   const uint16_t* src = is_q ? p.qg + ((size_t)e * p.Hq + h) * (p.fused ? 2 : 1) * HD : p.k + ((size_t)e * p.Hkv + kvh) * HD;
-  uint16_t* dst = p.q + (((size_t)(h / G) * p.B + b) * p.T + t) * G * HD + (size_t)(h % G) * HD;
+  float x[PER], w[PER];
+  uint2 v[PER / 4];
+  load_bf16(src + lane * PER, x);
+  if (p.fused) load_bf16((is_q ? p.q_norm_w : p.k_norm_w) + lane * PER, w);
   if (!is_q) {
+#pragma unroll
+    for (int i = 0; i < PER / 4; i++) v[i] = *reinterpret_cast<const uint2*>(p.v + ((size_t)e * p.Hkv + kvh) * HD + lane * PER + 4 * i);
+  }
+  const int at = row_of(p, b, t);
+  if (at < 0) return;
+  uint16_t* dst;
+  if (is_q) {
+    const int head = h / G;
+    dst = p.q + (((size_t)head * p.B + b) * p.T + t) * G * HD + (size_t)(h - head * G) * HD;
+  } else {
     const int page = p.table[(size_t)b * p.max_pages + at / p.page_rows];
     if (page < 0 || page >= p.n_pages) return;
     const size_t row = (((size_t)page * p.Hkv + kvh) * p.page_rows + at % p.page_rows) * HD;
     dst = p.k_pages + row;
-    const uint16_t* vs = p.v + ((size_t)e * p.Hkv + kvh) * HD;
 #pragma unroll
-    for (int i = 0; i < PER; i += 4) *reinterpret_cast<uint2*>(p.v_pages + row + lane * PER + i) = *reinterpret_cast<const uint2*>(vs + lane * PER + i);
+    for (int i = 0; i < PER / 4; i++) *reinterpret_cast<uint2*>(p.v_pages + row + lane * PER + 4 * i) = v[i];
   }
-  float x[PER];
-  load_bf16(src + lane * PER, x);
   if (p.fused) {
-    float w[PER], sum = 0.0f;
-    load_bf16((is_q ? p.q_norm_w : p.k_norm_w) + lane * PER, w);
+    const float *cr = p.cos_t + (size_t)at * p.rot_half, *sr = p.sin_t + (size_t)at * p.rot_half;
+    float sum = 0.0f;
 #pragma unroll
     for (int i = 0; i < PER; i++) sum = fmaf(x[i], x[i], sum);
     const float rstd = bk_rcp_sqrt(__fadd_rn(__fdiv_rn(bk_warp_sum(sum), (float)HD), p.eps));
 #pragma unroll
     for (int i = 0; i < PER; i++) y_s[warp][lane * PER + i] = __fmul_rn(__fmul_rn(x[i], rstd), __fadd_rn(1.0f, w[i]));
     __syncwarp();
-    const float *cr = p.cos_t + (size_t)at * p.rot_half, *sr = p.sin_t + (size_t)at * p.rot_half;
 #pragma unroll
     for (int i = 0; i < PER; i++) {
       const int d = lane * PER + i;
