@@ -429,6 +429,15 @@ BK_DEVINL float exp2_approx(float x) {   // 2^x to 2 ulp or so; 2^-inf = 0
   return y;
 }
 
+// two bf16 values, zeros in the place of those that are not finite
+BK_DEVINL uint32_t finite_pair(uint32_t v) {
+  return ((v & 0x7f80u) == 0x7f80u ? 0u : v & 0xffffu) | ((v & 0x7f800000u) == 0x7f800000u ? 0u : v & 0xffff0000u);
+}
+// an f32 sum, plus a bf16 value if that is not finite
+BK_DEVINL uint32_t odd_value(uint32_t sum, uint16_t v) {
+  return (v & 0x7f80u) == 0x7f80u ? __float_as_uint(__fadd_rn(__uint_as_float(sum), bk_bf16_to_f32(v))) : sum;
+}
+
 // positions in the stream of a piece's tiles: K0, K1, V0, K2, V1, ..., V(n-1)
 BK_DEVINL int stream_v(int i, int n) { return i < n - 1 ? 2 * i + 2 : 2 * n - 1; }
 
@@ -436,6 +445,7 @@ template <int kStages>
 struct TileShared {   // behind the tiles
   uint64_t full[kStages], empty[kStages], q_here, q_empty, q_full, s_full[2], p_full[2], o_full[2];
   float m_s[2][2][kRows];   // [tile & 1][half of the keys]: largest score
+  int odd_from[3], odd_to[3];   // [piece mod 3]: keys between which values were not finite and were taken out, see there
   uint32_t tmem_slot;
   int dead;
 };
@@ -472,6 +482,10 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     dead_s = 0;
+    for (int i = 0; i < 3; i++) {
+      sh.odd_from[i] = 0x7fffffff;
+      sh.odd_to[i] = -1;
+    }
     for (int i = 0; i < C::kStages; i++) {
       mbar_init(smem_u32(full + i), 1);
       mbar_init(smem_u32(empty + i), 1);
@@ -708,6 +722,25 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
         if (mine) limit = min(row_of(p, b, t) + 1, key1);
         __syncwarp();
         const bool warp_on = __any_sync(0xffffffffu, mine);
+        // Tiles from this key on have a row that does not see all of them.  There a value that is not finite must not meet a zero probability (0 * inf):
+        // it is taken out of the tile, and given back at the end to the rows that see it.
+        int seen_by_all = key1;
+        if (q.seq >= 0) {
+          const int first = q.mt * kRows / (p.Hq / p.Hkv), count = p.n_new ? min(p.n_new[q.seq], p.T) : p.T;
+          seen_by_all = max(0, p.lens[q.seq] - count + first) + 1;
+        } else {
+          int uneven;
+          asm volatile("{ .reg .pred a, b; setp.ne.s32 a, %1, 0; barrier.cta.red.or.pred b, 5, 256, a; selp.s32 %0, 1, 0, b; }"
+                       : "=r"(uneven)
+                       : "r"((int)(mine && limit > 0 && limit < key1))
+                       : "memory");
+          if (uneven) seen_by_all = 0;
+        }
+        const int odd = pieces % 3;
+        if (threadIdx.x == 0) {   // the next piece's; who read these two pieces ago has moved its queries since
+          sh.odd_from[(pieces + 1) % 3] = 0x7fffffff;
+          sh.odd_to[(pieces + 1) % 3] = -1;
+        }
         // queries into tensor memory, half of the dims a group (the MMAs that read the ones before have completed: their output was there)
         bar_wait_warp(smem_u32(&q_here), pieces & 1, P.status, dead);
         tc_after();
@@ -738,7 +771,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
           const uint32_t s_at = lanes + C::kS + (tile & 1) * kTile;
           bar_wait_warp(smem_u32(s_full + (tile & 1)), (tile >> 1) & 1, P.status, dead);
           tc_after();
-          if (there < kTile) {   // values past the end count as zeros, whatever the page holds there
+          const bool mixed = tile_key + there > seen_by_all;
+          if (there < kTile || mixed) {   // values past the end count as zeros, whatever the page holds there
             const int v_pos = stream + stream_v(i, n), v_stage = v_pos % C::kStages;
             bar_wait_warp(smem_u32(full + v_stage), (v_pos / C::kStages) & 1, P.status, dead);
             uint8_t* v_at = ring + (size_t)v_stage * C::kStage;
@@ -746,6 +780,17 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
               const int row = there + y / (HD / 8), piece = y % (HD / 8);
               *reinterpret_cast<uint4*>(v_at + (piece >> 3) * (kTile * 128) + row * 128 + (piece & 7) * 16) = make_uint4(0, 0, 0, 0);
             }
+            if (mixed)
+              for (int y = threadIdx.x; y < there * (HD / 8); y += 256) {
+                const int row = y / (HD / 8), piece = y % (HD / 8);
+                uint4* at = reinterpret_cast<uint4*>(v_at + (piece >> 3) * (kTile * 128) + row * 128 + (piece & 7) * 16);
+                const uint4 v = *at, w = make_uint4(finite_pair(v.x), finite_pair(v.y), finite_pair(v.z), finite_pair(v.w));
+                if (((v.x ^ w.x) | (v.y ^ w.y) | (v.z ^ w.z) | (v.w ^ w.w)) != 0) {
+                  *at = w;
+                  atomicMin(&sh.odd_from[odd], tile_key + row);
+                  atomicMax(&sh.odd_to[odd], tile_key + row);
+                }
+              }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
           }
@@ -828,6 +873,14 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
             uint32_t o[32];
             tmem_ld32(lanes + C::kO + d * 32, o);
             if (mine) {
+              const int last = min(limit - 1, *reinterpret_cast<volatile int*>(&sh.odd_to[odd]));
+              for (int key = *reinterpret_cast<volatile int*>(&sh.odd_from[odd]); key <= last; key++) {   // (nearly always none)
+                const int page = __ldg(p.table + (size_t)max(q.seq, 0) * p.max_pages + key / p.page_rows);
+                const uint16_t* v = p.v_pages + (((size_t)page * p.Hkv + q.kvh) * p.page_rows + key % p.page_rows) * HD + d * 32;
+                if (page >= 0 && page < p.n_pages)
+#pragma unroll
+                  for (int y = 0; y < 32; y++) o[y] = odd_value(o[y], v[y]);
+              }
 #pragma unroll
               for (int y = 0; y < 32; y += 4) o_to[(size_t)(d * 8 + y / 4) * rows] = make_uint4(o[y], o[y + 1], o[y + 2], o[y + 3]);
             }

@@ -470,6 +470,44 @@ def test_attention_where_nothing_is_there(bk):
     c.check()
 
 
+@pytest.mark.parametrize("HD,rows", [(128, 16), (256, 64)])
+def test_attention_keeps_what_is_not_finite_to_the_tokens_that_see_it(bk, HD, rows):
+    """Infinities and NaN in keys and values of later tokens, and of common rows behind a short sequence's end, do not reach a token; those it
+    sees make its dims infinite or NaN."""
+    T = 12
+    c = Case(51, 2, T, 40, [30, 12], HD=HD, Hq=6, Hkv=1, rows=rows, fused=False, gate=False)
+    c.v[7 * 2 + 0, 0, 3], c.v[7 * 2 + 0, 0, HD - 1], c.v[11 * 2 + 0, 0, 5], c.k[9 * 2 + 1, 0, 1] = 0x7F80, 0xFF80, 0x7FC0, 0x7FC0
+    with np.errstate(invalid="ignore"):
+        want, kp, vp = c.want()
+    ops.paged_attn(c.args())
+    assert R.cuSync() == 0, R.last_error()
+    got = val(c.out.download(np.uint16, (T * 2, c.Hq, HD))).reshape(T, 2, c.Hq, HD)
+    want = want.reshape(T, 2, c.Hq, HD)
+    odd = np.zeros(want.shape, bool)
+    odd[7:, 0, :, 3] = odd[7:, 0, :, HD - 1] = True
+    odd[11:, 0, :, 5] = True
+    odd[9:, 1] = True                                            # a NaN key: every later token of that sequence, all dims
+    assert np.array_equal(~np.isfinite(want), odd)               # (the plain form says so too)
+    assert np.array_equal(~np.isfinite(got), odd)
+    assert np.array_equal(np.isnan(got[odd]), np.isnan(want[odd])) and (got[7:, 0, :, 3] == np.inf).all() and (got[7:, 0, :, HD - 1] == -np.inf).all()
+    vmax = np.abs(val(vp)[np.isfinite(val(vp))]).max()
+    assert (np.abs(got[~odd] - want[~odd]) <= 2.0 ** -8 * np.abs(want[~odd]) + 2.0 ** -13 * vmax).all()
+    # common rows behind the end of a short sequence
+    c = Case(52, 3, 1, 128, [10, 0, 3], HD=HD, fused=False, gate=False, rows=rows)
+    c.lens = np.array([138, 50, 131], np.int32)
+    page, row = c.table[0, 100 // rows], 100 % rows
+    c.vp[page, 0, row, 2] = 0x7FC0
+    with np.errstate(invalid="ignore"):
+        want, kp, vp = c.want()
+    ops.paged_attn(c.args())
+    assert R.cuSync() == 0, R.last_error()
+    got = val(c.out.download(np.uint16, (3, c.Hq, HD)))
+    odd = np.zeros(want.shape, bool)
+    odd[[0, 2], :, 2] = True
+    assert np.array_equal(~np.isfinite(want), odd) and np.array_equal(~np.isfinite(got), odd)
+    assert (np.abs(got[~odd] - want[~odd]) <= 2.0 ** -8 * np.abs(want[~odd]) + 2.0 ** -13 * np.abs(val(vp)[np.isfinite(val(vp))]).max()).all()
+
+
 def test_attention_over_scores_of_all_sizes(bk):
     """Large scores (softmax of one row), a running maximum that rises from tile to tile, equal scores."""
     Case(11, 2, 1, 128, [100, 300], HD=128, std=6.0, fused=False).check()
