@@ -290,6 +290,59 @@ export function runGraphDecode(model: BunkerModel, prompt: number[], genLen: num
   return out;
 }
 
+/** A cache in pages (bkPages, 88 bytes): the pool, its tables, lengths and reference counts are device buffers of the caller. */
+export interface Pages {
+  base: bigint; planeBytes: bigint; ref: bigint; table: bigint; lens: bigint; scratch: bigint; scratchBytes: bigint;
+  nPlanes: number; nPages: number; heads: number; pageRows: number; rowBytes: number; nSeqs: number; maxPages: number;
+}
+export function packPages(p: Pages): Buffer {
+  const b = Buffer.alloc(88);
+  [p.base, p.planeBytes, p.ref, p.table, p.lens, p.scratch, p.scratchBytes].forEach((v, i) => b.writeBigUInt64LE(v, 8 * i));
+  [p.nPlanes, p.nPages, p.heads, p.pageRows, p.rowBytes, p.nSeqs, p.maxPages].forEach((v, i) => b.writeInt32LE(v, 56 + 4 * i));
+  return b;
+}
+export function pagesCopy(from: Buffer, to: Buffer, src: bigint, dst: bigint, n: number): void { check(cu().bkPagesCopy(from, to, src, dst, n), "bkPagesCopy"); }
+export function pagesFork(pool: Buffer, src: bigint, dst: bigint, n: number, ok = 0n): void { check(cu().bkPagesFork(pool, src, dst, n, ok), "bkPagesFork"); }
+export function pagesGrow(pool: Buffer, seqs: bigint, add: bigint, n: number, ok = 0n): void { check(cu().bkPagesGrow(pool, seqs, add, n, ok), "bkPagesGrow"); }
+export function pagesFree(pool: Buffer, seqs: bigint, n: number): void { check(cu().bkPagesFree(pool, seqs, n), "bkPagesFree"); }
+export function pagesCompact(pool: Buffer, tableOut: bigint, refOut: bigint, map: bigint, used: bigint): void {
+  check(cu().bkPagesCompact(pool, tableOut, refOut, map, used), "bkPagesCompact");
+}
+
+/** Attention over pages (bkPagedAttnArgs, 184 bytes). */
+export interface PagedAttn {
+  qg: bigint; k?: bigint; v?: bigint; gate?: bigint; qNormW?: bigint; kNormW?: bigint; cosT?: bigint; sinT?: bigint; kPages: bigint; vPages: bigint;
+  table: bigint; lens: bigint; nNew?: bigint; out: bigint; scratch: bigint; scratchBytes: bigint;
+  B: number; T: number; Hq: number; Hkv: number; HD: number; rotHalf?: number; nPages: number; pageRows: number; maxPages: number; prefixRows: number;
+  maxLen: number; fusedNormRope: boolean; scale: number; eps?: number;
+}
+export function pagedAttn(a: PagedAttn): void {
+  const b = Buffer.alloc(184);
+  [a.qg, a.k, a.v, a.gate, a.qNormW, a.kNormW, a.cosT, a.sinT, a.kPages, a.vPages, a.table, a.lens, a.nNew, a.out, a.scratch, a.scratchBytes]
+    .forEach((v, i) => b.writeBigUInt64LE(v ?? 0n, 8 * i));
+  [a.B, a.T, a.Hq, a.Hkv, a.HD, a.rotHalf ?? 0, a.nPages, a.pageRows, a.maxPages, a.prefixRows, a.maxLen, a.fusedNormRope ? 1 : 0]
+    .forEach((v, i) => b.writeInt32LE(v, 128 + 4 * i));
+  b.writeFloatLE(a.scale, 176); b.writeFloatLE(a.eps ?? 1e-6, 180);
+  check(cu().bkPagedAttn(b), "bkPagedAttn");
+}
+
+/** Adapters beside a shared projection (bkLoraArgs, 256 bytes): up to four row segments. */
+export interface LoraSeg { A: bigint; Bm: bigint; base?: bigint; out: bigint; nRows: number; dtype: number; ldOut: number; colOff?: number }
+export interface Lora {
+  K: number; B: number; rank: number; nAdapters: number; x: bigint; ids: bigint; scale?: bigint; scratch: bigint; scratchBytes: bigint; segs: LoraSeg[];
+}
+export function lora(a: Lora): void {
+  const b = Buffer.alloc(256);
+  [a.K, a.B, a.segs.length, a.rank, a.nAdapters].forEach((v, i) => b.writeInt32LE(v, 4 * i));
+  [a.x, a.ids, a.scale ?? 0n, a.scratch, a.scratchBytes].forEach((v, i) => b.writeBigUInt64LE(v, 24 + 8 * i));
+  a.segs.slice(0, 4).forEach((s, i) => {
+    const o = 64 + 48 * i;
+    [s.A, s.Bm, s.base ?? 0n, s.out].forEach((v, k) => b.writeBigUInt64LE(v, o + 8 * k));
+    [s.nRows, s.dtype, s.ldOut, s.colOff ?? 0].forEach((v, k) => b.writeInt32LE(v, o + 32 + 4 * k));
+  });
+  check(cu().bkLora(b), "bkLora");
+}
+
 /** Weight loader's quantiser: f32 / bf16 rows already on the device -> Q4_K rows (prototypes/decode.ts:64-76 uploads bf16). */
 export function quantizeQ4K(x: bigint, dtype: number, nRows: number | bigint, K: number, outQ4K: bigint): void {
   check(cu().bkQuantizeQ4K(x, dtype, BigInt(nRows), K, outQ4K), "bkQuantizeQ4K");

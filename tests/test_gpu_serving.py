@@ -645,6 +645,26 @@ def test_adapters_without_base_or_scale_in_place_and_in_columns(bk):
     assert (np.abs(got - want[0][0]) <= 340 * 2.0 ** -24 * want[0][1]).all()
 
 
+def test_adapters_of_segments_of_both_types(bk):
+    a32, k32, w32, hold32 = lora_case(11, 7, 512, [70, 300], 24, 3, [0, 2, -1, 0, 1, 2, 2], True)
+    a16, k16, w16, hold16 = lora_case(11, 7, 512, [70, 300], 24, 3, [0, 2, -1, 0, 1, 2, 2], False)
+    args = R.bkLoraArgs.from_buffer_copy(a32)
+    args.n_segs = 4
+    for i, s in enumerate((a16.segs[0], a32.segs[0], a16.segs[1], a32.segs[1])):
+        args.segs[i] = s
+    args.x = a16.x                     # (the same draw)
+    nb = ops.lora_scratch_bytes(512, 7, 24, 4)
+    scratch = R.DeviceBuffer(nb)
+    args.scratch, args.scratch_bytes = scratch.ptr, nb
+    ops.lora(args)
+    assert R.cuSync() == 0
+    for keep, want, f32 in ((k16, w16, False), (k32, w32, True)):
+        for (d, out, ld, n), (y, mag) in zip(keep, want):
+            raw = out.download(np.uint32 if f32 else np.uint16, (7, ld))
+            got = raw.view(np.float32).astype(np.float64) if f32 else val(raw)
+            assert (np.abs(got - y) <= 540 * 2.0 ** -24 * mag + (0 if f32 else 2.0 ** -8 * np.abs(y))).all()
+
+
 def test_adapters_keep_infinities_to_their_own_request(bk):
     """A request whose x holds inf or NaN does not reach the others, nor does an adapter that nobody has."""
     args, keep, want, (dx, di, ds, scratch) = lora_case(9, 4, 256, [64], 8, 3, [0, 0, 1, -1], True)
@@ -680,3 +700,63 @@ def test_adapters_refusals(bk):
     with pytest.raises(ValueError):
         ops.lora_args(x=1, K=8, B=1, rank=8, n_adapters=1, ids=1, segs=[], scratch=1, scratch_bytes=1)
     assert R.cuSync() == 0
+
+
+# ---- all of it together ------------------------------------------------------------------
+
+def test_requests_behind_one_prompt(bk):
+    """The example layer: prompt, forks, steps with adapters, dropped requests, compaction.  Sharing changes only the order of sums; compaction
+    changes nothing; and a request's attention is what bkAttnDecode gives over a contiguous cache of the same rows (it rounds q
+    and k after the norm too: 2^-6 of the largest value)."""
+    from bunker_b200 import shared_prompt as S
+    from bunker_b200.model import CONFIG_TINY as cfg
+    w, lora = S.random_layer(cfg, seed=3)
+    n, rows, steps = 5, 75, 3
+    rng = np.random.default_rng(4)
+    x = dev(rnd(rng, rows, cfg.hidden))
+    xs = [dev(rnd(rng, n, cfg.hidden)) for _ in range(steps)]
+    adapters = [0, -1, 2, 1, 0]
+    runs = []
+    for share in (True, False):
+        s = S.SharedPrompt(cfg, w, lora, n, rows + steps + 5, n_pages=30)
+        s.prompt(x.ptr, rows)
+        s.fork(range(n))
+        outs = []
+        for t in range(steps):
+            if t == 2:
+                s.drop([1, 3])
+                if share:
+                    s.compact()
+            s.step(xs[t].ptr, adapters, share)
+            assert R.cuSync() == 0, R.last_error()
+            outs.append(val(s.out.download(np.uint16, (n, cfg.hidden))))
+            att = val(s.att.download(np.uint16, (n, cfg.attn_q_heads * cfg.head_dim)))
+            assert (s.ok.download(np.int32, (n,)) == 1).all()
+        runs.append(outs)
+        assert not att[[1, 3]].any() and att[[0, 2, 4]].any()      # dropped requests attend to nothing
+        assert s.lens.download(np.int32, (n + 1,)).tolist() == [rows, rows + 3, 0, rows + 3, 0, rows + 3]
+        if share:
+            # 5 pages of the prompt; of three requests the copied page and, for one of 3 rows more than 75, nothing else
+            assert s.used.download(np.int32, (1,))[0] == 5 + 3 and (np.sort(np.nonzero(s.ref.download(np.int32, (30,)))[0]) == np.arange(8)).all()
+    for a, b in zip(*runs):
+        assert (np.abs(a - b) <= 2.0 ** -6 * np.abs(b).max()).all()
+
+    # request 2 over a contiguous cache: the rows that the pages hold, the last step's q, k, v
+    hd, Hq, Hkv, last = cfg.head_dim, cfg.attn_q_heads, cfg.attn_kv_heads, rows + steps - 1
+    table = s.table.download(np.int32, (n + 1, s.max_pages))[3]
+    planes = [s.data.download(np.uint16, (2, 30, Hkv, 16, hd))[i][table[:-(-(last + 1) // 16)]].transpose(1, 0, 2, 3).reshape(Hkv, -1, hd) for i in range(2)]
+    L = planes[0].shape[1]
+    kc, vc = dev(planes[0]), dev(planes[1])
+    row = lambda b, width: dev(b.download(np.uint16, (n, width))[2:3])  # noqa: E731
+    qg, k, v = row(s.qg, Hq * 2 * hd), row(s.k, Hkv * hd), row(s.v, Hkv * hd)
+    split, _ = ops.attn_plan(L, 1, Hkv)
+    scratch = R.DeviceBuffer.zeros(ops.attn_scratch_bytes(1, Hq, hd, L, split))
+    out, pos = R.DeviceBuffer(Hq * hd * 2), dev(i32(last))
+    cos_t, sin_t = ops.rope_tables(L, cfg.rot_dim, cfg.rope_theta)
+    dc, dsn = dev(cos_t), dev(sin_t)
+    ops.attn_decode(qg=qg.ptr, k=k.ptr, v=v.ptr, q_norm_w=w["q_norm"].ptr, k_norm_w=w["k_norm"].ptr, cos_t=dc.ptr, sin_t=dsn.ptr, k_cache=kc.ptr, v_cache=vc.ptr,
+                    pos=pos.ptr, out=out.ptr, scratch=scratch.ptr, B=1, Hq=Hq, Hkv=Hkv, HD=hd, rot_half=cfg.rot_dim // 2, max_len=L, split_len=split,
+                    max_pos=L - 1, scale=1 / math.sqrt(hd), fused_norm_rope=1)
+    assert R.cuSync() == 0, R.last_error()
+    want = val(out.download(np.uint16, (Hq * hd,)))
+    assert (np.abs(att[2] - want) <= 2.0 ** -6 * np.abs(val(planes[1])).max()).all()
