@@ -1028,7 +1028,7 @@ int32_t bkPagedAttn(const bkPagedAttnArgs* args) {
   BK_ARG(args != nullptr, "bkPagedAttn: args is null");
   const bkPagedAttnArgs& a = *args;
   BK_ARG(a.HD == 128 || a.HD == 256, "bkPagedAttn: head_dim %d unsupported (128 and 256)", a.HD);
-  BK_ARG(a.Hq > 0 && a.Hkv > 0 && a.Hq % a.Hkv == 0 && a.Hq / a.Hkv <= 16, "bkPagedAttn: bad head counts Hq=%d Hkv=%d (group size 1..16)", a.Hq, a.Hkv);
+  BK_ARG(a.Hq > 0 && a.Hkv > 0 && a.Hq % a.Hkv == 0 && a.Hq / a.Hkv <= 16 && a.Hkv <= 1024, "bkPagedAttn: bad head counts Hq=%d Hkv=%d (group size 1..16, at most 1024 KV heads)", a.Hq, a.Hkv);
   BK_ARG(a.B > 0 && a.T > 0 && (long long)a.B * a.T * (a.Hq + a.Hkv) < (1 << 24), "bkPagedAttn: B=%d T=%d of %d heads", a.B, a.T, a.Hq + a.Hkv);
   BK_ARG(a.page_rows >= 16 && a.page_rows <= 1024 && (a.page_rows & (a.page_rows - 1)) == 0, "bkPagedAttn: page_rows=%d must be a power of two, 16 to 1024", a.page_rows);
   BK_ARG(a.n_pages > 0 && a.max_pages > 0 && (long long)a.n_pages * a.Hkv * a.page_rows < (1ll << 31), "bkPagedAttn: n_pages=%d max_pages=%d (n_pages * Hkv * page_rows below 2^31)", a.n_pages, a.max_pages);

@@ -130,7 +130,7 @@ BK_DEVINL void copy_vecs(uint4* dst, const uint4* src, int n, int lane) {
   uint4 v[kCopyVecs];
 #pragma unroll
   for (int e = 0; e < kCopyVecs; e++)
-    if (lane + 32 * e < n) v[e] = __ldcs(src + lane + 32 * e);
+    if (lane + 32 * e < n) v[e] = __ldcg(src + lane + 32 * e);   // (several forks read one page)
 #pragma unroll
   for (int e = 0; e < kCopyVecs; e++)
     if (lane + 32 * e < n) __stcs(dst + lane + 32 * e, v[e]);

@@ -324,7 +324,7 @@ typedef struct bkPagedAttnArgs {
   uint64_t out;
   uint64_t scratch;      /* bkPagedAttnScratchBytes() bytes, 16-byte aligned; contents need not survive a call */
   uint64_t scratch_bytes;
-  int32_t B, T, Hq, Hkv, HD; /* HD 128 or 256; Hq / Hkv 1..16 */
+  int32_t B, T, Hq, Hkv, HD; /* HD 128 or 256; Hq / Hkv 1..16; Hkv at most 1024 */
   int32_t rot_half;
   int32_t n_pages, page_rows, max_pages; /* page_rows: a power of two, 16..1024 */
   int32_t prefix_rows;

@@ -460,6 +460,41 @@ def test_attention_of_many_rows_and_row_tiles(bk):
     Case(6, 2, 40, 130, [40, 95], Hq=8, Hkv=1, HD=128).check()                                         # 320 rows of one sequence
 
 
+def test_attention_of_more_jobs_than_shared_memory_plans(bk):
+    Case(61, 300, 1, 70, [1 + 7 * i % 40 for i in range(300)], Hq=4, Hkv=4, HD=128).check()            # 1,204 jobs
+    Case(62, 130, 1, 0, [i % 3 for i in range(130)], new=[min(1, i % 3) for i in range(130)], Hq=8, Hkv=8, HD=128).check()   # 1,040, a third of them empty
+
+
+def test_attention_of_a_long_piece_of_prompt(bk):
+    """One sequence, 150 new tokens of 8 heads: ten row tiles, with and without common rows, in one line and cut at the same keys."""
+    Case(63, 1, 150, 0, [600], Hq=8, Hkv=1, HD=128).check()
+    Case(64, 1, 150, 2000, [150], Hq=8, Hkv=1, HD=128, rows=64).check()
+    Case(65, 2, 70, 1300, [70, 75], new=[70, 31], Hq=16, Hkv=2, HD=256, rows=128).check()
+
+
+def test_attention_over_pages_beyond_32_bits(bk):
+    """Pools of 5 GB of keys and of values: the pages in use lie at their end."""
+    c = Case(66, 2, 1, 80, [40, 100], Hq=8, Hkv=2, HD=256, rows=64)
+    page = 2 * 64 * 256 * 2
+    far = (5 << 30) // page
+    shift = far - c.n_pages
+    want, kp, vp = c.want()
+    big = [R.DeviceBuffer(5 << 30) for _ in range(2)]
+    for b, host in zip(big, (c.kp, c.vp)):
+        R.cuHtoD(b.ptr + shift * page, host)
+    table = dev(np.where(c.table >= 0, c.table + shift, -1).astype(np.int32))
+    ops.paged_attn(c.args(k_pages=big[0].ptr, v_pages=big[1].ptr, table=table.ptr, n_pages=far))
+    assert R.cuSync() == 0, R.last_error()
+    got = val(c.out.download(np.uint16, (2, c.Hq, 256)))
+    vmax = np.abs(val(vp)[np.isfinite(val(vp))]).max()
+    assert (np.abs(got - want) <= 2.0 ** -8 * np.abs(want) + 2.0 ** -7 * vmax).all()
+    back = np.empty_like(c.vp)
+    R.cuDtoH(back, big[1].ptr + shift * page)
+    assert np.array_equal(back, vp)
+    for b in big:
+        b.free()
+
+
 def test_attention_where_nothing_is_there(bk):
     Case(1, 3, 1, 0, [0, 5, 0], new=[0, 1, 0], HD=128).check()
     Case(2, 2, 1, 0, [0, 0], new=[0, 0], HD=256).check()                        # no work at all
