@@ -68,8 +68,9 @@ __global__ void __launch_bounds__(kThreads) lora_shrink_kernel(const __grid_cons
   constexpr int U = MT <= 2 ? 4 : MT <= 4 ? 2 : 1;   // of 32 values of K requested together: up to 8 KB of weights a warp
   __shared__ int list[kMaxB];
   __shared__ float part_s[kWarps][MT * 16][8];
-  bk_pdl_trigger();
+  // The wait comes first: a launch behind this call may read, before its own wait, what a launch before this call wrote (weights, settled caches).
   bk_pdl_wait();
+  bk_pdl_trigger();
   int a;
   const unsigned long long cols = columns_of(p, blockIdx.y, &a);
   if (!cols) return;

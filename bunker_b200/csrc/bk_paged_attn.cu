@@ -45,7 +45,7 @@ BK_DEVINL void load_bf16(const uint16_t* src, float (&y)[PER]) {
 // out in one line and cut into equal pieces, one per CTA, so that a long prefix and many short sequences keep every SM busy until the end.
 // Where common keys have several row tiles, all of those are cut at the same keys, one range a CTA, and the line is for the other CTAs: the row tiles
 // of a KV head then read the same keys at the same time, once from memory (in one line they read them at times that hang on the cuts: 64
-// sequences, 24 heads on 4, 32,768 common rows 100 to 118 us by the overhead that the line counts with, so @T1@).
+// sequences, 24 heads on 4, 32,768 common rows 100 to 118 us by the overhead that the line counts with, so 97).
 // The plan is made on the device (lengths are there), by one CTA of the first launch.
 constexpr int kTile = 64;       // keys of a step
 constexpr int kRows = 128;      // rows of a job: the lanes of tensor memory
@@ -288,8 +288,9 @@ template <int HD>
 __global__ void __launch_bounds__(kPrepThreads) paged_prepare_kernel(const PagedParams p, const Layout L, uint8_t* scratch) {
   constexpr int PER = HD / 32;
   __shared__ float y_s[kPrepThreads / 32][HD];
-  bk_pdl_trigger();
+  // The wait comes first: a launch behind this call may read, before its own wait, what a launch before this call wrote (weights, settled caches).
   bk_pdl_wait();
+  bk_pdl_trigger();
   if (blockIdx.x == 0) {   // (first: it takes longest)
     if (L.n_p + L.n_s <= kPlanned) plan_jobs<true>(p, L, scratch);
     else plan_jobs<false>(p, L, scratch);

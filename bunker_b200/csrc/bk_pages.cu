@@ -91,6 +91,9 @@ BK_DEVINL int find_free(const Pool& p, long long want, int* fresh, long long* wa
   return (int)min((long long)found, want);
 }
 
+// The first launch of each call waits before it lets the next one start: a launch behind the call may read, before its own wait, what a launch
+// before the call wrote (weights, settled caches).
+
 struct ForkPlan {   // of one fork, in the scratch buffer
   int src, dst, rows, fresh;   // rows: -1 = not served; fresh: page of the partial rows, -1 = none
 };
@@ -101,8 +104,8 @@ __global__ void __launch_bounds__(kPlanThreads) pages_fork_plan_kernel(const Poo
   __shared__ __align__(16) int dst_s[kPlanThreads];
   __shared__ int total_s;
   __shared__ long long want_s;
-  bk_pdl_trigger();
   bk_pdl_wait();
+  bk_pdl_trigger();
   const int i = threadIdx.x;
   const int s = i < n ? src[i] : -1, d = i < n ? dst[i] : -1;
   dst_s[i] = d;
@@ -179,8 +182,8 @@ __global__ void __launch_bounds__(kPlanThreads) pages_grow_kernel(const Pool p, 
   __shared__ __align__(16) int list_s[kPlanThreads];
   __shared__ int need_s[kPlanThreads], before_s[kPlanThreads], total_s;
   __shared__ long long want_s;
-  bk_pdl_trigger();
   bk_pdl_wait();
+  bk_pdl_trigger();
   const int i = threadIdx.x;
   const int s = i < n ? seqs[i] : -1;
   const int more = i < n ? add[i] : -1;
@@ -215,8 +218,8 @@ __global__ void __launch_bounds__(kPlanThreads) pages_grow_kernel(const Pool p, 
 
 // One CTA per entry of the list.
 __global__ void __launch_bounds__(kCopyThreads) pages_free_kernel(const Pool p, const int* seqs) {
-  bk_pdl_trigger();
   bk_pdl_wait();
+  bk_pdl_trigger();
   const int i = blockIdx.x, s = seqs[i];
   if (s < 0 || s >= p.n_seqs) return;
   bool again = false;
@@ -239,8 +242,8 @@ __global__ void __launch_bounds__(kCopyThreads) pages_free_kernel(const Pool p, 
 __global__ void __launch_bounds__(kPlanThreads) pages_compact_plan_kernel(const Pool p, int* ref_out, int* map, int* used_out, int* moves) {
   __shared__ long long warp_sums[32];
   __shared__ int total_s[2];
-  bk_pdl_trigger();
   bk_pdl_wait();
+  bk_pdl_trigger();
   int mine = 0;
   for (int q = threadIdx.x; q < p.n_pages; q += kPlanThreads) mine += p.ref[q] > 0;
   const long long upto = block_scan(mine, warp_sums);
@@ -293,8 +296,8 @@ struct CopyJob {
   long long table_n;
 };
 __global__ void __launch_bounds__(kCopyThreads) pages_copy_kernel(const Pool from, const Pool to, const CopyJob job) {
-  bk_pdl_trigger();
   bk_pdl_wait();
+  bk_pdl_trigger();
   if (job.map)
     for (long long j = (long long)blockIdx.x * kCopyThreads + threadIdx.x; j < job.table_n; j += (long long)gridDim.x * kCopyThreads) {
       const int page = job.table_in[j];
