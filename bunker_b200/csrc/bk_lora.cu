@@ -147,7 +147,6 @@ __global__ void __launch_bounds__(kThreads, KS <= 2 ? 3 : KS <= 4 ? 2 : 1) lora_
   extern __shared__ __align__(16) uint16_t u_s[];   // [3][columns of the adapter][R]
   __shared__ int list[kMaxB];
   bk_pdl_trigger();
-  bk_pdl_wait();
   int seg = 0;
   while (seg + 1 < p.n_segs && (int)blockIdx.x >= p.segs[seg + 1].tile0) seg++;
   const LoraSeg& s = p.segs[seg];
@@ -159,6 +158,7 @@ __global__ void __launch_bounds__(kThreads, KS <= 2 ? 3 : KS <= 4 ? 2 : 1) lora_
   uint8_t* const out0 = reinterpret_cast<uint8_t*>(s.out);
   const int n_rows = s.n_rows, rank = p.rank, ld = s.ld_out, col_off = s.col_off;
   if (a < 0) {   // no adapter
+    bk_pdl_wait();
     if (base0 == out0) return;
     for (int row = row0 + lane; row < row_end; row += kThreads) {
       const size_t at = ((size_t)b * ld + col_off + row) * SZ;
@@ -166,7 +166,10 @@ __global__ void __launch_bounds__(kThreads, KS <= 2 ? 3 : KS <= 4 ? 2 : 1) lora_
     }
     return;
   }
-  if (!cols) return;
+  if (!cols) {
+    bk_pdl_wait();   // (no launch of this call outlives the one behind it)
+    return;
+  }
   const int n = __popcll(cols);
   // weights first: what is needed beside them is small and near
   const uint16_t* from = s.Bm + ((size_t)a * n_rows + q) * rank;
@@ -218,6 +221,7 @@ __global__ void __launch_bounds__(kThreads, KS <= 2 ? 3 : KS <= 4 ? 2 : 1) lora_
   };
   request_base(row0);
   const float scale = p.scale ? __ldg(p.scale + a) : 1.0f;
+  bk_pdl_wait();   // (all but u is older than this call, and the launch before this one began after that)
   for (int i = threadIdx.x; i < n * R; i += kThreads) {   // (zeros behind the rank)
     const int c = i / R, r = i % R;
     float y = 0.0f;

@@ -479,7 +479,6 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
   uint32_t& tmem_slot = sh.tmem_slot;
   int& dead_s = sh.dead;
   volatile int* dead = &dead_s;
-  bk_pdl_trigger();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     dead_s = 0;
@@ -513,6 +512,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
   tc_after();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(&tmem_slot);
   bk_pdl_wait();
+  bk_pdl_trigger();   // (the merge reads the plan before its own wait)
 
   const int4* jobs = jobs_of(L, P.scratch);
   const int cta = blockIdx.x, n_jobs = L.n_p + L.n_s;
@@ -912,14 +912,14 @@ __global__ void __launch_bounds__(256 * kSlices) paged_merge_kernel(const PagedP
   const int rp = (b * p.T + t) * G + g, rs = t * G + g;
   const int jp = kvh * L.mt_p + rp / kRows, js = (b * p.Hkv + kvh) * L.mt_s + rs / kRows;   // within their kind
   const uint16_t* gate = p.fused ? p.qg + ((size_t)e * p.Hq + kvh * G + g) * 2 * HD + HD : p.gate ? p.gate + ((size_t)e * p.Hq + kvh * G + g) * HD : nullptr;
-  bk_pdl_wait();
   const int4* jobs = jobs_of(L, scratch);
   const int2 qs = __ldcg(reinterpret_cast<const int2*>(&jobs[L.n_p + js].z));   // first slot; number and distance
   const int2 qp = L.n_p ? __ldcg(reinterpret_cast<const int2*>(&jobs[jp].z)) : make_int2(0, 0);
   const bool here = row_of(p, b, t) >= 0;
   uint2 gv = make_uint2(0, 0);
-  if (gate && slice == 0) gv = *reinterpret_cast<const uint2*>(gate + (d0 + d) * 4);
+  if (gate && slice == 0) gv = __ldcg(reinterpret_cast<const uint2*>(gate + (d0 + d) * 4));
   const int np = here ? qp.y & 0xffff : 0, n = here ? np + (qs.y & 0xffff) : 0;
+  bk_pdl_wait();   // (what is above was there when the launch before this one began its work)
   float m = -INFINITY, l = 0.0f;
   float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   constexpr int U = kSlices == 1 ? 6 : 4;   // pieces requested together
