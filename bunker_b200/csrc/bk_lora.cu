@@ -61,11 +61,13 @@ BK_DEVINL void list_columns(unsigned long long cols, int* list) {
   __syncthreads();
 }
 
-// grid (part of K, column, segment).  A warp takes every eighth 32 of the CTA's K: MT tiles of 16 rows of A and up to 8 columns of x.  Bound: memory,
-// and for few requests the latency of ids, then of the weights.
+// u[r] = sum over k of A[r][k] x[k].  grid (part of K, column, segment).  A warp takes every eighth 32 of the CTA's K: MT tiles of 16 rows of A and up to
+// 8 columns of x.  Bound: the latency of ids, then of the weights, then of the warps' sums: a CTA has its whole part in one or two requests.  64 requests
+// of 48 adapters, rank 32, K = 5,120 and two segments: about 8 us, 31 MB of weights at 4 TB/s.  Parts of K: about four CTAs an SM; with two the
+// call takes 33.5 us, with eight 31.3, with four 29.5.
 template <int MT>
 __global__ void __launch_bounds__(kThreads) lora_shrink_kernel(const __grid_constant__ LoraParams p) {
-  constexpr int U = MT <= 2 ? 4 : MT <= 4 ? 2 : 1;   // of 32 values of K requested together: up to 8 KB of weights a warp
+  constexpr int U = MT <= 1 ? 4 : MT <= 4 ? 2 : 1;   // of 32 values of K requested together: 4 KB of weights a warp and more (twice that at MT = 2: two CTAs an SM, 30.2 us)
   __shared__ int list[kMaxB];
   __shared__ float part_s[kWarps][MT * 16][8];
   // The wait comes first: a launch behind this call may read, before its own wait, what a launch before this call wrote (weights, settled caches).
@@ -132,8 +134,6 @@ BK_DEVINL void split3(float u, uint16_t (&o)[3]) {
   o[2] = sound ? bk_f32_to_bf16(__fsub_rn(r, bk_bf16_to_f32(o[1]))) : 0;
 }
 
-// grid (p.per tiles of 256 rows, column).  A warp has 32 rows of a tile, KS steps of 16 of the rank; the next tile's weights are requested before
-// these are multiplied.  WIDE (rank a multiple of 32): a lane's 16 bytes are two steps of a row.  Bound: memory.
 template <bool F32>
 BK_DEVINL float load_as(const uint8_t* at) { return F32 ? *reinterpret_cast<const float*>(at) : bk_bf16_to_f32(*reinterpret_cast<const uint16_t*>(at)); }
 template <bool F32>
@@ -141,6 +141,13 @@ BK_DEVINL void store_as(uint8_t* at, float v) {
   if (F32) *reinterpret_cast<float*>(at) = v;
   else *reinterpret_cast<uint16_t*>(at) = bk_f32_to_bf16(v);
 }
+template <int KS>
+constexpr int kAhead = KS <= 4 ? 2 : 1;   // tiles requested ahead where one or two columns share the weights (three spill: 35.1 us for 31.1)
+
+// out = base + Bm (s u).  grid (p.per tiles of 256 rows, column).  A warp has 32 rows of a tile, KS steps of 16 of the rank; the next tiles' weights are
+// requested before these are used up.  WIDE (rank a multiple of 32): a lane's 16 bytes are two steps of a row.  Bound: memory; 64 requests of 48 adapters,
+// rank 32, 2 x 17,408 rows: 21 us, 125 MB at 6 TB/s.  Instructions come next: with three MMAs for the parts of u and a store for
+// each of a row tile's eighths, adapters of one or two columns were bound by them (460 a warp and 32 rows; the call 37 us, now 29.5).
 template <int KS, bool WIDE, bool F32>
 __global__ void __launch_bounds__(kThreads, KS <= 2 ? 3 : KS <= 4 ? 2 : 1) lora_expand_kernel(const __grid_constant__ LoraParams p) {
   constexpr int R = KS * 16, SZ = F32 ? 4 : 2;
@@ -156,7 +163,7 @@ __global__ void __launch_bounds__(kThreads, KS <= 2 ? 3 : KS <= 4 ? 2 : 1) lora_
   const unsigned long long cols = columns_of(p, b, &a);
   const uint8_t* const base0 = reinterpret_cast<const uint8_t*>(s.base);   // (0: zeros)
   uint8_t* const out0 = reinterpret_cast<uint8_t*>(s.out);
-  const int n_rows = s.n_rows, rank = p.rank, ld = s.ld_out, col_off = s.col_off;
+  const int n_rows = s.n_rows, rank = WIDE ? R : p.rank, ld = s.ld_out, col_off = s.col_off;
   if (a < 0) {   // no adapter
     bk_pdl_wait();
     if (base0 == out0) return;
@@ -172,27 +179,105 @@ __global__ void __launch_bounds__(kThreads, KS <= 2 ? 3 : KS <= 4 ? 2 : 1) lora_
   }
   const int n = __popcll(cols);
   // weights first: what is needed beside them is small and near
-  const uint16_t* from = s.Bm + ((size_t)a * n_rows + q) * rank;
-  uint2 w[4][KS];
-  auto request = [&](int row) {
+  const uint16_t* from = s.Bm + ((size_t)a * n_rows + q) * rank + j * (WIDE ? 8 : 4);
+  auto request = [&](int row, uint2 (&w)[4][KS]) {   // rows below row_end
+    const uint16_t* at = from + (size_t)row * rank;
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-      const uint16_t* at = from + (size_t)(row + i * 8) * rank;
-      const bool in = row + i * 8 + q < n_rows;
+      const bool in = row + i * 8 + q < row_end;
       if (WIDE) {
 #pragma unroll
         for (int k = 0; k < KS; k += 2) {
-          const uint4 v = in ? __ldg(reinterpret_cast<const uint4*>(at + k * 16 + j * 8)) : make_uint4(0, 0, 0, 0);
+          const uint4 v = in ? __ldg(reinterpret_cast<const uint4*>(at + i * 8 * rank + k * 16)) : make_uint4(0, 0, 0, 0);
           w[i][k] = make_uint2(v.x, v.y);
           w[i][k + 1 < KS ? k + 1 : k] = make_uint2(v.z, v.w);
         }
       } else {
 #pragma unroll
-        for (int k = 0; k < KS; k++) w[i][k] = in && k * 16 + j * 4 < rank ? __ldg(reinterpret_cast<const uint2*>(at + k * 16 + j * 4)) : make_uint2(0, 0);
+        for (int k = 0; k < KS; k++) w[i][k] = in && k * 16 + j * 4 < rank ? __ldg(reinterpret_cast<const uint2*>(at + i * 8 * rank + k * 16)) : make_uint2(0, 0);
       }
     }
   };
-  request(row0);
+  // u of the adapter's columns into u_s; whole CTA
+  auto take_u = [&]() {
+    const float scale = p.scale ? __ldg(p.scale + a) : 1.0f;
+    bk_pdl_wait();   // (all but u is older than this call, and the launch before this one began after that)
+    for (int i = threadIdx.x; i < n * R; i += kThreads) {   // (zeros behind the rank)
+      const int c = i / R, r = i % R;
+      float y = 0.0f;
+      if (r < rank) {
+        const float* u = p.u + ((size_t)s.u_seg * p.B + list[c]) * rank + r;
+#pragma unroll 4
+        for (int part = 0; part < p.parts; part++) y = __fadd_rn(y, __ldcg(u + (size_t)part * p.u_segs * p.B * rank));
+      }
+      uint16_t o[3];
+      split3(__fmul_rn(scale, y), o);
+#pragma unroll
+      for (int t = 0; t < 3; t++) u_s[(size_t)t * n * R + i] = o[t];
+    }
+    __syncthreads();
+  };
+  auto u_at = [&](int t, int c, int k) {   // part t of column c, this lane's values of step k
+    return *reinterpret_cast<const uint2*>(u_s + ((size_t)t * n + c) * R + (WIDE ? (k >> 1) * 32 + j * 8 + (k & 1) * 4 : k * 16 + j * 4));
+  };
+
+  if (n <= 2) {
+    // One or two columns: their three parts side by side as six of the eight columns of one operand B, a third of the MMAs.  The parts then lie in lanes
+    // j = 0, 1, 2 of a row's four, which add them up and keep one of the tile's four rows q each.
+    constexpr int D = kAhead<KS>;
+    uint2 w[D][4][KS];
+    float base[D][2];
+#pragma unroll
+    for (int d = 0; d < D; d++) request(row0 + d * kThreads, w[d]);
+    list_columns(cols, list);
+    const int mine = (j & 1) * 16 + (j >> 1) * 8 + q;
+    size_t col[2];
+#pragma unroll
+    for (int c = 0; c < 2; c++) col[c] = ((size_t)list[min(c, n - 1)] * ld + col_off + mine) * SZ;
+    auto request_base = [&](int row, float (&base)[2]) {
+#pragma unroll
+      for (int c = 0; c < 2; c++) base[c] = base0 && c < n && row + mine < row_end ? load_as<F32>(base0 + col[c] + (size_t)row * SZ) : 0.0f;
+    };
+#pragma unroll
+    for (int d = 0; d < D; d++) request_base(row0 + d * kThreads, base[d]);
+    take_u();
+    uint2 u[KS];
+#pragma unroll
+    for (int k = 0; k < KS; k++) u[k] = q < 6 && (q & 1) < n ? u_at(q >> 1, q & 1, k) : make_uint2(0, 0);
+#pragma unroll 1
+    for (int first = row0; first < row_end; first += D * kThreads) {
+#pragma unroll
+      for (int d = 0; d < D; d++) {
+        const int row = first + d * kThreads;
+        float v[2][4];
+#pragma unroll
+        for (int t = 0; t < 2; t++)
+#pragma unroll
+          for (int e = 0; e < 4; e++) v[t][e] = 0.0f;
+#pragma unroll
+        for (int k = 0; k < KS; k++)
+#pragma unroll
+          for (int t = 0; t < 2; t++) mma_bf16(v[t], w[d][2 * t][k].x, w[d][2 * t + 1][k].x, w[d][2 * t][k].y, w[d][2 * t + 1][k].y, u[k].x, u[k].y);
+        request(row + D * kThreads, w[d]);
+        float half[4], sum[2];
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          if (j == 3) v[0][e] = v[1][e] = 0.0f;   // (a weight that is not finite made it NaN)
+          half[e] = __fadd_rn(j & 1 ? v[1][e] : v[0][e], __shfl_xor_sync(0xffffffffu, j & 1 ? v[0][e] : v[1][e], 1));
+        }
+#pragma unroll
+        for (int c = 0; c < 2; c++) {
+          sum[c] = __fadd_rn(j & 2 ? half[2 + c] : half[c], __shfl_xor_sync(0xffffffffu, j & 2 ? half[c] : half[2 + c], 2));
+          if (c < n && row + mine < row_end) store_as<F32>(out0 + col[c] + (size_t)row * SZ, __fadd_rn(base[d][c], sum[c]));
+        }
+        request_base(row + D * kThreads, base[d]);
+      }
+    }
+    return;
+  }
+
+  uint2 w[4][KS];
+  request(row0, w);
   list_columns(cols, list);
   // this lane's two of eight columns, at row q; base a tile ahead where these are all
   size_t col[2];
@@ -220,31 +305,13 @@ __global__ void __launch_bounds__(kThreads, KS <= 2 ? 3 : KS <= 4 ? 2 : 1) lora_
     }
   };
   request_base(row0);
-  const float scale = p.scale ? __ldg(p.scale + a) : 1.0f;
-  bk_pdl_wait();   // (all but u is older than this call, and the launch before this one began after that)
-  for (int i = threadIdx.x; i < n * R; i += kThreads) {   // (zeros behind the rank)
-    const int c = i / R, r = i % R;
-    float y = 0.0f;
-    if (r < rank) {
-      const float* u = p.u + ((size_t)s.u_seg * p.B + list[c]) * rank + r;
-#pragma unroll 4
-      for (int part = 0; part < p.parts; part++) y = __fadd_rn(y, __ldcg(u + (size_t)part * p.u_segs * p.B * rank));
-    }
-    uint16_t o[3];
-    split3(__fmul_rn(scale, y), o);
-#pragma unroll
-    for (int t = 0; t < 3; t++) u_s[(size_t)t * n * R + i] = o[t];
-  }
-  __syncthreads();
+  take_u();
   uint2 u[3][KS];   // operand B of eight columns
   auto columns_from = [&](int c0) {
 #pragma unroll
     for (int t = 0; t < 3; t++)
 #pragma unroll
-      for (int k = 0; k < KS; k++) {
-        const int r = WIDE ? (k >> 1) * 32 + j * 8 + (k & 1) * 4 : k * 16 + j * 4;
-        u[t][k] = c0 + q < n ? *reinterpret_cast<const uint2*>(u_s + ((size_t)t * n + c0 + q) * R + r) : make_uint2(0, 0);
-      }
+      for (int k = 0; k < KS; k++) u[t][k] = c0 + q < n ? u_at(t, c0 + q, k) : make_uint2(0, 0);
   };
   columns_from(0);
 #pragma unroll 1
@@ -273,7 +340,7 @@ __global__ void __launch_bounds__(kThreads, KS <= 2 ? 3 : KS <= 4 ? 2 : 1) lora_
 #pragma unroll
         for (int i = 0; i < 4; i++) now[e][i] = __fadd_rn(base[e][i], d[i >> 1][(i & 1) * 2 + e]);
       if (c0 + 8 >= n && row + kThreads < row_end) {   // (the last use of these weights)
-        request(row + kThreads);
+        request(row + kThreads, w);
         if (n <= 8) request_base(row + kThreads);
       }
 #pragma unroll
@@ -288,12 +355,14 @@ __global__ void __launch_bounds__(kThreads, KS <= 2 ? 3 : KS <= 4 ? 2 : 1) lora_
   }
 }
 
-// A CTA takes one tile where there are few, else as many as leave eight CTAs an SM.
+// A CTA takes one tile where there are few, else as many as leave eight CTAs an SM, in whole turns of what it requests ahead (an odd one costs a turn
+// of MMAs on nothing: 31.2 us with five tiles, 30.1 with four, six or eight).
 template <int KS, bool WIDE, bool F32>
 int32_t launch_expand_as(LoraParams& p) {
   long long tiles = 0;
   for (int i = 0; i < p.n_segs; i++) tiles += (p.segs[i].n_rows + kThreads - 1) / kThreads;
-  p.per = (int)std::max(1ll, std::min(16ll, tiles * std::min(p.B, p.n_adapters) / (8 * bk_ctx().sm_count)));
+  p.per = (int)std::min(16ll, tiles * std::min(p.B, p.n_adapters) / (8 * bk_ctx().sm_count));
+  p.per = std::max(1, p.per / kAhead<KS> * kAhead<KS>);
   int ctas = 0;
   for (int i = 0; i < p.n_segs; i++) {
     p.segs[i].tile0 = ctas;
