@@ -63,7 +63,7 @@ BK_DEVINL void list_columns(unsigned long long cols, int* list) {
 
 // u[r] = sum over k of A[r][k] x[k].  grid (part of K, column, segment).  A warp takes every eighth 32 of the CTA's K: MT tiles of 16 rows of A and up to
 // 8 columns of x.  Bound: the latency of ids, then of the weights, then of the warps' sums: a CTA has its whole part in one or two requests.  64 requests
-// of 48 adapters, rank 32, K = 5,120 and two segments: about 8 us, 31 MB of weights at 4 TB/s.  Parts of K: about four CTAs an SM; with two the
+// of 42 adapters, rank 32, K = 5,120 and two segments: about 8 us, 28 MB of weights at 3.4 TB/s.  Parts of K: about four CTAs an SM; with two the
 // call takes 33.5 us, with eight 31.3, with four 29.5.
 template <int MT>
 __global__ void __launch_bounds__(kThreads) lora_shrink_kernel(const __grid_constant__ LoraParams p) {
@@ -145,8 +145,8 @@ template <int KS>
 constexpr int kAhead = KS <= 4 ? 2 : 1;   // tiles requested ahead where one or two columns share the weights (three spill: 35.1 us for 31.1)
 
 // out = base + Bm (s u).  grid (p.per tiles of 256 rows, column).  A warp has 32 rows of a tile, KS steps of 16 of the rank; the next tiles' weights are
-// requested before these are used up.  WIDE (rank a multiple of 32): a lane's 16 bytes are two steps of a row.  Bound: memory; 64 requests of 48 adapters,
-// rank 32, 2 x 17,408 rows: 21 us, 125 MB at 6 TB/s.  Instructions come next: with three MMAs for the parts of u and a store for
+// requested before these are used up.  WIDE (rank a multiple of 32): a lane's 16 bytes are two steps of a row.  Bound: memory; 64 requests of 42 adapters,
+// rank 32, 2 x 17,408 rows: 21 us, 111 MB at 5.3 TB/s.  Instructions come next: with three MMAs for the parts of u and a store for
 // each of a row tile's eighths, adapters of one or two columns were bound by them (460 a warp and 32 rows; the call 37 us, now 29.5).
 template <int KS, bool WIDE, bool F32>
 __global__ void __launch_bounds__(kThreads, KS <= 2 ? 3 : KS <= 4 ? 2 : 1) lora_expand_kernel(const __grid_constant__ LoraParams p) {
