@@ -1,5 +1,11 @@
 // bk_paged_attn.cu -- attention of many sequences over pages of keys and values (bkPagedAttn in bunker_cuda.h has the rules).
 //
+// o[r] = sum over keys j <= row of r of 2^(S[r][j] - m[r]) v[j] / sum of the same without v, S = q k^T scale log2(e).  Three launches: queries and new
+// rows (with the plan of the next), tiles of rows and keys, the pieces' results together.  Each hides little of the one before: a tile CTA takes all of an
+// SM's shared memory.  One sequence of 300 rows, 16 heads on 2: 15 us, nearly all of it the three launches' latency; 32 sequences behind 8,192
+// common rows: 29 us; 64 behind 32,768, 24 heads on 4: 92 us (110 where the power limit sets the clock for long), 0.34 of the bf16 rate by
+// the operations that the result needs, half of it again in operations done.
+//
 // No counterpart in the reference (one contiguous cache of 128 rows, src/emitters.ts:188-226).
 #include <math.h>
 #include <string.h>
@@ -46,7 +52,8 @@ BK_DEVINL void load_bf16(const uint16_t* src, float (&y)[PER]) {
 // Where common keys have several row tiles, all of those are cut at the same keys, one range a CTA, and the line is for the other CTAs: the row tiles
 // of a KV head then read the same keys at the same time, once from memory (in one line they read them at times that hang on the cuts: 64
 // sequences, 24 heads on 4, 32,768 common rows 100 to 118 us by the overhead that the line counts with, so 97).
-// The plan is made on the device (lengths are there), by one CTA of the first launch.
+// The plan is made on the device (lengths are there), by one CTA of the first launch.  (Every CTA of the second making it for itself, in shared memory
+// and without records, starts later than that one, since an SM has no room for it beside a CTA of the first: 29.2 to 32.6 us, 22.4 to 25.8.)
 constexpr int kTile = 64;       // keys of a step
 constexpr int kRows = 128;      // rows of a job: the lanes of tensor memory
 constexpr int kOverhead = 3;    // what a job's start and end cost, in steps
@@ -283,7 +290,10 @@ BK_DEVINL bool row_at(const PagedParams& p, const Job& q, int i, int* b, int* t,
   return r < p.B * p.T * G;
 }
 
-// One warp per (token row, head): q heads to the scratch buffer, k and v heads into their page.  The first CTA lays out the work of the next launch.
+// One warp per (token row, head): y = x / sqrt(mean(x^2) + eps) (1 + w), then the rotation of pairs (d, d + rot_half), in f32; q heads to the scratch
+// buffer, k and v heads into their page, rounded to bf16: operands of the tensor cores (q's rounding is what the result's error is made of, 0.0023 of
+// its norm against 0.0017 for exact arithmetic rounded once).  The first CTA lays out the work of the next launch.  Bound: latency, 5 us for 32
+// sequences and 7 for 64 of 24 heads, most of it that CTA's.
 template <int HD>
 __global__ void __launch_bounds__(kPrepThreads) paged_prepare_kernel(const PagedParams p, const Layout L, uint8_t* scratch) {
   constexpr int PER = HD / 32;
@@ -465,6 +475,8 @@ constexpr int kCopyWarp = 8, kMmaWarp = 9, kQueryWarp = 10, kTileThreads = 352; 
 // memory, by TMA.  Q comes by TMA too, ahead of its turn, and is moved by the lanes that own the rows.  P = 2^(S c - m) with the running maximum m of the row; it overwrites its S as two bf16 matrices, the
 // rounded values and what rounding left (16 bits of the value; with 8 the result's error against exact arithmetic is 1.7 times that of its own rounding).
 // m is only moved when a score passes it by more than 2^8, since O must be rescaled then.  Row sums are in f32, by the lane that owns the row.
+// Bound: the MMAs, 1,650 of the 2,000 cycles that a step of 128 rows and 64 keys takes (HD 256): QK^T once, P V twice for the two matrices.  With P
+// rounded once the call of 64 sequences takes 85 us for 92 but the error is 0.0029.  Four stages in the ring for five: 92 us for 90.4.
 template <int HD>
 __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __grid_constant__ TileParams P) {
   using C = TileCfg<HD>;
@@ -608,7 +620,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
     } else if (warp == kMmaWarp) {
       // ================= MMAs =================
       // Scores of tile i, then the output of tile i - 1.  What the second half of a batch does not need is waited for ahead of it, while the
-      // first half runs.  Bound: the MMAs (1,600 cycles a step: 16 of 128 x 64 and 8 of 128 x 256) and, while little is queued, what this warp does
+      // first half runs.  Bound: the MMAs (1,650 cycles a step: 16 of 128 x 64 and 8 of 128 x 256) and, while little is queued, what this warp does
       // between them, so addresses are counted up, not made from positions.
       constexpr uint32_t kShapeS = mma_shape(kTile, false), kShapeO = mma_shape(HD, true);
       const uint64_t k_desc0 = smem_desc(smem_u32(ring), 16, 1024), v_desc0 = smem_desc(smem_u32(ring), kTile * 128, 1024);
@@ -900,8 +912,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
 
 // The pieces' results of a token row and KV head together: a CTA takes 64 dims of the group's heads, whose rows lie side by side in the
 // partial results; a thread 4 dims of one head, from every kSlices-th piece.  The common keys' pieces first, each kind in the order of the line.
-// Bound: latency, of a chain of loads.  Few CTAs have many pieces to a row, which four slices take together; many CTAs hide one another's
-// latency better when they are small.
+// Bound: latency, of a chain of loads: the lists of pieces, their sums and results; 2.6 us of a call for one sequence, 5.5 for 32, 6.4 for 64.
+// Few CTAs have many pieces to a row, which four slices take together; many CTAs hide one another's latency better when they are small (two
+// slices for 64 sequences of 24 heads: 1.5 us more).
 template <int HD, int kSlices>
 __global__ void __launch_bounds__(256 * kSlices) paged_merge_kernel(const PagedParams p, const Layout L, uint8_t* scratch) {
   __shared__ __align__(16) float4 o_s[kSlices > 1 ? kSlices - 1 : 1][16 * 16];
