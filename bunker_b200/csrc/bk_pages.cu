@@ -99,7 +99,7 @@ struct ForkPlan {   // of one fork, in the scratch buffer
 };
 
 // One CTA: which forks are served, and the fresh page of each.  A thread per fork; the free pages come from one pass over the counts, which ends when
-// enough are found.  Bound: latency of that chain, 3 to 4 us with the launch.
+// enough are found.  Bound: latency of that chain.
 __global__ void __launch_bounds__(kPlanThreads) pages_fork_plan_kernel(const Pool p, const int* src, const int* dst, int n, int* ok, ForkPlan* plan, int* fresh) {
   __shared__ long long warp_sums[32];
   __shared__ __align__(16) int dst_s[kPlanThreads];
