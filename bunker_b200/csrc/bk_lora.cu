@@ -1,15 +1,16 @@
 // bk_lora.cu -- low-rank adapters of many requests beside a shared projection: out[b] = base[b] + s_a Bm_a (A_a x_b), a = ids[b].
 //
 // No counterpart in the reference.  Two launches: u = A x, split over K so that few requests fill the GPU too, then out = base + s Bm u.
-// A CTA takes all columns of one adapter (it belongs to the first of them), so an adapter's weights are read once whatever the number
+// A CTA takes all columns of one adapter, so an adapter's weights are read once whatever the number
 // of requests that share it.  Both products are m16n8k16 MMAs on fragments that lanes load from memory as they lie: the order of the
 // contraction's index is free as long as both operands have the same, so a lane takes 8 or 16 consecutive bytes of a row.  (With one row of weights
 // a thread, or a few lanes, and FMAs, unpacking and reducing were 200 instructions for 32 rows and a column.)  x and the weights are
 // bf16, exact; u goes in as three bf16 matrices, what is left of its 24 bits after each rounding in the next.  Sums in f32, the parts of K added
-// in ascending order: results do not depend on the launch.
+// in ascending order: the same call gives the same bits.
 #include <string.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "bk_common.cuh"
 #include "bk_internal.h"
@@ -30,20 +31,20 @@ struct LoraParams {
   const int* ids;
   const float* scale;
   float* u;   // [part of K][segment][column][rank]
-  int K, B, n_segs, rank, n_adapters, parts, chunk, per, u_segs;   // u_segs: segments that u has
+  int K, B, n_segs, rank, n_adapters, parts, chunk, per, u_segs, by_adapter;   // u_segs: segments that u has
   LoraSeg segs[4];
 };
 
-// Column b's adapter and the columns that share it, a bit each, if b is the first of them (0: it is not, or has no adapter: *adapter = -1).  Whole
-// warps call.
-BK_DEVINL unsigned long long columns_of(const LoraParams& p, int b, int* adapter) {
+// The adapter of CTAs y and its columns, a bit each.  by_adapter: adapter y, if there are as few; else column y's, for the first of its columns
+// (64 columns of 7 adapters by columns: 57 of 64 CTAs come to find nothing to do, 24 us for 13).  0: nothing here; *adapter -1: no adapter.  Whole warps call.
+BK_DEVINL unsigned long long columns_of(const LoraParams& p, int y, int* adapter) {
   const int lane = threadIdx.x & 31;
   const int lo = lane < p.B ? __ldg(p.ids + lane) : -1, hi = lane + 32 < p.B ? __ldg(p.ids + lane + 32) : -1;
-  const int a = __shfl_sync(0xffffffffu, b < 32 ? lo : hi, b & 31);
+  const int a = p.by_adapter ? y : __shfl_sync(0xffffffffu, y < 32 ? lo : hi, y & 31);
   const bool there = a >= 0 && a < p.n_adapters;
   *adapter = there ? a : -1;
   const unsigned long long same = (unsigned long long)__ballot_sync(0xffffffffu, hi == a) << 32 | __ballot_sync(0xffffffffu, lo == a);
-  return there && __ffsll(same) - 1 == b ? same : 0;
+  return there && (p.by_adapter || __ffsll(same) - 1 == y) ? same : 0;
 }
 
 // D += A B; a: rows lane/4 and +8, two pairs of the contraction's index; b: column lane/4, the same pairs; d: rows lane/4 and +8, columns 2(lane mod 4), +1
@@ -61,15 +62,16 @@ BK_DEVINL void list_columns(unsigned long long cols, int* list) {
   __syncthreads();
 }
 
-// u[r] = sum over k of A[r][k] x[k].  grid (part of K, column, segment).  A warp takes every eighth 32 of the CTA's K: MT tiles of 16 rows of A and up to
-// 8 columns of x.  Bound: the latency of ids, then of the weights, then of the warps' sums: a CTA has its whole part in one or two requests.  64 requests
-// of 42 adapters, rank 32, K = 5,120 and two segments: about 8 us, 28 MB of weights at 3.4 TB/s.  Parts of K: about four CTAs an SM; with two the
-// call takes 33.5 us, with eight 31.3, with four 29.5.
+// u[r] = sum over k of A[r][k] x[k].  grid (part of K, adapter or column, segment).  A warp has 16 rows of A, up to 8 columns of x and every S-th 32 of
+// the CTA's K, 8 KB of weights on the way.  (All rows a warp, with what a long rank leaves of the registers: 56 adapters of rank 128, K = N = 5,120
+// 62 us, so 29; rank 64 32, so 20.)  Bound: memory for long ranks (73 MB in 15 us), else the latency of ids, weights and the warps' sums: 42 adapters of
+// rank 32, K = 5,120, two segments about 8 us, 28 MB at 3.4 TB/s.  Parts of K: as many CTAs as stay on the GPU, two an SM (three with half as much on
+// the way: rank 128 30.0, rank 64 20.9; four: 34.1 and 24.5).
 template <int MT>
-__global__ void __launch_bounds__(kThreads) lora_shrink_kernel(const __grid_constant__ LoraParams p) {
-  constexpr int U = MT <= 1 ? 4 : MT <= 4 ? 2 : 1;   // of 32 values of K requested together: 4 KB of weights a warp and more (twice that at MT = 2: two CTAs an SM, 30.2 us)
+__global__ void __launch_bounds__(kThreads, 2) lora_shrink_kernel(const __grid_constant__ LoraParams p) {
+  constexpr int S = kWarps / MT, U = 8;   // U: of 32 values of K requested together
   __shared__ int list[kMaxB];
-  __shared__ float part_s[kWarps][MT * 16][8];
+  __shared__ float part_s[S][MT * 16][8];
   // The wait comes first: a launch behind this call may read, before its own wait, what a launch before this call wrote (weights, settled caches).
   bk_pdl_wait();
   bk_pdl_trigger();
@@ -77,49 +79,40 @@ __global__ void __launch_bounds__(kThreads) lora_shrink_kernel(const __grid_cons
   const unsigned long long cols = columns_of(p, blockIdx.y, &a);
   if (!cols) return;
   list_columns(cols, list);
-  const int n = __popcll(cols), lane = threadIdx.x & 31, warp = threadIdx.x >> 5, q = lane >> 2, j = lane & 3;
+  const int n = __popcll(cols), lane = threadIdx.x & 31, warp = threadIdx.x >> 5, q = lane >> 2, j = lane & 3, r0 = warp / S * 16, slice = warp % S;
   const int k0 = blockIdx.x * p.chunk, k1 = min(p.K, k0 + p.chunk);
-  const uint16_t* A = p.segs[blockIdx.z].A + ((size_t)a * p.rank + q) * p.K + j * 8;
+  const bool row[2] = {r0 < p.rank, r0 + 8 < p.rank};   // (the rank is a multiple of 8)
+  const uint16_t* A = p.segs[blockIdx.z].A + ((size_t)a * p.rank + r0 + q) * p.K + j * 8;
   const uint4 zero = make_uint4(0, 0, 0, 0);
   for (int c0 = 0; c0 < n; c0 += 8) {
     const uint16_t* x = p.x + (size_t)list[min(c0 + q, n - 1)] * p.K + j * 8;
     const bool col = c0 + q < n;
-    float d[MT][4];
-#pragma unroll
-    for (int t = 0; t < MT; t++)
-#pragma unroll
-      for (int e = 0; e < 4; e++) d[t][e] = 0.0f;
-    for (int kb = k0 + warp * 32; kb < k1; kb += kWarps * 32 * U) {
-      uint4 w[U][MT][2], v[U];
+    float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int kb = k0 + slice * 32; kb < k1; kb += S * 32 * U) {
+      uint4 w[U][2], v[U];
 #pragma unroll
       for (int u = 0; u < U; u++) {
-        const int k = kb + u * kWarps * 32;
+        const int k = kb + u * S * 32;
         const bool in = k + j * 8 < k1;   // (K and the parts are multiples of 8)
+#pragma unroll
+        for (int h = 0; h < 2; h++) w[u][h] = in && row[h] ? __ldg(reinterpret_cast<const uint4*>(A + (size_t)(h * 8) * p.K + k)) : zero;
         v[u] = in && col ? __ldg(reinterpret_cast<const uint4*>(x + k)) : zero;
-#pragma unroll
-        for (int t = 0; t < MT; t++)
-#pragma unroll
-          for (int h = 0; h < 2; h++) w[u][t][h] = in && t * 16 + h * 8 < p.rank ? __ldg(reinterpret_cast<const uint4*>(A + (size_t)(t * 16 + h * 8) * p.K + k)) : zero;
       }
 #pragma unroll
-      for (int u = 0; u < U; u++)
-#pragma unroll
-        for (int t = 0; t < MT; t++) {
-          mma_bf16(d[t], w[u][t][0].x, w[u][t][1].x, w[u][t][0].y, w[u][t][1].y, v[u].x, v[u].y);
-          mma_bf16(d[t], w[u][t][0].z, w[u][t][1].z, w[u][t][0].w, w[u][t][1].w, v[u].z, v[u].w);
-        }
+      for (int u = 0; u < U; u++) {
+        mma_bf16(d, w[u][0].x, w[u][1].x, w[u][0].y, w[u][1].y, v[u].x, v[u].y);
+        mma_bf16(d, w[u][0].z, w[u][1].z, w[u][0].w, w[u][1].w, v[u].z, v[u].w);
+      }
     }
     if (c0) __syncthreads();   // the sums before have been taken
 #pragma unroll
-    for (int t = 0; t < MT; t++)
-#pragma unroll
-      for (int e = 0; e < 4; e++) part_s[warp][t * 16 + (e >> 1) * 8 + q][2 * j + (e & 1)] = d[t][e];
+    for (int e = 0; e < 4; e++) part_s[slice][r0 + (e >> 1) * 8 + q][2 * j + (e & 1)] = d[e];
     __syncthreads();
     for (int i = threadIdx.x; i < p.rank * 8; i += kThreads) {
       const int r = i >> 3, c = c0 + (i & 7);
       float y = 0.0f;
 #pragma unroll
-      for (int w = 0; w < kWarps; w++) y = __fadd_rn(y, part_s[w][r][i & 7]);
+      for (int w = 0; w < S; w++) y = __fadd_rn(y, part_s[w][r][i & 7]);
       if (c < n) p.u[(((size_t)blockIdx.x * p.n_segs + blockIdx.z) * p.B + list[c]) * p.rank + r] = y;
     }
   }
@@ -146,10 +139,10 @@ constexpr int kAhead = KS <= 4 ? 2 : 1;   // tiles requested ahead where one or 
 
 // out = base + Bm (s u).  grid (p.per tiles of 256 rows, column).  A warp has 32 rows of a tile, KS steps of 16 of the rank; the next tiles' weights are
 // requested before these are used up.  WIDE (rank a multiple of 32): a lane's 16 bytes are two steps of a row.  Bound: memory; 64 requests of 42 adapters,
-// rank 32, 2 x 17,408 rows: 21 us, 111 MB at 5.3 TB/s.  Instructions come next: with three MMAs for the parts of u and a store for
+// rank 32, 2 x 17,408 rows: 20 us, 111 MB at 5.5 TB/s.  Instructions come next: with three MMAs for the parts of u and a store for
 // each of a row tile's eighths, adapters of one or two columns were bound by them (460 a warp and 32 rows; the call 37 us, now 29.5).
 template <int KS, bool WIDE, bool F32>
-__global__ void __launch_bounds__(kThreads, KS <= 2 ? 3 : KS <= 4 ? 2 : 1) lora_expand_kernel(const __grid_constant__ LoraParams p) {
+__global__ void __launch_bounds__(kThreads, KS <= 2 ? 3 : 2) lora_expand_kernel(const __grid_constant__ LoraParams p) {
   constexpr int R = KS * 16, SZ = F32 ? 4 : 2;
   extern __shared__ __align__(16) uint16_t u_s[];   // [3][columns of the adapter][R]
   __shared__ int list[kMaxB];
@@ -157,19 +150,24 @@ __global__ void __launch_bounds__(kThreads, KS <= 2 ? 3 : KS <= 4 ? 2 : 1) lora_
   int seg = 0;
   while (seg + 1 < p.n_segs && (int)blockIdx.x >= p.segs[seg + 1].tile0) seg++;
   const LoraSeg& s = p.segs[seg];
-  const int lane = threadIdx.x & 31, q = lane >> 2, j = lane & 3, b = blockIdx.y;
+  const int lane = threadIdx.x & 31, q = lane >> 2, j = lane & 3;
   const int row0 = ((int)blockIdx.x - s.tile0) * (p.per * kThreads) + (threadIdx.x >> 5) * 32, row_end = min(s.n_rows, row0 + p.per * kThreads);   // of this warp
   int a;
-  const unsigned long long cols = columns_of(p, b, &a);
+  const unsigned long long cols = columns_of(p, blockIdx.y, &a);
   const uint8_t* const base0 = reinterpret_cast<const uint8_t*>(s.base);   // (0: zeros)
   uint8_t* const out0 = reinterpret_cast<uint8_t*>(s.out);
   const int n_rows = s.n_rows, rank = WIDE ? R : p.rank, ld = s.ld_out, col_off = s.col_off;
-  if (a < 0) {   // no adapter
+  if (a < 0) {   // no adapter: this column, or those of eight
     bk_pdl_wait();
     if (base0 == out0) return;
-    for (int row = row0 + lane; row < row_end; row += kThreads) {
-      const size_t at = ((size_t)b * ld + col_off + row) * SZ;
-      store_as<F32>(out0 + at, base0 ? load_as<F32>(base0 + at) : 0.0f);
+    const int b0 = p.by_adapter ? ((int)blockIdx.y - p.n_adapters) * 8 : (int)blockIdx.y, b1 = p.by_adapter ? min(p.B, b0 + 8) : b0 + 1;
+    for (int b = b0; b < b1; b++) {
+      const int id = __ldg(p.ids + b);
+      if (id >= 0 && id < p.n_adapters) continue;
+      for (int row = row0 + lane; row < row_end; row += kThreads) {
+        const size_t at = ((size_t)b * ld + col_off + row) * SZ;
+        store_as<F32>(out0 + at, base0 ? load_as<F32>(base0 + at) : 0.0f);
+      }
     }
     return;
   }
@@ -198,22 +196,32 @@ __global__ void __launch_bounds__(kThreads, KS <= 2 ? 3 : KS <= 4 ? 2 : 1) lora_
       }
     }
   };
-  // u of the adapter's columns into u_s; whole CTA
-  auto take_u = [&]() {
+  // u of the adapter's columns into u_s, V values a thread at a time; whole CTA
+  auto take_u = [&](auto width) {
+    constexpr int V = decltype(width)::value;
     const float scale = p.scale ? __ldg(p.scale + a) : 1.0f;
     bk_pdl_wait();   // (all but u is older than this call, and the launch before this one began after that)
-    for (int i = threadIdx.x; i < n * R; i += kThreads) {   // (zeros behind the rank)
+    for (int i = threadIdx.x * V; i < n * R; i += kThreads * V) {   // (zeros behind the rank, a multiple of 8)
       const int c = i / R, r = i % R;
-      float y = 0.0f;
+      float y[V] = {};
       if (r < rank) {
         const float* u = p.u + ((size_t)s.u_seg * p.B + list[c]) * rank + r;
 #pragma unroll 4
-        for (int part = 0; part < p.parts; part++) y = __fadd_rn(y, __ldcg(u + (size_t)part * p.u_segs * p.B * rank));
-      }
-      uint16_t o[3];
-      split3(__fmul_rn(scale, y), o);
+        for (int part = 0; part < p.parts; part++) {
+          alignas(16) float x[V];
+          if (V == 4) *reinterpret_cast<float4*>(x) = __ldcg(reinterpret_cast<const float4*>(u + (size_t)part * p.u_segs * p.B * rank));
+          else x[0] = __ldcg(u + (size_t)part * p.u_segs * p.B * rank);
 #pragma unroll
-      for (int t = 0; t < 3; t++) u_s[(size_t)t * n * R + i] = o[t];
+          for (int e = 0; e < V; e++) y[e] = __fadd_rn(y[e], x[e]);
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < V; e++) {
+        uint16_t o[3];
+        split3(__fmul_rn(scale, y[e]), o);
+#pragma unroll
+        for (int t = 0; t < 3; t++) u_s[(size_t)t * n * R + i + e] = o[t];
+      }
     }
     __syncthreads();
   };
@@ -240,7 +248,7 @@ __global__ void __launch_bounds__(kThreads, KS <= 2 ? 3 : KS <= 4 ? 2 : 1) lora_
     };
 #pragma unroll
     for (int d = 0; d < D; d++) request_base(row0 + d * kThreads, base[d]);
-    take_u();
+    take_u(std::integral_constant<int, 1>());
     uint2 u[KS];
 #pragma unroll
     for (int k = 0; k < KS; k++) u[k] = q < 6 && (q & 1) < n ? u_at(q >> 1, q & 1, k) : make_uint2(0, 0);
@@ -305,13 +313,14 @@ __global__ void __launch_bounds__(kThreads, KS <= 2 ? 3 : KS <= 4 ? 2 : 1) lora_
     }
   };
   request_base(row0);
-  take_u();
-  uint2 u[3][KS];   // operand B of eight columns
+  take_u(std::integral_constant<int, 4>());   // (64 columns of one adapter: 25.8 us with one value, 20.5 with four)
+  constexpr bool kKeep = KS <= 2;   // operand B of eight columns in registers (longer ranks: from shared memory each time, for two CTAs an SM: 8 columns, rank 128 37.9 us with one CTA, 24.5 with two)
+  uint2 u[3][kKeep ? KS : 1];
   auto columns_from = [&](int c0) {
 #pragma unroll
     for (int t = 0; t < 3; t++)
 #pragma unroll
-      for (int k = 0; k < KS; k++) u[t][k] = c0 + q < n ? u_at(t, c0 + q, k) : make_uint2(0, 0);
+      for (int k = 0; k < (kKeep ? KS : 0); k++) u[t][k] = c0 + q < n ? u_at(t, c0 + q, k) : make_uint2(0, 0);
   };
   columns_from(0);
 #pragma unroll 1
@@ -331,9 +340,11 @@ __global__ void __launch_bounds__(kThreads, KS <= 2 ? 3 : KS <= 4 ? 2 : 1) lora_
 #pragma unroll
       for (int part = 2; part >= 0; part--)   // the smallest first
 #pragma unroll
-        for (int k = 0; k < KS; k++)
+        for (int k = 0; k < KS; k++) {
+          const uint2 y = kKeep ? u[part][kKeep ? k : 0] : c0 + q < n ? u_at(part, c0 + q, k) : make_uint2(0, 0);
 #pragma unroll
-          for (int t = 0; t < 2; t++) mma_bf16(d[t], w[2 * t][k].x, w[2 * t + 1][k].x, w[2 * t][k].y, w[2 * t + 1][k].y, u[part][k].x, u[part][k].y);
+          for (int t = 0; t < 2; t++) mma_bf16(d[t], w[2 * t][k].x, w[2 * t + 1][k].x, w[2 * t][k].y, w[2 * t + 1][k].y, y.x, y.y);
+        }
       float now[2][4];
 #pragma unroll
       for (int e = 0; e < 2; e++)
@@ -355,13 +366,14 @@ __global__ void __launch_bounds__(kThreads, KS <= 2 ? 3 : KS <= 4 ? 2 : 1) lora_
   }
 }
 
-// A CTA takes one tile where there are few, else as many as leave eight CTAs an SM, in whole turns of what it requests ahead (an odd one costs a turn
-// of MMAs on nothing: 31.2 us with five tiles, 30.1 with four, six or eight).
+// A CTA takes one tile where there are few, else as many as leave four CTAs an SM: its start, a chain of ids, u and the first weights, costs several
+// tiles' time (eight an SM: 56 adapters of rank 16 to 17,408 rows 23.1 us for 17.0; three: 42 of rank 32 to 34,816 31.9 for 28.7).  In whole turns of what
+// it requests ahead: an odd one costs a turn of MMAs on nothing (five tiles 31.2 us, four or six 30.0).
 template <int KS, bool WIDE, bool F32>
 int32_t launch_expand_as(LoraParams& p) {
   long long tiles = 0;
   for (int i = 0; i < p.n_segs; i++) tiles += (p.segs[i].n_rows + kThreads - 1) / kThreads;
-  p.per = (int)std::min(16ll, tiles * std::min(p.B, p.n_adapters) / (8 * bk_ctx().sm_count));
+  p.per = (int)std::min(16ll, (tiles * std::min(p.B, p.n_adapters) + 2 * bk_ctx().sm_count) / (4 * bk_ctx().sm_count));
   p.per = std::max(1, p.per / kAhead<KS> * kAhead<KS>);
   int ctas = 0;
   for (int i = 0; i < p.n_segs; i++) {
@@ -374,7 +386,13 @@ int32_t launch_expand_as(LoraParams& p) {
     BK_CUDA(cudaFuncSetAttribute(lora_expand_kernel<KS, WIDE, F32>, cudaFuncAttributeMaxDynamicSharedMemorySize, 3 * kMaxB * KS * 16 * 2));
     configured = true;
   }
-  BK_CUDA(bk_launch_pdl(lora_expand_kernel<KS, WIDE, F32>, dim3(ctas, p.B), dim3(kThreads), smem, p));
+  int ys = p.B;
+  if (p.by_adapter) {
+    ys = p.n_adapters;
+    for (int i = 0; i < p.n_segs; i++)
+      if (p.segs[i].base != p.segs[i].out) ys = p.n_adapters + (p.B + 7) / 8;
+  }
+  BK_CUDA(bk_launch_pdl(lora_expand_kernel<KS, WIDE, F32>, dim3(ctas, ys), dim3(kThreads), smem, p));
   BK_CHECK_LAUNCH();
   return BK_OK;
 }
@@ -398,7 +416,7 @@ int32_t launch_expand(const LoraParams& all) {
 }
 template <int MT>
 int32_t launch_shrink(LoraParams& p) {
-  BK_CUDA(bk_launch_pdl(lora_shrink_kernel<MT>, dim3(p.parts, p.B, p.n_segs), dim3(kThreads), 0, p));
+  BK_CUDA(bk_launch_pdl(lora_shrink_kernel<MT>, dim3(p.parts, p.by_adapter ? p.n_adapters : p.B, p.n_segs), dim3(kThreads), 0, p));
   BK_CHECK_LAUNCH();
   return BK_OK;
 }
@@ -427,7 +445,7 @@ int32_t bkLora(const bkLoraArgs* args) {
   LoraParams p;
   memset(&p, 0, sizeof(p));
   p.x = bk_ptr<uint16_t>(a.x); p.ids = bk_ptr<int>(a.ids); p.scale = bk_ptr<float>(a.scale); p.u = bk_ptr<float>(a.scratch);
-  p.K = a.K; p.B = a.B; p.n_segs = p.u_segs = a.n_segs; p.rank = a.rank; p.n_adapters = a.n_adapters;
+  p.K = a.K; p.B = a.B; p.n_segs = p.u_segs = a.n_segs; p.rank = a.rank; p.n_adapters = a.n_adapters; p.by_adapter = a.n_adapters <= a.B;
   for (int i = 0; i < a.n_segs; i++) {
     const bkLoraSeg& s = a.segs[i];
     BK_ARG(s.n_rows > 0 && s.n_rows < (1 << 30) && s.col_off >= 0 && (long long)s.col_off + s.n_rows <= s.ld_out, "bkLora: segment %d: n_rows=%d col_off=%d ld_out=%d", i, s.n_rows, s.col_off,
@@ -437,9 +455,9 @@ int32_t bkLora(const bkLoraArgs* args) {
     BK_ARG(s.A && s.Bm && s.out && ((s.A | s.Bm) & 15) == 0 && ((s.base | s.out) & mask) == 0, "bkLora: segment %d: A and Bm must be 16-byte aligned, out non-null, base and out aligned to their type", i);
     p.segs[i] = LoraSeg{bk_ptr<uint16_t>(s.A), bk_ptr<uint16_t>(s.Bm), bk_ptr<void>(s.base), bk_ptr<void>(s.out), s.n_rows, s.dtype == BK_DTYPE_F32, s.ld_out, s.col_off, i, 0};
   }
-  // Parts of K, multiples of 256 (32 a warp): about four CTAs an SM, no more than 16 for the expanding launch to add up.
+  // Parts of K, multiples of 256: about two CTAs an SM, no more than 16 for the expanding launch to add up.
   const int units = (a.K + 255) / 256;
-  const int parts = std::max(1, std::min({units, 16, 4 * bk_ctx().sm_count / (a.n_segs * std::min(a.B, a.n_adapters))}));
+  const int parts = std::max(1, std::min({units, 16, 2 * bk_ctx().sm_count / (a.n_segs * std::min(a.B, a.n_adapters))}));
   p.chunk = (units + parts - 1) / parts * 256;
   p.parts = (a.K + p.chunk - 1) / p.chunk;
   const int32_t rc = a.rank <= 16 ? launch_shrink<1>(p) : a.rank <= 32 ? launch_shrink<2>(p) : a.rank <= 64 ? launch_shrink<4>(p) : launch_shrink<8>(p);

@@ -661,6 +661,34 @@ def test_adapters_of_many_requests(bk, B, K, rows, rank, n_adapters, ids, f32):
         first = bits
 
 
+@pytest.mark.parametrize("rank", [8, 16, 24, 32, 56, 64, 80, 96, 128])
+@pytest.mark.parametrize("B,n_adapters,ids", [
+    (5, 9, [7, 2, 7, -1, 7]),                    # more adapters than requests: three columns, one, none
+    (4, 4, [3, 1, 3, 1]),                        # two columns each; two adapters without any
+    (10, 2, [1, -1, 1, 1, 0, 1, 1, 2, 1, 1]),    # seven columns and one; two without
+])
+def test_adapters_of_every_rank(bk, rank, B, n_adapters, ids):
+    for rows in ([2500], [31, 257]):             # tiles that end inside
+        args, keep, want, hold = lora_case(rank + B, B, 1032, rows, rank, n_adapters, ids, True)
+        ops.lora(args)
+        assert R.cuSync() == 0, R.last_error()
+        for (d, out, ld, n), (y, mag) in zip(keep, want):
+            got = out.download(np.float32, (B, ld)).astype(np.float64)
+            assert (np.abs(got - y) <= (1032 + rank + 4) * 2.0 ** -24 * mag).all()
+
+
+@pytest.mark.parametrize("rank,shared", [(8, 1), (32, 1), (8, 4), (64, 2), (128, 3)])
+def test_adapters_of_many_rows(bk, rank, shared):
+    """So many rows and adapters that a CTA goes through several tiles; every adapter has `shared` columns."""
+    B = 40
+    args, keep, want, hold = lora_case(rank, B, 64, [9001 if rank > 32 else 17377], rank, B, [-1 if b == 7 else b // shared for b in range(B)], True)
+    ops.lora(args)
+    assert R.cuSync() == 0, R.last_error()
+    for (d, out, ld, n), (y, mag) in zip(keep, want):
+        got = out.download(np.float32, (B, ld)).astype(np.float64)
+        assert (np.abs(got - y) <= (64 + rank + 4) * 2.0 ** -24 * mag).all()
+
+
 def test_adapters_without_base_or_scale_in_place_and_in_columns(bk):
     for kw in ({"with_base": False}, {"with_scale": False}, {"pad": 5}):
         args, keep, want, hold = lora_case(7, 4, 320, [100, 30], 16, 3, [0, 2, -1, 0], True, **kw)
