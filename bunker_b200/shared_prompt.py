@@ -52,7 +52,7 @@ class SharedPrompt:
         nb = ops.lora_scratch_bytes(H, c, lora["rank"], 3)
         self.lora_scratch, self.lora_bytes = R.DeviceBuffer(nb), nb
         self.att_scratch, self.att_bytes = R.DeviceBuffer(16), 16
-        self.lists = {k: R.DeviceBuffer(4 * c) for k in ("seqs", "src", "add", "new", "ids")}
+        self.lists = {k: R.DeviceBuffer(4 * c) for k in ("seqs", "src", "add", "ids")}
         self.prompt_rows = 0
         self.active = np.zeros(requests, bool)
 
@@ -102,10 +102,12 @@ class SharedPrompt:
         self.active[list(requests)] = True
 
     def step(self, x: int, adapters: Sequence[int], share: bool = True) -> int:
-        """One token of every active request: x bf16 [requests][H] -> out bf16 [requests][H] (rows of others: what the residual gives)."""
+        """One token of every active request: x bf16 [requests][H] -> out bf16 [requests][H] (rows of others: what the residual gives).
+        ``ok`` (int32 [requests], on the device) says who had room.  A request without room has no token in this step: its ok is its number of new
+        tokens, so nothing is stored for it (the row before its next one may be the prompt's, which all share).  An inactive one has no rows."""
         new = self.active.astype(np.int32)
         self.pool.grow(self._list("seqs", np.arange(1, self.n + 1)), self._list("add", new), self.n, self.ok.ptr)
-        return self._layer(x, self.n, self.n, 1, 1, self._list("new", new), adapters, self.prompt_rows if share and new[0] else 0)
+        return self._layer(x, self.n, self.n, 1, 1, self.ok.ptr, adapters, self.prompt_rows if share and new[0] else 0)
 
     def drop(self, requests: Sequence[int]) -> None:
         self.pool.free(self._list("seqs", [r + 1 for r in requests]), len(requests))

@@ -307,6 +307,8 @@ BK_API int32_t bkPagesCompact(const bkPages* pool, uint64_t table_out, uint64_t 
 /* Attention of B sequences with up to T new tokens each over pages of keys and values, [n_pages][Hkv][page_rows][HD] bf16 (one plane
  * each of a bkPages pool).  Token t of sequence b is row t*B + b of every input and output; it stands at row lens[b] - n_new[b] + t of its
  * sequence and attends to the rows up to its own.  A token t >= n_new[b], or at a row outside [0, max_len), is not there: its out is 0.
+ * lens counts rows that have their room: where bkPagesGrow refused a sequence (ok = 0) n_new must be 0, or its tokens take the place of rows that
+ * are there, which other sequences may share.  For one token a sequence, ok itself can be n_new.
  * The first prefix_rows rows are the same for all sequences: their whole pages are read through sequence 0's table, once for all.
  *   fused_norm_rope = 1: qg bf16 [T*B][Hq][2*HD] = q | gate; q and k get their head RMSNorm (times 1 + w) and the partial rotary at the
  *     token's row, in f32 with one rounding to bf16; k and v [T*B][Hkv][HD] are stored into the pages; out = attention * sigmoid(gate).
