@@ -89,12 +89,15 @@ class SharedPrompt:
         return self.out.ptr
 
     def prompt(self, x: int, rows: int, adapter: int = -1) -> None:
-        """The prompt's rows x bf16 [rows][H] into sequence 0."""
+        """The prompt's rows x bf16 [rows][H] into sequence 0.  Waits for each chunk's room; where the pool has none left, the chunks before are
+        the prompt and RuntimeError says how many rows that is."""
         for at in range(0, rows, self.CHUNK):
             n = min(self.CHUNK, rows - at)
             self.pool.grow(self._list("seqs", [0]), self._list("add", [n]), 1, self.ok.ptr)
+            if not self.ok.download(np.int32, (1,))[0]:
+                raise RuntimeError(f"no room for the prompt: {at} of {rows} rows are in")
             self._layer(x + at * self.cfg.hidden * 2, n, 1, n, 0, 0, [adapter] * n, 0)
-        self.prompt_rows += rows
+            self.prompt_rows += n
 
     def fork(self, requests: Sequence[int]) -> None:
         """These requests begin behind the prompt."""

@@ -93,3 +93,14 @@ def test_a_step_past_the_longest_sequence_changes_nothing(layer, x):
     after, lens = held(s)
     assert lens == [62, 64, 0, 64] and not attended(s).any()
     assert all(np.array_equal(a, b) for a, b in zip(before, after))
+
+
+@pytest.mark.parametrize("max_rows,n_pages", [(112, 4), (64, 20)])    # the pages run out, or the table's row
+def test_a_prompt_that_does_not_fit_says_so_and_keeps_what_did(layer, x, max_rows, n_pages):
+    s, fits = make(layer, max_rows, n_pages), make(layer, 112, 20)
+    fits.prompt(x.ptr, 64)
+    with pytest.raises(RuntimeError, match="64 of 100"):
+        s.prompt(x.ptr, 100)
+    assert R.cuSync() == 0 and s.prompt_rows == 64
+    rows, lens = held(s)
+    assert lens[0] == 64 and np.array_equal(rows[0], held(fits)[0][0])
