@@ -99,10 +99,14 @@ class SharedPrompt:
             self._layer(x + at * self.cfg.hidden * 2, n, 1, n, 0, 0, [adapter] * n, 0)
             self.prompt_rows += n
 
-    def fork(self, requests: Sequence[int]) -> None:
-        """These requests begin behind the prompt."""
-        self.pool.fork(self._list("src", [0] * len(requests)), self._list("seqs", [r + 1 for r in requests]), len(requests), self.ok.ptr)
-        self.active[list(requests)] = True
+    def fork(self, requests: Sequence[int]) -> np.ndarray:
+        """These requests begin behind the prompt.  Waits for the pool's answer: which of them were served (a prompt that ends inside a page takes
+        a page for each); the others stay as they were."""
+        n = len(requests)
+        self.pool.fork(self._list("src", [0] * n), self._list("seqs", [r + 1 for r in requests]), n, self.ok.ptr)
+        served = self.ok.download(np.int32, (n,)) != 0
+        self.active[np.asarray(requests, np.int64)[served]] = True
+        return served
 
     def step(self, x: int, adapters: Sequence[int], share: bool = True) -> int:
         """One token of every active request: x bf16 [requests][H] -> out bf16 [requests][H] (rows of others: what the residual gives).

@@ -104,3 +104,14 @@ def test_a_prompt_that_does_not_fit_says_so_and_keeps_what_did(layer, x, max_row
     assert R.cuSync() == 0 and s.prompt_rows == 64
     rows, lens = held(s)
     assert lens[0] == 64 and np.array_equal(rows[0], held(fits)[0][0])
+
+
+def test_a_request_whose_fork_found_no_page_is_not_active(layer, x):
+    s = make(layer, 64, 4)
+    s.prompt(x.ptr, 40)                      # three pages, the last one partial: every fork needs one
+    assert s.fork([1, 0, 2]).tolist() == [True, False, False]
+    assert s.active.tolist() == [False, True, False]
+    assert s.fork([1]).tolist() == [False] and s.active.tolist() == [False, True, False]     # (it is not empty)
+    s.step(x.ptr, ADAPTERS)
+    rows, lens = held(s)
+    assert lens == [40, 0, 41, 0] and not attended(s)[[0, 2]].any() and attended(s)[1].any()
