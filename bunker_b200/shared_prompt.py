@@ -90,7 +90,10 @@ class SharedPrompt:
 
     def prompt(self, x: int, rows: int, adapter: int = -1) -> None:
         """The prompt's rows x bf16 [rows][H] into sequence 0.  Waits for each chunk's room; where the pool has none left, the chunks before are
-        the prompt and RuntimeError says how many rows that is."""
+        the prompt and RuntimeError says how many rows that is.  Only while no request is active: the requests' steps read the prompt's rows as
+        common ones, and those that have begun would not have the new ones."""
+        if self.active.any():
+            raise RuntimeError(f"the prompt cannot grow behind {int(self.active.sum())} active requests")
         for at in range(0, rows, self.CHUNK):
             n = min(self.CHUNK, rows - at)
             self.pool.grow(self._list("seqs", [0]), self._list("add", [n]), 1, self.ok.ptr)

@@ -115,3 +115,18 @@ def test_a_request_whose_fork_found_no_page_is_not_active(layer, x):
     s.step(x.ptr, ADAPTERS)
     rows, lens = held(s)
     assert lens == [40, 0, 41, 0] and not attended(s)[[0, 2]].any() and attended(s)[1].any()
+
+
+def test_a_prompt_cannot_grow_under_its_requests(layer, x):
+    """Rows added then would be read as common rows by requests that do not have them."""
+    s = make(layer, 96, 20)
+    s.prompt(x.ptr, 32)
+    s.fork([0, 1])
+    before, lens = held(s)
+    with pytest.raises(RuntimeError, match="request"):
+        s.prompt(x.ptr, 16)
+    after, now = held(s)
+    assert s.prompt_rows == 32 and now == lens and all(np.array_equal(a, b) for a, b in zip(before, after))
+    s.drop([0, 1])
+    s.prompt(x.ptr, 16)
+    assert s.prompt_rows == 48 and s.fork([2]).all() and held(s)[1] == [48, 0, 0, 48]
