@@ -60,6 +60,11 @@ class SharedPrompt:
         self.lists[name].upload(np.asarray(values, np.int32))
         return self.lists[name].ptr
 
+    def _check_requests(self, requests: Sequence[int]) -> None:
+        for r in requests:
+            if not 0 <= r < self.n:
+                raise IndexError(f"request {r} of {self.n}")
+
     def _layer(self, x: int, cols: int, B: int, T: int, first_seq: int, n_new: int, ids: Sequence[int], prefix: int) -> int:
         """x bf16 [cols][H] of B sequences from first_seq on, T columns each -> out bf16 [cols][H] (device pointer)"""
         cfg, w, lo, H, hd = self.cfg, self.w, self.lora, self.cfg.hidden, self.hd
@@ -105,6 +110,7 @@ class SharedPrompt:
     def fork(self, requests: Sequence[int]) -> np.ndarray:
         """These requests begin behind the prompt.  Waits for the pool's answer: which of them were served (a prompt that ends inside a page takes
         a page for each); the others stay as they were."""
+        self._check_requests(requests)
         n = len(requests)
         self.pool.fork(self._list("src", [0] * n), self._list("seqs", [r + 1 for r in requests]), n, self.ok.ptr)
         served = self.ok.download(np.int32, (n,)) != 0
@@ -115,11 +121,14 @@ class SharedPrompt:
         """One token of every active request: x bf16 [requests][H] -> out bf16 [requests][H] (rows of others: what the residual gives).
         ``ok`` (int32 [requests], on the device) says who had room.  A request without room has no token in this step: its ok is its number of new
         tokens, so nothing is stored for it (the row before its next one may be the prompt's, which all share).  An inactive one has no rows."""
+        if len(adapters) != self.n:
+            raise ValueError(f"{len(adapters)} adapters for {self.n} requests")
         new = self.active.astype(np.int32)
         self.pool.grow(self._list("seqs", np.arange(1, self.n + 1)), self._list("add", new), self.n, self.ok.ptr)
         return self._layer(x, self.n, self.n, 1, 1, self.ok.ptr, adapters, self.prompt_rows if share and new[0] else 0)
 
     def drop(self, requests: Sequence[int]) -> None:
+        self._check_requests(requests)
         self.pool.free(self._list("seqs", [r + 1 for r in requests]), len(requests))
         self.active[list(requests)] = False
 

@@ -130,3 +130,20 @@ def test_a_prompt_cannot_grow_under_its_requests(layer, x):
     s.drop([0, 1])
     s.prompt(x.ptr, 16)
     assert s.prompt_rows == 48 and s.fork([2]).all() and held(s)[1] == [48, 0, 0, 48]
+
+
+def test_requests_that_are_none_are_refused(layer, x):
+    """Request -1 would be the prompt's own sequence."""
+    s = make(layer, 64, 20)
+    s.prompt(x.ptr, 32)
+    s.fork([0])
+    before, lens = held(s)
+    for bad in ([-1], [0, 3]):
+        with pytest.raises(IndexError):
+            s.drop(bad)
+        with pytest.raises(IndexError):
+            s.fork(bad)
+    with pytest.raises(ValueError):
+        s.step(x.ptr, ADAPTERS[:2])
+    after, now = held(s)
+    assert now == lens and all(np.array_equal(a, b) for a, b in zip(before, after)) and s.active.tolist() == [True, False, False]
