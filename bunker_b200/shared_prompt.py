@@ -166,8 +166,9 @@ def main() -> None:
     a = ap.parse_args()
     cfg = CONFIG_TINY
     w, lora = random_layer(cfg)
-    rows = a.prompt + a.steps + 1
-    layer = SharedPrompt(cfg, w, lora, a.requests, rows, n_pages=-(-rows // 16) + a.requests * (-(-a.steps // 16) + 2))
+    half = max(1, (a.steps - 2) // 2)
+    rows = a.prompt + 2 * (1 + half) + 1    # (both ways of reading the prompt, each with a step ahead of the timed ones, and one at the end)
+    layer = SharedPrompt(cfg, w, lora, a.requests, rows, n_pages=-(-a.prompt // 16) + a.requests * (-(-rows // 16) - a.prompt // 16))
     rng = synth.rng_for(1, 72)
     x = R.DeviceBuffer.from_numpy(synth.normal_bf16(rng, (max(a.prompt, a.requests), cfg.hidden)))
     layer.prompt(x.ptr, a.prompt)
@@ -176,7 +177,6 @@ def main() -> None:
     for share in (False, True):
         layer.step(x.ptr, adapters, share)      # warm
         e0, e1 = R.Event().record(), R.Event()
-        half = max(1, (a.steps - 2) // 2)
         for _ in range(half):
             layer.step(x.ptr, adapters, share)
         e1.record().synchronize()

@@ -147,3 +147,20 @@ def test_requests_that_are_none_are_refused(layer, x):
         s.step(x.ptr, ADAPTERS[:2])
     after, now = held(s)
     assert now == lens and all(np.array_equal(a, b) for a, b in zip(before, after)) and s.active.tolist() == [True, False, False]
+
+
+@pytest.mark.parametrize("steps", [1, 2, 3, 20])
+def test_the_command_has_room_for_its_steps(bk, monkeypatch, steps):
+    """Every step that the command takes is served."""
+    seen = []
+    step = S.SharedPrompt.step
+
+    def watched(self, *a, **kw):
+        out = step(self, *a, **kw)
+        seen.append(bool(self.ok.download(np.int32, (self.n,)).all()))
+        return out
+
+    monkeypatch.setattr(S.SharedPrompt, "step", watched)
+    monkeypatch.setattr("sys.argv", ["shared_prompt", "--requests", "4", "--prompt", "46", "--steps", str(steps)])
+    S.main()
+    assert seen and all(seen)
