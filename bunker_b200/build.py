@@ -16,7 +16,7 @@ LIB = os.path.join(HERE, "libbunker_cuda.so")
 TOK_LIB = os.path.join(HERE, "libbunker_tok.so")
 TOK_SRC = os.path.join(CSRC, "bk_tokenizer.cpp")
 SOURCES = ["bk_runtime.cu", "bk_gemv.cu", "bk_gemv_mma.cu", "bk_ops.cu", "bk_attn.cu", "bk_launch.cu", "bk_model.cu", "bk_comm.cu", "bk_persist.cu", "bk_quantize.cu", "bk_gemv_umma.cu", "bk_sample.cu", "bk_pages.cu", "bk_paged_attn.cu", "bk_lora.cu"]
-HEADERS = ["bk_common.cuh", "bk_internal.h", "bk_gemv_shared.cuh", "bk_gemv_dp4a.cuh", "bk_gdn.cuh",
+HEADERS = ["bk_common.cuh", "bk_internal.h", "bk_gemv_shared.cuh", "bk_gemv_dp4a.cuh", "bk_gdn.cuh", "bk_ring.h",
            os.path.join("..", "..", "include", "bunker_cuda.h"), os.path.join("..", "..", "include", "bunker_cuda_diag.h")]
 
 NVCC_FLAGS = [

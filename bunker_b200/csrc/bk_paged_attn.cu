@@ -14,6 +14,7 @@
 
 #include "bk_common.cuh"
 #include "bk_internal.h"
+#include "bk_ring.h"
 
 namespace {
 
@@ -413,17 +414,26 @@ BK_DEVINL bool elect_lane() {
   asm volatile("{ .reg .pred p; elect.sync _|p, 0xffffffff; selp.u32 %0, 1, 0, p; }" : "=r"(p));
   return p != 0;
 }
-// A wait of a warp that stays together.  Bounded by time (a poll may sleep): the first wait of a CTA that gives up, after 2^31 cycles, sets the
-// status word and `dead`, after which the others return at once and the kernel runs to its end.
-BK_DEVINL void bar_wait_warp(uint32_t bar, uint32_t parity, int* status, volatile int* dead) {
-  if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return;
+// A wait of a warp that stays together: whether the phase has completed.  Bounded by time (a poll may sleep): the first wait of a CTA that gives up, after
+// 2^31 cycles, sets the status word and `dead`, after which the others return at once and the kernel runs to its end.  Who was to arm a barrier, issue a copy
+// or MMAs after a wait that gave up does not, so that what is on its way can be waited for at the end.
+BK_DEVINL bool bar_wait_warp(uint32_t bar, uint32_t parity, int* status, volatile int* dead) {
+  if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
   const long long from = clock64();
 #pragma unroll 1
   do {
-    if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity) || *dead)) return;
+    const bool here = mbar_try_wait(bar, parity);
+    if (__all_sync(0xffffffffu, here || *dead)) return __all_sync(0xffffffffu, here);
   } while (__any_sync(0xffffffffu, clock64() - from < (1ll << 31)));
   *dead = 1;
   atomicExch(status, 10003 /* BK_ERR_TIMEOUT */);
+  return false;
+}
+// The end of a CTA where a wait gave up: no longer than 2^16 polls.
+BK_DEVINL void bar_settle(uint32_t bar, uint32_t parity) {
+#pragma unroll 1
+  for (int it = 0; it < (1 << 16) && !mbar_try_wait(bar, parity); it++) {
+  }
 }
 BK_DEVINL void tma_load(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
   asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar)
@@ -454,7 +464,7 @@ BK_DEVINL int stream_v(int i, int n) { return i < n - 1 ? 2 * i + 2 : 2 * n - 1;
 
 template <int kStages>
 struct TileShared {   // behind the tiles
-  uint64_t full[kStages], empty[kStages], q_here, q_empty, q_full, s_full[2], p_full[2], o_full[2];
+  uint64_t full[kStages], empty[kStages], q_here, q_empty, q_full, s_full[2], p_full[2], o_full[2], settled;
   float m_s[2][2][kRows];   // [tile & 1][half of the keys]: largest score
   int odd_from[3], odd_to[3];   // [piece mod 3]: keys between which values were not finite and were taken out, see there
   uint32_t tmem_slot;
@@ -505,6 +515,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
     mbar_init(smem_u32(&q_here), 1);
     mbar_init(smem_u32(&q_empty), 8);
     mbar_init(smem_u32(&q_full), 8);
+    mbar_init(smem_u32(&sh.settled), 1);
     for (int i = 0; i < 2; i++) {
       mbar_init(smem_u32(s_full + i), 1);
       mbar_init(smem_u32(p_full + i), 8);
@@ -564,6 +575,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
     return false;
   };
   Piece x;
+  int armed = 0;   // copies' barriers so far: of the ring, of the queries
 
   {
     if (warp == kCopyWarp) {
@@ -576,7 +588,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
       const uint32_t box_at = block * (kTile * 128) + chunk * P.box_rows * 128;
       int stage = 0;
       uint32_t parity = 1;
-      while (next_piece(&x)) {
+      bool going = true;
+      while (going && next_piece(&x)) {
         const Job q = x.q;
         const int t0 = x.t0, t1 = x.t1, key1 = x.key1;
         const int* table = p.table + (size_t)max(q.seq, 0) * p.max_pages;
@@ -587,7 +600,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
           return page >= 0 && page < p.n_pages ? (page * p.Hkv + q.kvh) * p.page_rows + key % p.page_rows : no_row;
         };
         auto load = [&](const CUtensorMap* map, int row) {
-          bar_wait_warp(smem_u32(empty + stage), parity, P.status, dead);
+          if (!bar_wait_warp(smem_u32(empty + stage), parity, P.status, dead)) return false;
+          armed++;
           const uint32_t bar = smem_u32(full + stage);
           if (lane == 0) mbar_expect_tx(bar, C::kStage);
           __syncwarp();
@@ -596,25 +610,15 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
             stage = 0;
             parity ^= 1u;
           }
+          return true;
         };
         int next = row_of_tile(t0), before = 0;
-        for (int i = t0; i <= t1; i++) {
+        for (int i = t0; going && i <= t1; i++) {
           const int row = next;
           next = row_of_tile(i + 1);
-          if (i < t1) load(&P.k_map, row);
-          if (i > t0) load(&P.v_map, before);
+          if (i < t1) going = load(&P.k_map, row);
+          if (going && i > t0) going = load(&P.v_map, before);
           before = row;
-        }
-      }
-      // the last copies have landed before the CTA ends: the MMAs waited for them (or the waits below do, where a wait gave up)
-      if (*dead) {
-        for (int i = 0; i < C::kStages; i++) {
-          for (int it = 0; it < (1 << 16) && !mbar_try_wait(smem_u32(full + stage), parity ^ 1u); it++) {
-          }
-          if (++stage == C::kStages) {
-            stage = 0;
-            parity ^= 1u;
-          }
         }
       }
     } else if (warp == kMmaWarp) {
@@ -633,7 +637,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
           parity ^= 1u;
         }
       };
-      auto wait = [&](uint32_t bar, uint32_t par) { bar_wait_warp(bar, par, P.status, dead); };
+      bool going = true;
+      auto wait = [&](uint32_t bar, uint32_t par) { going = bar_wait_warp(bar, par, P.status, dead) && going; };
       auto scores = [&](int half, uint64_t desc, int t) {   // (the probabilities that this buffer held have been multiplied: MMAs run in order)
         const uint32_t d = tmem + C::kS + (t & 1) * kTile;
 #pragma unroll
@@ -652,10 +657,11 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
           else tc_mma<true>(tmem + C::kO, p_at + ks * 8, desc + ks * (2048 / 16), kShapeO);
         }
       };
-      while (next_piece(&x)) {
+      while (going && next_piece(&x)) {
         const int n = x.t1 - x.t0;
         wait(full0 + stage * 8, parity);
         wait(smem_u32(&q_full), pieces & 1);
+        if (!going) break;
         tc_after();
         // the first tile's scores
         if (elect_lane()) {
@@ -678,6 +684,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
           const uint32_t v_bar = empty0 + stage * 8;
           wait(p_full0 + (t & 1) * 8, (t >> 1) & 1);
           wait(full0 + stage * 8, parity);
+          if (!going) break;
           tc_after();
           next_stage();
           if (elect_lane()) {
@@ -707,7 +714,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
         const bool common = x.q.seq < 0;
         const CUtensorMap* map = P.q_map + common;
         const int rows = P.q_rows[common], row = common ? x.q.kvh * p.B * p.T * (p.Hq / p.Hkv) : (x.q.kvh * p.B + x.q.seq) * p.T * (p.Hq / p.Hkv);
-        bar_wait_warp(smem_u32(&q_empty), parity, P.status, dead);
+        if (!bar_wait_warp(smem_u32(&q_empty), parity, P.status, dead)) break;
+        armed++;
         if (lane == 0) mbar_expect_tx(smem_u32(&q_here), rows * HD * 2);
         __syncwarp();
         if (lane < HD / 64) tma_load(smem_u32(q_s) + lane * (kRows * 128), map, lane * 64, row + x.q.mt * kRows, smem_u32(&q_here));
@@ -907,6 +915,21 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
   tc_before();
   __syncthreads();
   tc_after();
+  // The MMAs have waited for every copy, and the rows for every MMA, unless a wait gave up: then what is on its way is waited for here.
+  if (*dead) {
+    if (warp == kCopyWarp) {
+      for (int i = 0; i < C::kStages; i++) {
+        const int last = bk_ring_last_parity(armed, i, C::kStages);
+        if (last >= 0) bar_settle(smem_u32(full + i), last);
+      }
+    } else if (warp == kQueryWarp) {
+      if (armed) bar_settle(smem_u32(&q_here), bk_ring_last_parity(armed, 0, 1));
+    } else if (warp == kMmaWarp) {
+      if (elect_lane()) tc_commit(smem_u32(&sh.settled));
+      bar_settle(smem_u32(&sh.settled), 0);
+    }
+    __syncwarp();
+  }
   if (warp == kMmaWarp) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
 }
 
