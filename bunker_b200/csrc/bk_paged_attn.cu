@@ -975,7 +975,11 @@ __global__ void __launch_bounds__(256 * kSlices) paged_merge_kernel(const PagedP
     }
     float mn = m;
 #pragma unroll
-    for (int k = 0; k < U; k++) mn = fmaxf(mn, x[k].x);
+    for (int k = 0; k < U; k++) {
+      // Maxima pass over NaN, sums do not: a piece with a sum and no maximum has NaN scores only, and any maximum will do to bring that in.
+      if (x[k].x == -INFINITY && __fadd_rn(x[k].y, x[k].z) != 0.0f) x[k].x = 0.0f;
+      mn = fmaxf(mn, x[k].x);
+    }
     if (mn == -INFINITY) continue;
     const float f = exp2_approx(__fsub_rn(m, mn));   // (m = -inf: 0)
     l = __fmul_rn(l, f);
@@ -997,7 +1001,7 @@ __global__ void __launch_bounds__(256 * kSlices) paged_merge_kernel(const PagedP
 #pragma unroll
   for (int k = 0; k < kSlices; k++) M = fmaxf(M, ml_s[k][g].x);
   float sum = 0.0f, y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-  if (M != -INFINITY) {
+  if (here) {   // (a token sees its own row at least: without a maximum, -inf, its scores are all -inf, and 0 / 0 it is)
 #pragma unroll
     for (int k = 0; k < kSlices; k++) {
       const float2 x = ml_s[k][g];
