@@ -459,6 +459,35 @@ BK_DEVINL uint32_t odd_value(uint32_t sum, uint16_t v) {
   return (v & 0x7f80u) == 0x7f80u ? __float_as_uint(__fadd_rn(__uint_as_float(sum), bk_bf16_to_f32(v))) : sum;
 }
 
+// Adds to a row's sums of 32 dims, d and on, the values of keys k0 to k1 - 1 below the row's limit that are not finite.  Whole warps, of one job.
+// (A call: in line it is in the way of every piece, 0.2 us of a short call.)
+__device__ __noinline__ void add_odd_values(const PagedParams& p, const Job& q, int HD, int d, int k0, int k1, int limit, uint32_t* o) {
+  const int lane = threadIdx.x & 31;
+  auto values = [&](int key) {   // (nullptr: rows of zeros)
+    const int page = __ldg(p.table + (size_t)max(q.seq, 0) * p.max_pages + key / p.page_rows);
+    return page >= 0 && page < p.n_pages ? p.v_pages + (((size_t)page * p.Hkv + q.kvh) * p.page_rows + key % p.page_rows) * HD + d : nullptr;
+  };
+#pragma unroll 1
+  for (int k = k0; k < k1; k += 8) {   // eight keys at once, a lane eight dims of one
+    uint4 v = make_uint4(0, 0, 0, 0);
+    if (k + (lane >> 2) < k1) {
+      const uint16_t* at = values(k + (lane >> 2));
+      if (at) v = *reinterpret_cast<const uint4*>(at + (lane & 3) * 8);
+    }
+    const bool odd = ((v.x ^ finite_pair(v.x)) | (v.y ^ finite_pair(v.y)) | (v.z ^ finite_pair(v.z)) | (v.w ^ finite_pair(v.w))) != 0;
+    uint32_t found = __ballot_sync(0xffffffffu, odd);
+    while (found) {
+      const int i = (__ffs(found) - 1) >> 2;
+      found &= ~(15u << (4 * i));
+      const uint16_t* at = values(k + i);
+      if (k + i < limit) {
+#pragma unroll
+        for (int y = 0; y < 32; y++) o[y] = odd_value(o[y], at[y]);
+      }
+    }
+  }
+}
+
 // positions in the stream of a piece's tiles: K0, K1, V0, K2, V1, ..., V(n-1)
 BK_DEVINL int stream_v(int i, int n) { return i < n - 1 ? 2 * i + 2 : 2 * n - 1; }
 
@@ -893,15 +922,30 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
           for (int d = group * (HD / 64); d < (group + 1) * (HD / 64); d++) {
             uint32_t o[32];
             tmem_ld32(lanes + C::kO + d * 32, o);
-            if (mine) {
-              const int last = min(limit - 1, *reinterpret_cast<volatile int*>(&sh.odd_to[odd]));
-              for (int key = *reinterpret_cast<volatile int*>(&sh.odd_from[odd]); key <= last; key++) {   // (nearly always none)
-                const int page = __ldg(p.table + (size_t)max(q.seq, 0) * p.max_pages + key / p.page_rows);
-                const uint16_t* v = p.v_pages + (((size_t)page * p.Hkv + q.kvh) * p.page_rows + key % p.page_rows) * HD + d * 32;
-                if (page >= 0 && page < p.n_pages)
+            int k0 = *reinterpret_cast<volatile int*>(&sh.odd_from[odd]), k1 = *reinterpret_cast<volatile int*>(&sh.odd_to[odd]) + 1;
+            // Where all rows see a value that is not finite it went through the MMAs, and what the two parts of a probability, one of them zero or
+            // negative, make of an infinity is NaN.  Sums that are NaN are made anew, of all the piece's values that are not finite; if there are none
+            // that this row sees, it is the scores that are NaN.
+            const float2 zero = make_float2(0.0f, 0.0f);
+            float2 probe[4] = {zero, zero, zero, zero};   // stay zeros while sums are finite (one chain is 0.1 us more)
 #pragma unroll
-                  for (int y = 0; y < 32; y++) o[y] = odd_value(o[y], v[y]);
-              }
+            for (int y = 0; y < 16; y++) probe[y & 3] = bk_fma2(make_float2(__uint_as_float(o[2 * y]), __uint_as_float(o[2 * y + 1])), zero, probe[y & 3]);
+            const float2 all = bk_add2(bk_add2(probe[0], probe[1]), bk_add2(probe[2], probe[3]));
+            const bool anew = __any_sync(0xffffffffu, mine && limit > 0 && __fadd_rn(all.x, all.y) != 0.0f);
+            if (anew) {
+              k0 = q.key0 + t0 * kTile;
+              k1 = min(key1, k0 + n * kTile);
+            }
+            if (k0 < k1) {   // (nearly never)
+              uint32_t z[32];
+#pragma unroll
+              for (int y = 0; y < 32; y++) z[y] = anew && isnan(__uint_as_float(o[y])) ? 0u : o[y];
+              add_odd_values(p, q, HD, d * 32, k0, k1, limit, z);
+#pragma unroll
+              for (int y = 0; y < 32; y++)
+                if (!(isnan(__uint_as_float(o[y])) && isfinite(__uint_as_float(z[y])))) o[y] = z[y];
+            }
+            if (mine) {
 #pragma unroll
               for (int y = 0; y < 32; y += 4) o_to[(size_t)(d * 8 + y / 4) * rows] = make_uint4(o[y], o[y + 1], o[y + 2], o[y + 3]);
             }
@@ -931,6 +975,12 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
     __syncwarp();
   }
   if (warp == kMmaWarp) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+}
+
+// 2^x, x <= 0, as the weight of a piece: never zero, so that what is infinite stays so (NaN stays NaN)
+BK_DEVINL float weight_of(float x) {
+  const float w = exp2_approx(x);
+  return w < 1.17549435e-38f ? 1.17549435e-38f : w;
 }
 
 // The pieces' results of a token row and KV head together: a CTA takes 64 dims of the group's heads, whose rows lie side by side in the
@@ -981,14 +1031,14 @@ __global__ void __launch_bounds__(256 * kSlices) paged_merge_kernel(const PagedP
       mn = fmaxf(mn, x[k].x);
     }
     if (mn == -INFINITY) continue;
-    const float f = exp2_approx(__fsub_rn(m, mn));   // (m = -inf: 0)
+    const float f = weight_of(__fsub_rn(m, mn));   // (m = -inf: of zeros)
     l = __fmul_rn(l, f);
     o.x = __fmul_rn(o.x, f); o.y = __fmul_rn(o.y, f); o.z = __fmul_rn(o.z, f); o.w = __fmul_rn(o.w, f);
     m = mn;
 #pragma unroll
     for (int k = 0; k < U; k++)
       if (x[k].x != -INFINITY) {
-        const float w = exp2_approx(__fsub_rn(x[k].x, m));
+        const float w = weight_of(__fsub_rn(x[k].x, m));
         l = fmaf(w, __fadd_rn(x[k].y, x[k].z), l);
         o.x = fmaf(w, v[k].x, o.x); o.y = fmaf(w, v[k].y, o.y); o.z = fmaf(w, v[k].z, o.z); o.w = fmaf(w, v[k].w, o.w);
       }
@@ -1005,7 +1055,7 @@ __global__ void __launch_bounds__(256 * kSlices) paged_merge_kernel(const PagedP
 #pragma unroll
     for (int k = 0; k < kSlices; k++) {
       const float2 x = ml_s[k][g];
-      const float w = exp2_approx(__fsub_rn(x.x, M));
+      const float w = weight_of(__fsub_rn(x.x, M));
       const float4 v = k ? o_s[k - 1][d * 16 + g] : o;
       sum = fmaf(w, x.y, sum);
       y[0] = fmaf(w, v.x, y[0]); y[1] = fmaf(w, v.y, y[1]); y[2] = fmaf(w, v.z, y[2]); y[3] = fmaf(w, v.w, y[3]);

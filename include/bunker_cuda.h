@@ -314,7 +314,8 @@ BK_API int32_t bkPagesCompact(const bkPages* pool, uint64_t table_out, uint64_t 
  *     token's row, in f32 with one rounding to bf16; k and v [T*B][Hkv][HD] are stored into the pages; out = attention * sigmoid(gate).
  *   fused_norm_rope = 0: qg holds ready q [T*B][Hq][HD]; k, v (ready, or both 0 where the pages have them) are stored as they are;
  *     gate bf16 [T*B][Hq][HD], or 0 for none.
- * A token whose scores are not numbers, or all -inf, gets NaN, as the softmax of its scores is.
+ * A token whose scores are not numbers, or all -inf, gets NaN, as the softmax of its scores is.  A value that is not finite makes the dim infinite, or NaN,
+ * of the tokens that see it, whatever its weight, and of no others.
  * out bf16 [T*B][Hq*HD].  Rows of a page past a sequence's end are never part of a result, whatever they hold.  Nothing is stored
  * through a table entry that names no page; read, such an entry is rows of zeros (the calls above leave none among a sequence's rows). */
 typedef struct bkPagedAttnArgs {

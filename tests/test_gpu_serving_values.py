@@ -85,3 +85,48 @@ def test_infinite_scores(bk, HD):
     c.q[:] = bf16(np.full(c.q.shape, 0.25))
     c.kp[c.table[1, 0], 0, 3, 9] = INF
     assert np.isnan(as_defined(c)[1]).all()
+
+
+# ---- values that are not finite, seen by every row of a tile ---------------------------------------
+
+def put(c, b, key, dim, what):
+    c.vp[c.table[b, key // c.rows], :, key % c.rows, dim] = what
+
+
+@pytest.mark.parametrize("HD,rows", [(128, 16), (256, 64)])
+@pytest.mark.parametrize("std", [1.0, 16.0])     # (16: one key has nearly all of the weight, and some have none in 32 bits)
+def test_values_that_are_infinite_for_single_tokens(bk, HD, rows, std):
+    # one sequence, keys in the first, a middle and the last tile, and the new row itself
+    c = Case(141, 1, 1, 0, [700], HD=HD, Hq=8, Hkv=1, rows=rows, fused=False, std=std)
+    for key, dim, what in ((0, 0, INF), (33, 1, NINF), (300, 2, INF), (301, 2, INF), (640, HD - 1, NINF), (10, 40, INF), (600, 40, NINF), (77, 64, NAN), (698, 65, INF)):
+        put(c, 0, key, dim, what)
+    c.v[0, 0, 70] = INF
+    for key in (33, 300, 640):                      # scores of four times the size: far below or far above the others
+        at = c.table[0, key // rows], slice(None), key % rows
+        c.kp[at] = bf16(4 * val(c.kp[at]))
+    w = as_defined(c)
+    assert (w[:, :, [0, 2, 65, 70]] == np.inf).all() and (w[:, :, [1, HD - 1]] == -np.inf).all() and np.isnan(w[:, :, [40, 64]]).all()
+    # common rows of several sequences, rows of one sequence, and both at once
+    c = Case(142, 5, 1, 450, [1, 100, 20, 0, 64], HD=HD, Hq=12, Hkv=2, rows=rows, fused=False, std=std)
+    for b, key, dim, what in ((0, 5, 3, INF), (0, 200, 4, NINF), (0, 430, 60, NAN), (1, 500, 3, INF), (1, 460, 4, INF), (4, 455, 9, NINF)):
+        put(c, b, key, dim, what)
+    w = as_defined(c)
+    assert (w[1, :, 3] == np.inf).all() and np.isnan(w[1, :, 4]).all() and (w[4, :, 9] == -np.inf).all()
+
+
+@pytest.mark.parametrize("HD", [128, 256])
+def test_values_that_are_infinite_for_pieces_of_prompts(bk, HD):
+    """The same row of V does the same in tiles that all rows see and in those that some see."""
+    T = 12
+    c = Case(151, 2, T, 300, [140, 12], HD=HD, Hq=6, Hkv=1, rows=32, fused=False)
+    for key, dim, what in ((3, 0, INF), (299, 1, NINF), (330, 2, INF), (420, 3, NINF), (3, 5, INF), (425, 5, NINF)):
+        put(c, 0, key, dim, what)
+    c.v[7 * 2, 0, 8], c.v[9 * 2 + 1, 0, 9] = NINF, INF
+    assert not np.isfinite(as_defined(c)).all()
+
+
+def test_values_that_are_infinite_in_row_tiles_cut_at_the_same_keys(bk):
+    c = Case(161, 2, 70, 1300, [70, 75], new=[70, 31], Hq=16, Hkv=2, HD=256, rows=128, fused=False)
+    for key, dim, what in ((0, 0, INF), (640, 1, NINF), (1200, 2, INF), (1310, 3, INF), (64, 200, NINF)):
+        put(c, 0, key, dim, what)
+    as_defined(c)
