@@ -5,7 +5,7 @@
 // of requests that share it.  Both products are m16n8k16 MMAs on fragments that lanes load from memory as they lie: the order of the
 // contraction's index is free as long as both operands have the same, so a lane takes 8 or 16 consecutive bytes of a row.  (With one row of weights
 // a thread, or a few lanes, and FMAs, unpacking and reducing were 200 instructions for 32 rows and a column.)  x and the weights are
-// bf16, exact; u goes in as three bf16 matrices, what is left of its 24 bits after each rounding in the next.  Sums in f32, the parts of K added
+// bf16, exact; u goes in as three bf16 matrices, eight of its 24 bits in each.  Sums in f32, the parts of K added
 // in ascending order: the same call gives the same bits.
 #include <string.h>
 
@@ -125,13 +125,19 @@ __global__ void __launch_bounds__(kThreads, 2) lora_shrink_kernel(const __grid_c
   }
 }
 
-// u as three bf16 values; one that is not finite stays whole in the first
+// u as three bf16 values, eight of its 24 bits each, cut off: none has another sign than u, and where a part would be zero beside a u that is not it is the
+// least normal value, 2^-126.  So an infinite weight, or an infinite u, makes the sum of the products infinite and not NaN (inf * 0, inf - inf).
 BK_DEVINL void split3(float u, uint16_t (&o)[3]) {
-  o[0] = bk_f32_to_bf16(u);
+  const uint32_t bits = __float_as_uint(u);
+  o[0] = isnan(u) ? 0x7fc0 : bits >> 16;
   const float r = isfinite(u) ? __fsub_rn(u, bk_bf16_to_f32(o[0])) : 0.0f;
-  const bool sound = isfinite(r);   // (rounding may pass the largest f32)
-  o[1] = sound ? bk_f32_to_bf16(r) : 0;
-  o[2] = sound ? bk_f32_to_bf16(__fsub_rn(r, bk_bf16_to_f32(o[1]))) : 0;
+  o[1] = __float_as_uint(r) >> 16;
+  o[2] = __float_as_uint(__fsub_rn(r, bk_bf16_to_f32(o[1]))) >> 16;
+  if (u != 0.0f) {
+#pragma unroll
+    for (int t = 0; t < 3; t++)
+      if ((o[t] & 0x7fff) == 0) o[t] = (bits >> 16 & 0x8000) | 0x0080;
+  }
 }
 
 template <bool F32>

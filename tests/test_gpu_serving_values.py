@@ -1,4 +1,4 @@
-"""Attention over pages where values are not finite.
+"""Attention over pages and adapters where values are not finite.
 
 What is infinite or NaN by the definition (64 bits) is the same infinity or NaN in the result, and nothing else is.  The rest is held to the
 tolerances of the ready-query form: 2^-8 |o| for the rounding of the output and 2^-13 of the largest |v|.
@@ -8,7 +8,7 @@ import pytest
 
 from bunker_b200 import ops
 from bunker_b200 import runtime as R
-from tests.test_gpu_serving import Case, bf16, val
+from tests.test_gpu_serving import Case, bf16, lora_case, val
 
 pytestmark = pytest.mark.gpu
 
@@ -130,3 +130,39 @@ def test_values_that_are_infinite_in_row_tiles_cut_at_the_same_keys(bk):
     for key, dim, what in ((0, 0, INF), (640, 1, NINF), (1200, 2, INF), (1310, 3, INF), (64, 200, NINF)):
         put(c, 0, key, dim, what)
     as_defined(c)
+
+
+# ---- adapters -------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("B,n_adapters,ids", [(1, 2, [1]), (2, 2, [1, 1]), (3, 5, [1, 4, 1]), (4, 2, [1, 0, 1, 1]), (13, 3, [1] * 11 + [0, -1])])
+@pytest.mark.parametrize("rank", [8, 24, 32, 64, 72, 128])
+@pytest.mark.parametrize("f32", [True, False])
+def test_a_weight_that_is_infinite_makes_its_row_infinite(bk, B, n_adapters, ids, rank, f32):
+    K, rows = 264, [300]
+    args, keep, want, (dx, di, ds, scratch) = lora_case(rank + B, B, K, rows, rank, n_adapters, ids, f32)
+    (dA, dM, dbase), out, ld, n = keep[0]
+    A, M, x = dA.download(np.uint16, (n_adapters, rank, K)), dM.download(np.uint16, (n_adapters, n, rank)), dx.download(np.uint16, (B, K))
+    A[1, rank - 1] = bf16(np.full(K, 0.5))
+    x[0] = bf16(np.ones(K) * 0.25)               # u of the last row of A is 33 exactly: a bf16 value, whose other parts are zeros
+    M[1, 0, rank - 1], M[1, 17, 3], M[1, 299, 0], M[1, 299, rank - 1], M[1, 40, 5] = INF, NINF, INF, NINF, NAN
+    for d, a in ((dA, A), (dM, M), (dx, x)):
+        d.upload(a)
+    base = dbase.download(np.float32 if f32 else np.uint16, (B, ld))
+    scale = ds.download(np.float32, (n_adapters,))
+    y = base.astype(np.float64) if f32 else val(base)
+    mag = np.abs(y)
+    with np.errstate(invalid="ignore"):
+        for b, a in enumerate(ids):
+            if a >= 0:
+                y[b] += float(scale[a]) * (val(M[a]) @ (val(A[a]) @ val(x[b])))
+                mag[b] += float(scale[a]) * (np.abs(val(M[a])) @ (np.abs(val(A[a])) @ np.abs(val(x[b]))))
+    assert y[0, 0] == np.inf and np.isnan(y[0, 40])
+    ops.lora(args)
+    assert R.cuSync() == 0, R.last_error()
+    raw = out.download(np.uint32 if f32 else np.uint16, (B, ld))
+    got = raw.view(np.float32).astype(np.float64) if f32 else val(raw)
+    assert np.array_equal(np.isnan(got), np.isnan(y))
+    fine = np.isfinite(y)
+    assert np.array_equal(got[~fine & ~np.isnan(y)], y[~fine & ~np.isnan(y)]) and np.isfinite(got[fine]).all()
+    got, y, mag = got[fine], y[fine], mag[fine]
+    assert (np.abs(got - y) <= (K + rank + 4) * 2.0 ** -24 * mag + (0 if f32 else 2.0 ** -8 * np.abs(y))).all()
