@@ -1,7 +1,8 @@
-"""Attention over pages and adapters where values are not finite.
+"""Attention over pages and adapters where values are not finite, and where many row tiles share a long prefix.
 
 What is infinite or NaN by the definition (64 bits) is the same infinity or NaN in the result, and nothing else is.  The rest is held to the
-tolerances of the ready-query form: 2^-8 |o| for the rounding of the output and 2^-13 of the largest |v|.
+tolerances of the ready-query form: 2^-8 |o| for the rounding of the output and 2^-13 of the largest |v|.  Two results from the same
+bits of q, k and v by two plans are each within that of the exact one: 2^-7 |o| + 2^-12 of the largest |v| of one another.
 """
 import numpy as np
 import pytest
@@ -166,3 +167,31 @@ def test_a_weight_that_is_infinite_makes_its_row_infinite(bk, B, n_adapters, ids
     assert np.array_equal(got[~fine & ~np.isnan(y)], y[~fine & ~np.isnan(y)]) and np.isfinite(got[fine]).all()
     got, y, mag = got[fine], y[fine], mag[fine]
     assert (np.abs(got - y) <= (K + rank + 4) * 2.0 ** -24 * mag + (0 if f32 else 2.0 ** -8 * np.abs(y))).all()
+
+
+# ---- row tiles that are cut at the same common keys ----------------------------------------------
+
+LONG = [(64, 1, 150, 2000, [150], None, 8, 1, 128, 64), (65, 2, 70, 1300, [70, 75], [70, 31], 16, 2, 256, 128), (63, 1, 150, 0, [600], None, 8, 1, 128, 16),
+        (67, 40, 1, 2500, [1 + 7 * (i % 11) for i in range(40)], None, 8, 1, 256, 64)]
+
+
+@pytest.mark.parametrize("seed,B,T,prefix,own_rows,new,Hq,Hkv,HD,rows", LONG)
+def test_attention_of_many_row_tiles_with_ready_queries(bk, seed, B, T, prefix, own_rows, new, Hq, Hkv, HD, rows):
+    """The plan that cuts several row tiles at the same keys, held to the bound without the norm's roundings: a tile of keys left out or taken
+    twice moves the result by many times that (tests/test_serving_cpu.py)."""
+    Case(seed, B, T, prefix, own_rows, new=new, Hq=Hq, Hkv=Hkv, HD=HD, rows=rows, fused=False).check()
+
+
+@pytest.mark.parametrize("seed,B,T,prefix,own_rows,new,Hq,Hkv,HD,rows", [c for c in LONG if c[3]])
+def test_attention_of_many_row_tiles_is_the_same_whatever_is_shared(bk, seed, B, T, prefix, own_rows, new, Hq, Hkv, HD, rows):
+    """The same with norm and rotation: both ways read the same bits of q, k and v."""
+    c = Case(seed, B, T, prefix, own_rows, new=new, Hq=Hq, Hkv=Hkv, HD=HD, rows=rows)
+    got = []
+    for P in (prefix, 0, prefix // 2):
+        ops.paged_attn(c.args(prefix_rows=P))
+        assert R.cuSync() == 0, R.last_error()
+        got.append(val(c.out.download(np.uint16, (T * B, Hq, HD))))
+    vmax = np.abs(val(c.vp)[np.isfinite(val(c.vp))]).max()
+    vmax = max(vmax, np.abs(val(c.v)).max())
+    for g in got[1:]:
+        assert (np.abs(g - got[0]) <= 2.0 ** -7 * np.abs(got[0]) + 2.0 ** -12 * vmax).all()

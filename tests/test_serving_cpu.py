@@ -1,6 +1,7 @@
 """Host side of the paged cache, the attention over it and the adapters: struct layouts and argument packing, without a GPU."""
 import ctypes as C
 
+import numpy as np
 import pytest
 
 from bunker_b200 import ops, pages
@@ -48,3 +49,21 @@ def test_the_plan_of_the_example_is_refused_for_too_many_requests():
     for n in (0, 65):
         with pytest.raises(ValueError):
             SharedPrompt(CONFIG_TINY, {}, {"rank": 8, "n_adapters": 1}, n, 100, 10)
+
+
+@pytest.mark.parametrize("keys,HD", [(2150, 128), (1375, 256), (2577, 256)])
+def test_the_bound_of_ready_queries_sees_a_tile_of_keys(keys, HD):
+    """What the tests of attention over pages with ready queries allow (2^-8 |o| + 2^-13 of the largest |v|), against an oracle that leaves out a tile of
+    64 keys, or 16 keys, or takes them twice: every row of queries has values outside."""
+    rng = np.random.default_rng(keys)
+    k, v, q = (rng.normal(0, 1, (n, HD)) for n in (keys, keys, 48))
+    s = q @ k.T / np.sqrt(HD)
+    w = np.exp(s - s.max(1, keepdims=True))
+    o = w @ v / w.sum(1, keepdims=True)
+    tol = 2.0 ** -8 * np.abs(o) + 2.0 ** -13 * np.abs(v).max()
+    for first, n in [(64 * i, 64) for i in range(keys // 64)] + [(64 * i + 48, 16) for i in range(keys // 64)]:
+        for times in (0, 2):
+            z = w.copy()
+            z[:, first:first + n] *= times
+            wrong = z @ v / z.sum(1, keepdims=True)
+            assert (np.abs(wrong - o) > tol).any(1).all(), (first, n, times)
