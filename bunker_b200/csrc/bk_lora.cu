@@ -153,7 +153,7 @@ constexpr int kAhead = KS <= 4 ? 2 : 1;   // tiles requested ahead where one or 
 // out = base + Bm (s u).  grid (p.per tiles of 256 rows, column).  A warp has 32 rows of a tile, KS steps of 16 of the rank; the next tiles' weights are
 // requested before these are used up.  WIDE (rank a multiple of 32): a lane's 16 bytes are two steps of a row.  Bound: memory; 64 requests of 42 adapters,
 // rank 32, 2 x 17,408 rows: 20 us, 111 MB at 5.5 TB/s.  Instructions come next: with three MMAs for the parts of u and a store for
-// each of a row tile's eighths, adapters of one or two columns were bound by them (460 a warp and 32 rows; the call 37 us, now 29.5).
+// each of a row tile's eighths, adapters of one or two columns were bound by them (460 a warp and 32 rows; the call 37 us, now 28.7).
 template <int KS, bool WIDE, bool F32>
 __global__ void __launch_bounds__(kThreads, KS <= 2 ? 3 : 2) lora_expand_kernel(const __grid_constant__ LoraParams p) {
   constexpr int R = KS * 16, SZ = F32 ? 4 : 2;

@@ -2,9 +2,9 @@
 //
 // o[r] = sum over keys j <= row of r of 2^(S[r][j] - m[r]) v[j] / sum of the same without v, S = q k^T scale log2(e).  Three launches: queries and new
 // rows (with the plan of the next), tiles of rows and keys, the pieces' results together.  Each hides little of the one before: a tile CTA takes all of an
-// SM's shared memory.  One sequence of 300 rows, 16 heads on 2: 15 us, nearly all of it the three launches' latency; 32 sequences behind 8,192
-// common rows: 29 us; 64 behind 32,768, 24 heads on 4: 92 us (110 where the power limit sets the clock for long), 0.34 of the bf16 rate by
-// the operations that the result needs, half of it again in operations done.
+// SM's shared memory.  One sequence of 300 rows, 16 heads on 2: 16 us, nearly all of it the three launches' latency; 32 sequences behind 8,192
+// common rows: 30 us; 64 behind 32,768, 24 heads on 4: 96 us, 114 where the power limit sets the clock for long: 0.33 and 0.28 of the bf16 rate by
+// the operations that the result needs, half of it again in operations done; 32 sequences of 8,192 rows that share nothing: 98 us, 5.5 TB/s.
 //
 // No counterpart in the reference (one contiguous cache of 128 rows, src/emitters.ts:188-226).
 #include <math.h>
@@ -223,7 +223,7 @@ BK_DEVINL void plan_jobs(const PagedParams& p, const Layout& L, uint8_t* scratch
     }
     ranges = __reduce_min_sync(0xffffffffu, best) & 255;
   }
-  const int c0 = L.n_p * ranges, C = max(c0 + 1, min(all_ctas, c0 + tiles_all));   // the line's CTAs: from c0 on, and every one of them has a tile to do
+  const int c0 = L.n_p * ranges, C = max(c0 + 1, min(all_ctas, c0 + tiles_all));   // the line's CTAs: from c0 on, no more than there are tiles (a short piece may be a job's start alone)
   for (int c = threadIdx.x; c <= C; c += kPrepThreads) {
     // (a quotient that is no whole number is at least 1 / C away from one, so the double below it is too)
     const int share = units < (1 << 23) ? (int)((unsigned int)units * (unsigned int)max(0, c - c0) / (unsigned int)(C - c0)) : (int)((double)units * (c - c0) / (C - c0));
@@ -292,7 +292,7 @@ BK_DEVINL bool row_at(const PagedParams& p, const Job& q, int i, int* b, int* t,
 }
 
 // One warp per (token row, head): y = x / sqrt(mean(x^2) + eps) (1 + w), then the rotation of pairs (d, d + rot_half), in f32; q heads to the scratch
-// buffer, k and v heads into their page, rounded to bf16: operands of the tensor cores (q's rounding is what the result's error is made of, 0.0023 of
+// buffer, k and v heads into their page, rounded to bf16: operands of the tensor cores (q's rounding is what the result's error is made of, 0.0024 of
 // its norm against 0.0017 for exact arithmetic rounded once).  The first CTA lays out the work of the next launch.  Bound: latency, 5 us for 32
 // sequences and 7 for 64 of 24 heads, most of it that CTA's.
 template <int HD>
@@ -515,7 +515,7 @@ constexpr int kCopyWarp = 8, kMmaWarp = 9, kQueryWarp = 10, kTileThreads = 352; 
 // rounded values and what rounding left (16 bits of the value; with 8 the result's error against exact arithmetic is 1.7 times that of its own rounding).
 // m is only moved when a score passes it by more than 2^8, since O must be rescaled then.  Row sums are in f32, by the lane that owns the row.
 // Bound: the MMAs, 1,650 of the 2,000 cycles that a step of 128 rows and 64 keys takes (HD 256): QK^T once, P V twice for the two matrices.  With P
-// rounded once the call of 64 sequences takes 85 us for 92 but the error is 0.0029.  Four stages in the ring for five: 92 us for 90.4.
+// rounded once the call of 64 sequences took 85 us for 92 but the error is 0.0029.  Four stages in the ring for five: 92 us for 90.4.
 template <int HD>
 __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __grid_constant__ TileParams P) {
   using C = TileCfg<HD>;

@@ -290,8 +290,8 @@ __global__ void __launch_bounds__(kPlanThreads) pages_compact_plan_kernel(const 
 }
 
 // Whole pages: pair i is src[i] of `from`, dst[i] of `to`.  n_dev: the number of pairs lies on the device.  The tables of a compaction
-// are rewritten beside the copies.  Bound: memory.  500 pages of 64 rows, 2 heads, 12 planes (786 MB read and written): 126 us, 6.25 TB/s, 0.95 of a
-// plain copy of the device; 490 of 2,048 such pages moved by a compaction: 127 us.  Whole warps on 4 KB pieces, eight CTAs an SM: no page is too
+// are rewritten beside the copies.  Bound: memory.  500 pages of 64 rows, 2 heads, 12 planes (786 MB read and written): 128 us, 6.15 TB/s, 0.94 of a
+// plain copy of the device; 490 of 2,048 such pages moved by a compaction: 126 to 132 us.  Whole warps on 4 KB pieces, eight CTAs an SM: no page is too
 // small or too large for an even spread.
 struct CopyJob {
   const int *src, *dst, *n_dev;

@@ -5,7 +5,9 @@
 The prompt is written once, in chunks of up to 64 tokens; every request is a fork of it (whole pages shared, a partial last page
 copied); a step of all requests is RMSNorm, the shared Q4_K projections with the requests' adapters beside them, the attention
 that computes the prompt's rows once for all, and the output projection with the residual.  Finished requests give their pages
-back, and the pool can be compacted at any time.  All of it is enqueued on the library stream; nothing waits for the GPU.
+back, and the pool can be compacted at any time.  All of it is enqueued on the library stream.  The host waits for the GPU where it
+uploads a list (three times a step; a server would keep lists that stay in their place) and where it asks the pool what was served
+(``prompt``, ``fork``; not ``step``, whose answer is ``ok``).
 """
 from __future__ import annotations
 
@@ -180,7 +182,7 @@ def main() -> None:
         for _ in range(half):
             layer.step(x.ptr, adapters, share)
         e1.record().synchronize()
-        print(f"{a.requests} requests behind {a.prompt} rows, prompt {'once for all' if share else 'by every request'}: {e0.elapsed_ms(e1) * 1e3 / half:.1f} us a step")
+        print(f"{a.requests} requests behind {a.prompt} rows, prompt {'once for all' if share else 'by every request'}: {e0.elapsed_ms(e1) * 1e3 / half:.1f} us a step, the waits for its lists among them")
     layer.drop(range(0, a.requests, 2))
     layer.compact()
     layer.step(x.ptr, adapters, False)
