@@ -11,6 +11,7 @@
 #include <string.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "bk_common.cuh"
 #include "bk_internal.h"
@@ -29,11 +30,51 @@ struct PagedParams {
   float scale, eps;
 };
 
+// What a call for trees (bkTreeAttn) has besides.  Its rows see the keys before the tree and the nodes whose bits are set; where new rows go and
+// where their rotation stands is given.
+struct TreeParams {
+  const int *pos, *slot;
+  const uint32_t* mask;   // [T * B][words]
+  int words, max_pos;
+};
+struct NoTree {};
+template <bool TREE>
+struct Params : PagedParams, std::conditional<TREE, TreeParams, NoTree>::type {};
+
 // row of its sequence at which token t of sequence b stands, -1 where it is not there
-BK_DEVINL int row_of(const PagedParams& p, int b, int t) {
+BK_DEVINL int row_of(const Params<false>& p, int b, int t) {
   const int n = p.n_new ? min(p.n_new[b], p.T) : p.T;
   const long long at = (long long)p.lens[b] - n + t;
   return t < n && at >= 0 && at < p.max_rows ? (int)at : -1;
+}
+// the tree of sequence b: its nodes (0: none is there), and the row of the first, which is the number of keys that all of them see
+struct Tree {
+  int n, base;
+};
+BK_DEVINL Tree tree_of(const Params<true>& p, int b) {
+  Tree r;
+  r.n = p.n_new ? max(0, min(p.n_new[b], p.T)) : p.T;
+  const int len = p.lens[b];
+  r.base = len - r.n;
+  if (len < r.n || len > p.max_rows) r.n = r.base = 0;
+  return r;
+}
+BK_DEVINL int row_of(const Params<true>& p, int b, int t) {
+  const Tree r = tree_of(p, b);
+  return t < r.n ? r.base + t : -1;
+}
+// word i of the nodes that a row sees, of n; all ones before the first
+BK_DEVINL uint32_t node_word(const uint32_t* bits, int n, int i) {
+  if (i < 0) return 0xffffffffu;
+  const int left = n - 32 * i;
+  return left <= 0 ? 0u : __ldg(bits + i) & (left >= 32 ? 0xffffffffu : (1u << left) - 1u);
+}
+// Which of the keys key, key + 1, ... key + 31 a row sees: bit for bit.  Those before the tree, and nodes whose bits are set.
+BK_DEVINL uint32_t seen_keys(const uint32_t* bits, const Tree& r, int key) {
+  const int o = key - r.base;
+  if (o <= -32) return 0xffffffffu;
+  const int i = o >> 5;
+  return __funnelshift_r(node_word(bits, r.n, i), node_word(bits, r.n, i + 1), o & 31);
 }
 
 template <int PER>
@@ -100,8 +141,9 @@ inline Layout make_layout(int B, int T, int Hq, int Hkv, int HD, int prefix_rows
   return L;
 }
 
+template <bool TREE>
 struct TileParams {
-  PagedParams g;
+  Params<TREE> g;
   Layout L;
   uint8_t* scratch;
   int* status;
@@ -130,8 +172,13 @@ BK_DEVINL Job job_of(const PagedParams& p, const Layout& L, int j) {
   q.key0 = L.P;
   return q;
 }
-// the end of its keys: behind the row of the last of the tile's tokens that is there
-BK_DEVINL int keys_end(const PagedParams& p, const Layout& L, const Job& q) {
+// the end of its keys: behind the row of the last of the tile's tokens that is there; a node may see any other of its tree
+BK_DEVINL int keys_end(const Params<true>& p, const Layout& L, const Job& q) {
+  if (q.seq < 0) return L.P;
+  const Tree r = tree_of(p, q.seq);
+  return max(L.P, r.base + r.n);
+}
+BK_DEVINL int keys_end(const Params<false>& p, const Layout& L, const Job& q) {
   if (q.seq < 0) return L.P;
   const int G = p.Hq / p.Hkv, n = p.n_new ? min(p.n_new[q.seq], p.T) : p.T, last = min(n, (min(p.T * G, (q.mt + 1) * kRows) - 1) / G + 1) - 1;
   for (int t = last; t >= 0 && t >= q.mt * kRows / G; t--) {   // (one turn but for tokens past max_len)
@@ -157,8 +204,8 @@ BK_DEVINL void piece_of(int s, int n, int u0, int u1, int* t0, int* t1) {
 constexpr int kPrepThreads = 256, kPlanned = 1024;   // jobs whose starts fit in shared memory
 // SMEM: no more than kPlanned jobs, whose lines are worked on in shared memory; otherwise in the records themselves.  What it takes is on every
 // call's way: a chain of loads from L2 costs 0.6 us a link.
-template <bool SMEM>
-BK_DEVINL void plan_jobs(const PagedParams& p, const Layout& L, uint8_t* scratch) {
+template <bool SMEM, bool TREE>
+BK_DEVINL void plan_jobs(const Params<TREE>& p, const Layout& L, uint8_t* scratch) {
   __shared__ int warp_s[kPrepThreads / 32][2], starts_s[SMEM ? kPlanned + 1 : 1], ends_s[SMEM ? kPlanned : 1], bounds_s[kPrepThreads + 1];
   int4* jobs = jobs_of(L, scratch);
   int4* pieces = pieces_of(L, scratch);
@@ -295,16 +342,16 @@ BK_DEVINL bool row_at(const PagedParams& p, const Job& q, int i, int* b, int* t,
 // buffer, k and v heads into their page, rounded to bf16: operands of the tensor cores (q's rounding is what the result's error is made of, 0.0024 of
 // its norm against 0.0017 for exact arithmetic rounded once).  The first CTA lays out the work of the next launch.  Bound: latency, 5 us for 32
 // sequences and 7 for 64 of 24 heads, most of it that CTA's.
-template <int HD>
-__global__ void __launch_bounds__(kPrepThreads) paged_prepare_kernel(const PagedParams p, const Layout L, uint8_t* scratch) {
+template <int HD, bool TREE>
+__global__ void __launch_bounds__(kPrepThreads) paged_prepare_kernel(const Params<TREE> p, const Layout L, uint8_t* scratch) {
   constexpr int PER = HD / 32;
   __shared__ float y_s[kPrepThreads / 32][HD];
   // The wait comes first: a launch behind this call may read, before its own wait, what a launch before this call wrote (weights, settled caches).
   bk_pdl_wait();
   bk_pdl_trigger();
   if (blockIdx.x == 0) {   // (first: it takes longest)
-    if (L.n_p + L.n_s <= kPlanned) plan_jobs<true>(p, L, scratch);
-    else plan_jobs<false>(p, L, scratch);
+    if (L.n_p + L.n_s <= kPlanned) plan_jobs<true, TREE>(p, L, scratch);
+    else plan_jobs<false, TREE>(p, L, scratch);
     return;
   }
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -324,16 +371,29 @@ __global__ void __launch_bounds__(kPrepThreads) paged_prepare_kernel(const Paged
 #pragma unroll
     for (int i = 0; i < PER / 4; i++) v[i] = *reinterpret_cast<const uint2*>(p.v + ((size_t)e * p.Hkv + kvh) * HD + lane * PER + 4 * i);
   }
-  const int at = row_of(p, b, t);
+  int at = row_of(p, b, t);
   if (at < 0) return;
+  int page, row_in;
+  if constexpr (TREE) {
+    const int slot = is_q ? 0 : p.slot[e];
+    page = slot >= 0 ? slot / p.page_rows : -1;
+    row_in = slot - page * p.page_rows;
+    if (p.fused) {
+      at = p.pos[e];
+      if (at < 0 || at >= p.max_pos) return;
+    }
+  }
   uint16_t* dst;
   if (is_q) {
     const int head = h / G;
     dst = p.q + (((size_t)head * p.B + b) * p.T + t) * G * HD + (size_t)(h - head * G) * HD;
   } else {
-    const int page = p.table[(size_t)b * p.max_pages + at / p.page_rows];
+    if constexpr (!TREE) {
+      page = p.table[(size_t)b * p.max_pages + at / p.page_rows];
+      row_in = at % p.page_rows;
+    }
     if (page < 0 || page >= p.n_pages) return;
-    const size_t row = (((size_t)page * p.Hkv + kvh) * p.page_rows + at % p.page_rows) * HD;
+    const size_t row = (((size_t)page * p.Hkv + kvh) * p.page_rows + row_in) * HD;
     dst = p.k_pages + row;
 #pragma unroll
     for (int i = 0; i < PER / 4; i++) *reinterpret_cast<uint2*>(p.v_pages + row + lane * PER + 4 * i) = v[i];
@@ -461,7 +521,9 @@ BK_DEVINL uint32_t odd_value(uint32_t sum, uint16_t v) {
 
 // Adds to a row's sums of 32 dims, d and on, the values of keys k0 to k1 - 1 below the row's limit that are not finite.  Whole warps, of one job.
 // (A call: in line it is in the way of every piece, 0.2 us of a short call.)
-__device__ __noinline__ void add_odd_values(const PagedParams& p, const Job& q, int HD, int d, int k0, int k1, int limit, uint32_t* o) {
+// (bits, tree: of a row of a tree, whose limit is its first node)
+template <bool TREE>
+__device__ __noinline__ void add_odd_values(const PagedParams& p, const Job& q, int HD, int d, int k0, int k1, int limit, const uint32_t* bits, Tree tree, uint32_t* o) {
   const int lane = threadIdx.x & 31;
   auto values = [&](int key) {   // (nullptr: rows of zeros)
     const int page = __ldg(p.table + (size_t)max(q.seq, 0) * p.max_pages + key / p.page_rows);
@@ -480,7 +542,9 @@ __device__ __noinline__ void add_odd_values(const PagedParams& p, const Job& q, 
       const int i = (__ffs(found) - 1) >> 2;
       found &= ~(15u << (4 * i));
       const uint16_t* at = values(k + i);
-      if (k + i < limit) {
+      bool sees = k + i < limit;
+      if constexpr (TREE) sees = sees || (bits && (seen_keys(bits, tree, k + i) & 1u));
+      if (sees) {
 #pragma unroll
         for (int y = 0; y < 32; y++) o[y] = odd_value(o[y], at[y]);
       }
@@ -516,10 +580,10 @@ constexpr int kCopyWarp = 8, kMmaWarp = 9, kQueryWarp = 10, kTileThreads = 352; 
 // m is only moved when a score passes it by more than 2^8, since O must be rescaled then.  Row sums are in f32, by the lane that owns the row.
 // Bound: the MMAs, 1,650 of the 2,000 cycles that a step of 128 rows and 64 keys takes (HD 256): QK^T once, P V twice for the two matrices.  With P
 // rounded once the call of 64 sequences took 85 us for 92 but the error is 0.0029.  Four stages in the ring for five: 92 us for 90.4.
-template <int HD>
-__global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __grid_constant__ TileParams P) {
+template <int HD, bool TREE>
+__global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __grid_constant__ TileParams<TREE> P) {
   using C = TileCfg<HD>;
-  const PagedParams& p = P.g;
+  const Params<TREE>& p = P.g;
   const Layout& L = P.L;
   extern __shared__ __align__(1024) uint8_t q_s[];   // queries [HD / 64][kRows][64], then the ring: stages [HD / 64][kTile][64]
   uint8_t* ring = q_s + C::kQuery;
@@ -769,20 +833,34 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
         const int t0 = x.t0, n = x.t1 - t0, key1 = x.key1;
         int b, t, g, limit = 0x7fffffff;   // (lanes without a row: never masked, never read)
         const bool mine = row_at(p, q, i_row, &b, &t, &g);
-        if (mine) limit = min(row_of(p, b, t) + 1, key1);
+        Tree tree = {0, 0};
+        const uint32_t* bits = nullptr;   // of a row of a tree that is there
+        if constexpr (TREE) {
+          if (mine) {
+            tree = tree_of(p, b);
+            if (t < tree.n) bits = p.mask + ((size_t)t * p.B + b) * p.words;
+            limit = bits ? min(tree.base, key1) : 0;
+          }
+        } else if (mine) {
+          limit = min(row_of(p, b, t) + 1, key1);
+        }
         __syncwarp();
         const bool warp_on = __any_sync(0xffffffffu, mine);
         // Tiles from this key on have a row that does not see all of them.  There a value that is not finite must not meet a zero probability (0 * inf):
         // it is taken out of the tile, and given back at the end to the rows that see it.
         int seen_by_all = key1;
         if (q.seq >= 0) {
-          const int first = q.mt * kRows / (p.Hq / p.Hkv), count = p.n_new ? min(p.n_new[q.seq], p.T) : p.T;
-          seen_by_all = max(0, p.lens[q.seq] - count + first) + 1;
+          if constexpr (TREE) {
+            seen_by_all = tree_of(p, q.seq).base;
+          } else {
+            const int first = q.mt * kRows / (p.Hq / p.Hkv), count = p.n_new ? min(p.n_new[q.seq], p.T) : p.T;
+            seen_by_all = max(0, p.lens[q.seq] - count + first) + 1;
+          }
         } else {
           int uneven;
           asm volatile("{ .reg .pred a, b; setp.ne.s32 a, %1, 0; barrier.cta.red.or.pred b, 5, 256, a; selp.s32 %0, 1, 0, b; }"
                        : "=r"(uneven)
-                       : "r"((int)(mine && limit > 0 && limit < key1))
+                       : "r"((int)(mine && (TREE ? bits != nullptr : limit > 0) && limit < key1))
                        : "memory");
           if (uneven) seen_by_all = 0;
         }
@@ -819,6 +897,13 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
         for (int i = 0; i < n; i++, tile++) {
           const int tile_key = q.key0 + (t0 + i) * kTile, there = min(kTile, key1 - tile_key), key = tile_key + group * 32;
           const uint32_t s_at = lanes + C::kS + (tile & 1) * kTile;
+          uint32_t seen = 0xffffffffu;   // of a tree's row, these keys
+          if constexpr (TREE) {
+            if (mine && key + 32 > limit) {   // (ahead of the wait: its loads are on the way meanwhile)
+              seen = bits ? seen_keys(bits, tree, key) : 0u;
+              if (key + 32 > key1) seen &= key >= key1 ? 0u : (1u << (key1 - key)) - 1u;
+            }
+          }
           bar_wait_warp(smem_u32(s_full + (tile & 1)), (tile >> 1) & 1, P.status, dead);
           tc_after();
           const bool mixed = tile_key + there > seen_by_all;
@@ -849,7 +934,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
             tmem_ld32(s_at + group * 32, s);
             if (!__all_sync(0xffffffffu, key + 32 <= limit)) {
 #pragma unroll
-              for (int y = 0; y < 32; y++) s[y] = key + y < limit ? s[y] : 0xff800000u;
+              for (int y = 0; y < 32; y++) s[y] = (TREE ? (seen >> y & 1u) != 0u : key + y < limit) ? s[y] : 0xff800000u;
             }
             float top[4];   // four chains: one alone is 32 results of the instruction before
 #pragma unroll
@@ -931,7 +1016,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
 #pragma unroll
             for (int y = 0; y < 16; y++) probe[y & 3] = bk_fma2(make_float2(__uint_as_float(o[2 * y]), __uint_as_float(o[2 * y + 1])), zero, probe[y & 3]);
             const float2 all = bk_add2(bk_add2(probe[0], probe[1]), bk_add2(probe[2], probe[3]));
-            const bool anew = __any_sync(0xffffffffu, mine && limit > 0 && __fadd_rn(all.x, all.y) != 0.0f);
+            const bool anew = __any_sync(0xffffffffu, mine && (TREE ? bits != nullptr : limit > 0) && __fadd_rn(all.x, all.y) != 0.0f);
             if (anew) {
               k0 = q.key0 + t0 * kTile;
               k1 = min(key1, k0 + n * kTile);
@@ -940,7 +1025,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
               uint32_t z[32];
 #pragma unroll
               for (int y = 0; y < 32; y++) z[y] = anew && isnan(__uint_as_float(o[y])) ? 0u : o[y];
-              add_odd_values(p, q, HD, d * 32, k0, k1, limit, z);
+              add_odd_values<TREE>(p, q, HD, d * 32, k0, k1, limit, bits, tree, z);
 #pragma unroll
               for (int y = 0; y < 32; y++)
                 if (!(isnan(__uint_as_float(o[y])) && isfinite(__uint_as_float(z[y])))) o[y] = z[y];
@@ -988,8 +1073,8 @@ BK_DEVINL float weight_of(float x) {
 // Bound: latency, of a chain of loads: the lists of pieces, their sums and results; 2.6 us of a call for one sequence, 5.5 for 32, 6.4 for 64.
 // Few CTAs have many pieces to a row, which four slices take together; many CTAs hide one another's latency better when they are small (two
 // slices for 64 sequences of 24 heads: 1.5 us more).
-template <int HD, int kSlices>
-__global__ void __launch_bounds__(256 * kSlices) paged_merge_kernel(const PagedParams p, const Layout L, uint8_t* scratch) {
+template <int HD, int kSlices, bool TREE>
+__global__ void __launch_bounds__(256 * kSlices) paged_merge_kernel(const Params<TREE> p, const Layout L, uint8_t* scratch) {
   __shared__ __align__(16) float4 o_s[kSlices > 1 ? kSlices - 1 : 1][16 * 16];
   __shared__ float2 ml_s[kSlices][16];
   bk_pdl_trigger();
@@ -1001,7 +1086,16 @@ __global__ void __launch_bounds__(256 * kSlices) paged_merge_kernel(const PagedP
   const int4* jobs = jobs_of(L, scratch);
   const int2 qs = __ldcg(reinterpret_cast<const int2*>(&jobs[L.n_p + js].z));   // first slot; number and distance
   const int2 qp = L.n_p ? __ldcg(reinterpret_cast<const int2*>(&jobs[jp].z)) : make_int2(0, 0);
-  const bool here = row_of(p, b, t) >= 0;
+  bool here = row_of(p, b, t) >= 0;
+  if constexpr (TREE) {   // a node that sees nothing gets zeros
+    const Tree tree = tree_of(p, b);
+    if (here && p.fused) here = p.pos[e] >= 0 && p.pos[e] < p.max_pos;
+    if (here && tree.base == 0) {
+      uint32_t any = 0;
+      for (int i = 0; i < p.words; i++) any |= node_word(p.mask + (size_t)e * p.words, tree.n, i);
+      here = any != 0;
+    }
+  }
   uint2 gv = make_uint2(0, 0);
   if (gate && slice == 0) gv = __ldcg(reinterpret_cast<const uint2*>(gate + (d0 + d) * 4));
   const int np = here ? qp.y & 0xffff : 0, n = here ? np + (qs.y & 0xffff) : 0;
@@ -1070,9 +1164,9 @@ __global__ void __launch_bounds__(256 * kSlices) paged_merge_kernel(const PagedP
   *reinterpret_cast<uint2*>(p.out + ((size_t)e * p.Hq + kvh * G + g) * HD + (d0 + d) * 4) = make_uint2(bk_f32x2_to_bf16x2(y[0], y[1]), bk_f32x2_to_bf16x2(y[2], y[3]));
 }
 
-template <int HD>
-int32_t launch_paged(const PagedParams& p, const Layout& L, uint64_t scratch) {
-  TileParams P;
+template <int HD, bool TREE>
+int32_t launch_paged(const Params<TREE>& p, const Layout& L, uint64_t scratch) {
+  TileParams<TREE> P;
   P.g = p;
   P.L = L;
   P.scratch = bk_ptr<uint8_t>(scratch);
@@ -1089,19 +1183,57 @@ int32_t launch_paged(const PagedParams& p, const Layout& L, uint64_t scratch) {
       return bk_fail(BK_ERR_UNSUPPORTED, "bkPagedAttn: the driver refuses a tensor map of %llu rows of %d queries", (unsigned long long)q_rows, HD);
   }
   const int heads = p.Hq + (p.k ? p.Hkv : 0);
-  BK_CUDA(bk_launch_pdl(paged_prepare_kernel<HD>, dim3((p.T * p.B * heads + kPrepThreads / 32 - 1) / (kPrepThreads / 32) + 1), dim3(kPrepThreads), 0, p, L, P.scratch));
+  BK_CUDA(bk_launch_pdl(paged_prepare_kernel<HD, TREE>, dim3((p.T * p.B * heads + kPrepThreads / 32 - 1) / (kPrepThreads / 32) + 1), dim3(kPrepThreads), 0, p, L, P.scratch));
   BK_CHECK_LAUNCH();
   static bool configured = false;
   if (!configured) {
-    BK_CUDA(cudaFuncSetAttribute(paged_tile_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, TileCfg<HD>::kSmem));
+    BK_CUDA(cudaFuncSetAttribute(paged_tile_kernel<HD, TREE>, cudaFuncAttributeMaxDynamicSharedMemorySize, TileCfg<HD>::kSmem));
     configured = true;
   }
-  BK_CUDA(bk_launch_pdl(paged_tile_kernel<HD>, dim3(L.ctas), dim3(kTileThreads), TileCfg<HD>::kSmem, P));
+  BK_CUDA(bk_launch_pdl(paged_tile_kernel<HD, TREE>, dim3(L.ctas), dim3(kTileThreads), TileCfg<HD>::kSmem, P));
   BK_CHECK_LAUNCH();
   const dim3 merge(p.T * p.B, p.Hkv * (HD / 64));
-  if ((long long)merge.x * merge.y <= 2 * bk_ctx().sm_count) BK_CUDA(bk_launch_pdl(paged_merge_kernel<HD, 4>, merge, dim3(p.Hq / p.Hkv * 64), 0, p, L, P.scratch));
-  else BK_CUDA(bk_launch_pdl(paged_merge_kernel<HD, 1>, merge, dim3(p.Hq / p.Hkv * 16), 0, p, L, P.scratch));
+  if ((long long)merge.x * merge.y <= 2 * bk_ctx().sm_count) BK_CUDA(bk_launch_pdl(paged_merge_kernel<HD, 4, TREE>, merge, dim3(p.Hq / p.Hkv * 64), 0, p, L, P.scratch));
+  else BK_CUDA(bk_launch_pdl(paged_merge_kernel<HD, 1, TREE>, merge, dim3(p.Hq / p.Hkv * 16), 0, p, L, P.scratch));
   BK_CHECK_LAUNCH();
+  return BK_OK;
+}
+
+// the checks of a call, its parameters and layout
+template <typename P>
+int32_t read_args(const char* what, const bkPagedAttnArgs& a, P* out, Layout* layout) {
+  BK_ARG(a.HD == 128 || a.HD == 256, "%s: head_dim %d unsupported (128 and 256)", what, a.HD);
+  BK_ARG(a.Hq > 0 && a.Hkv > 0 && a.Hq % a.Hkv == 0 && a.Hq / a.Hkv <= 16 && a.Hkv <= 1024, "%s: bad head counts Hq=%d Hkv=%d (group size 1..16, at most 1024 KV heads)", what, a.Hq, a.Hkv);
+  BK_ARG(a.B > 0 && a.T > 0 && (long long)a.B * a.T * (a.Hq + a.Hkv) < (1 << 24), "%s: B=%d T=%d of %d heads", what, a.B, a.T, a.Hq + a.Hkv);
+  BK_ARG(a.page_rows >= 16 && a.page_rows <= 1024 && (a.page_rows & (a.page_rows - 1)) == 0, "%s: page_rows=%d must be a power of two, 16 to 1024", what, a.page_rows);
+  BK_ARG(a.n_pages > 0 && a.max_pages > 0 && (long long)a.n_pages * a.Hkv * a.page_rows < (1ll << 31), "%s: n_pages=%d max_pages=%d (n_pages * Hkv * page_rows below 2^31)", what, a.n_pages, a.max_pages);
+  BK_ARG(a.max_len > 0 && a.prefix_rows >= 0 && a.prefix_rows <= a.max_len, "%s: prefix_rows=%d max_len=%d", what, a.prefix_rows, a.max_len);
+  BK_ARG(a.scale > 0.0f && a.scale < INFINITY, "%s: scale=%g must be positive", what, (double)a.scale);
+  BK_ARG(a.qg && a.k_pages && a.v_pages && a.table && a.lens && a.out && a.scratch, "%s: null pointer", what);
+  BK_ARG(((a.qg | a.k | a.v | a.gate | a.k_pages | a.v_pages | a.out | a.scratch) & 15) == 0, "%s: tensors must be 16-byte aligned", what);
+  BK_ARG(((a.table | a.lens | a.n_new) & 3) == 0, "%s: table, lens and n_new must be int32 arrays", what);
+  BK_ARG((a.k != 0) == (a.v != 0), "%s: k and v go together", what);
+  if (a.fused_norm_rope) {
+    BK_ARG(a.k && a.q_norm_w && a.k_norm_w && a.cos_t && a.sin_t, "%s: fused mode needs k, v, norm weights and tables", what);
+    BK_ARG(((a.q_norm_w | a.k_norm_w) & 15) == 0 && ((a.cos_t | a.sin_t) & 3) == 0, "%s: norm weights must be 16-byte aligned, tables f32 arrays", what);
+    BK_ARG(a.rot_half > 0 && 2 * a.rot_half <= a.HD, "%s: rot_half=%d", what, a.rot_half);
+    BK_ARG(a.gate == 0, "%s: fused mode takes the gate from qg", what);
+  }
+  const uint64_t need = bkPagedAttnScratchBytes(a.B, a.T, a.Hq, a.Hkv, a.HD, a.prefix_rows);
+  BK_ARG(a.scratch_bytes >= need, "%s: scratch of %llu bytes, %llu needed", what, (unsigned long long)a.scratch_bytes, (unsigned long long)need);
+  P& p = *out;
+  memset(&p, 0, sizeof(p));
+  p.qg = bk_ptr<uint16_t>(a.qg); p.k = bk_ptr<uint16_t>(a.k); p.v = bk_ptr<uint16_t>(a.v); p.gate = bk_ptr<uint16_t>(a.gate);
+  p.q_norm_w = bk_ptr<uint16_t>(a.q_norm_w); p.k_norm_w = bk_ptr<uint16_t>(a.k_norm_w); p.cos_t = bk_ptr<float>(a.cos_t); p.sin_t = bk_ptr<float>(a.sin_t);
+  p.k_pages = bk_ptr<uint16_t>(a.k_pages); p.v_pages = bk_ptr<uint16_t>(a.v_pages);
+  p.table = bk_ptr<int>(a.table); p.lens = bk_ptr<int>(a.lens); p.n_new = bk_ptr<int>(a.n_new); p.out = bk_ptr<uint16_t>(a.out);
+  p.q = bk_ptr<uint16_t>(a.scratch);
+  p.B = a.B; p.T = a.T; p.Hq = a.Hq; p.Hkv = a.Hkv; p.rot_half = a.rot_half; p.n_pages = a.n_pages; p.page_rows = a.page_rows; p.max_pages = a.max_pages;
+  p.max_rows = (int)std::min<long long>(a.max_len, (long long)a.max_pages * a.page_rows); p.fused = a.fused_norm_rope != 0; p.scale = a.scale; p.eps = a.eps;
+  Layout& L = *layout;
+  L = make_layout(a.B, a.T, a.Hq, a.Hkv, a.HD, a.prefix_rows, a.page_rows, bk_ctx().sm_count);
+  BK_ARG((long long)(L.n_p + L.n_s) * ((long long)p.max_rows / kTile + 1 + kOverhead) < (1ll << 31), "%s: B=%d T=%d Hkv=%d with %d rows a sequence: too much for one call", what, a.B,
+         a.T, a.Hkv, p.max_rows);
   return BK_OK;
 }
 
@@ -1117,39 +1249,31 @@ uint64_t bkPagedAttnScratchBytes(int32_t B, int32_t T, int32_t Hq, int32_t Hkv, 
 int32_t bkPagedAttn(const bkPagedAttnArgs* args) {
   BK_REQUIRE_INIT();
   BK_ARG(args != nullptr, "bkPagedAttn: args is null");
-  const bkPagedAttnArgs& a = *args;
-  BK_ARG(a.HD == 128 || a.HD == 256, "bkPagedAttn: head_dim %d unsupported (128 and 256)", a.HD);
-  BK_ARG(a.Hq > 0 && a.Hkv > 0 && a.Hq % a.Hkv == 0 && a.Hq / a.Hkv <= 16 && a.Hkv <= 1024, "bkPagedAttn: bad head counts Hq=%d Hkv=%d (group size 1..16, at most 1024 KV heads)", a.Hq, a.Hkv);
-  BK_ARG(a.B > 0 && a.T > 0 && (long long)a.B * a.T * (a.Hq + a.Hkv) < (1 << 24), "bkPagedAttn: B=%d T=%d of %d heads", a.B, a.T, a.Hq + a.Hkv);
-  BK_ARG(a.page_rows >= 16 && a.page_rows <= 1024 && (a.page_rows & (a.page_rows - 1)) == 0, "bkPagedAttn: page_rows=%d must be a power of two, 16 to 1024", a.page_rows);
-  BK_ARG(a.n_pages > 0 && a.max_pages > 0 && (long long)a.n_pages * a.Hkv * a.page_rows < (1ll << 31), "bkPagedAttn: n_pages=%d max_pages=%d (n_pages * Hkv * page_rows below 2^31)", a.n_pages, a.max_pages);
-  BK_ARG(a.max_len > 0 && a.prefix_rows >= 0 && a.prefix_rows <= a.max_len, "bkPagedAttn: prefix_rows=%d max_len=%d", a.prefix_rows, a.max_len);
-  BK_ARG(a.scale > 0.0f && a.scale < INFINITY, "bkPagedAttn: scale=%g must be positive", (double)a.scale);
-  BK_ARG(a.qg && a.k_pages && a.v_pages && a.table && a.lens && a.out && a.scratch, "bkPagedAttn: null pointer");
-  BK_ARG(((a.qg | a.k | a.v | a.gate | a.k_pages | a.v_pages | a.out | a.scratch) & 15) == 0, "bkPagedAttn: tensors must be 16-byte aligned");
-  BK_ARG(((a.table | a.lens | a.n_new) & 3) == 0, "bkPagedAttn: table, lens and n_new must be int32 arrays");
-  BK_ARG((a.k != 0) == (a.v != 0), "bkPagedAttn: k and v go together");
-  if (a.fused_norm_rope) {
-    BK_ARG(a.k && a.q_norm_w && a.k_norm_w && a.cos_t && a.sin_t, "bkPagedAttn: fused mode needs k, v, norm weights and tables");
-    BK_ARG(((a.q_norm_w | a.k_norm_w) & 15) == 0 && ((a.cos_t | a.sin_t) & 3) == 0, "bkPagedAttn: norm weights must be 16-byte aligned, tables f32 arrays");
-    BK_ARG(a.rot_half > 0 && 2 * a.rot_half <= a.HD, "bkPagedAttn: rot_half=%d", a.rot_half);
-    BK_ARG(a.gate == 0, "bkPagedAttn: fused mode takes the gate from qg");
-  }
-  const uint64_t need = bkPagedAttnScratchBytes(a.B, a.T, a.Hq, a.Hkv, a.HD, a.prefix_rows);
-  BK_ARG(a.scratch_bytes >= need, "bkPagedAttn: scratch of %llu bytes, %llu needed", (unsigned long long)a.scratch_bytes, (unsigned long long)need);
-  PagedParams p;
-  memset(&p, 0, sizeof(p));
-  p.qg = bk_ptr<uint16_t>(a.qg); p.k = bk_ptr<uint16_t>(a.k); p.v = bk_ptr<uint16_t>(a.v); p.gate = bk_ptr<uint16_t>(a.gate);
-  p.q_norm_w = bk_ptr<uint16_t>(a.q_norm_w); p.k_norm_w = bk_ptr<uint16_t>(a.k_norm_w); p.cos_t = bk_ptr<float>(a.cos_t); p.sin_t = bk_ptr<float>(a.sin_t);
-  p.k_pages = bk_ptr<uint16_t>(a.k_pages); p.v_pages = bk_ptr<uint16_t>(a.v_pages);
-  p.table = bk_ptr<int>(a.table); p.lens = bk_ptr<int>(a.lens); p.n_new = bk_ptr<int>(a.n_new); p.out = bk_ptr<uint16_t>(a.out);
-  p.q = bk_ptr<uint16_t>(a.scratch);
-  p.B = a.B; p.T = a.T; p.Hq = a.Hq; p.Hkv = a.Hkv; p.rot_half = a.rot_half; p.n_pages = a.n_pages; p.page_rows = a.page_rows; p.max_pages = a.max_pages;
-  p.max_rows = (int)std::min<long long>(a.max_len, (long long)a.max_pages * a.page_rows); p.fused = a.fused_norm_rope != 0; p.scale = a.scale; p.eps = a.eps;
-  const Layout L = make_layout(a.B, a.T, a.Hq, a.Hkv, a.HD, a.prefix_rows, a.page_rows, bk_ctx().sm_count);
-  BK_ARG((long long)(L.n_p + L.n_s) * ((long long)p.max_rows / kTile + 1 + kOverhead) < (1ll << 31), "bkPagedAttn: B=%d T=%d Hkv=%d with %d rows a sequence: too much for one call", a.B,
-         a.T, a.Hkv, p.max_rows);
-  return a.HD == 256 ? launch_paged<256>(p, L, a.scratch) : launch_paged<128>(p, L, a.scratch);
+  Params<false> p;
+  Layout L;
+  const int32_t rc = read_args("bkPagedAttn", *args, &p, &L);
+  if (rc) return rc;
+  return args->HD == 256 ? launch_paged<256, false>(p, L, args->scratch) : launch_paged<128, false>(p, L, args->scratch);
+}
+
+uint64_t bkTreeAttnScratchBytes(int32_t B, int32_t T, int32_t Hq, int32_t Hkv, int32_t HD, int32_t prefix_rows) {
+  return bkPagedAttnScratchBytes(B, T, Hq, Hkv, HD, prefix_rows);
+}
+
+int32_t bkTreeAttn(const bkTreeAttnArgs* args) {
+  BK_REQUIRE_INIT();
+  BK_ARG(args != nullptr, "bkTreeAttn: args is null");
+  const bkTreeAttnArgs& a = *args;
+  Params<true> p;
+  Layout L;
+  const int32_t rc = read_args("bkTreeAttn", a.attn, &p, &L);
+  if (rc) return rc;
+  BK_ARG(a.mask && (a.mask & 3) == 0 && a.mask_words >= (a.attn.T + 31) / 32, "bkTreeAttn: mask must be a uint32 array of at least %d words a node (mask_words=%d)", (a.attn.T + 31) / 32,
+         a.mask_words);
+  BK_ARG((a.pos & 3) == 0 && (a.pos || !a.attn.fused_norm_rope), "bkTreeAttn: fused mode needs pos, an int32 array");
+  BK_ARG((a.slot & 3) == 0 && (a.slot || !a.attn.k), "bkTreeAttn: k and v need slot, an int32 array");
+  p.pos = bk_ptr<int>(a.pos); p.slot = bk_ptr<int>(a.slot); p.mask = bk_ptr<uint32_t>(a.mask); p.words = a.mask_words; p.max_pos = a.attn.max_len;
+  return a.attn.HD == 256 ? launch_paged<256, true>(p, L, a.attn.scratch) : launch_paged<128, true>(p, L, a.attn.scratch);
 }
 
 }  // extern "C"

@@ -14,6 +14,7 @@ namespace {
 
 constexpr int kPlanThreads = 1024;   // also the longest list
 constexpr int kCopyThreads = 256;
+constexpr int kMaxNodes = 1024;      // of a drafted tree
 constexpr int kCopyVecs = 8;         // 16-byte vectors that a lane has on the way: a warp moves 4 KB at a time, 256 KB an SM
 
 struct Pool {
@@ -324,6 +325,193 @@ __global__ void __launch_bounds__(kCopyThreads) pages_copy_kernel(const Pool fro
   }
 }
 
+// ---- drafted trees ---------------------------------------------------------------------
+
+struct BatchParams {
+  const int *seqs, *n_new, *parent;
+  int *table, *lens, *pos, *slot;
+  uint32_t* mask;
+  int n, T, words;
+};
+
+// Maps of a batch: a CTA row per sequence, its CTAs share the table; the nodes are the first one's, a thread each.  A node's ancestors have lower numbers, so a walk up
+// the tree writes the words of its mask from the last to the first, each once.  Bound: latency, of a chain of loads (list, length, table) and the walk.
+__global__ void __launch_bounds__(kCopyThreads) pages_batch_kernel(const Pool p, const BatchParams a) {
+  __shared__ int parent_s[kMaxNodes];
+  bk_pdl_wait();
+  bk_pdl_trigger();
+  const int i = blockIdx.x, s = a.seqs[i];
+  int len = s >= 0 && s < p.n_seqs ? __ldcg(p.lens + s) : 0;
+  if (len < 0 || len > p.max_pages * p.page_rows) len = 0;
+  const int held = pages_of(len, p.page_rows);
+  const int* from = p.table + (size_t)max(s, 0) * p.max_pages;
+  if (a.table) {
+    int* to = a.table + (size_t)i * p.max_pages;
+    for (int j = blockIdx.y * kCopyThreads + threadIdx.x; j < p.max_pages; j += gridDim.y * kCopyThreads) to[j] = j < held ? __ldcg(from + j) : -1;
+  }
+  if (blockIdx.y) return;
+  if (a.lens && threadIdx.x == 0) a.lens[i] = len;
+  if (!a.pos && !a.slot && !a.mask) return;
+  int n = a.n_new ? max(0, min(a.n_new[i], a.T)) : a.T;
+  const int base = len - n;
+  if (base < 0) n = 0;
+  if (a.parent) {
+    for (int t = threadIdx.x; t < n; t += kCopyThreads) parent_s[t] = a.parent[(size_t)t * a.n + i];
+    __syncthreads();
+  }
+  for (int t = threadIdx.x; t < a.T; t += kCopyThreads) {
+    const size_t e = (size_t)t * a.n + i;
+    uint32_t* words = a.mask ? a.mask + e * a.words : nullptr;
+    int w = a.words - 1, depth = -1;
+    if (t < n) {
+      uint32_t bits = 0;
+      int top = w;   // the last word that a bit can be in
+      if (words)
+        for (; top > t >> 5; top--) words[top] = 0;
+      else
+        top = t >> 5;
+      w = top;
+      for (int u = t; u >= 0;) {
+        if (u >> 5 != w) {
+          if (words) {
+            words[w] = bits;
+            for (w--; w > u >> 5; w--) words[w] = 0;
+          }
+          w = u >> 5;
+          bits = 0;
+        }
+        bits |= 1u << (u & 31);
+        depth++;
+        const int up = a.parent ? parent_s[u] : u - 1;
+        u = up < u ? up : -1;
+      }
+      if (words) words[w] = bits;
+      w--;
+    }
+    if (words)
+      for (; w >= 0; w--) words[w] = 0;
+    if (a.pos) a.pos[e] = t < n ? base + depth : -1;
+    if (a.slot) {
+      int slot = -1;
+      if (t < n) {
+        const int row = base + t, page = __ldcg(from + row / p.page_rows);
+        if (page >= 0 && page < p.n_pages) slot = page * p.page_rows + row % p.page_rows;
+      }
+      a.slot[e] = slot;
+    }
+  }
+}
+
+struct CommitParams {
+  const int *seqs, *n_new, *parent, *token, *target;
+  int *path, *n_path, *next, *ok, *history, *hist_len;
+  int n, T, history_ld;
+};
+
+// A cluster of CTAs per sequence.  Each finds the path for itself: every node that the model agrees with tells its parent, the lowest child stays, and one thread follows
+// the children.  Then the CTAs' warps move rows: a warp has 512 bytes of a row of one head and plane, of all rows that move, which it takes in order (row i of the
+// tree is written after it was read, since a path's node i has a number of at least i).  What the others still read (table, counts, lengths) is changed by the
+// first CTA behind the cluster's barrier; other sequences read none of it, for pages of a tree belong to one sequence alone.  Bound: latency of that chain for small
+// batches.
+__global__ void __launch_bounds__(kCopyThreads) pages_commit_kernel(const Pool p, const CommitParams a) {
+  __shared__ int child_s[kMaxNodes], path_s[kMaxNodes], n_s, refused_s;
+  const int tid = threadIdx.x, rank = blockIdx.x, ranks = gridDim.x, i = blockIdx.y;   // (a cluster is a row of the grid)
+  bk_pdl_wait();
+  bk_pdl_trigger();
+  const int s = a.seqs[i], n = a.n_new ? a.n_new[i] : a.T;
+  bool again = false;
+  for (int j = tid; j < i; j += kCopyThreads) again |= a.seqs[j] == s;
+  const bool named = s >= 0 && s < p.n_seqs && n >= 1 && n <= a.T;
+  const int len = named ? __ldcg(p.lens + s) : 0, base = len - n;
+  bool good = named && base >= 0 && len <= p.max_pages * p.page_rows;
+  int* table = p.table + (size_t)max(s, 0) * p.max_pages;
+  if (good) {   // (of the whole CTA)
+    // pages of the tree's rows: this sequence's alone
+    for (int j = base / p.page_rows + tid; j < pages_of(len, p.page_rows); j += kCopyThreads) {
+      const int page = __ldcg(table + j);
+      again |= page < 0 || page >= p.n_pages || __ldcg(p.ref + page) != 1;
+    }
+    for (int t = tid; t < n; t += kCopyThreads) child_s[t] = kMaxNodes;
+  }
+  if (tid == 0) n_s = 0;
+  good = !__syncthreads_or(again) && good;
+  if (good) {
+    for (int t = 1 + tid; t < n; t += kCopyThreads) {
+      const int up = a.parent[(size_t)t * a.n + i];
+      if (up >= 0 && up < t && a.token[(size_t)t * a.n + i] == a.target[(size_t)up * a.n + i]) atomicMin(child_s + up, t);
+    }
+    __syncthreads();
+    if (tid == 0) {
+      int m = 0;
+      for (int t = 0; t < kMaxNodes; t = child_s[t]) path_s[m++] = t;
+      n_s = m;
+      refused_s = 0;
+      if (a.history) {
+        const int h = __ldcg(a.hist_len + s);
+        refused_s = h < 0 || h > a.history_ld - m;
+      }
+    }
+    __syncthreads();
+    good = refused_s == 0;
+  }
+  const int m = good ? n_s : 0;
+  if (rank == 0) {
+    if (a.path)
+      for (int t = tid; t < a.T; t += kCopyThreads) a.path[(size_t)t * a.n + i] = t < m ? path_s[t] : -1;
+    if (tid == 0) {
+      if (a.n_path) a.n_path[i] = m;
+      if (a.next) a.next[i] = good ? a.target[(size_t)path_s[m - 1] * a.n + i] : -1;
+      if (a.ok) a.ok[i] = good;
+    }
+  }
+  if (!good) return;   // (of the whole cluster: its CTAs have read the same)
+  // the rows that move: from the first whose place is another
+  int first = 0;
+  while (first < m && path_s[first] == first) first++;
+  if (first < m) {
+    const int lane = tid & 31, chunks = (p.row_bytes / 16 + 31) / 32;
+    const long long items = (long long)p.n_planes * p.heads * chunks;
+    for (long long it = rank * (kCopyThreads / 32) + (tid >> 5); it < items; it += (long long)ranks * (kCopyThreads / 32)) {
+      const int chunk = (int)(it % chunks), run = (int)(it / chunks), head = run % p.heads, plane = run / p.heads, vec = chunk * 32 + lane;
+      uint8_t* at = p.base + plane * p.plane_bytes + (size_t)head * p.page_rows * p.row_bytes + (size_t)vec * 16;
+      auto row_at = [&](int t) {
+        const int row = base + t;
+        return reinterpret_cast<uint4*>(at + __ldcg(table + row / p.page_rows) * p.page_bytes + (size_t)(row % p.page_rows) * p.row_bytes);
+      };
+      if (vec < p.row_bytes / 16)
+        for (int k = first; k < m; k += kCopyVecs) {
+          uint4 v[kCopyVecs];
+#pragma unroll
+          for (int e = 0; e < kCopyVecs; e++)
+            if (k + e < m) v[e] = *row_at(path_s[k + e]);
+#pragma unroll
+          for (int e = 0; e < kCopyVecs; e++)
+            if (k + e < m) *row_at(k + e) = v[e];
+        }
+    }
+  }
+  if (ranks > 1) {
+    asm volatile("barrier.cluster.arrive;" ::: "memory");
+    asm volatile("barrier.cluster.wait;" ::: "memory");
+  } else {
+    __syncthreads();
+  }
+  if (rank) return;
+  for (int j = pages_of(base + m, p.page_rows) + tid; j < pages_of(len, p.page_rows); j += kCopyThreads) {
+    p.ref[table[j]] = 0;
+    table[j] = -1;
+  }
+  if (a.history) {
+    const int h = a.hist_len[s];
+    int* to = a.history + (size_t)s * a.history_ld + h;
+    for (int t = 1 + tid; t < m; t += kCopyThreads) to[t - 1] = a.token[(size_t)path_s[t] * a.n + i];
+    if (tid == 0) to[m - 1] = a.target[(size_t)path_s[m - 1] * a.n + i];
+    __syncthreads();
+    if (tid == 0) a.hist_len[s] = h + m;
+  }
+  if (tid == 0) p.lens[s] = base + m;
+}
+
 int32_t read_pool(const bkPages* a, const char* what, Pool* out) {
   BK_ARG(a != nullptr, "%s: the pool is null", what);
   BK_ARG(a->n_planes > 0 && a->n_pages > 0 && a->heads > 0 && a->page_rows > 0 && a->row_bytes > 0 && a->row_bytes % 16 == 0 && a->n_seqs > 0 && a->max_pages > 0,
@@ -445,6 +633,63 @@ int32_t bkPagesCompact(const bkPages* pool, uint64_t table_out, uint64_t ref_out
   job.table_in = p.table; job.map = bk_ptr<int>(map); job.table_out = bk_ptr<int>(table_out); job.table_n = (long long)p.n_seqs * p.max_pages;
   const long long items = (long long)(p.n_pages + 1) / 2 * p.n_planes * (((long long)p.page_bytes / 16 + 32 * kCopyVecs - 1) / (32 * kCopyVecs));
   BK_CUDA(bk_launch_pdl(pages_copy_kernel, dim3(copy_ctas(items)), dim3(kCopyThreads), 0, p, p, job));
+  BK_CHECK_LAUNCH();
+  return BK_OK;
+}
+
+int32_t bkPagesBatch(const bkPages* pool, const bkPagesBatchArgs* args) {
+  BK_REQUIRE_INIT();
+  Pool p;
+  TRY(read_pool(pool, "bkPagesBatch", &p));
+  BK_ARG(args != nullptr, "bkPagesBatch: args is null");
+  const bkPagesBatchArgs& a = *args;
+  TRY(check_list("bkPagesBatch", a.n, a.seqs, a.seqs));
+  BK_ARG(a.T >= 1 && a.T <= kMaxNodes, "bkPagesBatch: T=%d (1 to %d)", a.T, kMaxNodes);
+  BK_ARG(((a.n_new | a.parent | a.table | a.lens | a.pos | a.slot | a.mask) & 3) == 0, "bkPagesBatch: all arrays are of 32-bit words");
+  BK_ARG(!a.mask || a.mask_words >= (a.T + 31) / 32, "bkPagesBatch: mask_words=%d for %d nodes", a.mask_words, a.T);
+  BK_ARG(!a.slot || (long long)p.n_pages * p.page_rows < (1ll << 31), "bkPagesBatch: %d pages of %d rows: a slot has 31 bits", p.n_pages, p.page_rows);
+  if (a.n == 0) return BK_OK;
+  const BatchParams b = {bk_ptr<int>(a.seqs), bk_ptr<int>(a.n_new), bk_ptr<int>(a.parent), bk_ptr<int>(a.table), bk_ptr<int>(a.lens), bk_ptr<int>(a.pos), bk_ptr<int>(a.slot),
+                         bk_ptr<uint32_t>(a.mask), a.n, a.T, a.mask_words};
+  // CTAs a sequence: 1,024 entries of its table each, no more than fill the GPU twice
+  const int y = a.table ? std::max(1, std::min((p.max_pages + 4 * kCopyThreads - 1) / (4 * kCopyThreads), 2 * bk_ctx().sm_count / a.n)) : 1;
+  BK_CUDA(bk_launch_pdl(pages_batch_kernel, dim3(a.n, y), dim3(kCopyThreads), 0, p, b));
+  BK_CHECK_LAUNCH();
+  return BK_OK;
+}
+
+int32_t bkPagesCommit(const bkPages* pool, const bkPagesCommitArgs* args) {
+  BK_REQUIRE_INIT();
+  Pool p;
+  TRY(read_pool(pool, "bkPagesCommit", &p));
+  BK_ARG(args != nullptr, "bkPagesCommit: args is null");
+  const bkPagesCommitArgs& a = *args;
+  TRY(check_list("bkPagesCommit", a.n, a.seqs, a.seqs));
+  BK_ARG(a.T >= 1 && a.T <= kMaxNodes, "bkPagesCommit: T=%d (1 to %d)", a.T, kMaxNodes);
+  BK_ARG(a.n == 0 || (a.parent && a.token && a.target), "bkPagesCommit: parent, token and target must be non-null int32 arrays");
+  BK_ARG(((a.n_new | a.parent | a.token | a.target | a.path | a.n_path | a.next | a.ok | a.history | a.hist_len) & 3) == 0, "bkPagesCommit: all arrays are of int32");
+  BK_ARG((a.history != 0) == (a.hist_len != 0) && (!a.history || a.history_ld > 0), "bkPagesCommit: history and hist_len go together (history_ld=%d)", a.history_ld);
+  if (a.n == 0) return BK_OK;
+  const CommitParams c = {bk_ptr<int>(a.seqs), bk_ptr<int>(a.n_new), bk_ptr<int>(a.parent), bk_ptr<int>(a.token), bk_ptr<int>(a.target), bk_ptr<int>(a.path), bk_ptr<int>(a.n_path),
+                          bk_ptr<int>(a.next), bk_ptr<int>(a.ok), bk_ptr<int>(a.history), bk_ptr<int>(a.hist_len), a.n, a.T, a.history_ld};
+  // CTAs a sequence: as many as its warps have runs of rows for, at most 8 (a cluster) and four an SM
+  const long long items = (long long)p.n_planes * p.heads * ((p.row_bytes / 16 + 31) / 32);
+  int ranks = 1;
+  while (ranks < 8 && ranks * (kCopyThreads / 32) < items && (long long)2 * ranks * a.n <= 4 * bk_ctx().sm_count) ranks *= 2;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(ranks, a.n);
+  cfg.blockDim = dim3(kCopyThreads);
+  cfg.stream = bk_ctx().stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = ranks;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  BK_CUDA(cudaLaunchKernelEx(&cfg, pages_commit_kernel, p, c));
   BK_CHECK_LAUNCH();
   return BK_OK;
 }

@@ -179,6 +179,35 @@ def paged_attn(args: R.bkPagedAttnArgs) -> None:
     _check(cu().bkPagedAttn(C.byref(args)))
 
 
+def tree_attn_scratch_bytes(B: int, T: int, Hq: int, Hkv: int, HD: int, prefix_rows: int) -> int:
+    return int(cu().bkTreeAttnScratchBytes(B, T, Hq, Hkv, HD, prefix_rows))
+
+
+def tree_attn_args(*, mask: int, mask_words: int, pos: int = 0, slot: int = 0, **kw) -> R.bkTreeAttnArgs:
+    """The arguments of ``tree_attn``; the other keyword names are the fields of bkPagedAttnArgs, as for ``paged_attn_args``."""
+    return R.bkTreeAttnArgs(attn=paged_attn_args(**kw), pos=pos, slot=slot, mask=mask, mask_words=mask_words)
+
+
+def tree_attn(args: R.bkTreeAttnArgs) -> None:
+    """Attention of drafted trees over pages: a node sees the rows before its tree and the nodes of its mask (``PagePool.batch`` makes pos, slot and mask)."""
+    _check(cu().bkTreeAttn(C.byref(args)))
+
+
+def adjust_logits_args(**kw) -> R.bkLogitsArgs:
+    """The arguments of ``adjust_logits``; keyword names are the fields of bkLogitsArgs."""
+    a = R.bkLogitsArgs()
+    for k, v in kw.items():
+        if not hasattr(a, k):
+            raise TypeError(f"adjust_logits_args: bkLogitsArgs has no field {k!r}")
+        setattr(a, k, v)
+    return a
+
+
+def adjust_logits(args: R.bkLogitsArgs) -> None:
+    """Penalties for repeated tokens, biases and grammar masks on logits, in place (call it before ``sample`` or ``argmax``)."""
+    _check(cu().bkAdjustLogits(C.byref(args)))
+
+
 def lora_scratch_bytes(K: int, B: int, rank: int, n_segs: int) -> int:
     return int(R.load_library().bkLoraScratchBytes(K, B, rank, n_segs))
 

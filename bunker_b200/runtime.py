@@ -81,6 +81,26 @@ class bkPagedAttnArgs(C.Structure):
                                           "max_len", "fused_norm_rope")] + [("scale", C.c_float), ("eps", C.c_float)]
 
 
+class bkPagesBatchArgs(C.Structure):
+    _fields_ = [(n, C.c_uint64) for n in ("seqs", "n_new", "parent", "table", "lens", "pos", "slot", "mask")] + \
+               [(n, C.c_int32) for n in ("n", "T", "mask_words", "reserved")]
+
+
+class bkTreeAttnArgs(C.Structure):
+    _fields_ = [("attn", bkPagedAttnArgs)] + [(n, C.c_uint64) for n in ("pos", "slot", "mask")] + [("mask_words", C.c_int32), ("reserved", C.c_int32)]
+
+
+class bkLogitsArgs(C.Structure):
+    _fields_ = [(n, C.c_uint64) for n in ("logits", "seqs", "history", "hist_len", "prompt_len", "repetition", "presence", "frequency", "draft", "path",
+                                           "bias_token", "bias_value", "bias_n", "allowed", "mask_id")] + \
+               [(n, C.c_int32) for n in ("B", "T", "V", "ld", "n_seqs", "history_ld", "bias_ld", "path_words", "n_masks", "allowed_words")]
+
+
+class bkPagesCommitArgs(C.Structure):
+    _fields_ = [(n, C.c_uint64) for n in ("seqs", "n_new", "parent", "token", "target", "path", "n_path", "next", "ok", "history", "hist_len")] + \
+               [(n, C.c_int32) for n in ("n", "T", "history_ld", "reserved")]
+
+
 class bkLoraSeg(C.Structure):
     _fields_ = [("A", C.c_uint64), ("Bm", C.c_uint64), ("base", C.c_uint64), ("out", C.c_uint64), ("n_rows", C.c_int32), ("dtype", C.c_int32),
                 ("ld_out", C.c_int32), ("col_off", C.c_int32)]
@@ -164,6 +184,11 @@ SIGNATURES = {
     "bkPagesCompact": (_I32, [C.POINTER(bkPages), _U64, _U64, _U64, _U64]),
     "bkPagedAttn": (_I32, [C.POINTER(bkPagedAttnArgs)]),
     "bkPagedAttnScratchBytes": (_U64, [_I32, _I32, _I32, _I32, _I32, _I32]),
+    "bkPagesBatch": (_I32, [C.POINTER(bkPages), C.POINTER(bkPagesBatchArgs)]),
+    "bkPagesCommit": (_I32, [C.POINTER(bkPages), C.POINTER(bkPagesCommitArgs)]),
+    "bkTreeAttn": (_I32, [C.POINTER(bkTreeAttnArgs)]),
+    "bkTreeAttnScratchBytes": (_U64, [_I32, _I32, _I32, _I32, _I32, _I32]),
+    "bkAdjustLogits": (_I32, [C.POINTER(bkLogitsArgs)]),
     "bkLora": (_I32, [C.POINTER(bkLoraArgs)]),
     "bkLoraScratchBytes": (_U64, [_I32, _I32, _I32, _I32]),
     "bkLaunch": (_I32, [_I32, _PU64, _I32]),

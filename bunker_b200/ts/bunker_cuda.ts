@@ -74,8 +74,13 @@ const SYMBOLS = {
   bkPagesGrow: { args: ["ptr", "u64", "u64", "i32", "u64"], returns: "i32" },
   bkPagesFree: { args: ["ptr", "u64", "i32"], returns: "i32" },
   bkPagesCompact: { args: ["ptr", "u64", "u64", "u64", "u64"], returns: "i32" },
+  bkPagesBatch: { args: ["ptr", "ptr"], returns: "i32" },
+  bkPagesCommit: { args: ["ptr", "ptr"], returns: "i32" },
   bkPagedAttn: { args: ["ptr"], returns: "i32" },
   bkPagedAttnScratchBytes: { args: ["i32", "i32", "i32", "i32", "i32", "i32"], returns: "u64" },
+  bkTreeAttn: { args: ["ptr"], returns: "i32" },
+  bkTreeAttnScratchBytes: { args: ["i32", "i32", "i32", "i32", "i32", "i32"], returns: "u64" },
+  bkAdjustLogits: { args: ["ptr"], returns: "i32" },
   bkLora: { args: ["ptr"], returns: "i32" },
   bkLoraScratchBytes: { args: ["i32", "i32", "i32", "i32"], returns: "u64" },
   bkModelCreate: { args: ["ptr", "ptr"], returns: "i32" },
@@ -316,14 +321,63 @@ export interface PagedAttn {
   B: number; T: number; Hq: number; Hkv: number; HD: number; rotHalf?: number; nPages: number; pageRows: number; maxPages: number; prefixRows: number;
   maxLen: number; fusedNormRope: boolean; scale: number; eps?: number;
 }
-export function pagedAttn(a: PagedAttn): void {
-  const b = Buffer.alloc(184);
+function packPagedAttn(b: Buffer, a: PagedAttn): void {
   [a.qg, a.k, a.v, a.gate, a.qNormW, a.kNormW, a.cosT, a.sinT, a.kPages, a.vPages, a.table, a.lens, a.nNew, a.out, a.scratch, a.scratchBytes]
     .forEach((v, i) => b.writeBigUInt64LE(v ?? 0n, 8 * i));
   [a.B, a.T, a.Hq, a.Hkv, a.HD, a.rotHalf ?? 0, a.nPages, a.pageRows, a.maxPages, a.prefixRows, a.maxLen, a.fusedNormRope ? 1 : 0]
     .forEach((v, i) => b.writeInt32LE(v, 128 + 4 * i));
   b.writeFloatLE(a.scale, 176); b.writeFloatLE(a.eps ?? 1e-6, 180);
+}
+export function pagedAttn(a: PagedAttn): void {
+  const b = Buffer.alloc(184);
+  packPagedAttn(b, a);
   check(cu().bkPagedAttn(b), "bkPagedAttn");
+}
+
+/** Maps of a step (bkPagesBatchArgs, 80 bytes): tables, lengths, positions, slots and masks of a list of sequences and their drafted trees. */
+export interface PagesBatch {
+  seqs: bigint; nNew?: bigint; parent?: bigint; table?: bigint; lens?: bigint; pos?: bigint; slot?: bigint; mask?: bigint; n: number; T: number; maskWords?: number;
+}
+export function pagesBatch(pool: Buffer, a: PagesBatch): void {
+  const b = Buffer.alloc(80);
+  [a.seqs, a.nNew, a.parent, a.table, a.lens, a.pos, a.slot, a.mask].forEach((v, i) => b.writeBigUInt64LE(v ?? 0n, 8 * i));
+  [a.n, a.T, a.maskWords ?? 0].forEach((v, i) => b.writeInt32LE(v, 64 + 4 * i));
+  check(cu().bkPagesBatch(pool, b), "bkPagesBatch");
+}
+
+/** Attention of drafted trees over pages (bkTreeAttnArgs, 216 bytes): as pagedAttn, with the nodes that each row sees. */
+export function treeAttn(a: PagedAttn & { pos?: bigint; slot?: bigint; mask: bigint; maskWords: number }): void {
+  const b = Buffer.alloc(216);
+  packPagedAttn(b, a);
+  [a.pos, a.slot, a.mask].forEach((v, i) => b.writeBigUInt64LE(v ?? 0n, 184 + 8 * i));
+  b.writeInt32LE(a.maskWords, 208);
+  check(cu().bkTreeAttn(b), "bkTreeAttn");
+}
+
+/** Penalties, biases and grammar masks on logits in place (bkLogitsArgs, 160 bytes). */
+export interface AdjustLogits {
+  logits: bigint; seqs?: bigint; history?: bigint; histLen?: bigint; promptLen?: bigint; repetition?: bigint; presence?: bigint; frequency?: bigint;
+  draft?: bigint; path?: bigint; biasToken?: bigint; biasValue?: bigint; biasN?: bigint; allowed?: bigint; maskId?: bigint;
+  B: number; T: number; V: number; ld?: number; nSeqs?: number; historyLd?: number; biasLd?: number; pathWords?: number; nMasks?: number; allowedWords?: number;
+}
+export function adjustLogits(a: AdjustLogits): void {
+  const b = Buffer.alloc(160);
+  [a.logits, a.seqs, a.history, a.histLen, a.promptLen, a.repetition, a.presence, a.frequency, a.draft, a.path, a.biasToken, a.biasValue, a.biasN, a.allowed, a.maskId]
+    .forEach((v, i) => b.writeBigUInt64LE(v ?? 0n, 8 * i));
+  [a.B, a.T, a.V, a.ld, a.nSeqs, a.historyLd, a.biasLd, a.pathWords, a.nMasks, a.allowedWords].forEach((v, i) => b.writeInt32LE(v ?? 0, 120 + 4 * i));
+  check(cu().bkAdjustLogits(b), "bkAdjustLogits");
+}
+
+/** What the model agrees with stays (bkPagesCommitArgs, 104 bytes): the longest path of every drafted tree. */
+export interface PagesCommit {
+  seqs: bigint; nNew?: bigint; parent: bigint; token: bigint; target: bigint; path?: bigint; nPath?: bigint; next?: bigint; ok?: bigint; history?: bigint; histLen?: bigint;
+  n: number; T: number; historyLd?: number;
+}
+export function pagesCommit(pool: Buffer, a: PagesCommit): void {
+  const b = Buffer.alloc(104);
+  [a.seqs, a.nNew, a.parent, a.token, a.target, a.path, a.nPath, a.next, a.ok, a.history, a.histLen].forEach((v, i) => b.writeBigUInt64LE(v ?? 0n, 8 * i));
+  [a.n, a.T, a.historyLd ?? 0].forEach((v, i) => b.writeInt32LE(v, 88 + 4 * i));
+  check(cu().bkPagesCommit(pool, b), "bkPagesCommit");
 }
 
 /** Adapters beside a shared projection (bkLoraArgs, 256 bytes): up to four row segments. */

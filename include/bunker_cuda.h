@@ -340,6 +340,87 @@ BK_API int32_t bkPagedAttn(const bkPagedAttnArgs* args);
 /* (after bkInit: it depends on the number of SMs) */
 BK_API uint64_t bkPagedAttnScratchBytes(int32_t B, int32_t T, int32_t Hq, int32_t Hkv, int32_t HD, int32_t prefix_rows);
 
+/* ---- drafted trees of tokens: maps of a step, attention, logits, and what stays -----------------------------------
+ * A request's draft is a tree of up to T tokens: node 0 is the last token that is certain, every other node continues an earlier one.  Its
+ * nodes are the last rows of the sequence (bkPagesGrow makes room for them), node t of request i is entry t*n + i of every array of nodes.  A step:
+ * bkPagesGrow, bkPagesBatch, then the layers with bkTreeAttn, bkAdjustLogits, bkSample or bkArgmax on all nodes, bkPagesCommit. */
+
+/* For a list of n (at most 1024) sequences, in the list's order, what the calls of a step take.  Any result may be 0 = not wanted.
+ *   table  int32 [n][max_pages]: the sequence's pages, -1 behind them;  lens int32 [n]
+ *   pos    int32 [T][n]: row of the sequence's first new token + how many tokens of the node's path come before the node: where its rotation stands
+ *   slot   int32 [T][n]: page * page_rows + row in the page, of the node's own row (n_pages * page_rows below 2^31)
+ *   mask   uint32 [T][n][mask_words]: bit u is set for the nodes u of the node's path, itself among them
+ * parent int32 [T][n]: the node that it continues, -1 (or any that is not an earlier node): none; parent = 0: each token continues the one before.
+ * n_new int32 [n]: how many of a sequence's rows are new, 0..T (less than 0 counts as 0, more than T as T); 0 = T of each.  A token t >= n_new, or of a
+ * sequence that has fewer than n_new rows, is not there: pos and slot are -1, its mask 0.  An entry that names no sequence has no rows.  The
+ * same sequence may be in the list twice.  The pool is not changed. */
+typedef struct bkPagesBatchArgs {
+  uint64_t seqs;         /* int32 [n] */
+  uint64_t n_new;
+  uint64_t parent;
+  uint64_t table, lens, pos, slot, mask;
+  int32_t n, T, mask_words, reserved; /* T 1..1024; mask_words >= (T + 31) / 32 */
+} bkPagesBatchArgs;
+BK_API int32_t bkPagesBatch(const bkPages* pool, const bkPagesBatchArgs* args);
+
+/* Attention of drafted trees over pages: bkPagedAttn (whose fields, layouts and rules it has), but token t of sequence b sees the rows before its
+ * tree, [0, lens[b] - n_new[b]), and of the tree's rows those whose bit is set in its mask.  Bits at n_new[b] and behind count as 0; a token's
+ * own bit is a bit like the others.  A token that sees nothing gets zeros.  k and v go into the rows that slot names (a slot that is in no page of the pool: nowhere);
+ * fused_norm_rope takes the tables' row pos[t*B + b] (a token whose pos is outside [0, max_len) is not there).  A sequence with
+ * fewer than n_new[b] rows, or more than max_len or its table's pages hold, has no tokens that are there. */
+typedef struct bkTreeAttnArgs {
+  bkPagedAttnArgs attn;
+  uint64_t pos;          /* int32 [T*B]; 0 where fused_norm_rope is 0 */
+  uint64_t slot;         /* int32 [T*B]; 0 where k is 0 */
+  uint64_t mask;         /* uint32 [T*B][mask_words] */
+  int32_t mask_words;
+  int32_t reserved;
+} bkTreeAttnArgs;
+BK_API int32_t bkTreeAttn(const bkTreeAttnArgs* args);
+BK_API uint64_t bkTreeAttnScratchBytes(int32_t B, int32_t T, int32_t Hq, int32_t Hkv, int32_t HD, int32_t prefix_rows);
+
+/* Penalties for repeated tokens, biases and grammar masks on logits f32 [T*B][ld], in place; row t*B + b is token t of request b.  For token v, with
+ * n = how often v stands in the request's history behind its prompt, plus how often on the row's path:
+ *   x = logits[v];   if v stands in the history or on the path:  x = x > 0 ? x / repetition : x * repetition,  x -= frequency * n + presence * [n > 0];
+ *   x += bias of v (a token that a request names several times gets the sum, in the list's order);   x = -inf where the row's mask does not allow v.
+ * A logit that nothing names is neither read nor written, unless its mask hides one of its three neighbours (then it may be rewritten as it is).  NaN stays NaN where it is allowed. */
+#define BK_LOGITS_MAX_BIAS 1024
+typedef struct bkLogitsArgs {
+  uint64_t logits;
+  uint64_t seqs;         /* int32 [B]: the request's row in the arrays [n_seqs]; 0 = request b is row b.  One outside [0, n_seqs) has none of them */
+  uint64_t history;      /* int32 [n_seqs][history_ld]; tokens outside [0, V) count for nothing */
+  uint64_t hist_len, prompt_len;            /* int32 [n_seqs]: tokens in the history (0..history_ld), and how many of them are the prompt's; prompt_len 0 = none */
+  uint64_t repetition, presence, frequency; /* f32 [n_seqs]; 0 = 1, 0, 0 for all */
+  uint64_t draft;        /* int32 [T*B]: token of each node */
+  uint64_t path;         /* uint32 [T*B][path_words]: nodes on the row's path (bkPagesBatch's mask); draft and path 0 = none */
+  uint64_t bias_token;   /* int32 [n_seqs][bias_ld]; bias_token, bias_value and bias_n 0 = none */
+  uint64_t bias_value;   /* f32 [n_seqs][bias_ld] */
+  uint64_t bias_n;       /* int32 [n_seqs], 0..bias_ld */
+  uint64_t allowed;      /* uint32 [n_masks][allowed_words]: bit v % 32 of word v / 32 allows token v; allowed and mask_id 0 = all allowed */
+  uint64_t mask_id;      /* int32 [T*B]: the row's mask; outside [0, n_masks): all allowed */
+  int32_t B, T, V;
+  int32_t ld;            /* floats between rows of logits; 0 = V */
+  int32_t n_seqs;        /* 0 = B */
+  int32_t history_ld, bias_ld, path_words, n_masks, allowed_words;
+} bkLogitsArgs;
+BK_API int32_t bkAdjustLogits(const bkLogitsArgs* args);
+
+/* What the model agrees with stays.  target int32 [T][n] is the model's token after each node, token int32 [T][n] the node's own.  From node 0 the path
+ * goes on to the lowest child whose token is the target of the node before, as long as there is one.  The rows of the path move up
+ * behind the rows before the tree, in all planes; the others are given up, with the pages that only they had.
+ *   path int32 [T][n]: nodes of the path, -1 behind it (0 = not wanted); n_path int32 [n]; next int32 [n]: the target of the last (a token without a row yet)
+ *   history int32 [n_seqs][history_ld], hist_len int32 [n_seqs] (0 = none): the tokens of the path but node 0's, then next, are appended
+ * ok[i] (0 to skip): 1, or 0 where nothing is changed, n_path is 0, next and path are -1: the entry names no sequence or one named before, n_new[i] is not
+ * in 1..T, the sequence has fewer rows, a page that holds rows of its tree is shared (or none of the pool's), or its history has no room (or a length below 0). */
+typedef struct bkPagesCommitArgs {
+  uint64_t seqs, n_new;  /* int32 [n]; n_new 0 = T of each */
+  uint64_t parent, token, target;
+  uint64_t path, n_path, next, ok;
+  uint64_t history, hist_len;
+  int32_t n, T, history_ld, reserved; /* T 1..1024 */
+} bkPagesCommitArgs;
+BK_API int32_t bkPagesCommit(const bkPages* pool, const bkPagesCommitArgs* args);
+
 /* Low-rank adapters of many requests beside a shared projection: for every segment
  *   out[b] = base[b] + scale[a] * Bm[a] (A[a] x[b]),   a = ids[b];   out[b] = base[b] where a is outside [0, n_adapters).
  * Sums and A x in f32, one rounding at the end.  Call it after the projection (bkGemvQ4K) that wrote base. */
