@@ -1,9 +1,10 @@
 // bk_logits.cu -- penalties for repeated tokens, biases and grammar masks on logits, in place (bkAdjustLogits in bunker_cuda.h has the rules).
 //
-// What a row needs is sparse (the tokens of a history, of a path in a drafted tree, of a list of biases) but for the mask, so a row is not read as a
-// whole: a CTA has a slice of the vocabulary of one request, counts the request's tokens of that slice in shared memory, and reads and writes only the
-// quads of logits that something names; quads that a mask hides whole are written without being read.  Rows of one request (the nodes of its tree) share the
-// counts: a row adds its path's tokens and takes them back.  Counts are integers, so results do not depend on the order of threads.
+// Two kinds of CTAs, of one launch, which never touch the same logit.  Some hide what the masks forbid: a warp has 1,024 tokens of a row, a lane's mask word
+// at a time for all lanes, and only writes.  The others do what is named (tokens of a history, of a path in a drafted tree, of a list of biases), which is sparse: a CTA has a
+// slice of the vocabulary of one request (every 2^k-th block of 64 tokens, since frequent tokens have numbers near one another), counts the tokens of the history that
+// lie there in shared memory (a word for each token of the slice, or, for short histories, a table of those that occur), lists them, and goes over (listed token, row) pairs; the rows of a request, the nodes of its tree, share counts and list.  Tokens that are
+// drafted somewhere in the tree, or have a bias, are marked and left to a loop of their own.  Counts are integers, so results do not depend on the order of threads.
 //
 // No counterpart in the reference, which takes the argmax of the logits as they are (prototypes/decode.ts:749-791).
 #include <math.h>
@@ -16,13 +17,15 @@
 namespace {
 
 constexpr int kThreads = 512;
-constexpr int kQuads = 4;   // quads of logits that a thread has on the way
+constexpr int kUnits = 4;        // logits that a thread has on the way
+constexpr int kMaxNodes = 1024;  // of a tree
+constexpr int kMaxSlice = 16384; // words
+constexpr int kMaxTable = 8192;  // entries of a table (of 8 bytes), a quarter of them free
+constexpr int kBlock = 64;       // tokens that lie together in a slice
+constexpr int kAhead = 1;        // groups of four tokens of the history that a thread asks for before it knows the history's length
 
-// A token's word: how often it was said (20 bits), 1 + the place of its bias (11 bits), whether it is in the prompt.
-constexpr uint32_t kSaid = (1u << 20) - 1, kInPrompt = 1u << 31;
-constexpr int kBiasShift = 20;
-constexpr int kMaxHistory = (1 << 20) - 1 - 1024;   // with a path of up to 1,024 nodes behind it
-constexpr int kMaxNodes = 1024;
+// A token's word: how often it was said, whether the last loop has it, whether it is in the prompt.
+constexpr uint32_t kSaid = (1u << 30) - 1, kMarked = 1u << 30, kInPrompt = 1u << 31;
 
 struct LogitsParams {
   float* logits;
@@ -36,178 +39,294 @@ struct LogitsParams {
   const uint32_t* allowed;
   const int* mask_id;
   int B, T, V, n_seqs, history_ld, bias_ld, path_words, n_masks, allowed_words;
-  int slice, rows;   // tokens, and rows of a request, that a CTA has
+  int shift, slice, rows, parts;   // log2 of the number of slices; words, and rows of a request, that a CTA has; CTAs that share a request's rows
+  int naming, hiding;              // CTAs of each kind
   long long ld;
 };
 
 struct Penalty {
-  float repetition, presence, frequency;
+  float down, up, presence, frequency;   // of positive and other logits: 1 / repetition, rounded (a second rounding beside the product's), and repetition
 };
-BK_DEVINL float adjusted(float x, uint32_t w, const Penalty& a, const float* bias) {
-  const uint32_t n = w & kSaid, at = w >> kBiasShift & 2047u;
-  if (n || w & kInPrompt) {
-    x = x > 0.0f ? __fdiv_rn(x, a.repetition) : __fmul_rn(x, a.repetition);
-    x = __fsub_rn(x, __fadd_rn(__fmul_rn(a.frequency, (float)n), n ? a.presence : 0.0f));
+BK_DEVINL float taken(uint32_t n, const Penalty& a) { return fmaf(a.frequency, (float)n, n ? a.presence : 0.0f); }
+BK_DEVINL float adjusted(float x, float sub, const Penalty& a) { return fmaf(x, x > 0.0f ? a.down : a.up, -sub); }
+
+// Hides what the masks forbid.  Bound: the writes, 4 bytes a token at least (a sector that is written in part is read by the memory beside it).
+BK_DEVINL void hide(const LogitsParams& p, int cta) {
+  const int lane = threadIdx.x & 31, chunks = (p.V + 1023) / 1024;
+  const long long items = (long long)p.T * p.B * chunks, warps = (long long)p.hiding * (kThreads / 32), w = (long long)cta * (kThreads / 32) + (threadIdx.x >> 5);
+  const long long i1 = items * (w + 1) / warps;
+  long long i = items * w / warps;
+  long long row = i / chunks;
+  int chunk = (int)(i - row * chunks);
+  auto id_of = [&]() {
+    const int id = i < i1 ? __ldg(p.mask_id + row) : -1;
+    return id >= 0 && id < p.n_masks ? id : -1;
+  };
+  auto word_of = [&](int id) {   // this lane's 32 tokens; one behind the vocabulary is not hidden
+    const int at = chunk * 32 + lane, left = p.V - at * 32;
+    if (id < 0 || left <= 0) return 0xffffffffu;
+    return __ldg(p.allowed + (size_t)id * p.allowed_words + at) | (left < 32 ? 0xffffffffu << left : 0u);
+  };
+  int id = id_of();
+  uint32_t word = word_of(id);
+  while (i < i1) {
+    float* x = p.logits + row * p.ld + chunk * 1024 + lane;
+    const uint32_t now = word;
+    i++;
+    if (++chunk == chunks) {
+      chunk = 0;
+      row++;
+      id = id_of();
+    }
+    word = i < i1 ? word_of(id) : 0xffffffffu;
+    if (!__any_sync(0xffffffffu, now != 0xffffffffu)) continue;
+#pragma unroll
+    for (int j = 0; j < 32; j++)
+      if (!(__shfl_sync(0xffffffffu, now, j) >> lane & 1u)) x[j * 32] = -INFINITY;
   }
-  return at ? __fadd_rn(x, bias[at - 1]) : x;
 }
 
-// VEC: rows start on 16 bytes
-template <bool VEC>
-__global__ void __launch_bounds__(kThreads) adjust_logits_kernel(const __grid_constant__ LogitsParams p) {
-  extern __shared__ __align__(16) uint32_t word_s[];   // [slice]
-  __shared__ int bias_at_s[BK_LOGITS_MAX_BIAS], warp_s[kThreads / 32];
-  __shared__ float bias_s[BK_LOGITS_MAX_BIAS];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, b = blockIdx.y, lo = blockIdx.x * p.slice, n = min(p.slice, p.V - lo);
-  for (int i = tid; i < p.slice / 4; i += kThreads) reinterpret_cast<uint4*>(word_s)[i] = make_uint4(0, 0, 0, 0);
+// TABLE: words belong to the tokens of a table (open addressing), not to all of the slice's
+template <bool TABLE>
+__global__ void __launch_bounds__(kThreads, 3) adjust_logits_kernel(const __grid_constant__ LogitsParams p) {
+  extern __shared__ __align__(16) uint32_t word_s[];        // [slice], then lists, see there
+  __shared__ int node_s[kMaxNodes], warp_s[kThreads / 32];  // nodes whose token lies in the slice: node << 16 | place
+  __shared__ int n_node_s, n_marked_s, n_listed_s, mask_s[kMaxNodes];   // mask_s: of each row, -1 where it has none
   bk_pdl_wait();
   bk_pdl_trigger();
+  if ((int)blockIdx.x >= p.naming) {
+    hide(p, blockIdx.x - p.naming);
+    return;
+  }
+  const int marks = p.bias_ld + (p.path ? p.T : 0);
+  float* const bias_s = reinterpret_cast<float*>(word_s + p.slice);           // [bias_ld]: the slice's biases
+  float* const sum_s = bias_s + p.bias_ld;                                    // [marks]: of a marked token
+  uint16_t* const marked_s = reinterpret_cast<uint16_t*>(sum_s + marks);      // [marks]
+  uint16_t* const bias_at_s = marked_s + marks;                               // [bias_ld]
+  uint16_t* const listed_s = bias_at_s + p.bias_ld;                           // [slice]: places of tokens that something but a mark names
+  int* const key_s = reinterpret_cast<int*>(listed_s + p.slice + ((marks + p.bias_ld) & 1));   // TABLE: [slice] tokens, -1: free
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, part = blockIdx.x & ((1 << p.shift) - 1), group = blockIdx.x >> p.shift, b = group / p.parts,
+            t0 = (group - b * p.parts) * p.rows, rows = min(p.rows, p.T - t0);
+  if (rows <= 0) return;
+  // token -> its place in the slice, -1: not in it; place -> token
+  auto place = [&](int token) {
+    const uint32_t block = (uint32_t)token / kBlock;
+    if ((uint32_t)token >= (uint32_t)p.V || (block & ((1u << p.shift) - 1u)) != (uint32_t)part) return -1;
+    if (!TABLE) return (int)(block >> p.shift) * kBlock + token % kBlock;
+    int at = (int)((uint32_t)token * 2654435761u >> 16 & (uint32_t)(p.slice - 1));
+    while (true) {   // (ends: the table has more entries than the request names tokens)
+      int there = *reinterpret_cast<volatile int*>(key_s + at);   // (most are there already: equal addresses are one read, but one atomic after the other)
+      if (there == -1) there = atomicCAS(key_s + at, -1, token);
+      if (there == -1 || there == token) return at;
+      at = (at + 1) & (p.slice - 1);
+    }
+  };
+  auto token_of = [&](int at) { return TABLE ? key_s[at] : ((at / kBlock << p.shift) + part) * kBlock + at % kBlock; };
   const int s = p.seqs ? p.seqs[b] : b;
   const bool known = s >= 0 && s < p.n_seqs;
-  Penalty a = {1.0f, 0.0f, 0.0f};
+  // everything that the request has is asked for at once, beyond what counts where its arrays are longer
+  Penalty a = {1.0f, 1.0f, 0.0f, 0.0f};
+  int said = 0, prompt = 0, listed = 0, head = 0;
+  const int* h = p.history + (known ? (size_t)s * p.history_ld : 0);
+  int4 ahead[kAhead];
+  int bias_token[BK_LOGITS_MAX_BIAS / kThreads], draft[kMaxNodes / kThreads];
+  float bias_value[BK_LOGITS_MAX_BIAS / kThreads];
   if (known) {
-    if (p.repetition) a.repetition = p.repetition[s];
+    if (p.history) {
+      said = p.hist_len[s];
+      head = min(p.history_ld, (int)((16 - ((uintptr_t)h & 15)) & 15) / 4);
+#pragma unroll
+      for (int k = 0; k < kAhead; k++)
+        if (head + 4 * (tid + k * kThreads) + 4 <= p.history_ld) ahead[k] = __ldcg(reinterpret_cast<const int4*>(h + head) + tid + k * kThreads);
+    }
+    if (p.prompt_len) prompt = p.prompt_len[s];
+    if (p.repetition) a.up = p.repetition[s];
     if (p.presence) a.presence = p.presence[s];
     if (p.frequency) a.frequency = p.frequency[s];
+    if (p.bias_ld) {
+      listed = p.bias_n[s];
+#pragma unroll
+      for (int k = 0; k < BK_LOGITS_MAX_BIAS / kThreads; k++) {
+        const int i = tid + k * kThreads;
+        if (i < p.bias_ld) {
+          bias_token[k] = p.bias_token[(size_t)s * p.bias_ld + i];
+          bias_value[k] = p.bias_value[(size_t)s * p.bias_ld + i];
+        }
+      }
+    }
   }
+  if (p.path) {
+#pragma unroll
+    for (int k = 0; k < kMaxNodes / kThreads; k++)
+      if (tid + k * kThreads < p.T) draft[k] = p.draft[(size_t)(tid + k * kThreads) * p.B + b];
+  }
+  for (int t = tid; t < rows; t += kThreads) {
+    const int id = p.mask_id ? p.mask_id[(size_t)(t0 + t) * p.B + b] : -1;
+    mask_s[t] = id >= 0 && id < p.n_masks ? id : -1;
+  }
+  for (int i = tid; i < p.slice / 4; i += kThreads) reinterpret_cast<uint4*>(word_s)[i] = make_uint4(0, 0, 0, 0);
+  if (TABLE)
+    for (int i = tid; i < p.slice; i += kThreads) key_s[i] = -1;
+  if (tid == 0) n_node_s = n_marked_s = n_listed_s = 0;
+  said = max(0, min(said, p.history_ld));
+  listed = max(0, min(listed, p.bias_ld));
+  a.down = __fdiv_rn(1.0f, a.up);
   __syncthreads();
-  if (known && p.history) {
-    const int said = max(0, min(p.hist_len[s], p.history_ld)), prompt = p.prompt_len ? p.prompt_len[s] : 0;
-    const int* h = p.history + (size_t)s * p.history_ld;
+  if (said) {
+    head = min(head, said);
     auto count = [&](int token, int i) {
-      const uint32_t o = (uint32_t)token - (uint32_t)lo;
-      if (o < (uint32_t)n) {
+      const int o = place(token);
+      if (o >= 0) {
         if (i < prompt) atomicOr(word_s + o, kInPrompt);
         else atomicAdd(word_s + o, 1u);
       }
     };
-    const int head = min(said, (int)((16 - ((uintptr_t)h & 15)) & 15) / 4), quads = (said - head) / 4;
-    if (tid < head) count(h[tid], tid);
-#pragma unroll 4
-    for (int q = tid; q < quads; q += kThreads) {
-      const int4 v = __ldcg(reinterpret_cast<const int4*>(h + head) + q);
+    const int quads = (said - head) / 4;
+    auto count4 = [&](int4 v, int q) {
       const int i = head + 4 * q;
       count(v.x, i); count(v.y, i + 1); count(v.z, i + 2); count(v.w, i + 3);
-    }
+    };
+    if (tid < head) count(h[tid], tid);
+#pragma unroll
+    for (int k = 0; k < kAhead; k++)
+      if (tid + k * kThreads < quads) count4(ahead[k], tid + k * kThreads);
+#pragma unroll 4
+    for (int q = tid + kAhead * kThreads; q < quads; q += kThreads) count4(__ldcg(reinterpret_cast<const int4*>(h + head) + q), q);
     const int i = head + 4 * quads + tid;
     if (i < said) count(h[i], i);
   }
-  if (known && p.bias_token) {
-    // the slice's entries, in the list's order
-    const int listed = max(0, min(p.bias_n[s], p.bias_ld));
-    int m = 0;
-    for (int i0 = 0; i0 < listed; i0 += kThreads) {
-      const int i = i0 + tid;
-      const uint32_t o = i < listed ? (uint32_t)p.bias_token[(size_t)s * p.bias_ld + i] - (uint32_t)lo : 0xffffffffu;
-      const bool mine = o < (uint32_t)n;
-      const uint32_t votes = __ballot_sync(0xffffffffu, mine);
-      if (lane == 0) warp_s[warp] = __popc(votes);
-      __syncthreads();
-      int at = m + __popc(votes & ((1u << lane) - 1u));
-      for (int w = 0; w < kThreads / 32; w++) {
-        if (w < warp) at += warp_s[w];
-        m += warp_s[w];
-      }
-      if (mine) {
-        bias_at_s[at] = (int)o;
-        bias_s[at] = p.bias_value[(size_t)s * p.bias_ld + i];
-      }
-      __syncthreads();
-    }
-    // a token's first entry gets the sum of all of its (a thread may only write its own, so sums are stored behind a barrier)
-    float sum[BK_LOGITS_MAX_BIAS / kThreads];
-    int first = 0;   // bit k: entry tid + k * kThreads is its token's first
+  // marked tokens: who sets a token's mark writes it down
+  auto mark = [&](int o) {
+    if (!(atomicOr(word_s + o, kMarked) & kMarked)) marked_s[atomicAdd(&n_marked_s, 1)] = (uint16_t)o;
+  };
+  int m = 0;   // biases of the slice, in the list's order
 #pragma unroll
-    for (int k = 0; k < BK_LOGITS_MAX_BIAS / kThreads; k++) {
-      const int i = tid + k * kThreads;
-      if (i >= m) continue;
-      const int o = bias_at_s[i];
-      bool earlier = false;
-      float y = 0.0f;
-      for (int j = 0; j < m; j++)
-        if (bias_at_s[j] == o) {
-          if (j < i) earlier = true;
-          else y = j == i ? bias_s[j] : __fadd_rn(y, bias_s[j]);
-        }
-      sum[k] = y;
-      if (!earlier) first |= 1 << k;
-    }
+  for (int k = 0; k < BK_LOGITS_MAX_BIAS / kThreads; k++) {
+    if (k * kThreads >= listed) break;
+    const int o = tid + k * kThreads < listed ? place(bias_token[k]) : -1;
+    const uint32_t votes = __ballot_sync(0xffffffffu, o >= 0);
+    if (k) __syncthreads();
+    if (lane == 0) warp_s[warp] = __popc(votes);
     __syncthreads();
+    int at = m + __popc(votes & ((1u << lane) - 1u));
+    for (int w = 0; w < kThreads / 32; w++) {
+      if (w < warp) at += warp_s[w];
+      m += warp_s[w];
+    }
+    if (o >= 0) {
+      bias_at_s[at] = (uint16_t)o;
+      bias_s[at] = bias_value[k];
+      mark(o);
+    }
+  }
+  if (p.path) {
 #pragma unroll
-    for (int k = 0; k < BK_LOGITS_MAX_BIAS / kThreads; k++)
-      if (first >> k & 1) {
-        const int i = tid + k * kThreads;
-        bias_s[i] = sum[k];
-        atomicOr(word_s + bias_at_s[i], (uint32_t)(i + 1) << kBiasShift);
+    for (int k = 0; k < kMaxNodes / kThreads; k++) {
+      const int u = tid + k * kThreads, o = u < p.T ? place(draft[k]) : -1;
+      if (o >= 0) {
+        node_s[atomicAdd(&n_node_s, 1)] = u << 16 | o;
+        mark(o);
       }
+    }
+  }
+  __syncthreads();
+  const int marked = n_marked_s, nodes = n_node_s;
+  for (int i = tid; i < marked; i += kThreads) {   // the sum of a marked token's biases, in the list's order
+    const int o = marked_s[i];
+    float y = 0.0f;
+    bool any = false;
+    for (int j = 0; j < m; j++)
+      if (bias_at_s[j] == o) {
+        y = any ? __fadd_rn(y, bias_s[j]) : bias_s[j];
+        any = true;
+      }
+    sum_s[i] = any ? y : -0.0f;   // (adds nothing, not even to a zero's sign)
+  }
+  if (said) {   // the others that are named: a warp's in one piece
+    for (int q0 = warp * 32; q0 < p.slice / 4; q0 += kThreads) {
+      const int q = q0 + lane;
+      uint4 w = make_uint4(0, 0, 0, 0);
+      if (q < p.slice / 4) w = reinterpret_cast<const uint4*>(word_s)[q];
+      auto here = [](uint32_t u) { return u != 0 && !(u & kMarked); };
+      const int n = here(w.x) + here(w.y) + here(w.z) + here(w.w);
+      if (!__any_sync(0xffffffffu, n)) continue;
+      int upto = n;
+#pragma unroll
+      for (int off = 1; off < 32; off <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, upto, off);
+        if (lane >= off) upto += y;
+      }
+      int at = 0;
+      if (lane == 31) at = atomicAdd(&n_listed_s, upto);
+      at = __shfl_sync(0xffffffffu, at, 31) + upto - n;
+      if (here(w.x)) listed_s[at++] = (uint16_t)(4 * q);
+      if (here(w.y)) listed_s[at++] = (uint16_t)(4 * q + 1);
+      if (here(w.z)) listed_s[at++] = (uint16_t)(4 * q + 2);
+      if (here(w.w)) listed_s[at++] = (uint16_t)(4 * q + 3);
+    }
   }
   __syncthreads();
 
-  const int t1 = min(p.T, (int)(blockIdx.z + 1) * p.rows);
-  for (int t = blockIdx.z * p.rows; t < t1; t++) {
-    const size_t row = (size_t)t * p.B + b;
-    // the path's tokens, for this row only
-    auto path = [&](uint32_t by) {
-      for (int u = tid; u < p.T; u += kThreads)
-        if (p.path[row * p.path_words + (u >> 5)] >> (u & 31) & 1u) {
-          const uint32_t o = (uint32_t)p.draft[(size_t)u * p.B + b] - (uint32_t)lo;
-          if (o < (uint32_t)n) atomicAdd(word_s + o, by);
-        }
-    };
-    if (p.path) {
-      path(1u);
-      __syncthreads();
-    }
-    const int id = p.mask_id ? p.mask_id[row] : -1;
-    const uint32_t* allowed = id >= 0 && id < p.n_masks ? p.allowed + (size_t)id * p.allowed_words + lo / 32 : nullptr;
-    float* x = p.logits + row * p.ld + lo;
-    const int quads = (n + 3) / 4;
-    for (int q0 = tid; q0 < quads; q0 += kThreads * kQuads) {
-      uint4 w[kQuads];
-      uint32_t open[kQuads];   // bit e: token e of the quad is allowed
-      float v[kQuads][4];
-      int todo = 0;
+  // (named token, row) pairs, rows next to one another in turn, kUnits pairs of a thread at once
+  const int n_listed = n_listed_s;
+  const size_t next = (size_t)p.B * p.ld;   // floats from a row to the request's next
+  float* const x0 = p.logits + ((size_t)t0 * p.B + b) * p.ld;
+  auto hidden = [&](int t, int token) {
+    const int id = mask_s[t];
+    return id >= 0 && !(__ldg(p.allowed + (size_t)id * p.allowed_words + (token >> 5)) >> (token & 31) & 1u);
+  };
+  if (rows == 1) {
+    for (int i0 = tid; i0 < n_listed; i0 += kThreads * kUnits) {
+      float* at[kUnits];
+      float x[kUnits];
+      uint32_t w[kUnits];
 #pragma unroll
-      for (int k = 0; k < kQuads; k++) {
-        const int q = q0 + k * kThreads;
-        w[k] = make_uint4(0, 0, 0, 0);
-        open[k] = 15;
-        if (q >= quads) continue;
-        w[k] = reinterpret_cast<const uint4*>(word_s)[q];
-        if (allowed) open[k] = __ldg(allowed + (q >> 3)) >> (q & 7) * 4 & 15u;
-        if ((w[k].x | w[k].y | w[k].z | w[k].w) == 0 && open[k] == 15) continue;
-        todo |= 1 << k;
-        if (open[k] == 0) continue;   // (written without being read)
-        if (VEC && 4 * q + 4 <= n) {
-          const float4 y = __ldcg(reinterpret_cast<const float4*>(x) + q);
-          v[k][0] = y.x; v[k][1] = y.y; v[k][2] = y.z; v[k][3] = y.w;
-        } else {
-#pragma unroll
-          for (int e = 0; e < 4; e++)
-            if (4 * q + e < n) v[k][e] = __ldcg(x + 4 * q + e);
-        }
+      for (int k = 0; k < kUnits; k++) {
+        const int i = i0 + k * kThreads;
+        at[k] = nullptr;
+        if (i >= n_listed) continue;
+        const int o = listed_s[i], token = token_of(o);
+        w[k] = word_s[o];
+        if (!hidden(0, token)) at[k] = x0 + token;
+        x[k] = __ldcg(x0 + token);
       }
 #pragma unroll
-      for (int k = 0; k < kQuads; k++) {
-        if (!(todo >> k & 1)) continue;
-        const int q = q0 + k * kThreads;
-        const uint32_t words[4] = {w[k].x, w[k].y, w[k].z, w[k].w};
+      for (int k = 0; k < kUnits; k++)
+        if (at[k]) *at[k] = adjusted(x[k], taken(w[k] & kSaid, a), a);
+    }
+  } else {
+    for (int i = tid; i < n_listed; i += kThreads) {
+      const int o = listed_s[i], token = token_of(o);
+      const float sub = taken(word_s[o] & kSaid, a);
+      float* at = x0 + token;
+      for (int t = 0; t < rows; t += kUnits, at += kUnits * next) {
+        float x[kUnits];
+        bool on[kUnits];
 #pragma unroll
-        for (int e = 0; e < 4; e++) v[k][e] = open[k] >> e & 1 ? words[e] ? adjusted(v[k][e], words[e], a, bias_s) : v[k][e] : -INFINITY;
-        if (VEC && 4 * q + 4 <= n) {
-          reinterpret_cast<float4*>(x)[q] = make_float4(v[k][0], v[k][1], v[k][2], v[k][3]);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 4; e++)
-            if (4 * q + e < n) x[4 * q + e] = v[k][e];
+        for (int k = 0; k < kUnits; k++) {
+          on[k] = t + k < rows && !hidden(t + k, token);
+          if (on[k]) x[k] = __ldcg(at + k * next);
         }
+#pragma unroll
+        for (int k = 0; k < kUnits; k++)
+          if (on[k]) at[k * next] = adjusted(x[k], sub, a);
       }
     }
-    if (p.path && t + 1 < t1) {
-      __syncthreads();
-      path(0xffffffffu);
-      __syncthreads();
+  }
+  for (int it = tid; it < marked * rows; it += kThreads) {
+    const int t = it / marked, i = it - t * marked, o = marked_s[i], token = token_of(o);
+    if (hidden(t, token)) continue;
+    const size_t row = (size_t)(t0 + t) * p.B + b;
+    const uint32_t w = word_s[o];
+    uint32_t said_here = w & kSaid;
+    for (int j = 0; j < nodes; j++) {
+      const int u = node_s[j] >> 16;
+      if ((node_s[j] & 0xffff) == o) said_here += __ldg(p.path + row * p.path_words + (u >> 5)) >> (u & 31) & 1u;
     }
+    float* x = x0 + t * next + token;
+    float y = __ldcg(x);
+    if (said_here || w & kInPrompt) y = adjusted(y, taken(said_here, a), a);
+    *x = __fadd_rn(y, sum_s[i]);
   }
 }
 
@@ -223,7 +342,7 @@ extern "C" int32_t bkAdjustLogits(const bkLogitsArgs* args) {
   BK_ARG(a.n_seqs >= 0, "bkAdjustLogits: n_seqs=%d", a.n_seqs);
   BK_ARG(((a.seqs | a.history | a.hist_len | a.prompt_len | a.repetition | a.presence | a.frequency | a.draft | a.path | a.bias_token | a.bias_value | a.bias_n | a.allowed | a.mask_id) & 3) == 0,
          "bkAdjustLogits: all arrays are of 32-bit words");
-  BK_ARG(!a.history || (a.hist_len && a.history_ld > 0 && a.history_ld <= kMaxHistory), "bkAdjustLogits: history needs hist_len and history_ld (%d; 1 to %d)", a.history_ld, kMaxHistory);
+  BK_ARG(!a.history || (a.hist_len && a.history_ld > 0 && a.history_ld <= (1 << 29)), "bkAdjustLogits: history needs hist_len and history_ld (%d; 1 to 2^29)", a.history_ld);
   BK_ARG((a.path != 0) == (a.draft != 0) && (!a.path || a.path_words >= (a.T + 31) / 32), "bkAdjustLogits: draft and path go together, path_words=%d for %d nodes", a.path_words, a.T);
   BK_ARG((a.bias_token != 0) == (a.bias_value != 0) && (a.bias_token != 0) == (a.bias_n != 0) && (!a.bias_token || (a.bias_ld > 0 && a.bias_ld <= BK_LOGITS_MAX_BIAS)),
          "bkAdjustLogits: bias_token, bias_value and bias_n go together, bias_ld=%d (1 to %d)", a.bias_ld, BK_LOGITS_MAX_BIAS);
@@ -232,18 +351,40 @@ extern "C" int32_t bkAdjustLogits(const bkLogitsArgs* args) {
   LogitsParams p = {bk_ptr<float>(a.logits), bk_ptr<int>(a.seqs), bk_ptr<int>(a.history), bk_ptr<int>(a.hist_len), bk_ptr<int>(a.prompt_len), bk_ptr<float>(a.repetition),
                     bk_ptr<float>(a.presence), bk_ptr<float>(a.frequency), bk_ptr<int>(a.draft), bk_ptr<uint32_t>(a.path), bk_ptr<int>(a.bias_token), bk_ptr<float>(a.bias_value),
                     bk_ptr<int>(a.bias_n), bk_ptr<uint32_t>(a.allowed), bk_ptr<int>(a.mask_id), a.B, a.T, a.V, a.n_seqs ? a.n_seqs : a.B, a.history_ld, a.bias_ld, a.path_words,
-                    a.n_masks, a.allowed_words, 0, 0, a.ld ? a.ld : a.V};
-  // Slices of 8,192 tokens (32 KB of words, four CTAs an SM), shorter while that leaves SMs without one; then rows apart, until each SM has four.
+                    a.n_masks, a.allowed_words, 0, 0, 0, 0, 0, 0, a.ld ? a.ld : a.V};
+  if (!a.bias_token) p.bias_ld = 0;
+  // Who names: slices of at most 16,384 words (96 KB with the list, two CTAs an SM), shorter while that leaves SMs without a CTA, to 1,024; then rows apart, until each SM
+  // has four CTAs.  Where such a slice has more than 4,096 words and the request's tokens fit a table, fewer CTAs with a table each (64 requests, 5,000 tokens
+  // of 151,936: 25.5 us with 16 slices of words, 15.5 with four tables; one request, 700 tokens: 4.6 with 128 slices of words, 5.2 with as many tables).
+  // Who hides: four CTAs an SM, no more than have 4,096 tokens each.
   const long long sms = bk_ctx().sm_count;
-  p.slice = 8192;
-  while (p.slice > 1024 && (long long)((a.V + p.slice - 1) / p.slice) * a.B * a.T < sms) p.slice /= 2;
-  const long long ctas = (long long)((a.V + p.slice - 1) / p.slice) * a.B;
-  const int parts = (int)std::min<long long>(a.T, (4 * sms + ctas - 1) / ctas);
-  p.rows = (a.T + parts - 1) / parts;
-  const dim3 grid((a.V + p.slice - 1) / p.slice, a.B, (a.T + p.rows - 1) / p.rows);
-  const bool vec = (a.logits & 15) == 0 && p.ld % 4 == 0;
-  if (vec) BK_CUDA(bk_launch_pdl(adjust_logits_kernel<true>, grid, dim3(kThreads), (size_t)p.slice * 4, p));
-  else BK_CUDA(bk_launch_pdl(adjust_logits_kernel<false>, grid, dim3(kThreads), (size_t)p.slice * 4, p));
+  const int blocks = (a.V + kBlock - 1) / kBlock;
+  const long long names = (a.history ? a.history_ld : 0) + p.bias_ld + (a.path ? a.T : 0);
+  int table = 512;
+  while (table <= kMaxTable && 3ll * table < 4 * names) table *= 2;
+  auto slice_of = [&](int shift) { return ((blocks + (1 << shift) - 1) >> shift) * kBlock; };
+  while (slice_of(p.shift) > kMaxSlice || (slice_of(p.shift) > 1024 && ((long long)a.B * a.T << p.shift) < sms)) p.shift++;
+  p.slice = slice_of(p.shift);
+  const bool use_table = table <= kMaxTable && p.slice > 4096;
+  if (use_table) {
+    p.slice = table;
+    while (p.shift > 0 && ((long long)a.B * a.T << (p.shift - 1)) >= sms) p.shift--;
+  }
+  const long long ctas = (long long)a.B << p.shift;
+  p.parts = (int)std::min<long long>(a.T, (4 * sms + ctas - 1) / ctas);
+  p.rows = (a.T + p.parts - 1) / p.parts;
+  if (a.allowed) p.hiding = (int)std::max<long long>(1, std::min<long long>(4 * sms, (long long)a.T * a.B * a.V / 4096));
+  BK_ARG(ctas * p.parts + p.hiding < (1ll << 31), "bkAdjustLogits: B=%d rows of %d logits: too much for one call", a.B, a.V);
+  if (a.history || a.bias_token || a.path) p.naming = (int)ctas * p.parts;
+  if (p.naming + p.hiding == 0) return BK_OK;
+  const size_t marks = (size_t)p.bias_ld + (a.path ? a.T : 0), smem = (size_t)p.slice * (use_table ? 10 : 6) + (size_t)p.bias_ld * 6 + marks * 6 + 4;   // at most 96 + 6 + 12 KB
+  auto* kernel = use_table ? adjust_logits_kernel<true> : adjust_logits_kernel<false>;
+  static bool configured[2] = {false, false};
+  if (!configured[use_table]) {
+    BK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 116 << 10));
+    configured[use_table] = true;
+  }
+  BK_CUDA(bk_launch_pdl(kernel, dim3(p.naming + p.hiding), dim3(kThreads), smem, p));
   BK_CHECK_LAUNCH();
   return BK_OK;
 }

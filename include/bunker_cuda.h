@@ -383,7 +383,7 @@ BK_API uint64_t bkTreeAttnScratchBytes(int32_t B, int32_t T, int32_t Hq, int32_t
  * n = how often v stands in the request's history behind its prompt, plus how often on the row's path:
  *   x = logits[v];   if v stands in the history or on the path:  x = x > 0 ? x / repetition : x * repetition,  x -= frequency * n + presence * [n > 0];
  *   x += bias of v (a token that a request names several times gets the sum, in the list's order);   x = -inf where the row's mask does not allow v.
- * A logit that nothing names is neither read nor written, unless its mask hides one of its three neighbours (then it may be rewritten as it is).  NaN stays NaN where it is allowed. */
+ * A logit that nothing names or hides is neither read nor written.  NaN stays NaN where it is allowed. */
 #define BK_LOGITS_MAX_BIAS 1024
 typedef struct bkLogitsArgs {
   uint64_t logits;

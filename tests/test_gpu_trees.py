@@ -517,6 +517,15 @@ def test_logits_of_long_histories_of_few_tokens(bk):
     Logits(9, 2, 4, 151936, history=33333, n_bias=300, n_masks=2, tree=True).check()
 
 
+@pytest.mark.parametrize("B,T,V,history,n_bias", [(64, 1, 30000, 1, 0), (64, 1, 30000, 300, 5), (160, 1, 9000, 6000, 40), (150, 1, 16500, 6143, 1), (150, 1, 16500, 6145, 0),
+                                                  (20, 8, 20000, 5000, 1024), (150, 1, 40000, 9000, 3), (8, 40, 33000, 2000, 0)])
+def test_logits_of_many_requests(bk, B, T, V, history, n_bias):
+    """Slices of words and tables, histories around what a table holds, repeated tokens."""
+    c = Logits(B + history, B, T, V, history=history, n_bias=n_bias, n_masks=3, tree=T > 1)
+    c.hist[:, ::3] = c.hist[:, :1]
+    c.check()
+
+
 def test_logits_of_a_token_that_a_request_names_often(bk):
     c = Logits(10, 2, 1, 5000, history=30, n_bias=1024)
     c.bt[0, ::2], c.bt[1, 1000:] = 17, 4999
@@ -575,7 +584,7 @@ def test_logits_refuse_what_they_cannot_do(bk):
     refused("ld=", ld=99)
     refused("n_seqs", n_seqs=-1)
     refused("32-bit", draft=c.args().draft + 1)
-    for change in (dict(hist_len=0), dict(history_ld=0), dict(history_ld=1 << 20)):
+    for change in (dict(hist_len=0), dict(history_ld=0), dict(history_ld=(1 << 29) + 1)):
         refused("history", **change)
     for change in (dict(draft=0), dict(path=0), dict(path_words=0)):
         refused("path", **change)
