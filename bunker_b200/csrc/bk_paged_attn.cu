@@ -36,7 +36,15 @@ struct TreeParams {
   const int *pos, *slot;
   const uint32_t* mask;   // [T * B][words]
   int words, max_pos;
+  int each;               // heads that a warp makes ready
+  // In the scratch buffer, made by the first launch.  Ready queries and rows of jobs are those of tokens that are there, one sequence's behind the other's (with more
+  // than kCompact sequences: T for each).
+  int* first;             // [B + 1]: where a sequence's tokens begin; how many there are
+  int* token;             // [B * T]: t * B + b of each (up to kCompact sequences)
+  int* place;             // [T * B]: which of them a row is, -1: not there, or it sees nothing
+  int4* team;             // see plan_trees
 };
+constexpr int kCompact = 1024;
 struct NoTree {};
 template <bool TREE>
 struct Params : PagedParams, std::conditional<TREE, TreeParams, NoTree>::type {};
@@ -58,10 +66,6 @@ BK_DEVINL Tree tree_of(const Params<true>& p, int b) {
   r.base = len - r.n;
   if (len < r.n || len > p.max_rows) r.n = r.base = 0;
   return r;
-}
-BK_DEVINL int row_of(const Params<true>& p, int b, int t) {
-  const Tree r = tree_of(p, b);
-  return t < r.n ? r.base + t : -1;
 }
 // word i of the nodes that a row sees, of n; all ones before the first
 BK_DEVINL uint32_t node_word(const uint32_t* bits, int n, int i) {
@@ -172,12 +176,7 @@ BK_DEVINL Job job_of(const PagedParams& p, const Layout& L, int j) {
   q.key0 = L.P;
   return q;
 }
-// the end of its keys: behind the row of the last of the tile's tokens that is there; a node may see any other of its tree
-BK_DEVINL int keys_end(const Params<true>& p, const Layout& L, const Job& q) {
-  if (q.seq < 0) return L.P;
-  const Tree r = tree_of(p, q.seq);
-  return max(L.P, r.base + r.n);
-}
+// the end of its keys: behind the row of the last of the tile's tokens that is there
 BK_DEVINL int keys_end(const Params<false>& p, const Layout& L, const Job& q) {
   if (q.seq < 0) return L.P;
   const int G = p.Hq / p.Hkv, n = p.n_new ? min(p.n_new[q.seq], p.T) : p.T, last = min(n, (min(p.T * G, (q.mt + 1) * kRows) - 1) / G + 1) - 1;
@@ -204,8 +203,8 @@ BK_DEVINL void piece_of(int s, int n, int u0, int u1, int* t0, int* t1) {
 constexpr int kPrepThreads = 256, kPlanned = 1024;   // jobs whose starts fit in shared memory
 // SMEM: no more than kPlanned jobs, whose lines are worked on in shared memory; otherwise in the records themselves.  What it takes is on every
 // call's way: a chain of loads from L2 costs 0.6 us a link.
-template <bool SMEM, bool TREE>
-BK_DEVINL void plan_jobs(const Params<TREE>& p, const Layout& L, uint8_t* scratch) {
+template <bool SMEM>
+BK_DEVINL void plan_jobs(const Params<false>& p, const Layout& L, uint8_t* scratch) {
   __shared__ int warp_s[kPrepThreads / 32][2], starts_s[SMEM ? kPlanned + 1 : 1], ends_s[SMEM ? kPlanned : 1], bounds_s[kPrepThreads + 1];
   int4* jobs = jobs_of(L, scratch);
   int4* pieces = pieces_of(L, scratch);
@@ -322,6 +321,210 @@ BK_DEVINL void plan_jobs(const Params<TREE>& p, const Layout& L, uint8_t* scratc
   if (SMEM && threadIdx.x == 0) jobs[n] = make_int4(units, 0, 0, 0);
 }
 
+// ---- who does what, for trees --------------------------------------------------------------
+// A tree has many rows to a sequence, so most jobs are several row tiles over the same keys.  CTAs come in teams, each of which takes one row tile of the same keys at the
+// same time, so that the keys are read from memory once: a sequence's m row tiles (the common keys' too) are cut into as few teams of up to kTeam tiles as there can be, of
+// equal width but for one tile.  Teams of one width are jobs on a line of their own, which is cut into equal pieces for the line's share of the CTAs; shares are the
+// smallest longest piece.  (All row tiles on one line, 32 sequences of up to 16,384 rows and 64 nodes, 24 heads on 4: 704 us, the keys read once for each row tile;
+// so ???.)
+constexpr int kTeam = 4;
+// Team job i: {start on its line, job of its first row tile, end of its keys, slot of its first row tile's partial result for team 0}; the slots of a team job's pieces
+// are kTeam-wide steps: slot + w * team + rank, which no two pieces share since i + team grows from piece to piece of a line.  jobs[j] = {.., .., first slot, number and
+// distance of slots}; pieces[2c] = {start and end of CTA c's piece of its line, first team job in it, end of the line's team jobs}, pieces[2c + 1] = {w * team + rank, rank}.
+struct Teams {   // of m row tiles: `wide` teams of w + 1, `all - wide` of w
+  int all, wide, w;
+  BK_DEVINL explicit Teams(int m) {
+    all = (m + kTeam - 1) / kTeam;
+    w = all ? m / all : 0;
+    wide = m - all * w;
+  }
+  BK_DEVINL int of_width(int v) const { return v == w ? all - wide : v == w + 1 ? wide : 0; }
+};
+// floor((n t - less) / of)
+BK_DEVINL int share_of(int n, int t, int of, int less = 0) {
+  const unsigned long long x = (unsigned long long)n * t - less;
+  return x >> 32 ? (int)(x / of) : (int)((unsigned int)x / (unsigned int)of);
+}
+// one CTA
+BK_DEVINL void plan_trees(const Params<true>& p, const Layout& L, uint8_t* scratch) {
+  __shared__ int sum_s[2 * kTeam][kPrepThreads / 32], total_s[2 * kTeam];
+  __shared__ int teams_s[kTeam + 1], common_s[kTeam + 1], start_s[kPlanned];   // start_s: of the team jobs, as far as they fit
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, G = p.Hq / p.Hkv;
+  int4* jobs = jobs_of(L, scratch);
+  int4* pieces = pieces_of(L, scratch);
+  // exclusive sums over the block of n values a thread; the totals in total_s
+  auto scan = [&](int* v, int n) {
+    int up[2 * kTeam];
+#pragma unroll
+    for (int k = 0; k < 2 * kTeam; k++) {
+      if (k >= n) break;
+      up[k] = v[k];
+#pragma unroll
+      for (int off = 1; off < 32; off <<= 1) {
+        const int o = __shfl_up_sync(0xffffffffu, up[k], off);
+        if (lane >= off) up[k] += o;
+      }
+      if (lane == 31) sum_s[k][warp] = up[k];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < 2 * kTeam; k++) {
+      if (k >= n) break;
+      int before = up[k] - v[k], all = 0;
+#pragma unroll
+      for (int w = 0; w < kPrepThreads / 32; w++) {
+        if (w < warp) before += sum_s[k][w];
+        all += sum_s[k][w];
+      }
+      v[k] = before;
+      if (tid == 0) total_s[k] = all;
+    }
+    __syncthreads();
+  };
+  // where each sequence's tokens begin
+  const bool compact = p.B <= kCompact;
+  int tokens = p.B * p.T;
+  if (compact) {
+    constexpr int kEach = kCompact / kPrepThreads;
+    int n[kEach], at[1] = {0};
+    const int per = (p.B + kPrepThreads - 1) / kPrepThreads;
+#pragma unroll
+    for (int k = 0; k < kEach; k++) {
+      const int b = tid * per + k;
+      n[k] = k < per && b < p.B ? tree_of(p, b).n : 0;
+      at[0] += n[k];
+    }
+    scan(at, 1);
+    tokens = total_s[0];
+#pragma unroll
+    for (int k = 0; k < kEach; k++) {
+      const int b = tid * per + k;
+      if (k < per && b < p.B) p.first[b] = at[0];
+      at[0] += n[k];
+    }
+    if (tid == 0) p.first[p.B] = tokens;
+    __syncthreads();   // (total_s is used again)
+  }
+  // groups: the common keys of each KV head, then (sequence, KV head)
+  const int commons = L.n_p ? p.Hkv : 0, groups = commons + p.B * p.Hkv, per = (groups + kPrepThreads - 1) / kPrepThreads, g0 = min(groups, tid * per), g1 = min(groups, g0 + per);
+  const Teams common((int)(((long long)tokens * G + kRows - 1) / kRows));
+  const int common_tiles = tokens ? (L.P + kTile - 1) / kTile : 0;
+  auto group_of = [&](int g, Teams* teams, int* tiles, int* end) {
+    if (g < commons) {
+      *teams = common;
+      *tiles = common_tiles;
+      *end = L.P;
+      return;
+    }
+    const Tree r = tree_of(p, (g - commons) / p.Hkv);
+    *teams = Teams((r.n * G + kRows - 1) / kRows);
+    *end = max(L.P, r.base + r.n);
+    *tiles = r.n ? (*end - L.P + kTile - 1) / kTile : 0;
+  };
+  int v[2 * kTeam];   // of each width: team jobs, units
+#pragma unroll
+  for (int k = 0; k < 2 * kTeam; k++) v[k] = 0;
+  Teams teams(0);
+  int tiles, end;
+  for (int g = g0; g < g1; g++) {
+    group_of(g, &teams, &tiles, &end);
+    if (tiles == 0) continue;
+#pragma unroll
+    for (int k = 0; k < kTeam; k++) {
+      const int n = teams.of_width(k + 1);
+      v[k] += n;
+      v[kTeam + k] += n * (tiles + kOverhead);
+    }
+  }
+  scan(v, 2 * kTeam);
+  // shares: the smallest piece X for which the teams that it takes fit; one of 32 candidates between the mean and what surely fits
+  if (warp == 0) {
+    const int all_ctas = L.ctas;
+    float work = 0.0f;
+#pragma unroll
+    for (int k = 0; k < kTeam; k++) work += (float)(k + 1) * (float)total_s[kTeam + k];
+    const float lo = work / (float)all_ctas, hi = all_ctas > kTeam * (kTeam + 1) / 2 ? work / (float)(all_ctas - kTeam * (kTeam + 1) / 2) : 2.0f * work;
+    const float X = fmaxf(1.0f, lo + (hi - lo) * (float)(lane + 1) * (1.01f / 32.0f));
+    int take[kTeam], sum = 0;
+#pragma unroll
+    for (int k = 0; k < kTeam; k++) {
+      const int units = total_s[kTeam + k];
+      take[k] = units ? max(1, (int)ceilf((float)units / X)) : 0;
+      sum += (k + 1) * take[k];
+    }
+    const uint32_t fits = __ballot_sync(0xffffffffu, sum <= all_ctas);
+    const int best = fits ? __ffs(fits) - 1 : 31;
+#pragma unroll
+    for (int k = 0; k < kTeam; k++) {
+      take[k] = __shfl_sync(0xffffffffu, take[k], best);
+      if (!fits) take[k] = total_s[kTeam + k] ? 1 : 0;
+      if (lane == 0) teams_s[k + 1] = take[k];
+    }
+    if (lane <= kTeam) common_s[lane] = lane && common_tiles ? commons * common.of_width(lane) : 0;   // team jobs over common keys, at a line's front
+  }
+  __syncthreads();
+  // records of team jobs, of their row tiles and of the CTAs whose pieces begin in them
+  int list0[kTeam], slot_p[kTeam], slot_s[kTeam], cta0[kTeam];
+  {
+    int a = 0, b = 0, c = 0, d = 0;
+#pragma unroll
+    for (int k = 0; k < kTeam; k++) {
+      list0[k] = a;
+      slot_p[k] = b;
+      slot_s[k] = c;
+      cta0[k] = d;
+      a += total_s[k];
+      b += (common_s[k + 1] + teams_s[k + 1]) * (k + 1);
+      c += (total_s[k] - common_s[k + 1] + teams_s[k + 1]) * (k + 1);
+      d += teams_s[k + 1] * (k + 1);
+    }
+  }
+  for (int g = g0; g < g1; g++) {
+    group_of(g, &teams, &tiles, &end);
+    const bool is_common = g < commons;
+    const int j0 = is_common ? g * L.mt_p : L.n_p + (g - commons) * L.mt_s, row_tiles = is_common ? L.mt_p : L.mt_s;
+    int mt = 0;
+    for (int i = 0; tiles && i < teams.all; i++) {
+      const int w = i < teams.wide ? teams.w + 1 : teams.w;
+#pragma unroll
+      for (int k = 0; k < kTeam; k++)   // (registers, not indexes)
+        if (w == k + 1) {
+          const int at = v[k]++, start = v[kTeam + k], len = tiles + kOverhead, units = total_s[kTeam + k], K = teams_s[k + 1];
+          v[kTeam + k] += len;
+          const int slot = is_common ? slot_p[k] + at * w : slot_s[k] + (at - common_s[k + 1]) * w;
+          p.team[list0[k] + at] = make_int4(start, j0 + mt, end, slot);
+          // team t has units [units t / K, units (t + 1) / K): unit u is team ((u + 1) K - 1) / units's
+          auto team_at = [&](int u) { return share_of(K, u + 1, units, 1); };
+          const int t0 = team_at(start + kOverhead), t1 = team_at(start + len - 1);
+          for (int r = 0; r < w; r++) jobs[j0 + mt + r] = make_int4(0, 0, slot + t0 * w + r, (t1 - t0 + 1) | w << 16);
+          if (list0[k] + at < kPlanned) start_s[list0[k] + at] = start;
+        }
+      mt += w;
+    }
+    for (; mt < row_tiles; mt++) jobs[j0 + mt] = make_int4(0, 0, 0, 0);
+  }
+  __syncthreads();
+  for (int cta = tid; cta < L.ctas; cta += kPrepThreads) {
+    int4 piece = make_int4(0, 0, 0, 0), more = make_int4(0, 0, 0, 0);   // (without work)
+#pragma unroll
+    for (int k = 0; k < kTeam; k++) {
+      const int K = teams_s[k + 1], c = cta - cta0[k], t = c / (k + 1);
+      if (c < 0 || t >= K) continue;
+      const int u0 = share_of(total_s[kTeam + k], t, K), u1 = share_of(total_s[kTeam + k], t + 1, K);
+      int lo = list0[k], hi = list0[k] + total_s[k];   // the last that starts at u0 or before
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1, start = mid < kPlanned ? start_s[mid] : p.team[mid].x;
+        if (start <= u0) lo = mid;
+        else hi = mid;
+      }
+      piece = make_int4(u0, u1, lo, list0[k] + total_s[k]);
+      more = make_int4(c, c - t * (k + 1), 0, 0);
+    }
+    pieces[2 * cta] = piece;
+    pieces[2 * cta + 1] = more;
+  }
+}
+
 // row i of a job's tile -> token row e and query head of its group; false past the last
 BK_DEVINL bool row_at(const PagedParams& p, const Job& q, int i, int* b, int* t, int* g) {
   const int G = p.Hq / p.Hkv, r = q.mt * kRows + i;
@@ -338,25 +541,111 @@ BK_DEVINL bool row_at(const PagedParams& p, const Job& q, int i, int* b, int* t,
   return r < p.B * p.T * G;
 }
 
+template <int PER>
+BK_DEVINL void store_bf16(uint16_t* dst, const float (&x)[PER]) {
+#pragma unroll
+  for (int i = 0; i < PER; i += 4) *reinterpret_cast<uint2*>(dst + i) = make_uint2(bk_f32x2_to_bf16x2(x[i], x[i + 1]), bk_f32x2_to_bf16x2(x[i + 2], x[i + 3]));
+}
 // One warp per (token row, head): y = x / sqrt(mean(x^2) + eps) (1 + w), then the rotation of pairs (d, d + rot_half), in f32; q heads to the scratch
 // buffer, k and v heads into their page, rounded to bf16: operands of the tensor cores (q's rounding is what the result's error is made of, 0.0024 of
 // its norm against 0.0017 for exact arithmetic rounded once).  The first CTA lays out the work of the next launch.  Bound: latency, 5 us for 32
 // sequences and 7 for 64 of 24 heads, most of it that CTA's.
 template <int HD, bool TREE>
-__global__ void __launch_bounds__(kPrepThreads) paged_prepare_kernel(const Params<TREE> p, const Layout L, uint8_t* scratch) {
+__global__ void __launch_bounds__(kPrepThreads, TREE ? 3 : 0) paged_prepare_kernel(const Params<TREE> p, const Layout L, uint8_t* scratch) {
   constexpr int PER = HD / 32;
   __shared__ float y_s[kPrepThreads / 32][HD];
   // The wait comes first: a launch behind this call may read, before its own wait, what a launch before this call wrote (weights, settled caches).
   bk_pdl_wait();
   bk_pdl_trigger();
   if (blockIdx.x == 0) {   // (first: it takes longest)
-    if (L.n_p + L.n_s <= kPlanned) plan_jobs<true, TREE>(p, L, scratch);
-    else plan_jobs<false, TREE>(p, L, scratch);
+    if constexpr (TREE) plan_trees(p, L, scratch);
+    else if (L.n_p + L.n_s <= kPlanned) plan_jobs<true>(p, L, scratch);
+    else plan_jobs<false>(p, L, scratch);
     return;
   }
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int heads = p.Hq + (p.k ? p.Hkv : 0);
   const int item = (blockIdx.x - 1) * (kPrepThreads / 32) + warp;
+  if constexpr (TREE) {   // p.each heads of a token
+    const int turns = (heads + p.each - 1) / p.each;
+    if (item >= p.T * p.B * turns) return;
+    const int e = item / turns, h0 = (item - e * turns) * p.each, h1 = min(heads, h0 + p.each), t = e / p.B, b = e - t * p.B, G = p.Hq / p.Hkv;
+    float x[PER];
+    auto load = [&](int h) {
+      load_bf16((h < p.Hq ? p.qg + ((size_t)e * p.Hq + h) * (p.fused ? 2 : 1) * HD : p.k + ((size_t)e * p.Hkv + h - p.Hq) * HD) + lane * PER, x);
+    };
+    load(h0);   // (does not wait for what follows)
+    const Tree tree = tree_of(p, b);
+    const int at = p.fused ? p.pos[e] : 0;
+    const bool here = t < tree.n && at >= 0 && (!p.fused || at < p.max_pos);
+    int place = b * p.T + t;   // of the token among the ready queries
+    if (h0 < p.Hq && p.B <= kCompact) {
+      place = 0;
+      for (int i = lane; i < b; i += 32) place += tree_of(p, i).n;
+      place = __reduce_add_sync(0xffffffffu, place) + t;
+    }
+    if (h0 == 0) {
+      bool sees = here && tree.base > 0;
+      if (here && tree.base == 0)
+        for (int i = lane; i < (tree.n + 31) / 32; i += 32) sees = sees || node_word(p.mask + (size_t)e * p.words, tree.n, i);
+      sees = __any_sync(0xffffffffu, sees);
+      if (lane == 0) {
+        p.place[e] = sees ? place : -1;
+        if (t < tree.n && p.B <= kCompact) p.token[place] = e;
+      }
+    }
+    if (!here) return;
+    const int slot = h1 > p.Hq ? p.slot[e] : -1, page = slot >= 0 ? slot / p.page_rows : -1, row_in = slot - page * p.page_rows;
+    // what all heads of the token share: norm weights, and of each dim the cosine, the signed sine and the place of the other one of its pair
+    float w[PER], c[PER], sn[PER];
+    int other[PER];
+    auto weights = [&](const uint16_t* from) { load_bf16(from + lane * PER, w); };
+    if (p.fused) {
+      const float *cr = p.cos_t + (size_t)at * p.rot_half, *sr = p.sin_t + (size_t)at * p.rot_half;
+#pragma unroll
+      for (int i = 0; i < PER; i++) {
+        const int d = lane * PER + i, half = p.rot_half;
+        other[i] = d < half ? d + half : d < 2 * half ? d - half : -1;
+        c[i] = other[i] >= 0 ? cr[min(d, other[i])] : 1.0f;
+        sn[i] = other[i] < 0 ? 0.0f : d < half ? -sr[d] : sr[d - half];
+      }
+      weights(h0 < p.Hq ? p.q_norm_w : p.k_norm_w);
+    }
+    for (int h = h0; h < h1; h++) {
+      float y[PER];
+#pragma unroll
+      for (int i = 0; i < PER; i++) y[i] = x[i];
+      if (h + 1 < h1) load(h + 1);
+      uint16_t* dst;
+      if (h < p.Hq) {
+        const int head = h / G;
+        dst = p.q + ((size_t)head * p.B * p.T + place) * G * HD + (size_t)(h - head * G) * HD;
+      } else {
+        if (page < 0 || page >= p.n_pages) break;
+        const size_t row = (((size_t)page * p.Hkv + h - p.Hq) * p.page_rows + row_in) * HD;
+        dst = p.k_pages + row;
+#pragma unroll
+        for (int i = 0; i < PER; i += 4)
+          *reinterpret_cast<uint2*>(p.v_pages + row + lane * PER + i) = *reinterpret_cast<const uint2*>(p.v + ((size_t)e * p.Hkv + h - p.Hq) * HD + lane * PER + i);
+        if (p.fused && h == p.Hq) weights(p.k_norm_w);
+      }
+      if (p.fused) {
+        float sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < PER; i++) sum = fmaf(y[i], y[i], sum);
+        const float rstd = bk_rcp_sqrt(__fadd_rn(__fdiv_rn(bk_warp_sum(sum), (float)HD), p.eps));
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < PER; i++) y_s[warp][lane * PER + i] = y[i] = __fmul_rn(__fmul_rn(y[i], rstd), __fadd_rn(1.0f, w[i]));
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < PER; i++)
+          if (other[i] >= 0) y[i] = __fadd_rn(__fmul_rn(y[i], c[i]), __fmul_rn(y_s[warp][other[i]], sn[i]));
+      }
+      store_bf16(dst + lane * PER, y);
+    }
+    return;
+  } else {
   if (item >= p.T * p.B * heads) return;
   const int e = item / heads, h = item - e * heads, t = e / p.B, b = e - t * p.B;
   const bool is_q = h < p.Hq;
@@ -371,29 +660,16 @@ __global__ void __launch_bounds__(kPrepThreads) paged_prepare_kernel(const Param
 #pragma unroll
     for (int i = 0; i < PER / 4; i++) v[i] = *reinterpret_cast<const uint2*>(p.v + ((size_t)e * p.Hkv + kvh) * HD + lane * PER + 4 * i);
   }
-  int at = row_of(p, b, t);
+  const int at = row_of(p, b, t);
   if (at < 0) return;
-  int page, row_in;
-  if constexpr (TREE) {
-    const int slot = is_q ? 0 : p.slot[e];
-    page = slot >= 0 ? slot / p.page_rows : -1;
-    row_in = slot - page * p.page_rows;
-    if (p.fused) {
-      at = p.pos[e];
-      if (at < 0 || at >= p.max_pos) return;
-    }
-  }
   uint16_t* dst;
   if (is_q) {
     const int head = h / G;
     dst = p.q + (((size_t)head * p.B + b) * p.T + t) * G * HD + (size_t)(h - head * G) * HD;
   } else {
-    if constexpr (!TREE) {
-      page = p.table[(size_t)b * p.max_pages + at / p.page_rows];
-      row_in = at % p.page_rows;
-    }
+    const int page = p.table[(size_t)b * p.max_pages + at / p.page_rows];
     if (page < 0 || page >= p.n_pages) return;
-    const size_t row = (((size_t)page * p.Hkv + kvh) * p.page_rows + row_in) * HD;
+    const size_t row = (((size_t)page * p.Hkv + kvh) * p.page_rows + at % p.page_rows) * HD;
     dst = p.k_pages + row;
 #pragma unroll
     for (int i = 0; i < PER / 4; i++) *reinterpret_cast<uint2*>(p.v_pages + row + lane * PER + 4 * i) = v[i];
@@ -416,8 +692,8 @@ __global__ void __launch_bounds__(kPrepThreads) paged_prepare_kernel(const Param
       else x[i] = y;
     }
   }
-#pragma unroll
-  for (int i = 0; i < PER; i += 4) *reinterpret_cast<uint2*>(dst + lane * PER + i) = make_uint2(bk_f32x2_to_bf16x2(x[i], x[i + 1]), bk_f32x2_to_bf16x2(x[i + 2], x[i + 3]));
+  store_bf16(dst + lane * PER, x);
+  }
 }
 
 // ---- tensor memory and its instructions ------------------------------------------------
@@ -643,6 +919,19 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
   };
   bool began = false;
   auto next_piece = [&](Piece* x) {
+    if constexpr (TREE) {
+      while (++j < line.w) {
+        const int4 team = __ldcg(p.team + j);
+        if (team.x >= u1) return false;
+        x->q = job_of(p, L, team.y + first.y);
+        piece_of(team.x, (team.z - x->q.key0 + kTile - 1) / kTile, u0, u1, &x->t0, &x->t1);
+        if (x->t0 >= x->t1) continue;
+        x->key1 = team.z;
+        x->slot = team.w + first.x;
+        return true;
+      }
+      return false;
+    }
     if (!began) {
       began = true;
       if (line.w >= 0) {
@@ -806,7 +1095,11 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
       while (next_piece(&x)) {
         const bool common = x.q.seq < 0;
         const CUtensorMap* map = P.q_map + common;
-        const int rows = P.q_rows[common], row = common ? x.q.kvh * p.B * p.T * (p.Hq / p.Hkv) : (x.q.kvh * p.B + x.q.seq) * p.T * (p.Hq / p.Hkv);
+        const int rows = P.q_rows[common];
+        int row = common ? x.q.kvh * p.B * p.T * (p.Hq / p.Hkv) : (x.q.kvh * p.B + x.q.seq) * p.T * (p.Hq / p.Hkv);
+        if constexpr (TREE) {
+          if (!common && p.B <= kCompact) row = (x.q.kvh * p.B * p.T + __ldcg(p.first + x.q.seq)) * (p.Hq / p.Hkv);
+        }
         if (!bar_wait_warp(smem_u32(&q_empty), parity, P.status, dead)) break;
         armed++;
         if (lane == 0) mbar_expect_tx(smem_u32(&q_here), rows * HD * 2);
@@ -832,14 +1125,26 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
         const Job q = x.q;
         const int t0 = x.t0, n = x.t1 - t0, key1 = x.key1;
         int b, t, g, limit = 0x7fffffff;   // (lanes without a row: never masked, never read)
-        const bool mine = row_at(p, q, i_row, &b, &t, &g);
+        bool mine = row_at(p, q, i_row, &b, &t, &g);
+        if constexpr (TREE) {
+          if (q.seq < 0 && p.B <= kCompact) {
+            const int at = b * p.T + t;   // (row_at took the rows for T of each sequence)
+            mine = mine && at < __ldcg(p.first + p.B);
+            const int e = mine ? __ldcg(p.token + at) : 0;
+            t = e / p.B;
+            b = e - t * p.B;
+          }
+        }
         Tree tree = {0, 0};
-        const uint32_t* bits = nullptr;   // of a row of a tree that is there
+        const uint32_t* bits = nullptr;   // of a row of a tree
         if constexpr (TREE) {
           if (mine) {
             tree = tree_of(p, b);
-            if (t < tree.n) bits = p.mask + ((size_t)t * p.B + b) * p.words;
-            limit = bits ? min(tree.base, key1) : 0;
+            mine = t < tree.n;
+          }
+          if (mine) {
+            bits = p.mask + ((size_t)t * p.B + b) * p.words;
+            limit = min(tree.base, key1);
           }
         } else if (mine) {
           limit = min(row_of(p, b, t) + 1, key1);
@@ -860,7 +1165,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
           int uneven;
           asm volatile("{ .reg .pred a, b; setp.ne.s32 a, %1, 0; barrier.cta.red.or.pred b, 5, 256, a; selp.s32 %0, 1, 0, b; }"
                        : "=r"(uneven)
-                       : "r"((int)(mine && (TREE ? bits != nullptr : limit > 0) && limit < key1))
+                       : "r"((int)(mine && (TREE || limit > 0) && limit < key1))
                        : "memory");
           if (uneven) seen_by_all = 0;
         }
@@ -900,7 +1205,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
           uint32_t seen = 0xffffffffu;   // of a tree's row, these keys
           if constexpr (TREE) {
             if (mine && key + 32 > limit) {   // (ahead of the wait: its loads are on the way meanwhile)
-              seen = bits ? seen_keys(bits, tree, key) : 0u;
+              seen = seen_keys(bits, tree, key);
               if (key + 32 > key1) seen &= key >= key1 ? 0u : (1u << (key1 - key)) - 1u;
             }
           }
@@ -1016,7 +1321,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
 #pragma unroll
             for (int y = 0; y < 16; y++) probe[y & 3] = bk_fma2(make_float2(__uint_as_float(o[2 * y]), __uint_as_float(o[2 * y + 1])), zero, probe[y & 3]);
             const float2 all = bk_add2(bk_add2(probe[0], probe[1]), bk_add2(probe[2], probe[3]));
-            const bool anew = __any_sync(0xffffffffu, mine && (TREE ? bits != nullptr : limit > 0) && __fadd_rn(all.x, all.y) != 0.0f);
+            const bool anew = __any_sync(0xffffffffu, mine && (TREE || limit > 0) && __fadd_rn(all.x, all.y) != 0.0f);
             if (anew) {
               k0 = q.key0 + t0 * kTile;
               k1 = min(key1, k0 + n * kTile);
@@ -1073,8 +1378,8 @@ BK_DEVINL float weight_of(float x) {
 // Bound: latency, of a chain of loads: the lists of pieces, their sums and results; 2.6 us of a call for one sequence, 5.5 for 32, 6.4 for 64.
 // Few CTAs have many pieces to a row, which four slices take together; many CTAs hide one another's latency better when they are small (two
 // slices for 64 sequences of 24 heads: 1.5 us more).
-template <int HD, int kSlices, bool TREE>
-__global__ void __launch_bounds__(256 * kSlices) paged_merge_kernel(const Params<TREE> p, const Layout L, uint8_t* scratch) {
+template <int HD, int kSlices>
+__global__ void __launch_bounds__(256 * kSlices) paged_merge_kernel(const Params<false> p, const Layout L, uint8_t* scratch) {
   __shared__ __align__(16) float4 o_s[kSlices > 1 ? kSlices - 1 : 1][16 * 16];
   __shared__ float2 ml_s[kSlices][16];
   bk_pdl_trigger();
@@ -1086,16 +1391,7 @@ __global__ void __launch_bounds__(256 * kSlices) paged_merge_kernel(const Params
   const int4* jobs = jobs_of(L, scratch);
   const int2 qs = __ldcg(reinterpret_cast<const int2*>(&jobs[L.n_p + js].z));   // first slot; number and distance
   const int2 qp = L.n_p ? __ldcg(reinterpret_cast<const int2*>(&jobs[jp].z)) : make_int2(0, 0);
-  bool here = row_of(p, b, t) >= 0;
-  if constexpr (TREE) {   // a node that sees nothing gets zeros
-    const Tree tree = tree_of(p, b);
-    if (here && p.fused) here = p.pos[e] >= 0 && p.pos[e] < p.max_pos;
-    if (here && tree.base == 0) {
-      uint32_t any = 0;
-      for (int i = 0; i < p.words; i++) any |= node_word(p.mask + (size_t)e * p.words, tree.n, i);
-      here = any != 0;
-    }
-  }
+  const bool here = row_of(p, b, t) >= 0;
   uint2 gv = make_uint2(0, 0);
   if (gate && slice == 0) gv = __ldcg(reinterpret_cast<const uint2*>(gate + (d0 + d) * 4));
   const int np = here ? qp.y & 0xffff : 0, n = here ? np + (qs.y & 0xffff) : 0;
@@ -1164,6 +1460,130 @@ __global__ void __launch_bounds__(256 * kSlices) paged_merge_kernel(const Params
   *reinterpret_cast<uint2*>(p.out + ((size_t)e * p.Hq + kvh * G + g) * HD + (d0 + d) * 4) = make_uint2(bk_f32x2_to_bf16x2(y[0], y[1]), bk_f32x2_to_bf16x2(y[2], y[3]));
 }
 
+
+// The same for trees.  A thread has kQuads times 4 dims of one head, 64 apart; a CTA 64 kQuads dims of the group's heads, from kSlices slices of pieces.  Many rows have few
+// pieces each: one slice and all dims, so that the chain of loads (place, lists of pieces, sums and results) is there once a row and KV head.  Few rows may have a piece of
+// every CTA: as many slices as threads fill the GPU with.  (2,048 tokens, half of them there, 24 heads on 4: 76 us with 64 dims a CTA, so ???; one token, 16 heads on 2, 8,192
+// rows: 17.5 us with four slices, so ???.)
+template <int HD, int kSlices, int kQuads>
+__global__ void __launch_bounds__(256 * (kSlices > 4 ? 4 : kSlices)) tree_merge_kernel(const Params<true> p, const Layout L, uint8_t* scratch) {
+  constexpr int U = kQuads == 1 ? 4 : 2, kParts = HD / (64 * kQuads);   // U: pieces requested together
+  extern __shared__ __align__(16) uint8_t merge_smem[];
+  bk_pdl_trigger();
+  const int G = p.Hq / p.Hkv, e = blockIdx.x, kvh = blockIdx.y / kParts, d0 = blockIdx.y % kParts * 16 * kQuads, t = e / p.B, b = e - t * p.B;
+  const int g = threadIdx.x % G, d = threadIdx.x / G % 16, slice = threadIdx.x / (G * 16);
+  float4* const o_s = reinterpret_cast<float4*>(merge_smem);                                  // [kSlices - 1][kQuads][16][G]
+  float2* const ml_s = reinterpret_cast<float2*>(o_s + (kSlices - 1) * kQuads * 16 * G);      // [kSlices][G]
+  uint16_t* const out = p.out + ((size_t)e * p.Hq + kvh * G + g) * HD;
+  const uint16_t* gate = p.fused ? p.qg + ((size_t)e * p.Hq + kvh * G + g) * 2 * HD + HD : p.gate ? p.gate + ((size_t)e * p.Hq + kvh * G + g) * HD : nullptr;
+  uint2 gv[kQuads];
+#pragma unroll
+  for (int k = 0; k < kQuads; k++)
+    if (gate && slice == 0) gv[k] = __ldcg(reinterpret_cast<const uint2*>(gate + (d0 + 16 * k + d) * 4));
+  const int place = __ldcg(p.place + e);
+  if (place < 0) {
+    bk_pdl_wait();   // (nothing of an earlier call may still read or write what is overwritten)
+    if (slice == 0)
+#pragma unroll
+      for (int k = 0; k < kQuads; k++) *reinterpret_cast<uint2*>(out + (d0 + 16 * k + d) * 4) = make_uint2(0, 0);
+    return;
+  }
+  const int rp = place * G + g, rs = t * G + g;
+  const int4* jobs = jobs_of(L, scratch);
+  const int2 qs = __ldcg(reinterpret_cast<const int2*>(&jobs[L.n_p + (b * p.Hkv + kvh) * L.mt_s + rs / kRows].z));   // first slot; number and distance
+  const int2 qp = L.n_p ? __ldcg(reinterpret_cast<const int2*>(&jobs[kvh * L.mt_p + rp / kRows].z)) : make_int2(0, 0);
+  const int np = qp.y & 0xffff, n = np + (qs.y & 0xffff);
+  bk_pdl_wait();   // (what is above was there when the launch before this one began its work)
+  float m = -INFINITY, l = 0.0f;
+  float4 o[kQuads];
+#pragma unroll
+  for (int k = 0; k < kQuads; k++) o[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  for (int i0 = slice; i0 < n; i0 += kSlices * U) {
+    float4 v[U][kQuads], x[U];
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      const int i = i0 + u * kSlices;
+      x[u] = make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
+      if (i < n) {
+        const bool common = i < np;
+        const size_t slot = common ? qp.x + i * (qp.y >> 16) : qs.x + (i - np) * (qs.y >> 16);
+        const int rows = common ? kRows : L.rows_s, row = (common ? rp : rs) % kRows;
+        x[u] = __ldcg(reinterpret_cast<const float4*>(scratch + (common ? L.ml_p : L.ml_s)) + slot * rows + row);
+#pragma unroll
+        for (int k = 0; k < kQuads; k++)
+          v[u][k] = __ldcg(reinterpret_cast<const float4*>(scratch + (common ? L.o_p : L.o_s)) + (slot * (HD / 4) + d0 + 16 * k + d) * rows + row);
+      }
+    }
+    float mn = m;
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      // (a piece with a sum and no maximum has NaN scores only, see paged_merge_kernel)
+      if (x[u].x == -INFINITY && __fadd_rn(x[u].y, x[u].z) != 0.0f) x[u].x = 0.0f;
+      mn = fmaxf(mn, x[u].x);
+    }
+    if (mn == -INFINITY) continue;
+    const float f = weight_of(__fsub_rn(m, mn));   // (m = -inf: of zeros)
+    l = __fmul_rn(l, f);
+#pragma unroll
+    for (int k = 0; k < kQuads; k++) o[k] = make_float4(__fmul_rn(o[k].x, f), __fmul_rn(o[k].y, f), __fmul_rn(o[k].z, f), __fmul_rn(o[k].w, f));
+    m = mn;
+#pragma unroll
+    for (int u = 0; u < U; u++)
+      if (x[u].x != -INFINITY) {
+        const float w = weight_of(__fsub_rn(x[u].x, m));
+        l = fmaf(w, __fadd_rn(x[u].y, x[u].z), l);
+#pragma unroll
+        for (int k = 0; k < kQuads; k++) {
+          o[k].x = fmaf(w, v[u][k].x, o[k].x); o[k].y = fmaf(w, v[u][k].y, o[k].y); o[k].z = fmaf(w, v[u][k].z, o[k].z); o[k].w = fmaf(w, v[u][k].w, o[k].w);
+        }
+      }
+  }
+  if (kSlices > 1) {
+    if (slice)
+#pragma unroll
+      for (int k = 0; k < kQuads; k++) o_s[(((slice - 1) * kQuads + k) * 16 + d) * G + g] = o[k];
+    if (d == 0) ml_s[slice * G + g] = make_float2(m, l);
+    __syncthreads();
+    if (slice) return;
+    float M = -INFINITY;
+#pragma unroll
+    for (int s = 0; s < kSlices; s++) M = fmaxf(M, ml_s[s * G + g].x);
+    const float w0 = weight_of(__fsub_rn(m, M));
+    l = __fmul_rn(w0, l);
+#pragma unroll
+    for (int k = 0; k < kQuads; k++) o[k] = make_float4(__fmul_rn(w0, o[k].x), __fmul_rn(w0, o[k].y), __fmul_rn(w0, o[k].z), __fmul_rn(w0, o[k].w));
+#pragma unroll
+    for (int s = 1; s < kSlices; s++) {
+      const float2 x = ml_s[s * G + g];
+      const float w = weight_of(__fsub_rn(x.x, M));
+      l = fmaf(w, x.y, l);
+#pragma unroll
+      for (int k = 0; k < kQuads; k++) {
+        const float4 v = o_s[(((s - 1) * kQuads + k) * 16 + d) * G + g];
+        o[k].x = fmaf(w, v.x, o[k].x); o[k].y = fmaf(w, v.y, o[k].y); o[k].z = fmaf(w, v.z, o[k].z); o[k].w = fmaf(w, v.w, o[k].w);
+      }
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < kQuads; k++) {
+    const int at = (d0 + 16 * k + d) * 4;
+    float y[4] = {__fdiv_rn(o[k].x, l), __fdiv_rn(o[k].y, l), __fdiv_rn(o[k].z, l), __fdiv_rn(o[k].w, l)};
+    if (gate) {
+      const uint32_t gw[2] = {gv[k].x, gv[k].y};
+#pragma unroll
+      for (int i = 0; i < 4; i++) y[i] = __fmul_rn(y[i], bk_sigmoidf(__uint_as_float(i & 1 ? gw[i >> 1] & 0xffff0000u : gw[i >> 1] << 16)));
+    }
+    *reinterpret_cast<uint2*>(out + at) = make_uint2(bk_f32x2_to_bf16x2(y[0], y[1]), bk_f32x2_to_bf16x2(y[2], y[3]));
+  }
+}
+
+template <int HD, int kSlices, int kQuads>
+cudaError_t launch_tree_merge(const Params<true>& p, const Layout& L, uint8_t* scratch) {
+  const int G = p.Hq / p.Hkv;
+  const size_t smem = kSlices > 1 ? (size_t)(kSlices - 1) * kQuads * 16 * G * 16 + (size_t)kSlices * G * 8 : 0;   // at most 25 KB
+  return bk_launch_pdl(tree_merge_kernel<HD, kSlices, kQuads>, dim3(p.T * p.B, p.Hkv * (HD / (64 * kQuads))), dim3(G * 16 * kSlices), smem, p, L, scratch);
+}
+
 template <int HD, bool TREE>
 int32_t launch_paged(const Params<TREE>& p, const Layout& L, uint64_t scratch) {
   TileParams<TREE> P;
@@ -1182,7 +1602,8 @@ int32_t launch_paged(const Params<TREE>& p, const Layout& L, uint64_t scratch) {
     if (!bk_encode_map_2d(&P.q_map[common], CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, scratch + L.q, HD, q_rows, HD * 2, 64, P.q_rows[common], CU_TENSOR_MAP_SWIZZLE_128B))
       return bk_fail(BK_ERR_UNSUPPORTED, "bkPagedAttn: the driver refuses a tensor map of %llu rows of %d queries", (unsigned long long)q_rows, HD);
   }
-  const int heads = p.Hq + (p.k ? p.Hkv : 0);
+  int heads = p.Hq + (p.k ? p.Hkv : 0);
+  if constexpr (TREE) heads = (heads + p.each - 1) / p.each;
   BK_CUDA(bk_launch_pdl(paged_prepare_kernel<HD, TREE>, dim3((p.T * p.B * heads + kPrepThreads / 32 - 1) / (kPrepThreads / 32) + 1), dim3(kPrepThreads), 0, p, L, P.scratch));
   BK_CHECK_LAUNCH();
   static bool configured = false;
@@ -1193,11 +1614,25 @@ int32_t launch_paged(const Params<TREE>& p, const Layout& L, uint64_t scratch) {
   BK_CUDA(bk_launch_pdl(paged_tile_kernel<HD, TREE>, dim3(L.ctas), dim3(kTileThreads), TileCfg<HD>::kSmem, P));
   BK_CHECK_LAUNCH();
   const dim3 merge(p.T * p.B, p.Hkv * (HD / 64));
-  if ((long long)merge.x * merge.y <= 2 * bk_ctx().sm_count) BK_CUDA(bk_launch_pdl(paged_merge_kernel<HD, 4, TREE>, merge, dim3(p.Hq / p.Hkv * 64), 0, p, L, P.scratch));
-  else BK_CUDA(bk_launch_pdl(paged_merge_kernel<HD, 1, TREE>, merge, dim3(p.Hq / p.Hkv * 16), 0, p, L, P.scratch));
+  if constexpr (TREE) {
+    // by rows: eight slices of pieces (16 rows: 22 us a call, with four 34), four (1,024 rows: 25 and 32 us, with eight 30 and 42, with two 28 and 36), two (4,096 rows: 49 us, with
+    // four 53, with one 51), one (24,576 rows: 72 us, with two 80)
+    const long long rows = (long long)p.T * p.B * p.Hq, sms = bk_ctx().sm_count;
+    if (rows <= 2 * sms && p.Hq / p.Hkv <= 8) BK_CUDA((launch_tree_merge<HD, 8, 1>(p, L, P.scratch)));
+    else if (rows <= 10 * sms) BK_CUDA((launch_tree_merge<HD, 4, HD / 128>(p, L, P.scratch)));
+    else if (rows <= 40 * sms) BK_CUDA((launch_tree_merge<HD, 2, HD / 128>(p, L, P.scratch)));
+    else BK_CUDA((launch_tree_merge<HD, 1, HD / 128>(p, L, P.scratch)));
+  } else if ((long long)merge.x * merge.y <= 2 * bk_ctx().sm_count) {
+    BK_CUDA(bk_launch_pdl(paged_merge_kernel<HD, 4>, merge, dim3(p.Hq / p.Hkv * 64), 0, p, L, P.scratch));
+  } else {
+    BK_CUDA(bk_launch_pdl(paged_merge_kernel<HD, 1>, merge, dim3(p.Hq / p.Hkv * 16), 0, p, L, P.scratch));
+  }
   BK_CHECK_LAUNCH();
   return BK_OK;
 }
+
+// what the layout takes with what trees have behind it
+size_t tree_bytes(const Layout& L, int B, int T) { return L.bytes + (size_t)(L.n_p + L.n_s) * 16 + ((size_t)B + 1 + 2 * (size_t)B * T) * 4; }
 
 // the checks of a call, its parameters and layout
 template <typename P>
@@ -1257,7 +1692,8 @@ int32_t bkPagedAttn(const bkPagedAttnArgs* args) {
 }
 
 uint64_t bkTreeAttnScratchBytes(int32_t B, int32_t T, int32_t Hq, int32_t Hkv, int32_t HD, int32_t prefix_rows) {
-  return bkPagedAttnScratchBytes(B, T, Hq, Hkv, HD, prefix_rows);
+  if (bkPagedAttnScratchBytes(B, T, Hq, Hkv, HD, prefix_rows) == 0) return 0;
+  return tree_bytes(make_layout(B, T, Hq, Hkv, HD, prefix_rows, 1, bk_ctx().sm_count), B, T);
 }
 
 int32_t bkTreeAttn(const bkTreeAttnArgs* args) {
@@ -1272,6 +1708,15 @@ int32_t bkTreeAttn(const bkTreeAttnArgs* args) {
          a.mask_words);
   BK_ARG((a.pos & 3) == 0 && (a.pos || !a.attn.fused_norm_rope), "bkTreeAttn: fused mode needs pos, an int32 array");
   BK_ARG((a.slot & 3) == 0 && (a.slot || !a.attn.k), "bkTreeAttn: k and v need slot, an int32 array");
+  const uint64_t need = bkTreeAttnScratchBytes(a.attn.B, a.attn.T, a.attn.Hq, a.attn.Hkv, a.attn.HD, a.attn.prefix_rows);
+  BK_ARG(a.attn.scratch_bytes >= need, "bkTreeAttn: scratch of %llu bytes, %llu needed", (unsigned long long)a.attn.scratch_bytes, (unsigned long long)need);
+  // heads a warp: one while all warps are on the GPU at once (32 an SM)
+  const long long items = (long long)a.attn.B * a.attn.T * (a.attn.Hq + (a.attn.k ? a.attn.Hkv : 0));
+  p.each = (int)std::max<long long>(1, std::min<long long>(8, items / (32 * bk_ctx().sm_count)));
+  p.team = bk_ptr<int4>(a.attn.scratch + L.bytes);
+  p.first = reinterpret_cast<int*>(p.team + L.n_p + L.n_s);
+  p.token = p.first + a.attn.B + 1;
+  p.place = p.token + (size_t)a.attn.B * a.attn.T;
   p.pos = bk_ptr<int>(a.pos); p.slot = bk_ptr<int>(a.slot); p.mask = bk_ptr<uint32_t>(a.mask); p.words = a.mask_words; p.max_pos = a.attn.max_len;
   return a.attn.HD == 256 ? launch_paged<256, true>(p, L, a.attn.scratch) : launch_paged<128, true>(p, L, a.attn.scratch);
 }
