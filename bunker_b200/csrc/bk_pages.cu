@@ -328,8 +328,8 @@ __global__ void __launch_bounds__(kCopyThreads) pages_copy_kernel(const Pool fro
 // ---- drafted trees ---------------------------------------------------------------------
 
 struct BatchParams {
-  const int *seqs, *n_new, *parent;
-  int *table, *lens, *pos, *slot;
+  const int *seqs, *n_new, *parent, *ok;
+  int *table, *lens, *pos, *slot, *count;
   uint32_t* mask;
   int n, T, words;
 };
@@ -351,10 +351,12 @@ __global__ void __launch_bounds__(kCopyThreads) pages_batch_kernel(const Pool p,
   }
   if (blockIdx.y) return;
   if (a.lens && threadIdx.x == 0) a.lens[i] = len;
-  if (!a.pos && !a.slot && !a.mask) return;
   int n = a.n_new ? max(0, min(a.n_new[i], a.T)) : a.T;
+  if (a.ok && a.ok[i] == 0) n = 0;
   const int base = len - n;
   if (base < 0) n = 0;
+  if (a.count && threadIdx.x == 0) a.count[i] = n;
+  if (!a.pos && !a.slot && !a.mask) return;
   if (a.parent) {
     for (int t = threadIdx.x; t < n; t += kCopyThreads) parent_s[t] = a.parent[(size_t)t * a.n + i];
     __syncthreads();
@@ -411,56 +413,63 @@ struct CommitParams {
 // A cluster of CTAs per sequence.  Each finds the path for itself: every node that the model agrees with tells its parent, the lowest child stays, and one thread follows
 // the children.  Then the CTAs' warps move rows: a warp has 512 bytes of a row of one head and plane, of all rows that move, which it takes in order (row i of the
 // tree is written after it was read, since a path's node i has a number of at least i).  What the others still read (table, counts, lengths) is changed by the
-// first CTA behind the cluster's barrier; other sequences read none of it, for pages of a tree belong to one sequence alone.  Bound: latency of that chain for small
-// batches.
+// first CTA behind the cluster's barrier; other sequences read none of it, for pages of a tree belong to one sequence alone.  Bound: latency of the chain list, length,
+// pages, counts, rows; the tree is asked for ahead of it and the pages are kept (one sequence, with the call that makes room: ??? us; 64 of up to 64 nodes, 32 planes of 4 heads, 11.7 MB:
+// ???).
 __global__ void __launch_bounds__(kCopyThreads) pages_commit_kernel(const Pool p, const CommitParams a) {
-  __shared__ int child_s[kMaxNodes], path_s[kMaxNodes], n_s, refused_s;
+  __shared__ int child_s[kMaxNodes], path_s[kMaxNodes], target_s[kMaxNodes], page_s[kMaxNodes + 1], n_s, refused_s;
+  constexpr int kEach = kMaxNodes / kCopyThreads;
   const int tid = threadIdx.x, rank = blockIdx.x, ranks = gridDim.x, i = blockIdx.y;   // (a cluster is a row of the grid)
   bk_pdl_wait();
   bk_pdl_trigger();
   const int s = a.seqs[i], n = a.n_new ? a.n_new[i] : a.T;
-  bool again = false;
-  for (int j = tid; j < i; j += kCopyThreads) again |= a.seqs[j] == s;
+  int parent[kEach], token[kEach];
+#pragma unroll
+  for (int k = 0; k < kEach; k++) {
+    const int t = tid + k * kCopyThreads;
+    if (t >= a.T) break;
+    parent[k] = a.parent[(size_t)t * a.n + i];
+    token[k] = a.token[(size_t)t * a.n + i];
+    target_s[t] = a.target[(size_t)t * a.n + i];
+    child_s[t] = kMaxNodes;
+  }
+  bool bad = false;
+  for (int j = tid; j < i; j += kCopyThreads) bad |= a.seqs[j] == s;
   const bool named = s >= 0 && s < p.n_seqs && n >= 1 && n <= a.T;
-  const int len = named ? __ldcg(p.lens + s) : 0, base = len - n;
+  const int len = named ? __ldcg(p.lens + s) : 0, base = len - n, first_page = max(base, 0) / p.page_rows;
+  const int said = named && a.history ? __ldcg(a.hist_len + s) : 0;
   bool good = named && base >= 0 && len <= p.max_pages * p.page_rows;
   int* table = p.table + (size_t)max(s, 0) * p.max_pages;
-  if (good) {   // (of the whole CTA)
-    // pages of the tree's rows: this sequence's alone
-    for (int j = base / p.page_rows + tid; j < pages_of(len, p.page_rows); j += kCopyThreads) {
+  if (good)   // pages of the tree's rows: this sequence's alone
+    for (int j = first_page + tid; j < pages_of(len, p.page_rows); j += kCopyThreads) {
       const int page = __ldcg(table + j);
-      again |= page < 0 || page >= p.n_pages || __ldcg(p.ref + page) != 1;
+      page_s[j - first_page] = page;
+      bad |= page < 0 || page >= p.n_pages || __ldcg(p.ref + page) != 1;
     }
-    for (int t = tid; t < n; t += kCopyThreads) child_s[t] = kMaxNodes;
+  good = !__syncthreads_or(bad) && good;   // (of the whole CTA)
+#pragma unroll
+  for (int k = 0; k < kEach; k++) {
+    const int t = tid + k * kCopyThreads;
+    if (t >= a.T) break;
+    if (good && t >= 1 && t < n && parent[k] >= 0 && parent[k] < t && token[k] == target_s[parent[k]]) atomicMin(child_s + parent[k], t);
   }
-  if (tid == 0) n_s = 0;
-  good = !__syncthreads_or(again) && good;
-  if (good) {
-    for (int t = 1 + tid; t < n; t += kCopyThreads) {
-      const int up = a.parent[(size_t)t * a.n + i];
-      if (up >= 0 && up < t && a.token[(size_t)t * a.n + i] == a.target[(size_t)up * a.n + i]) atomicMin(child_s + up, t);
-    }
-    __syncthreads();
-    if (tid == 0) {
-      int m = 0;
+  __syncthreads();
+  if (tid == 0) {
+    int m = 0;
+    if (good)
       for (int t = 0; t < kMaxNodes; t = child_s[t]) path_s[m++] = t;
-      n_s = m;
-      refused_s = 0;
-      if (a.history) {
-        const int h = __ldcg(a.hist_len + s);
-        refused_s = h < 0 || h > a.history_ld - m;
-      }
-    }
-    __syncthreads();
-    good = refused_s == 0;
+    n_s = m;
+    refused_s = a.history && (said < 0 || said > a.history_ld - m);
   }
+  __syncthreads();
+  good = good && !refused_s;
   const int m = good ? n_s : 0;
   if (rank == 0) {
     if (a.path)
       for (int t = tid; t < a.T; t += kCopyThreads) a.path[(size_t)t * a.n + i] = t < m ? path_s[t] : -1;
     if (tid == 0) {
       if (a.n_path) a.n_path[i] = m;
-      if (a.next) a.next[i] = good ? a.target[(size_t)path_s[m - 1] * a.n + i] : -1;
+      if (a.next) a.next[i] = good ? target_s[path_s[m - 1]] : -1;
       if (a.ok) a.ok[i] = good;
     }
   }
@@ -475,8 +484,8 @@ __global__ void __launch_bounds__(kCopyThreads) pages_commit_kernel(const Pool p
       const int chunk = (int)(it % chunks), run = (int)(it / chunks), head = run % p.heads, plane = run / p.heads, vec = chunk * 32 + lane;
       uint8_t* at = p.base + plane * p.plane_bytes + (size_t)head * p.page_rows * p.row_bytes + (size_t)vec * 16;
       auto row_at = [&](int t) {
-        const int row = base + t;
-        return reinterpret_cast<uint4*>(at + __ldcg(table + row / p.page_rows) * p.page_bytes + (size_t)(row % p.page_rows) * p.row_bytes);
+        const int row = base + t, page = row / p.page_rows;
+        return reinterpret_cast<uint4*>(at + page_s[page - first_page] * p.page_bytes + (size_t)(row - page * p.page_rows) * p.row_bytes);
       };
       if (vec < p.row_bytes / 16)
         for (int k = first; k < m; k += kCopyVecs) {
@@ -498,16 +507,13 @@ __global__ void __launch_bounds__(kCopyThreads) pages_commit_kernel(const Pool p
   }
   if (rank) return;
   for (int j = pages_of(base + m, p.page_rows) + tid; j < pages_of(len, p.page_rows); j += kCopyThreads) {
-    p.ref[table[j]] = 0;
+    p.ref[page_s[j - first_page]] = 0;
     table[j] = -1;
   }
   if (a.history) {
-    const int h = a.hist_len[s];
-    int* to = a.history + (size_t)s * a.history_ld + h;
-    for (int t = 1 + tid; t < m; t += kCopyThreads) to[t - 1] = a.token[(size_t)path_s[t] * a.n + i];
-    if (tid == 0) to[m - 1] = a.target[(size_t)path_s[m - 1] * a.n + i];
-    __syncthreads();
-    if (tid == 0) a.hist_len[s] = h + m;
+    int* to = a.history + (size_t)s * a.history_ld + said;
+    for (int t = tid; t < m; t += kCopyThreads) to[t] = a.token[(size_t)path_s[t] * a.n + i];
+    if (tid == 0) a.hist_len[s] = said + m;
   }
   if (tid == 0) p.lens[s] = base + m;
 }
@@ -645,12 +651,12 @@ int32_t bkPagesBatch(const bkPages* pool, const bkPagesBatchArgs* args) {
   const bkPagesBatchArgs& a = *args;
   TRY(check_list("bkPagesBatch", a.n, a.seqs, a.seqs));
   BK_ARG(a.T >= 1 && a.T <= kMaxNodes, "bkPagesBatch: T=%d (1 to %d)", a.T, kMaxNodes);
-  BK_ARG(((a.n_new | a.parent | a.table | a.lens | a.pos | a.slot | a.mask) & 3) == 0, "bkPagesBatch: all arrays are of 32-bit words");
+  BK_ARG(((a.n_new | a.parent | a.table | a.lens | a.pos | a.slot | a.mask | a.ok | a.count) & 3) == 0, "bkPagesBatch: all arrays are of 32-bit words");
   BK_ARG(!a.mask || a.mask_words >= (a.T + 31) / 32, "bkPagesBatch: mask_words=%d for %d nodes", a.mask_words, a.T);
   BK_ARG(!a.slot || (long long)p.n_pages * p.page_rows < (1ll << 31), "bkPagesBatch: %d pages of %d rows: a slot has 31 bits", p.n_pages, p.page_rows);
   if (a.n == 0) return BK_OK;
-  const BatchParams b = {bk_ptr<int>(a.seqs), bk_ptr<int>(a.n_new), bk_ptr<int>(a.parent), bk_ptr<int>(a.table), bk_ptr<int>(a.lens), bk_ptr<int>(a.pos), bk_ptr<int>(a.slot),
-                         bk_ptr<uint32_t>(a.mask), a.n, a.T, a.mask_words};
+  const BatchParams b = {bk_ptr<int>(a.seqs), bk_ptr<int>(a.n_new), bk_ptr<int>(a.parent), bk_ptr<int>(a.ok), bk_ptr<int>(a.table), bk_ptr<int>(a.lens), bk_ptr<int>(a.pos),
+                         bk_ptr<int>(a.slot), bk_ptr<int>(a.count), bk_ptr<uint32_t>(a.mask), a.n, a.T, a.mask_words};
   // CTAs a sequence: 1,024 entries of its table each, no more than fill the GPU twice
   const int y = a.table ? std::max(1, std::min((p.max_pages + 4 * kCopyThreads - 1) / (4 * kCopyThreads), 2 * bk_ctx().sm_count / a.n)) : 1;
   BK_CUDA(bk_launch_pdl(pages_batch_kernel, dim3(a.n, y), dim3(kCopyThreads), 0, p, b));

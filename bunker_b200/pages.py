@@ -55,15 +55,13 @@ class PagePool:
         _check(cu().bkPagesCompact(C.byref(self.desc), table_out, ref_out, map_out, used_out))
 
     def batch(self, seqs: int, n: int, *, T: int = 1, n_new: int = 0, parent: int = 0, table: int = 0, lens: int = 0, pos: int = 0, slot: int = 0, mask: int = 0,
-              mask_words: int = 0) -> None:
+              mask_words: int = 0, ok: int = 0, count: int = 0) -> None:
         """What a step over sequences seqs[0..n) with up to T new tokens each takes: their tables and lengths in the list's order, and of every token (a node of a
-        drafted tree) its position, its row in the pool and the nodes on its path (bkPagesBatch)."""
-        _check(cu().bkPagesBatch(C.byref(self.desc), C.byref(R.bkPagesBatchArgs(seqs=seqs, n_new=n_new, parent=parent, table=table, lens=lens, pos=pos, slot=slot,
-                                                                                 mask=mask, n=n, T=T, mask_words=mask_words))))
+        drafted tree) its position, its row in the pool and the nodes on its path (bkPagesBatch).  ok: what ``grow`` said."""
+        _check(cu().bkPagesBatch(C.byref(self.desc), C.byref(R.bkPagesBatchArgs(seqs, n_new, parent, table, lens, pos, slot, mask, ok, count, n, T, mask_words))))
 
     def commit(self, seqs: int, n: int, *, T: int, parent: int, token: int, target: int, n_new: int = 0, path: int = 0, n_path: int = 0, next: int = 0,
                ok: int = 0, history: int = 0, hist_len: int = 0, history_ld: int = 0) -> None:
         """Of every drafted tree the path that agrees with target stays, the rest of its rows are given up (bkPagesCommit)."""
-        _check(cu().bkPagesCommit(C.byref(self.desc), C.byref(R.bkPagesCommitArgs(seqs=seqs, n_new=n_new, parent=parent, token=token, target=target, path=path,
-                                                                                   n_path=n_path, next=next, ok=ok, history=history, hist_len=hist_len, n=n,
-                                                                                   T=T, history_ld=history_ld))))
+        _check(cu().bkPagesCommit(C.byref(self.desc), C.byref(R.bkPagesCommitArgs(seqs, n_new, parent, token, target, path, n_path, next, ok, history, hist_len,
+                                                                                   n, T, history_ld))))

@@ -82,7 +82,7 @@ class bkPagedAttnArgs(C.Structure):
 
 
 class bkPagesBatchArgs(C.Structure):
-    _fields_ = [(n, C.c_uint64) for n in ("seqs", "n_new", "parent", "table", "lens", "pos", "slot", "mask")] + \
+    _fields_ = [(n, C.c_uint64) for n in ("seqs", "n_new", "parent", "table", "lens", "pos", "slot", "mask", "ok", "count")] + \
                [(n, C.c_int32) for n in ("n", "T", "mask_words", "reserved")]
 
 

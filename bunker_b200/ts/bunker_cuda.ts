@@ -334,14 +334,15 @@ export function pagedAttn(a: PagedAttn): void {
   check(cu().bkPagedAttn(b), "bkPagedAttn");
 }
 
-/** Maps of a step (bkPagesBatchArgs, 80 bytes): tables, lengths, positions, slots and masks of a list of sequences and their drafted trees. */
+/** Maps of a step (bkPagesBatchArgs, 96 bytes): tables, lengths, positions, slots and masks of a list of sequences and their drafted trees. */
 export interface PagesBatch {
-  seqs: bigint; nNew?: bigint; parent?: bigint; table?: bigint; lens?: bigint; pos?: bigint; slot?: bigint; mask?: bigint; n: number; T: number; maskWords?: number;
+  seqs: bigint; nNew?: bigint; parent?: bigint; table?: bigint; lens?: bigint; pos?: bigint; slot?: bigint; mask?: bigint; ok?: bigint; count?: bigint; n: number; T: number;
+  maskWords?: number;
 }
 export function pagesBatch(pool: Buffer, a: PagesBatch): void {
-  const b = Buffer.alloc(80);
-  [a.seqs, a.nNew, a.parent, a.table, a.lens, a.pos, a.slot, a.mask].forEach((v, i) => b.writeBigUInt64LE(v ?? 0n, 8 * i));
-  [a.n, a.T, a.maskWords ?? 0].forEach((v, i) => b.writeInt32LE(v, 64 + 4 * i));
+  const b = Buffer.alloc(96);
+  [a.seqs, a.nNew, a.parent, a.table, a.lens, a.pos, a.slot, a.mask, a.ok, a.count].forEach((v, i) => b.writeBigUInt64LE(v ?? 0n, 8 * i));
+  [a.n, a.T, a.maskWords ?? 0].forEach((v, i) => b.writeInt32LE(v, 80 + 4 * i));
   check(cu().bkPagesBatch(pool, b), "bkPagesBatch");
 }
 

@@ -351,14 +351,16 @@ BK_API uint64_t bkPagedAttnScratchBytes(int32_t B, int32_t T, int32_t Hq, int32_
  *   slot   int32 [T][n]: page * page_rows + row in the page, of the node's own row (n_pages * page_rows below 2^31)
  *   mask   uint32 [T][n][mask_words]: bit u is set for the nodes u of the node's path, itself among them
  * parent int32 [T][n]: the node that it continues, -1 (or any that is not an earlier node): none; parent = 0: each token continues the one before.
- * n_new int32 [n]: how many of a sequence's rows are new, 0..T (less than 0 counts as 0, more than T as T); 0 = T of each.  A token t >= n_new, or of a
- * sequence that has fewer than n_new rows, is not there: pos and slot are -1, its mask 0.  An entry that names no sequence has no rows.  The
+ * n_new int32 [n]: how many of a sequence's rows are new, 0..T (less than 0 counts as 0, more than T as T); 0 = T of each.  ok int32 [n] (0 = all): what bkPagesGrow
+ * said; where it is 0 the sequence got no room and has no new rows.  count int32 [n] gets how many it has then, which the attention and bkPagesCommit take as n_new.
+ * A token t >= count, or of a sequence that has fewer than n_new rows (count 0), is not there: pos and slot are -1, its mask 0.  An entry that names no sequence has no rows.  The
  * same sequence may be in the list twice.  The pool is not changed. */
 typedef struct bkPagesBatchArgs {
   uint64_t seqs;         /* int32 [n] */
   uint64_t n_new;
   uint64_t parent;
   uint64_t table, lens, pos, slot, mask;
+  uint64_t ok, count;
   int32_t n, T, mask_words, reserved; /* T 1..1024; mask_words >= (T + 31) / 32 */
 } bkPagesBatchArgs;
 BK_API int32_t bkPagesBatch(const bkPages* pool, const bkPagesBatchArgs* args);
@@ -380,7 +382,7 @@ BK_API int32_t bkTreeAttn(const bkTreeAttnArgs* args);
 BK_API uint64_t bkTreeAttnScratchBytes(int32_t B, int32_t T, int32_t Hq, int32_t Hkv, int32_t HD, int32_t prefix_rows);
 
 /* Penalties for repeated tokens, biases and grammar masks on logits f32 [T*B][ld], in place; row t*B + b is token t of request b.  For token v, with
- * n = how often v stands in the request's history behind its prompt, plus how often on the row's path:
+ * n = how often v stands in the request's history behind its prompt, plus how often on the row's path (whose tokens the history does not hold yet):
  *   x = logits[v];   if v stands in the history or on the path:  x = x > 0 ? x / repetition : x * repetition,  x -= frequency * n + presence * [n > 0];
  *   x += bias of v (a token that a request names several times gets the sum, in the list's order);   x = -inf where the row's mask does not allow v.
  * A logit that nothing names or hides is neither read nor written.  NaN stays NaN where it is allowed. */
@@ -409,7 +411,8 @@ BK_API int32_t bkAdjustLogits(const bkLogitsArgs* args);
  * goes on to the lowest child whose token is the target of the node before, as long as there is one.  The rows of the path move up
  * behind the rows before the tree, in all planes; the others are given up, with the pages that only they had.
  *   path int32 [T][n]: nodes of the path, -1 behind it (0 = not wanted); n_path int32 [n]; next int32 [n]: the target of the last (a token without a row yet)
- *   history int32 [n_seqs][history_ld], hist_len int32 [n_seqs] (0 = none): the tokens of the path but node 0's, then next, are appended
+ *   history int32 [n_seqs][history_ld], hist_len int32 [n_seqs] (0 = none): the tokens of the path are appended, node 0's first.  A history is then what has rows; next
+ *   comes with the next tree, as its node 0 (and bkAdjustLogits counts it with the path, not twice)
  * ok[i] (0 to skip): 1, or 0 where nothing is changed, n_path is 0, next and path are -1: the entry names no sequence or one named before, n_new[i] is not
  * in 1..T, the sequence has fewer rows, a page that holds rows of its tree is shared (or none of the pool's), or its history has no room (or a length below 0). */
 typedef struct bkPagesCommitArgs {

@@ -68,13 +68,14 @@ def test_batch_maps_of_lists_and_trees(bk, T, rows, extra):
     trees = [random_tree(rng, T, b % 2 == 0) for b in range(n)]
     trees[1][T - 1] = T + 3                              # not an earlier node
     trees[5][T // 2] = -7
-    for parent, counts in ((trees, new), (None, new), (trees, None)):
+    served = i32(1, 1, 1, 1, 1, 1, 0, 1)
+    for parent, counts, ok in ((trees, new, None), (None, new, served), (trees, None, served)):
         out = {k: R.DeviceBuffer.from_numpy(np.full(size, 0x5A5A5A5A, np.uint32)) for k, size in
-               (("table", n * p.max_pages), ("lens", n), ("pos", T * n), ("slot", T * n), ("mask", T * n * W))}
-        d = [dev(seqs), dev(new), dev(by_node(trees, T))]
-        pool.batch(d[0].ptr, n, T=T, n_new=d[1].ptr if counts is not None else 0, parent=d[2].ptr if parent else 0, mask_words=W, **{k: b.ptr for k, b in out.items()})
+               (("table", n * p.max_pages), ("lens", n), ("pos", T * n), ("slot", T * n), ("mask", T * n * W), ("count", n))}
+        d = [dev(seqs), dev(new), dev(by_node(trees, T)), dev(served)]
+        pool.batch(d[0].ptr, n, T=T, n_new=d[1].ptr if counts is not None else 0, parent=d[2].ptr if parent else 0, ok=d[3].ptr if ok is not None else 0, mask_words=W, **{k: b.ptr for k, b in out.items()})
         p.check("unchanged")
-        table, lens = np.full((n, p.max_pages), -1, np.int32), np.zeros(n, np.int32)
+        table, lens, count = np.full((n, p.max_pages), -1, np.int32), np.zeros(n, np.int32), np.zeros(n, np.int32)
         pos, slot, mask = np.full((T, n), -1, np.int32), np.full((T, n), -1, np.int32), np.zeros((T, n, W), np.uint32)
         for i, s in enumerate(seqs):
             if not 0 <= s < p.seqs:
@@ -83,16 +84,19 @@ def test_batch_maps_of_lists_and_trees(bk, T, rows, extra):
             held = p.np_pages(lens[i])
             table[i, :held] = p.table[s, :held]
             m = T if counts is None else min(max(int(new[i]), 0), T)
+            if ok is not None and not ok[i]:
+                m = 0
             base = int(lens[i]) - m
             if base < 0:
                 continue
+            count[i] = m
             path = paths(parent[i] if parent else list(range(-1, T - 1)))
             for t in range(m):
                 pos[t, i] = base + path[t].sum() - 1
                 page = p.table[s, (base + t) // rows]
                 slot[t, i] = page * rows + (base + t) % rows if 0 <= page < p.n_pages else -1
                 mask[t, i] = words(path[t], W)
-        for name, want in (("table", table), ("lens", lens), ("pos", pos), ("slot", slot), ("mask", mask)):
+        for name, want in (("table", table), ("lens", lens), ("pos", pos), ("slot", slot), ("mask", mask), ("count", count)):
             assert np.array_equal(out[name].download(want.dtype, want.shape), want), name
 
 
@@ -643,7 +647,7 @@ class Draft(Pool):
                 h = int(hist_len[s])
                 if h < 0 or h + len(walk) > history.shape[1]:
                     continue
-                history[s, h:h + len(walk)] = [self.token[t, i] for t in walk[1:]] + [self.target[walk[-1], i]]
+                history[s, h:h + len(walk)] = [self.token[t, i] for t in walk]
                 hist_len[s] += len(walk)
             ok[i], n_path[i], nxt[i] = 1, len(walk), self.target[walk[-1], i]
             path[:len(walk), i] = walk
@@ -804,3 +808,146 @@ def test_maps_and_commit_refuse_what_they_cannot_do(bk):
         assert fn(C.byref(pool.desc), None) == R.BK_ERR_ARG and fn(None, C.byref(x)) == R.BK_ERR_ARG
         assert fn(C.byref(desc), C.byref(x)) == R.BK_ERR_ARG
     p.check("nothing changed")
+
+
+# ---- all of it together ----------------------------------------------------------------
+
+def test_drafted_trees_give_the_tokens_of_single_steps(bk):
+    """A one-layer model served to four requests behind a prompt, greedy under penalties, biases and a grammar: token by token, then with drafted trees whose branches hold those
+    tokens and others.  Wherever the best logit is clear of the second, the same tokens come out, as many at once as were drafted right."""
+    from bunker_b200 import shared_prompt as S
+    from bunker_b200.model import CONFIG_TINY as cfg
+    rng = np.random.default_rng(77)
+    N, P, STEPS, T, H, V = 4, 83, 25, 9, cfg.hidden, cfg.vocab
+    w, lora = S.random_layer(cfg, seed=3)
+    f = dev(rng.normal(0, 1, (V, H)).astype(np.float32))
+    table = R.DeviceBuffer(V * H // 256 * 144)
+    ops.quantize_q4k(f.ptr, V, H, table.ptr)
+    adapters = [0, -1, 2, 1]
+    history = np.zeros((N, P + STEPS + 40), np.int32)
+    history[:, :P] = rng.integers(0, V, P)
+    history[:, P] = [5, 6, 7, 8]                                          # the first token of each
+    rules = dict(rep=np.array([1.3, 1.0, 1.1, 2.0], np.float32), pres=np.array([0.5, 0, 0.2, 0], np.float32), freq=np.array([0.1, 0.3, 0, 0], np.float32))
+    d_rules = {k: dev(v) for k, v in rules.items()}
+    prompt_len = dev(np.full(N, P, np.int32))
+    allowed = dev(words(rng.random((2, V)) < 0.5, V // 32))
+    bias_t, bias_v, bias_n = dev(rng.integers(0, V, (N, 3)).astype(np.int32)), dev(rng.normal(0, 3, (N, 3)).astype(np.float32)), dev(i32(3, 0, 2, 1))
+    ids, x, hq = R.DeviceBuffer(4 * 64), R.DeviceBuffer(64 * H * 2), R.DeviceBuffer(64 * H // 32 * 36)
+    logits, best, top = R.DeviceBuffer(64 * V * 4), R.DeviceBuffer(4 * 64), R.DeviceBuffer(4 * 64)
+    scratch = R.DeviceBuffer.zeros(ops.argmax_scratch_bytes(64))
+
+    def layer():
+        s = S.SharedPrompt(cfg, w, lora, N, P + STEPS + 60, 60)
+        ids_p, xp = dev(history[0, :P]), R.DeviceBuffer(P * H * 2)
+        for at in range(0, P, 64):
+            ops.embed(table.ptr, H, ids_p.ptr + 4 * at, min(64, P - at), xp.ptr + at * H * 2)
+        s.prompt(xp.ptr, P)
+        assert s.fork(range(N)).all()
+        return s
+
+    def head(out, rows, hist, hist_len, tree=None):
+        """logits of `rows` rows under the rules -> greedy tokens in `best`"""
+        ops.quant_q8_1(out, H, rows, hq.ptr, bf16=True)
+        ops.gemv(hq.ptr, H, rows, [ops.gemv_seg(table.ptr, V, logits.ptr)], order=1)
+        mask_id = dev(np.tile(i32(0, -1, 1, -1), rows // N))
+        more = dict(T=rows // N, draft=tree[0].ptr, path=tree[1], path_words=2) if tree else dict(T=1)
+        ops.adjust_logits(ops.adjust_logits_args(
+            logits=logits.ptr, V=V, B=N, history=hist.ptr, history_ld=history.shape[1], hist_len=hist_len.ptr, prompt_len=prompt_len.ptr, repetition=d_rules["rep"].ptr,
+            presence=d_rules["pres"].ptr, frequency=d_rules["freq"].ptr, bias_token=bias_t.ptr, bias_value=bias_v.ptr, bias_n=bias_n.ptr, bias_ld=3, allowed=allowed.ptr,
+            mask_id=mask_id.ptr, n_masks=2, allowed_words=V // 32, **more))
+        ops.argmax(logits.ptr, V, rows, best.ptr, top.ptr, scratch.ptr)
+        assert R.cuSync() == 0, R.last_error()      # (mask_id)
+
+    # token by token
+    s, said, clear = layer(), history.copy(), np.zeros((N, STEPS), bool)
+    for step in range(STEPS):
+        ids.upload(np.ascontiguousarray(said[:, P + step]))
+        ops.embed(table.ptr, H, ids.ptr, N, x.ptr)
+        h, n = dev(said), dev(np.full(N, P + step + 1, np.int32))           # (the token of this step among them: there is no path)
+        head(s.step(x.ptr, adapters), N, h, n)
+        y = np.sort(logits.download(np.float32, (N, V)), 1)
+        # results of attention that are rounded the other way move a logit by a few 2^-8 of the hidden state's part in it
+        clear[:, step] = y[:, -1] - y[:, -2] > 2.0 ** -4 * y[np.isfinite(y)].std()
+        said[:, P + step + 1] = best.download(np.int32, (N,))
+    assert clear.mean() > 0.5
+
+    # with trees: a spine of the tokens that will come, the last of them wrong in some, branches of other tokens
+    s, at, hist, hist_len = layer(), np.zeros(N, np.int64), dev(history), dev(np.full(N, P, np.int32))
+    many = 0
+    while at.min() < STEPS - T:
+        parent, token = np.zeros((T, N), np.int32), np.zeros((T, N), np.int32)
+        for i in range(N):
+            line = said[i, P + at[i]:P + at[i] + T]
+            parent[:, i] = [-1, 0, 0, 2, 3, 1, 4, 6, 2]                    # right: 0, 2, 3, 4, 6, 7
+            token[:, i] = [line[0], line[1] + 1, line[1], line[2], line[3], line[2], line[4], line[5] + i % 2, line[2] + 1]
+        token %= V
+        flat = dev(token.reshape(-1))
+        ops.embed(table.ptr, H, flat.ptr, T * N, x.ptr)
+        out = s.draft(x.ptr, parent, adapters)
+        head(out, T * N, hist, hist_len, (flat, s.b_mask.ptr))
+        target = best.download(np.int32, (T, N))
+        d = [dev(parent.reshape(-1)), s.lists["parent"]]
+        assert np.array_equal(d[0].download(np.int32, (T * N,)), d[1].download(np.int32, (64,))[:T * N])
+        kept, after = s.keep(token, best.ptr)
+        lens = s.lens.download(np.int32, (N + 1,))
+        h, n = hist.download(np.int32, history.shape), hist_len.download(np.int32, (N,))
+        for i in range(N):
+            assert 1 <= kept[i] <= 6 and lens[i + 1] == P + at[i] + kept[i]
+            right = [0, 2, 3, 4, 6, 7][:6 if i % 2 == 0 else 5]
+            for k, node in enumerate(right[:kept[i]]):
+                if clear[i, at[i] + k]:
+                    assert target[node, i] == said[i, P + at[i] + k + 1], (i, at[i], k)
+            if clear[i, at[i]:at[i] + len(right)].all():
+                assert kept[i] == len(right) and after[i] == said[i, P + at[i] + kept[i]]
+                many += 1
+            # go on along the tokens of the single steps
+            h[i, n[i]:n[i] + kept[i]] = said[i, P + at[i]:P + at[i] + kept[i]]
+        if (kept < [6, 5, 6, 5]).any() or any(said[i, P + at[i] + kept[i]] != after[i] for i in range(N)):
+            break                                                          # (a near tie: the streams part)
+        hist.upload(h)
+        hist_len.upload((n + kept).astype(np.int32))
+        at += kept
+    assert many >= 4
+
+
+def test_drafts_are_refused_where_they_do_not_fit(bk):
+    from bunker_b200 import shared_prompt as S
+    from bunker_b200.model import CONFIG_TINY as cfg
+    w, lora = S.random_layer(cfg, seed=4)
+    s = S.SharedPrompt(cfg, w, lora, 3, 64, 6)                              # six pages of 16 rows
+    x = dev(rnd(np.random.default_rng(1), 64, cfg.hidden))
+    s.prompt(x.ptr, 32)
+    assert s.fork([0, 2]).tolist() == [True, True]
+    chain = np.array([[-1] * 3] + [[t] * 3 for t in range(16)], np.int32)   # 17 nodes take two pages: four are free
+    for bad in (np.zeros((22, 3), np.int32), np.zeros((3, 2), np.int32), np.zeros((0, 3), np.int32)):
+        with pytest.raises(ValueError):
+            s.draft(x.ptr, bad, [-1] * 3)
+    for kw in (dict(adapters=[-1] * 2), dict(adapters=[-1] * 3, n_new=[1, 2]), dict(adapters=[-1] * 3, n_new=[18, 1, 1])):
+        with pytest.raises(ValueError):
+            s.draft(x.ptr, chain, **kw)
+    with pytest.raises(RuntimeError):
+        s.keep(chain, x.ptr)
+    s.draft(x.ptr, chain, [-1] * 3)
+    assert s.b_count.download(np.int32, (3,)).tolist() == [17, 0, 17]
+    for call in (lambda: s.step(x.ptr, [-1] * 3), lambda: s.draft(x.ptr, chain, [-1] * 3), lambda: s.fork([1]), lambda: s.drop([0]), lambda: s.prompt(x.ptr, 1)):
+        with pytest.raises(RuntimeError):
+            call()
+    with pytest.raises(ValueError):
+        s.keep(chain[:3], x.ptr)
+    token = np.arange(51, dtype=np.int32).reshape(17, 3)
+    target = np.full((17, 3), 99, np.int32)
+    target[:, 2] = np.append(token[1:, 2], 77)
+    t = dev(target)
+    kept, after = s.keep(token, t.ptr)
+    assert kept.tolist() == [1, 0, 17] and after.tolist() == [99, -1, 77]
+    assert s.lens.download(np.int32, (4,)).tolist() == [32, 33, 0, 49]
+    # request 2 holds two pages, request 0 one, one is free: 16 more nodes fit for the first of the list alone
+    s.draft(x.ptr, chain[:16], [-1] * 3, share=False)
+    assert s.b_count.download(np.int32, (3,)).tolist() == [16, 0, 0]
+    before, lens = s.data.download(np.uint16, (2, 6, 1, 16, cfg.head_dim)), s.lens.download(np.int32, (4,))
+    assert lens.tolist() == [32, 49, 0, 49]
+    kept, after = s.keep(token[:16], t.ptr)
+    assert kept.tolist() == [1, 0, 0] and s.lens.download(np.int32, (4,)).tolist() == [32, 34, 0, 49]
+    table = s.table.download(np.int32, (4, s.max_pages))
+    mine = table[3, :4]
+    assert np.array_equal(s.data.download(np.uint16, before.shape)[:, mine], before[:, mine])      # the refused one's rows are what they were

@@ -9,7 +9,7 @@ from bunker_b200 import runtime as R
 
 
 def test_struct_layouts_match_the_header():
-    assert C.sizeof(R.bkPagesBatchArgs) == 8 * 8 + 4 * 4 and R.bkPagesBatchArgs.n.offset == 64
+    assert C.sizeof(R.bkPagesBatchArgs) == 10 * 8 + 4 * 4 and R.bkPagesBatchArgs.n.offset == 80
     assert C.sizeof(R.bkTreeAttnArgs) == C.sizeof(R.bkPagedAttnArgs) + 3 * 8 + 8 and R.bkTreeAttnArgs.pos.offset == 184 and R.bkTreeAttnArgs.mask_words.offset == 208
     assert C.sizeof(R.bkLogitsArgs) == 15 * 8 + 10 * 4 and R.bkLogitsArgs.B.offset == 120
     assert C.sizeof(R.bkPagesCommitArgs) == 11 * 8 + 4 * 4 and R.bkPagesCommitArgs.T.offset == 92
