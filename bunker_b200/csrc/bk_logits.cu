@@ -2,7 +2,7 @@
 //
 // Two kinds of CTAs, of one launch, which never touch the same logit.  Some hide what the masks forbid: a warp has 1,024 tokens of a row, a lane's mask word
 // at a time for all lanes, and only writes.  The others do what is named (tokens of a history, of a path in a drafted tree, of a list of biases), which is sparse: a CTA has a
-// slice of the vocabulary of one request (every 2^k-th block of 64 tokens, since frequent tokens have numbers near one another), counts the tokens of the history that
+// slice of the vocabulary of one request (every 2^k-th block of 512 tokens, since frequent tokens have numbers near one another), counts the tokens of the history that
 // lie there in shared memory (a word for each token of the slice, or, for short histories, a table of those that occur), lists them, and goes over (listed token, row) pairs; the rows of a request, the nodes of its tree, share counts and list.  Tokens that are
 // drafted somewhere in the tree, or have a bias, are marked and left to a loop of their own.  Counts are integers, so results do not depend on the order of threads.
 //
@@ -17,11 +17,11 @@
 namespace {
 
 constexpr int kThreads = 512;
-constexpr int kUnits = 4;        // logits that a thread has on the way
+constexpr int kUnits = 6;        // logits that a thread has on the way
 constexpr int kMaxNodes = 1024;  // of a tree
-constexpr int kMaxSlice = 16384; // words
+constexpr int kMaxSlice = 8192;  // words
 constexpr int kMaxTable = 8192;  // entries of a table (of 8 bytes), a quarter of them free
-constexpr int kBlock = 64;       // tokens that lie together in a slice
+constexpr int kBlock = 512;      // tokens that lie together in a slice (64: 3 % slower, where memory is the bound)
 constexpr int kAhead = 1;        // groups of four tokens of the history that a thread asks for before it knows the history's length
 
 // A token's word: how often it was said, whether the last loop has it, whether it is in the prompt.
@@ -88,14 +88,18 @@ BK_DEVINL void hide(const LogitsParams& p, int cta) {
 
 // TABLE: words belong to the tokens of a table (open addressing), not to all of the slice's
 template <bool TABLE>
-__global__ void __launch_bounds__(kThreads, 3) adjust_logits_kernel(const __grid_constant__ LogitsParams p) {
+__global__ void __launch_bounds__(kThreads, 2) adjust_logits_kernel(const __grid_constant__ LogitsParams p) {
   extern __shared__ __align__(16) uint32_t word_s[];        // [slice], then lists, see there
   __shared__ int node_s[kMaxNodes], warp_s[kThreads / 32];  // nodes whose token lies in the slice: node << 16 | place
   __shared__ int n_node_s, n_marked_s, n_listed_s, mask_s[kMaxNodes];   // mask_s: of each row, -1 where it has none
   bk_pdl_wait();
   bk_pdl_trigger();
-  if ((int)blockIdx.x >= p.naming) {
-    hide(p, blockIdx.x - p.naming);
+  // Every third CTA hides, while there are two that name to one that hides: the ones are bound by memory, the others by latency (512 rows: 122 us with all that hide
+  // behind, 111 so).
+  const int triples = min(p.hiding, p.naming / 2), i_cta = blockIdx.x, behind = i_cta - 3 * triples;
+  const int i_name = behind < 0 ? (i_cta % 3 < 2 ? i_cta - i_cta / 3 : -1) : behind < p.naming - 2 * triples ? behind + 2 * triples : -1;
+  if (i_name < 0) {
+    hide(p, behind < 0 ? i_cta / 3 : behind - (p.naming - 2 * triples) + triples);
     return;
   }
   const int marks = p.bias_ld + (p.path ? p.T : 0);
@@ -105,7 +109,7 @@ __global__ void __launch_bounds__(kThreads, 3) adjust_logits_kernel(const __grid
   uint16_t* const bias_at_s = marked_s + marks;                               // [bias_ld]
   uint16_t* const listed_s = bias_at_s + p.bias_ld;                           // [slice]: places of tokens that something but a mark names
   int* const key_s = reinterpret_cast<int*>(listed_s + p.slice + ((marks + p.bias_ld) & 1));   // TABLE: [slice] tokens, -1: free
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, part = blockIdx.x & ((1 << p.shift) - 1), group = blockIdx.x >> p.shift, b = group / p.parts,
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, part = i_name & ((1 << p.shift) - 1), group = i_name >> p.shift, b = group / p.parts,
             t0 = (group - b * p.parts) * p.rows, rows = min(p.rows, p.T - t0);
   if (rows <= 0) return;
   // token -> its place in the slice, -1: not in it; place -> token
@@ -267,51 +271,31 @@ __global__ void __launch_bounds__(kThreads, 3) adjust_logits_kernel(const __grid
   }
   __syncthreads();
 
-  // (named token, row) pairs, rows next to one another in turn, kUnits pairs of a thread at once
-  const int n_listed = n_listed_s;
+  // (named token, row) pairs, tokens first: kUnits of a thread on the way at once
+  const int n_listed = n_listed_s, pairs = n_listed * rows;
   const size_t next = (size_t)p.B * p.ld;   // floats from a row to the request's next
   float* const x0 = p.logits + ((size_t)t0 * p.B + b) * p.ld;
   auto hidden = [&](int t, int token) {
     const int id = mask_s[t];
     return id >= 0 && !(__ldg(p.allowed + (size_t)id * p.allowed_words + (token >> 5)) >> (token & 31) & 1u);
   };
-  if (rows == 1) {
-    for (int i0 = tid; i0 < n_listed; i0 += kThreads * kUnits) {
-      float* at[kUnits];
-      float x[kUnits];
-      uint32_t w[kUnits];
+  for (int it0 = tid; it0 < pairs; it0 += kThreads * kUnits) {
+    float* at[kUnits];
+    float x[kUnits], sub[kUnits];
 #pragma unroll
-      for (int k = 0; k < kUnits; k++) {
-        const int i = i0 + k * kThreads;
-        at[k] = nullptr;
-        if (i >= n_listed) continue;
-        const int o = listed_s[i], token = token_of(o);
-        w[k] = word_s[o];
-        if (!hidden(0, token)) at[k] = x0 + token;
-        x[k] = __ldcg(x0 + token);
-      }
-#pragma unroll
-      for (int k = 0; k < kUnits; k++)
-        if (at[k]) *at[k] = adjusted(x[k], taken(w[k] & kSaid, a), a);
+    for (int k = 0; k < kUnits; k++) {
+      const int it = it0 + k * kThreads;
+      at[k] = nullptr;
+      if (it >= pairs) continue;
+      const int t = it / n_listed, o = listed_s[it - t * n_listed], token = token_of(o);
+      if (hidden(t, token)) continue;
+      at[k] = x0 + t * next + token;
+      x[k] = __ldcg(at[k]);
+      sub[k] = taken(word_s[o] & kSaid, a);
     }
-  } else {
-    for (int i = tid; i < n_listed; i += kThreads) {
-      const int o = listed_s[i], token = token_of(o);
-      const float sub = taken(word_s[o] & kSaid, a);
-      float* at = x0 + token;
-      for (int t = 0; t < rows; t += kUnits, at += kUnits * next) {
-        float x[kUnits];
-        bool on[kUnits];
 #pragma unroll
-        for (int k = 0; k < kUnits; k++) {
-          on[k] = t + k < rows && !hidden(t + k, token);
-          if (on[k]) x[k] = __ldcg(at + k * next);
-        }
-#pragma unroll
-        for (int k = 0; k < kUnits; k++)
-          if (on[k]) at[k * next] = adjusted(x[k], sub, a);
-      }
-    }
+    for (int k = 0; k < kUnits; k++)
+      if (at[k]) *at[k] = adjusted(x[k], sub[k], a);
   }
   for (int it = tid; it < marked * rows; it += kThreads) {
     const int t = it / marked, i = it - t * marked, o = marked_s[i], token = token_of(o);
@@ -353,9 +337,10 @@ extern "C" int32_t bkAdjustLogits(const bkLogitsArgs* args) {
                     bk_ptr<int>(a.bias_n), bk_ptr<uint32_t>(a.allowed), bk_ptr<int>(a.mask_id), a.B, a.T, a.V, a.n_seqs ? a.n_seqs : a.B, a.history_ld, a.bias_ld, a.path_words,
                     a.n_masks, a.allowed_words, 0, 0, 0, 0, 0, 0, a.ld ? a.ld : a.V};
   if (!a.bias_token) p.bias_ld = 0;
-  // Who names: slices of at most 16,384 words (96 KB with the list, two CTAs an SM), shorter while that leaves SMs without a CTA, to 1,024; then rows apart, until each SM
-  // has four CTAs.  Where such a slice has more than 4,096 words and the request's tokens fit a table, fewer CTAs with a table each (64 requests, 5,000 tokens
-  // of 151,936: 25.5 us with 16 slices of words, 15.5 with four tables; one request, 700 tokens: 4.6 with 128 slices of words, 5.2 with as many tables).
+  // Who names: slices of at most 8,192 words (48 KB with the list; 512 rows behind 16,000 tokens 117 us, with twice as many words 118), shorter while that leaves SMs without a
+  // CTA, to 1,024; then rows apart, until each SM has two (111 us; with four 117, none apart 159).  Where such a slice has more than 4,096 words and the request's tokens fit a table,
+  // fewer CTAs with a table each (64 requests, 5,000 tokens of 151,936: 25 us with slices of words, 15 with four tables; one request, 700 tokens: 4.6 with 128 slices of
+  // words, 5.2 with as many tables).
   // Who hides: four CTAs an SM, no more than have 4,096 tokens each.
   const long long sms = bk_ctx().sm_count;
   const int blocks = (a.V + kBlock - 1) / kBlock;
@@ -371,13 +356,13 @@ extern "C" int32_t bkAdjustLogits(const bkLogitsArgs* args) {
     while (p.shift > 0 && ((long long)a.B * a.T << (p.shift - 1)) >= sms) p.shift--;
   }
   const long long ctas = (long long)a.B << p.shift;
-  p.parts = (int)std::min<long long>(a.T, (4 * sms + ctas - 1) / ctas);
+  p.parts = (int)std::min<long long>(a.T, (2 * sms + ctas - 1) / ctas);
   p.rows = (a.T + p.parts - 1) / p.parts;
   if (a.allowed) p.hiding = (int)std::max<long long>(1, std::min<long long>(4 * sms, (long long)a.T * a.B * a.V / 4096));
   BK_ARG(ctas * p.parts + p.hiding < (1ll << 31), "bkAdjustLogits: B=%d rows of %d logits: too much for one call", a.B, a.V);
   if (a.history || a.bias_token || a.path) p.naming = (int)ctas * p.parts;
   if (p.naming + p.hiding == 0) return BK_OK;
-  const size_t marks = (size_t)p.bias_ld + (a.path ? a.T : 0), smem = (size_t)p.slice * (use_table ? 10 : 6) + (size_t)p.bias_ld * 6 + marks * 6 + 4;   // at most 96 + 6 + 12 KB
+  const size_t marks = (size_t)p.bias_ld + (a.path ? a.T : 0), smem = (size_t)p.slice * (use_table ? 10 : 6) + (size_t)p.bias_ld * 6 + marks * 6 + 4;   // at most 80 + 6 + 12 KB
   auto* kernel = use_table ? adjust_logits_kernel<true> : adjust_logits_kernel<false>;
   static bool configured[2] = {false, false};
   if (!configured[use_table]) {
