@@ -6,6 +6,11 @@
 // common rows: 30 us; 64 behind 32,768, 24 heads on 4: 96 us, 114 where the power limit sets the clock for long: 0.33 and 0.28 of the bf16 rate by
 // the operations that the result needs, half of it again in operations done; 32 sequences of 8,192 rows that share nothing: 98 us, 5.5 TB/s.
 //
+// bkTreeAttn is the same for drafted trees (TREE): a row sees the keys before its sequence's tree and those of its nodes whose bits are set.  Trees bring many rows to a
+// sequence, so its work is shared out by a plan of its own (plan_trees), over tokens that are there.  A step of 128 rows and 64 keys takes 1,900 cycles (HD 256; 1,755 for HD 128), 600 of them
+// exponentials (512 of the unit's), 1,536 (768) of the tensor cores beside them: both groups of rows wait for the same tile.  Four groups, groups that take turns at tiles, and the next
+// tile's scores asked for ahead of the wait for this one's probabilities were no faster.
+//
 // No counterpart in the reference (one contiguous cache of 128 rows, src/emitters.ts:188-226).
 #include <math.h>
 #include <string.h>
@@ -325,8 +330,9 @@ BK_DEVINL void plan_jobs(const Params<false>& p, const Layout& L, uint8_t* scrat
 // A tree has many rows to a sequence, so most jobs are several row tiles over the same keys.  CTAs come in teams, each of which takes one row tile of the same keys at the
 // same time, so that the keys are read from memory once: a sequence's m row tiles (the common keys' too) are cut into as few teams of up to kTeam tiles as there can be, of
 // equal width but for one tile.  Teams of one width are jobs on a line of their own, which is cut into equal pieces for the line's share of the CTAs; shares are the
-// smallest longest piece.  (All row tiles on one line, 32 sequences of up to 16,384 rows and 64 nodes, 24 heads on 4: 704 us, the keys read once for each row tile;
-// so ???.)
+// smallest longest piece.  (32 sequences of up to 16,384 rows and 64 nodes, 24 heads on 4, before the merge of today: teams of one 578 us, of up to two 543, three 520, four 527,
+// six 539; 16 behind 8,192 common rows, 16 on 2: 77, 69, 63, 63, 61.)  Only row tiles and tokens that are there have a place; with all of T for each sequence, half of
+// them there, the first took 704 us on one line.  The tiles are 313 us of the 476 that the call takes now; in a loop the power limit sets the clock.
 constexpr int kTeam = 4;
 // Team job i: {start on its line, job of its first row tile, end of its keys, slot of its first row tile's partial result for team 0}; the slots of a team job's pieces
 // are kTeam-wide steps: slot + w * team + rank, which no two pieces share since i + team grows from piece to piece of a line.  jobs[j] = {.., .., first slot, number and
@@ -549,7 +555,8 @@ BK_DEVINL void store_bf16(uint16_t* dst, const float (&x)[PER]) {
 // One warp per (token row, head): y = x / sqrt(mean(x^2) + eps) (1 + w), then the rotation of pairs (d, d + rot_half), in f32; q heads to the scratch
 // buffer, k and v heads into their page, rounded to bf16: operands of the tensor cores (q's rounding is what the result's error is made of, 0.0024 of
 // its norm against 0.0017 for exact arithmetic rounded once).  The first CTA lays out the work of the next launch.  Bound: latency, 5 us for 32
-// sequences and 7 for 64 of 24 heads, most of it that CTA's.
+// sequences and 7 for 64 of 24 heads, most of it that CTA's.  Trees: a warp takes up to eight heads of a token one after the other, once there are more than the GPU holds, with what
+// they share in registers (2,048 tokens of 28 heads: 42 us a warp for each, so 28; caches cold).
 template <int HD, bool TREE>
 __global__ void __launch_bounds__(kPrepThreads, TREE ? 3 : 0) paged_prepare_kernel(const Params<TREE> p, const Layout L, uint8_t* scratch) {
   constexpr int PER = HD / 32;
@@ -1463,8 +1470,8 @@ __global__ void __launch_bounds__(256 * kSlices) paged_merge_kernel(const Params
 
 // The same for trees.  A thread has kQuads times 4 dims of one head, 64 apart; a CTA 64 kQuads dims of the group's heads, from kSlices slices of pieces.  Many rows have few
 // pieces each: one slice and all dims, so that the chain of loads (place, lists of pieces, sums and results) is there once a row and KV head.  Few rows may have a piece of
-// every CTA: as many slices as threads fill the GPU with.  (2,048 tokens, half of them there, 24 heads on 4: 76 us with 64 dims a CTA, so ???; one token, 16 heads on 2, 8,192
-// rows: 17.5 us with four slices, so ???.)
+// every CTA: more slices (2,048 tokens, half of them there, 24 heads on 4: 76 us with 64 dims a CTA and every list read anew, so 35; one token, 16 heads on 2, 8,192 rows: 17.5 us
+// with four slices, so 12; caches cold).
 template <int HD, int kSlices, int kQuads>
 __global__ void __launch_bounds__(256 * (kSlices > 4 ? 4 : kSlices)) tree_merge_kernel(const Params<true> p, const Layout L, uint8_t* scratch) {
   constexpr int U = kQuads == 1 ? 4 : 2, kParts = HD / (64 * kQuads);   // U: pieces requested together

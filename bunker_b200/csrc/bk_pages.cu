@@ -1,6 +1,7 @@
-// bk_pages.cu -- a cache in pages: copying, forking, growing, freeing and compacting (bkPages in bunker_cuda.h has the rules).
+// bk_pages.cu -- a cache in pages: copying, forking, growing, freeing and compacting, maps of a step, and which drafted rows stay (bkPages in bunker_cuda.h
+// has the rules).
 //
-// No counterpart in the reference (one contiguous buffer of 128 rows, src/emitters.ts:202).  Each call is one or two launches: a plan by
+// No counterpart in the reference (one contiguous buffer of 128 rows, src/emitters.ts:202).  Each call that gives out or moves pages is one or two launches: a plan by
 // one CTA, which owns the order in which free pages are given out, then the copies by the whole GPU.  Everything is integer and
 // independent of the order in which threads run, so results are reproducible to the bit.
 #include <string.h>
@@ -335,7 +336,8 @@ struct BatchParams {
 };
 
 // Maps of a batch: a CTA row per sequence, its CTAs share the table; the nodes are the first one's, a thread each.  A node's ancestors have lower numbers, so a walk up
-// the tree writes the words of its mask from the last to the first, each once.  Bound: latency, of a chain of loads (list, length, table) and the walk.
+// the tree writes the words of its mask from the last to the first, each once.  Bound: latency, of a chain of loads (list, length, table) and the walk; a call of one sequence 5.0 us, of
+// 256 with tables of 2,048 pages and trees of up to 64 nodes 5.2: the host's launch.
 __global__ void __launch_bounds__(kCopyThreads) pages_batch_kernel(const Pool p, const BatchParams a) {
   __shared__ int parent_s[kMaxNodes];
   bk_pdl_wait();
@@ -414,8 +416,8 @@ struct CommitParams {
 // the children.  Then the CTAs' warps move rows: a warp has 512 bytes of a row of one head and plane, of all rows that move, which it takes in order (row i of the
 // tree is written after it was read, since a path's node i has a number of at least i).  What the others still read (table, counts, lengths) is changed by the
 // first CTA behind the cluster's barrier; other sequences read none of it, for pages of a tree belong to one sequence alone.  Bound: latency of the chain list, length,
-// pages, counts, rows; the tree is asked for ahead of it and the pages are kept (one sequence, with the call that makes room: ??? us; 64 of up to 64 nodes, 32 planes of 4 heads, 11.7 MB:
-// ???).
+// pages, counts, rows; the tree is asked for ahead of it and the pages are kept (with the call that makes room: one sequence 9.0 us; 64 of up to 64 nodes, 32 planes of 4 heads, 11.7 MB: 15.2 us, with the tree
+// and pages read where they are needed 17.8, with a CTA a sequence 25).
 __global__ void __launch_bounds__(kCopyThreads) pages_commit_kernel(const Pool p, const CommitParams a) {
   __shared__ int child_s[kMaxNodes], path_s[kMaxNodes], target_s[kMaxNodes], page_s[kMaxNodes + 1], n_s, refused_s;
   constexpr int kEach = kMaxNodes / kCopyThreads;
