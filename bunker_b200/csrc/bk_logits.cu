@@ -307,9 +307,11 @@ __global__ void __launch_bounds__(kThreads, 2) adjust_logits_kernel(const __grid
       const int u = node_s[j] >> 16;
       if ((node_s[j] & 0xffff) == o) said_here += __ldg(p.path + row * p.path_words + (u >> 5)) >> (u & 31) & 1u;
     }
+    const bool penalised = said_here || w & kInPrompt;
+    if (!penalised && __float_as_uint(sum_s[i]) == 0x80000000u) continue;   // (drafted elsewhere in the tree)
     float* x = x0 + t * next + token;
     float y = __ldcg(x);
-    if (said_here || w & kInPrompt) y = adjusted(y, taken(said_here, a), a);
+    if (penalised) y = adjusted(y, taken(said_here, a), a);
     *x = __fadd_rn(y, sum_s[i]);
   }
 }

@@ -265,6 +265,13 @@ def test_trees_of_many_row_tiles(bk):
     TreeCase(73, 300, 3, 64, [3 + i % 40 for i in range(300)], Hq=4, Hkv=4, HD=128, fused=False).check(1)                                             # 1,200 jobs and more
 
 
+def test_trees_of_more_sequences_than_are_packed(bk):
+    """From 1,025 sequences on ready queries lie T to a sequence."""
+    TreeCase(74, 1100, 2, 0, [2 + i % 7 for i in range(1100)], new=[2 - (i % 5 == 0) - (i % 11 == 0) for i in range(1100)], Hq=1, Hkv=1, HD=128, fused=False).check(1)
+    TreeCase(75, 1030, 1, 48, [1 + i % 3 for i in range(1030)], new=[int(i % 4 != 1) for i in range(1030)], Hq=2, Hkv=1, HD=128, fused=True).check(1)
+    TreeCase(76, 1024, 2, 32, [2 + i % 3 for i in range(1024)], new=[2 - i % 3 for i in range(1024)], Hq=1, Hkv=1, HD=128, fused=False, tree="any").check(1)
+
+
 def test_a_chain_is_what_attention_over_pages_gives(bk):
     """The same rows in the pages, and the same ready queries: each result is within 2^-8 |o| and 2^-13 of the largest |v| of the exact one for these queries."""
     for seed, prefix, fused in ((81, 0, True), (82, 100, True), (83, 64, False)):
@@ -490,6 +497,16 @@ class Logits:
         return got
 
 
+    def check_bits(self):
+        """what nothing names or hides has the bits that it had"""
+        ops.adjust_logits(self.args())
+        assert R.cuSync() == 0, R.last_error()
+        got = self.keep["logits"].download(np.uint32, (self.x.size + 8,))[:self.x.size].reshape(self.x.shape)
+        _, _, named = self.want()
+        assert np.array_equal(got[~named], self.x.view(np.uint32)[~named])
+        return got
+
+
 @pytest.mark.parametrize("V", [1, 2, 31, 33, 127, 1001, 4096, 8191, 8193, 40000, 151936])
 @pytest.mark.parametrize("what", ["history", "bias", "mask", "all"])
 def test_logits_by_vocabulary(bk, V, what):
@@ -558,6 +575,16 @@ def test_logits_that_are_not_finite(bk):
     c.pres[1] = c.freq[1] = 0
     c.bt[1, 1:] = -1
     c.check()
+
+
+def test_a_token_drafted_elsewhere_is_left_as_it_is(bk):
+    """A NaN's own bits, a zero's sign: rows whose path does not hold the token do not touch it."""
+    c = Logits(16, 1, 3, 300, tree=True)
+    c.draft[:] = [7, 8, 9]
+    c.sees[:, 0] = np.array([[1, 0, 0], [1, 1, 0], [1, 0, 1]], bool)
+    c.x.view(np.uint32)[:, 7:10] = [0x7FC12345, 0x80000000, 0xFFC00001]
+    got = c.check_bits()
+    assert (got[[0, 2], 8] == 0x80000000).all() and (got[[0, 1], 9] == 0xFFC00001).all()
 
 
 def test_logits_then_the_argmax_and_a_sample(bk):
