@@ -330,7 +330,7 @@ BK_DEVINL void plan_jobs(const Params<false>& p, const Layout& L, uint8_t* scrat
 // A tree has many rows to a sequence, so most jobs are several row tiles over the same keys.  CTAs come in teams, each of which takes one row tile of the same keys at the
 // same time, so that the keys are read from memory once: a sequence's m row tiles (the common keys' too) are cut into as few teams of up to kTeam tiles as there can be, of
 // equal width but for one tile.  Teams of one width are jobs on a line of their own, which is cut into equal pieces for the line's share of the CTAs; shares are the
-// smallest longest piece.  (32 sequences of up to 16,384 rows and 64 nodes, 24 heads on 4, before the merge of today: teams of one 578 us, of up to two 543, three 520, four 527,
+// smallest longest piece.  (32 sequences of up to 16,384 rows and 64 nodes, 24 heads on 4, with the merge that the calls had then: teams of one 578 us, of up to two 543, three 520, four 527,
 // six 539; 16 behind 8,192 common rows, 16 on 2: 77, 69, 63, 63, 61.)  Only row tiles and tokens that are there have a place; with all of T for each sequence, half of
 // them there, the first took 704 us on one line.  The tiles are 313 us of the 476 that the call takes now; in a loop the power limit sets the clock.
 constexpr int kTeam = 4;
