@@ -24,8 +24,9 @@ constexpr int kMaxTable = 8192;  // entries of a table (of 8 bytes), a quarter o
 constexpr int kBlock = 512;      // tokens that lie together in a slice (64: 3 % slower, where memory is the bound)
 constexpr int kAhead = 1;        // groups of four tokens of the history that a thread asks for before it knows the history's length
 
-// A token's word: how often it was said, whether the last loop has it, whether it is in the prompt.
-constexpr uint32_t kSaid = (1u << 30) - 1, kMarked = 1u << 30, kInPrompt = 1u << 31;
+// A token's word: how often it was said, whether the request names a bias of it again, whether the last loop has it, whether it is in the prompt.
+constexpr uint32_t kSaid = (1u << 29) - 1, kAgain = 1u << 29, kMarked = 1u << 30, kInPrompt = 1u << 31;
+constexpr int kMaxHistory = 1 << 28;
 
 struct LogitsParams {
   float* logits;
@@ -200,8 +201,14 @@ __global__ void __launch_bounds__(kThreads, 2) adjust_logits_kernel(const __grid
     if (i < said) count(h[i], i);
   }
   // marked tokens: who sets a token's mark writes it down
-  auto mark = [&](int o) {
-    if (!(atomicOr(word_s + o, kMarked) & kMarked)) marked_s[atomicAdd(&n_marked_s, 1)] = (uint16_t)o;
+  auto mark = [&](int o, bool bias, float value) {
+    if (!(atomicOr(word_s + o, kMarked) & kMarked)) {
+      const int i = atomicAdd(&n_marked_s, 1);
+      marked_s[i] = (uint16_t)o;
+      sum_s[i] = value;
+    } else if (bias) {
+      atomicOr(word_s + o, kAgain);
+    }
   };
   int m = 0;   // biases of the slice, in the list's order
 #pragma unroll
@@ -220,23 +227,25 @@ __global__ void __launch_bounds__(kThreads, 2) adjust_logits_kernel(const __grid
     if (o >= 0) {
       bias_at_s[at] = (uint16_t)o;
       bias_s[at] = bias_value[k];
-      mark(o);
+      mark(o, true, bias_value[k]);
     }
   }
+  if (p.bias_ld && p.path) __syncthreads();   // (a token that has a bias too is marked with that)
   if (p.path) {
 #pragma unroll
     for (int k = 0; k < kMaxNodes / kThreads; k++) {
       const int u = tid + k * kThreads, o = u < p.T ? place(draft[k]) : -1;
       if (o >= 0) {
         node_s[atomicAdd(&n_node_s, 1)] = u << 16 | o;
-        mark(o);
+        mark(o, false, -0.0f);   // (adds nothing, not even to a zero's sign)
       }
     }
   }
   __syncthreads();
   const int marked = n_marked_s, nodes = n_node_s;
-  for (int i = tid; i < marked; i += kThreads) {   // the sum of a marked token's biases, in the list's order
+  for (int i = tid; i < marked; i += kThreads) {   // several biases of a token: their sum, in the list's order
     const int o = marked_s[i];
+    if (!(word_s[o] & kAgain)) continue;
     float y = 0.0f;
     bool any = false;
     for (int j = 0; j < m; j++)
@@ -244,7 +253,7 @@ __global__ void __launch_bounds__(kThreads, 2) adjust_logits_kernel(const __grid
         y = any ? __fadd_rn(y, bias_s[j]) : bias_s[j];
         any = true;
       }
-    sum_s[i] = any ? y : -0.0f;   // (adds nothing, not even to a zero's sign)
+    sum_s[i] = y;
   }
   if (said) {   // the others that are named: a warp's in one piece
     for (int q0 = warp * 32; q0 < p.slice / 4; q0 += kThreads) {
@@ -328,7 +337,7 @@ extern "C" int32_t bkAdjustLogits(const bkLogitsArgs* args) {
   BK_ARG(a.n_seqs >= 0, "bkAdjustLogits: n_seqs=%d", a.n_seqs);
   BK_ARG(((a.seqs | a.history | a.hist_len | a.prompt_len | a.repetition | a.presence | a.frequency | a.draft | a.path | a.bias_token | a.bias_value | a.bias_n | a.allowed | a.mask_id) & 3) == 0,
          "bkAdjustLogits: all arrays are of 32-bit words");
-  BK_ARG(!a.history || (a.hist_len && a.history_ld > 0 && a.history_ld <= (1 << 29)), "bkAdjustLogits: history needs hist_len and history_ld (%d; 1 to 2^29)", a.history_ld);
+  BK_ARG(!a.history || (a.hist_len && a.history_ld > 0 && a.history_ld <= kMaxHistory), "bkAdjustLogits: history needs hist_len and history_ld (%d; 1 to 2^28)", a.history_ld);
   BK_ARG((a.path != 0) == (a.draft != 0) && (!a.path || a.path_words >= (a.T + 31) / 32), "bkAdjustLogits: draft and path go together, path_words=%d for %d nodes", a.path_words, a.T);
   BK_ARG((a.bias_token != 0) == (a.bias_value != 0) && (a.bias_token != 0) == (a.bias_n != 0) && (!a.bias_token || (a.bias_ld > 0 && a.bias_ld <= BK_LOGITS_MAX_BIAS)),
          "bkAdjustLogits: bias_token, bias_value and bias_n go together, bias_ld=%d (1 to %d)", a.bias_ld, BK_LOGITS_MAX_BIAS);
@@ -340,7 +349,8 @@ extern "C" int32_t bkAdjustLogits(const bkLogitsArgs* args) {
                     a.n_masks, a.allowed_words, 0, 0, 0, 0, 0, 0, a.ld ? a.ld : a.V};
   if (!a.bias_token) p.bias_ld = 0;
   // Who names: slices of at most 8,192 words (48 KB with the list; 512 rows behind 16,000 tokens 117 us, with twice as many words 118), shorter while that leaves SMs without a
-  // CTA, to 1,024; then rows apart, until each SM has two (111 us; with four 117, none apart 159).  Where such a slice has more than 4,096 words and the request's tokens fit a table,
+  // CTA, to 1,024; then rows apart, until each SM has two (111 us; with four 117, none apart 159), but no
+  // fewer rows than half the slices, each of which counts the whole history (4 requests, 10 rows behind 6,000 tokens, 32 slices: 13.8 us with four rows a CTA, 10.1 with ten).  Where such a slice has more than 4,096 words and the request's tokens fit a table,
   // fewer CTAs with a table each (64 requests, 5,000 tokens of 151,936: 25 us with slices of words, 15 with four tables; one request, 700 tokens: 4.6 with 128 slices of
   // words, 5.2 with as many tables).
   // Who hides: four CTAs an SM, no more than have 4,096 tokens each.
@@ -358,7 +368,7 @@ extern "C" int32_t bkAdjustLogits(const bkLogitsArgs* args) {
     while (p.shift > 0 && ((long long)a.B * a.T << (p.shift - 1)) >= sms) p.shift--;
   }
   const long long ctas = (long long)a.B << p.shift;
-  p.parts = (int)std::min<long long>(a.T, (2 * sms + ctas - 1) / ctas);
+  p.parts = (int)std::max<long long>(1, std::min<long long>(std::min<long long>(a.T, (2 * sms + ctas - 1) / ctas), 2ll * a.T >> p.shift));
   p.rows = (a.T + p.parts - 1) / p.parts;
   if (a.allowed) p.hiding = (int)std::max<long long>(1, std::min<long long>(4 * sms, (long long)a.T * a.B * a.V / 4096));
   BK_ARG(ctas * p.parts + p.hiding < (1ll << 31), "bkAdjustLogits: B=%d rows of %d logits: too much for one call", a.B, a.V);
