@@ -85,6 +85,23 @@ BK_DEVINL uint32_t seen_keys(const uint32_t* bits, const Tree& r, int key) {
   const int i = o >> 5;
   return __funnelshift_r(node_word(bits, r.n, i), node_word(bits, r.n, i + 1), o & 31);
 }
+// The same in two steps: the words as they lie in memory, asked for a tile ahead, and what they say.
+BK_DEVINL uint2 ask_seen(const uint32_t* bits, const Tree& r, int key) {
+  const int i = (key - r.base) >> 5;
+  uint2 w = make_uint2(0, 0);
+  if (i >= 0 && 32 * i < r.n) w.x = __ldg(bits + i);
+  if (i >= -1 && 32 * (i + 1) < r.n) w.y = __ldg(bits + i + 1);
+  return w;
+}
+BK_DEVINL uint32_t tell_seen(uint2 w, const Tree& r, int key) {
+  const int o = key - r.base, i = o >> 5;
+  if (o <= -32) return 0xffffffffu;
+  auto part = [&](uint32_t v, int j) {
+    const int left = r.n - 32 * j;
+    return j < 0 ? 0xffffffffu : left >= 32 ? v : left > 0 ? v & ((1u << left) - 1u) : 0u;
+  };
+  return __funnelshift_r(part(w.x, i), part(w.y, i + 1), o & 31);
+}
 
 template <int PER>
 BK_DEVINL void load_bf16(const uint16_t* src, float (&y)[PER]) {
@@ -199,9 +216,9 @@ BK_DEVINL int4* jobs_of(const Layout& L, uint8_t* scratch) { return reinterpret_
 BK_DEVINL int4* pieces_of(const Layout& L, uint8_t* scratch) { return reinterpret_cast<int4*>(scratch + L.pieces); }
 BK_DEVINL int tiles_of(const Layout& L, int j, int key1) { return (key1 - (j < L.n_p ? 0 : L.P) + kTile - 1) / kTile; }
 // the tiles of a job that starts at s and has n tiles which lie in units [u0, u1): [t0, t1)
-BK_DEVINL void piece_of(int s, int n, int u0, int u1, int* t0, int* t1) {
-  *t0 = max(0, min(n, u0 - s - kOverhead));
-  *t1 = max(0, min(n, u1 - s - kOverhead));
+BK_DEVINL void piece_of(int s, int n, int u0, int u1, int* t0, int* t1, int overhead = kOverhead) {
+  *t0 = max(0, min(n, u0 - s - overhead));
+  *t1 = max(0, min(n, u1 - s - overhead));
 }
 
 // one CTA
@@ -332,8 +349,12 @@ BK_DEVINL void plan_jobs(const Params<false>& p, const Layout& L, uint8_t* scrat
 // equal width but for one tile.  Teams of one width are jobs on a line of their own, which is cut into equal pieces for the line's share of the CTAs; shares are the
 // smallest longest piece.  (32 sequences of up to 16,384 rows and 64 nodes, 24 heads on 4, with the merge that the calls had then: teams of one 578 us, of up to two 543, three 520, four 527,
 // six 539; 16 behind 8,192 common rows, 16 on 2: 77, 69, 63, 63, 61.)  Only row tiles and tokens that are there have a place; with all of T for each sequence, half of
-// them there, the first took 704 us on one line.  The tiles are 313 us of the 476 that the call takes now; in a loop the power limit sets the clock.
+// them there, the first took 704 us on one line.  It takes 455 now, about 300 of them for the tiles; in a loop the power limit sets the clock.
 constexpr int kTeam = 4;
+// What a job's start and end cost, in steps: its queries and masks, the tile at its end whose rows are not seen by all, and the partial result, 4,500 cycles for 128 rows of 256.
+// (In us, at 3, 4, 5, 6 steps.  HD 256: one sequence of 16,384 rows and 64 nodes, 24 heads on 4: 82, 70, 65, 65; the same with 188: 151, 157, 130, 131; 16 behind 8,192 common rows,
+// 16 nodes, 16 on 2: 45.6, 44.2, 44.2, 44.2; 64 of 2,000 and one, 24 on 4: 58.8, 59.1, 59.9, 60.0.  HD 128, 4 of up to 4,300 and 100, 24 on 4: 60.9, 61.7, 64.1, 64.7, and 67.6 at 9.)
+__host__ __device__ constexpr int tree_overhead(int HD) { return HD == 256 ? 5 : 3; }
 // Team job i: {start on its line, job of its first row tile, end of its keys, slot of its first row tile's partial result for team 0}; the slots of a team job's pieces
 // are kTeam-wide steps: slot + w * team + rank, which no two pieces share since i + team grows from piece to piece of a line.  jobs[j] = {.., .., first slot, number and
 // distance of slots}; pieces[2c] = {start and end of CTA c's piece of its line, first team job in it, end of the line's team jobs}, pieces[2c + 1] = {w * team + rank, rank}.
@@ -352,6 +373,7 @@ BK_DEVINL int share_of(int n, int t, int of, int less = 0) {
   return x >> 32 ? (int)(x / of) : (int)((unsigned int)x / (unsigned int)of);
 }
 // one CTA
+template <int HD>
 BK_DEVINL void plan_trees(const Params<true>& p, const Layout& L, uint8_t* scratch) {
   __shared__ int sum_s[2 * kTeam][kPrepThreads / 32], total_s[2 * kTeam];
   __shared__ int teams_s[kTeam + 1], common_s[kTeam + 1], start_s[kPlanned];   // start_s: of the team jobs, as far as they fit
@@ -439,7 +461,7 @@ BK_DEVINL void plan_trees(const Params<true>& p, const Layout& L, uint8_t* scrat
     for (int k = 0; k < kTeam; k++) {
       const int n = teams.of_width(k + 1);
       v[k] += n;
-      v[kTeam + k] += n * (tiles + kOverhead);
+      v[kTeam + k] += n * (tiles + tree_overhead(HD));
     }
   }
   scan(v, 2 * kTeam);
@@ -495,13 +517,13 @@ BK_DEVINL void plan_trees(const Params<true>& p, const Layout& L, uint8_t* scrat
 #pragma unroll
       for (int k = 0; k < kTeam; k++)   // (registers, not indexes)
         if (w == k + 1) {
-          const int at = v[k]++, start = v[kTeam + k], len = tiles + kOverhead, units = total_s[kTeam + k], K = teams_s[k + 1];
+          const int at = v[k]++, start = v[kTeam + k], len = tiles + tree_overhead(HD), units = total_s[kTeam + k], K = teams_s[k + 1];
           v[kTeam + k] += len;
           const int slot = is_common ? slot_p[k] + at * w : slot_s[k] + (at - common_s[k + 1]) * w;
           p.team[list0[k] + at] = make_int4(start, j0 + mt, end, slot);
           // team t has units [units t / K, units (t + 1) / K): unit u is team ((u + 1) K - 1) / units's
           auto team_at = [&](int u) { return share_of(K, u + 1, units, 1); };
-          const int t0 = team_at(start + kOverhead), t1 = team_at(start + len - 1);
+          const int t0 = team_at(start + tree_overhead(HD)), t1 = team_at(start + len - 1);
           for (int r = 0; r < w; r++) jobs[j0 + mt + r] = make_int4(0, 0, slot + t0 * w + r, (t1 - t0 + 1) | w << 16);
           if (list0[k] + at < kPlanned) start_s[list0[k] + at] = start;
         }
@@ -565,7 +587,7 @@ __global__ void __launch_bounds__(kPrepThreads, TREE ? 3 : 0) paged_prepare_kern
   bk_pdl_wait();
   bk_pdl_trigger();
   if (blockIdx.x == 0) {   // (first: it takes longest)
-    if constexpr (TREE) plan_trees(p, L, scratch);
+    if constexpr (TREE) plan_trees<HD>(p, L, scratch);
     else if (L.n_p + L.n_s <= kPlanned) plan_jobs<true>(p, L, scratch);
     else plan_jobs<false>(p, L, scratch);
     return;
@@ -931,7 +953,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
         const int4 team = __ldcg(p.team + j);
         if (team.x >= u1) return false;
         x->q = job_of(p, L, team.y + first.y);
-        piece_of(team.x, (team.z - x->q.key0 + kTile - 1) / kTile, u0, u1, &x->t0, &x->t1);
+        piece_of(team.x, (team.z - x->q.key0 + kTile - 1) / kTile, u0, u1, &x->t0, &x->t1, tree_overhead(HD));
         if (x->t0 >= x->t1) continue;
         x->key1 = team.z;
         x->slot = team.w + first.x;
@@ -1128,7 +1150,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
         bar_wait_warp(smem_u32(o_full + (t & 1)), (t >> 1) & 1, P.status, dead);
         tc_after();
       };
-      for (; next_piece(&x); pieces++) {
+      // (Trees: the next piece is looked up while this one's last output is made; its loads in a row are 1,500 cycles.)
+      bool more = TREE && next_piece(&x);
+      for (; TREE ? more : next_piece(&x); pieces++) {
         const Job q = x.q;
         const int t0 = x.t0, n = x.t1 - t0, key1 = x.key1;
         int b, t, g, limit = 0x7fffffff;   // (lanes without a row: never masked, never read)
@@ -1181,6 +1205,11 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
           sh.odd_from[(pieces + 1) % 3] = 0x7fffffff;
           sh.odd_to[(pieces + 1) % 3] = -1;
         }
+        uint2 ahead = make_uint2(0, 0);
+        if constexpr (TREE) {
+          const int key = q.key0 + t0 * kTile + group * 32;
+          if (mine && key + 32 > limit) ahead = ask_seen(bits, tree, key);
+        }
         // queries into tensor memory, half of the dims a group (the MMAs that read the ones before have completed: their output was there)
         bar_wait_warp(smem_u32(&q_here), pieces & 1, P.status, dead);
         tc_after();
@@ -1209,17 +1238,15 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
         for (int i = 0; i < n; i++, tile++) {
           const int tile_key = q.key0 + (t0 + i) * kTile, there = min(kTile, key1 - tile_key), key = tile_key + group * 32;
           const uint32_t s_at = lanes + C::kS + (tile & 1) * kTile;
-          uint32_t seen = 0xffffffffu;   // of a tree's row, these keys
+          const uint2 nodes = ahead;   // of a tree's row, the words of these keys
           if constexpr (TREE) {
-            if (mine && key + 32 > limit) {   // (ahead of the wait: its loads are on the way meanwhile)
-              seen = seen_keys(bits, tree, key);
-              if (key + 32 > key1) seen &= key >= key1 ? 0u : (1u << (key1 - key)) - 1u;
-            }
+            if (mine && i + 1 < n && key + kTile + 32 > limit) ahead = ask_seen(bits, tree, key + kTile);
           }
           bar_wait_warp(smem_u32(s_full + (tile & 1)), (tile >> 1) & 1, P.status, dead);
           tc_after();
           const bool mixed = tile_key + there > seen_by_all;
-          if (there < kTile || mixed) {   // values past the end count as zeros, whatever the page holds there
+          // values past the end count as zeros, whatever the page holds there; those that are not finite are taken out where some row does not see them
+          auto settle_values = [&]() {
             const int v_pos = stream + stream_v(i, n), v_stage = v_pos % C::kStages;
             bar_wait_warp(smem_u32(full + v_stage), (v_pos / C::kStages) & 1, P.status, dead);
             uint8_t* v_at = ring + (size_t)v_stage * C::kStage;
@@ -1227,9 +1254,10 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
               const int row = there + y / (HD / 8), piece = y % (HD / 8);
               *reinterpret_cast<uint4*>(v_at + (piece >> 3) * (kTile * 128) + row * 128 + (piece & 7) * 16) = make_uint4(0, 0, 0, 0);
             }
-            if (mixed)
-              for (int y = threadIdx.x; y < there * (HD / 8); y += 256) {
+            auto take_out = [&](int from) {
+              for (int y = threadIdx.x; y < there * (HD / 8); y += 256) {   // (the same rows a thread as it looked at)
                 const int row = y / (HD / 8), piece = y % (HD / 8);
+                if (row < from) continue;
                 uint4* at = reinterpret_cast<uint4*>(v_at + (piece >> 3) * (kTile * 128) + row * 128 + (piece & 7) * 16);
                 const uint4 v = *at, w = make_uint4(finite_pair(v.x), finite_pair(v.y), finite_pair(v.z), finite_pair(v.w));
                 if (((v.x ^ w.x) | (v.y ^ w.y) | (v.z ^ w.z) | (v.w ^ w.w)) != 0) {
@@ -1238,13 +1266,45 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
                   atomicMax(&sh.odd_to[odd], tile_key + row);
                 }
               }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            };
+            if constexpr (TREE) {
+              // Most jobs of trees end with such tiles: one look at the rows of the tree (all see those before) with all loads on the way, and no fence where nothing was written.
+              bool wrote = there < kTile;
+              if (mixed) {
+                const int from = max(0, seen_by_all - tile_key);
+                uint32_t some = 0;   // bits 15 and 31 of a sum are set by an exponent of ones
+#pragma unroll
+                for (int z = 0; z < kTile * HD / 8; z += 256) {
+                  const int y = z + threadIdx.x, row = y / (HD / 8), piece = y % (HD / 8);
+                  if (row >= from && row < there) {
+                    const uint4 v = *reinterpret_cast<const uint4*>(v_at + (piece >> 3) * (kTile * 128) + row * 128 + (piece & 7) * 16);
+                    some |= ((v.x & 0x7f807f80u) + 0x00800080u) | ((v.y & 0x7f807f80u) + 0x00800080u) | ((v.z & 0x7f807f80u) + 0x00800080u) | ((v.w & 0x7f807f80u) + 0x00800080u);
+                  }
+                }
+                if (some & 0x80008000u) {
+                  take_out(from);
+                  wrote = true;
+                }
+              }
+              if (wrote) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            } else {
+              if (mixed) take_out(0);
+              asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            }
             __syncwarp();
-          }
+          };
+          // Trees: beside the probabilities, which need no values: 1,250 cycles a tile instead of 2,900 ahead of them, with the look above (16 sequences of 16 nodes: 49 to 45 us).
+          const bool settle = there < kTile || mixed;
+          if (!TREE && settle) settle_values();
           if (warp_on) {
             uint32_t s[32];
             tmem_ld32(s_at + group * 32, s);
             if (!__all_sync(0xffffffffu, key + 32 <= limit)) {
+              uint32_t seen = 0xffffffffu;
+              if (TREE && mine) {
+                seen = tell_seen(nodes, tree, key);
+                if (key + 32 > key1) seen &= key >= key1 ? 0u : (1u << (key1 - key)) - 1u;
+              }
 #pragma unroll
               for (int y = 0; y < 32; y++) s[y] = (TREE ? (seen >> y & 1u) != 0u : key + y < limit) ? s[y] : 0xff800000u;
             }
@@ -1297,17 +1357,20 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
             tmem_st16(s_at + 32 + group * 16, lo);
             tmem_wait_st();
           }
+          if (TREE && settle) settle_values();   // (a tree's rows are the last tiles of most jobs: their values come while probabilities are made)
           tc_before();
           __syncwarp();
           if (lane == 0) bar_arrive(smem_u32(p_full + (tile & 1)));
         }
         stream += 2 * n;
+        const size_t x_slot = x.slot;
+        if (TREE) more = next_piece(&x);
         // the piece's part of the result, half of the dims a group
         wait_output(tile - 1);
         if (warp_on) {
           const bool common = q.seq < 0;
           const int rows = common ? kRows : L.rows_s;
-          const size_t slot = x.slot * rows;
+          const size_t slot = x_slot * rows;
           float* ml = reinterpret_cast<float*>(P.scratch + (common ? L.ml_p : L.ml_s)) + (slot + i_row) * 4;
           uint4* o_to = reinterpret_cast<uint4*>(P.scratch + (common ? L.o_p : L.o_s)) + slot * (HD / 4) + i_row;   // [HD / 4][rows] x 4 dims: lanes side by side
           if (mine) {
@@ -1674,7 +1737,7 @@ int32_t read_args(const char* what, const bkPagedAttnArgs& a, P* out, Layout* la
   p.max_rows = (int)std::min<long long>(a.max_len, (long long)a.max_pages * a.page_rows); p.fused = a.fused_norm_rope != 0; p.scale = a.scale; p.eps = a.eps;
   Layout& L = *layout;
   L = make_layout(a.B, a.T, a.Hq, a.Hkv, a.HD, a.prefix_rows, a.page_rows, bk_ctx().sm_count);
-  BK_ARG((long long)(L.n_p + L.n_s) * ((long long)p.max_rows / kTile + 1 + kOverhead) < (1ll << 31), "%s: B=%d T=%d Hkv=%d with %d rows a sequence: too much for one call", what, a.B,
+  BK_ARG((long long)(L.n_p + L.n_s) * ((long long)p.max_rows / kTile + 1 + 16 * kOverhead) < (1ll << 31), "%s: B=%d T=%d Hkv=%d with %d rows a sequence: too much for one call", what, a.B,
          a.T, a.Hkv, p.max_rows);
   return BK_OK;
 }
