@@ -1737,7 +1737,8 @@ int32_t read_args(const char* what, const bkPagedAttnArgs& a, P* out, Layout* la
   p.max_rows = (int)std::min<long long>(a.max_len, (long long)a.max_pages * a.page_rows); p.fused = a.fused_norm_rope != 0; p.scale = a.scale; p.eps = a.eps;
   Layout& L = *layout;
   L = make_layout(a.B, a.T, a.Hq, a.Hkv, a.HD, a.prefix_rows, a.page_rows, bk_ctx().sm_count);
-  BK_ARG((long long)(L.n_p + L.n_s) * ((long long)p.max_rows / kTile + 1 + 16 * kOverhead) < (1ll << 31), "%s: B=%d T=%d Hkv=%d with %d rows a sequence: too much for one call", what, a.B,
+  const int overhead = std::is_same<P, Params<true>>::value ? tree_overhead(a.HD) : kOverhead;
+  BK_ARG((long long)(L.n_p + L.n_s) * ((long long)p.max_rows / kTile + 1 + overhead) < (1ll << 31), "%s: B=%d T=%d Hkv=%d with %d rows a sequence: too much for one call", what, a.B,
          a.T, a.Hkv, p.max_rows);
   return BK_OK;
 }

@@ -357,6 +357,7 @@ __global__ void __launch_bounds__(kCopyThreads) pages_batch_kernel(const Pool p,
   if (a.ok && a.ok[i] == 0) n = 0;
   const int base = len - n;
   if (base < 0) n = 0;
+  __syncthreads();   // (count may be what n_new or ok was read from)
   if (a.count && threadIdx.x == 0) a.count[i] = n;
   if (!a.pos && !a.slot && !a.mask) return;
   if (a.parent) {
@@ -676,6 +677,9 @@ int32_t bkPagesCommit(const bkPages* pool, const bkPagesCommitArgs* args) {
   BK_ARG(a.T >= 1 && a.T <= kMaxNodes, "bkPagesCommit: T=%d (1 to %d)", a.T, kMaxNodes);
   BK_ARG(a.n == 0 || (a.parent && a.token && a.target), "bkPagesCommit: parent, token and target must be non-null int32 arrays");
   BK_ARG(((a.n_new | a.parent | a.token | a.target | a.path | a.n_path | a.next | a.ok | a.history | a.hist_len) & 3) == 0, "bkPagesCommit: all arrays are of int32");
+  for (const uint64_t result : {a.path, a.n_path, a.next, a.ok})   // (a cluster's CTAs read while the first writes)
+    BK_ARG(result == 0 || (result != a.seqs && result != a.n_new && result != a.parent && result != a.token && result != a.target),
+           "bkPagesCommit: path, n_path, next and ok must lie apart from what the call reads");
   BK_ARG((a.history != 0) == (a.hist_len != 0) && (!a.history || a.history_ld > 0), "bkPagesCommit: history and hist_len go together (history_ld=%d)", a.history_ld);
   if (a.n == 0) return BK_OK;
   const CommitParams c = {bk_ptr<int>(a.seqs), bk_ptr<int>(a.n_new), bk_ptr<int>(a.parent), bk_ptr<int>(a.token), bk_ptr<int>(a.target), bk_ptr<int>(a.path), bk_ptr<int>(a.n_path),

@@ -352,7 +352,8 @@ BK_API uint64_t bkPagedAttnScratchBytes(int32_t B, int32_t T, int32_t Hq, int32_
  *   mask   uint32 [T][n][mask_words]: bit u is set for the nodes u of the node's path, itself among them
  * parent int32 [T][n]: the node that it continues, -1 (or any that is not an earlier node): none; parent = 0: each token continues the one before.
  * n_new int32 [n]: how many of a sequence's rows are new, 0..T (less than 0 counts as 0, more than T as T); 0 = T of each.  ok int32 [n] (0 = all): what bkPagesGrow
- * said; where it is 0 the sequence got no room and has no new rows.  count int32 [n] gets how many it has then, which the attention and bkPagesCommit take as n_new.
+ * said; where it is 0 the sequence got no room and has no new rows.  count int32 [n] gets how many it has then, which the attention and bkPagesCommit take as n_new
+ * (it may be the array of n_new or ok; the other results lie apart from what the call reads).
  * A token t >= count, or of a sequence that has fewer than n_new rows (count 0), is not there: pos and slot are -1, its mask 0.  An entry that names no sequence has no rows.  The
  * same sequence may be in the list twice.  The pool is not changed. */
 typedef struct bkPagesBatchArgs {
@@ -413,6 +414,7 @@ BK_API int32_t bkAdjustLogits(const bkLogitsArgs* args);
  *   path int32 [T][n]: nodes of the path, -1 behind it (0 = not wanted); n_path int32 [n]; next int32 [n]: the target of the last (a token without a row yet)
  *   history int32 [n_seqs][history_ld], hist_len int32 [n_seqs] (0 = none): the tokens of the path are appended, node 0's first.  A history is then what has rows; next
  *   comes with the next tree, as its node 0 (and bkAdjustLogits counts it with the path, not twice)
+ * path, n_path, next and ok lie apart from what the call reads.
  * ok[i] (0 to skip): 1, or 0 where nothing is changed, n_path is 0, next and path are -1: the entry names no sequence or one named before, n_new[i] is not
  * in 1..T, the sequence has fewer rows, a page that holds rows of its tree is shared (or none of the pool's), or its history has no room (or a length below 0). */
 typedef struct bkPagesCommitArgs {

@@ -114,6 +114,25 @@ def test_batch_gives_what_is_asked_for(bk):
     assert pos.download(np.int32, (2,)).tolist() == [38, 39] and lens.download(np.int32, (1,)).tolist() == [40]
 
 
+@pytest.mark.parametrize("place", ["n_new", "ok"])
+def test_batch_counts_in_place(bk, place):
+    rng = np.random.default_rng(6)
+    p = Pool(rng, n_pages=600, seqs=8, max_pages=66)
+    order = list(rng.permutation(600))
+    for s in range(8):
+        p.own(s, 150 * s, order)
+    pool = p.upload()
+    seqs = dev(np.tile(np.arange(8, dtype=np.int32), 32))
+    for _ in range(20):
+        d = {"n_new": dev(np.full(256, 2000, np.int32)), "ok": dev(np.full(256, 3, np.int32))}
+        slot = R.DeviceBuffer.from_numpy(np.full(300 * 256, 77, np.int32))
+        pool.batch(seqs.ptr, 256, T=300, n_new=d["n_new"].ptr, ok=d["ok"].ptr, count=d[place].ptr, slot=slot.ptr)
+        want = np.where(150 * (np.arange(256) % 8) >= 300, 300, 0)
+        assert np.array_equal(d[place].download(np.int32, (256,)), want)
+        assert np.array_equal((slot.download(np.int32, (300, 256)) >= 0).sum(0), want)
+    p.check("unchanged")
+
+
 def test_batch_of_a_full_list_with_long_tables(bk):
     rng = np.random.default_rng(6)
     p = Pool(rng, planes=1, n_pages=5000, heads=1, rows=2, row_vals=8, seqs=1100, max_pages=3001)
@@ -826,6 +845,9 @@ def test_maps_and_commit_refuse_what_they_cannot_do(bk):
     commit("parent", token=0)
     commit("parent", target=0)
     commit("arrays", ok=a.ptr + 1)
+    for result in ("path", "n_path", "next", "ok"):
+        commit("apart", **{result: a.ptr})
+        commit("apart", **{result: a.ptr + 64, "n_new": a.ptr + 64})
     commit("history", history=a.ptr)
     commit("history", hist_len=a.ptr)
     commit("history", history=a.ptr, hist_len=a.ptr)
