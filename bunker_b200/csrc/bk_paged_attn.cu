@@ -349,7 +349,7 @@ BK_DEVINL void plan_jobs(const Params<false>& p, const Layout& L, uint8_t* scrat
 // equal width but for one tile.  Teams of one width are jobs on a line of their own, which is cut into equal pieces for the line's share of the CTAs; shares are the
 // smallest longest piece.  (32 sequences of up to 16,384 rows and 64 nodes, 24 heads on 4, with the merge that the calls had then: teams of one 578 us, of up to two 543, three 520, four 527,
 // six 539; 16 behind 8,192 common rows, 16 on 2: 77, 69, 63, 63, 61.)  Only row tiles and tokens that are there have a place; with all of T for each sequence, half of
-// them there, the first took 704 us on one line.  It takes 455 now, about 300 of them for the tiles; in a loop the power limit sets the clock.
+// them there, the first took 704 us on one line.  It takes 449 to 469 now, about 300 of them for the tiles; in a loop the power limit sets the clock.
 constexpr int kTeam = 4;
 // What a job's start and end cost, in steps: its queries and masks, the tile at its end whose rows are not seen by all, and the partial result, 4,500 cycles for 128 rows of 256.
 // (In us, at 3, 4, 5, 6 steps.  HD 256: one sequence of 16,384 rows and 64 nodes, 24 heads on 4: 82, 70, 65, 65; the same with 188: 151, 157, 130, 131; 16 behind 8,192 common rows,
@@ -1293,7 +1293,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
             }
             __syncwarp();
           };
-          // Trees: beside the probabilities, which need no values: 1,250 cycles a tile instead of 2,900 ahead of them, with the look above (16 sequences of 16 nodes: 49 to 45 us).
+          // Trees: beside the probabilities, which need no values: 1,250 cycles a tile instead of 2,900 ahead of them, with the look above (16 sequences of 16 nodes: 49 to 46 us).
           const bool settle = there < kTile || mixed;
           if (!TREE && settle) settle_values();
           if (warp_on) {
