@@ -410,7 +410,7 @@ __global__ void __launch_bounds__(kCopyThreads) pages_batch_kernel(const Pool p,
 struct CommitParams {
   const int *seqs, *n_new, *parent, *token, *target;
   int *path, *n_path, *next, *ok, *history, *hist_len;
-  int n, T, history_ld;
+  int n, T, history_ld, values;
 };
 
 // A cluster of CTAs per sequence.  Each finds the path for itself: every node that the model agrees with tells its parent, the lowest child stays, and one thread follows
@@ -433,7 +433,9 @@ __global__ void __launch_bounds__(kCopyThreads) pages_commit_kernel(const Pool p
     if (t >= a.T) break;
     parent[k] = a.parent[(size_t)t * a.n + i];
     token[k] = a.token[(size_t)t * a.n + i];
-    target_s[t] = a.target[(size_t)t * a.n + i];
+    const int target = a.target[(size_t)t * a.n + i];
+    // (-inf: the best of what a grammar left, which is nothing)
+    target_s[t] = a.values && a.target[(size_t)(a.T + t) * a.n + i] == (int)0xff800000u ? -1 : target;
     child_s[t] = kMaxNodes;
   }
   bool bad = false;
@@ -454,7 +456,7 @@ __global__ void __launch_bounds__(kCopyThreads) pages_commit_kernel(const Pool p
   for (int k = 0; k < kEach; k++) {
     const int t = tid + k * kCopyThreads;
     if (t >= a.T) break;
-    if (good && t >= 1 && t < n && parent[k] >= 0 && parent[k] < t && token[k] == target_s[parent[k]]) atomicMin(child_s + parent[k], t);
+    if (good && t >= 1 && t < n && parent[k] >= 0 && parent[k] < t && token[k] >= 0 && token[k] == target_s[parent[k]]) atomicMin(child_s + parent[k], t);
   }
   __syncthreads();
   if (tid == 0) {
@@ -680,10 +682,11 @@ int32_t bkPagesCommit(const bkPages* pool, const bkPagesCommitArgs* args) {
   for (const uint64_t result : {a.path, a.n_path, a.next, a.ok})   // (a cluster's CTAs read while the first writes)
     BK_ARG(result == 0 || (result != a.seqs && result != a.n_new && result != a.parent && result != a.token && result != a.target),
            "bkPagesCommit: path, n_path, next and ok must lie apart from what the call reads");
+  BK_ARG(a.values == 0 || a.values == 1, "bkPagesCommit: values=%d (0 or 1)", a.values);
   BK_ARG((a.history != 0) == (a.hist_len != 0) && (!a.history || a.history_ld > 0), "bkPagesCommit: history and hist_len go together (history_ld=%d)", a.history_ld);
   if (a.n == 0) return BK_OK;
   const CommitParams c = {bk_ptr<int>(a.seqs), bk_ptr<int>(a.n_new), bk_ptr<int>(a.parent), bk_ptr<int>(a.token), bk_ptr<int>(a.target), bk_ptr<int>(a.path), bk_ptr<int>(a.n_path),
-                          bk_ptr<int>(a.next), bk_ptr<int>(a.ok), bk_ptr<int>(a.history), bk_ptr<int>(a.hist_len), a.n, a.T, a.history_ld};
+                          bk_ptr<int>(a.next), bk_ptr<int>(a.ok), bk_ptr<int>(a.history), bk_ptr<int>(a.hist_len), a.n, a.T, a.history_ld, a.values};
   // CTAs a sequence: as many as its warps have runs of rows for, at most 8 (a cluster) and four an SM
   const long long items = (long long)p.n_planes * p.heads * ((p.row_bytes / 16 + 31) / 32);
   int ranks = 1;

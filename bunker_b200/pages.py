@@ -61,7 +61,8 @@ class PagePool:
         _check(cu().bkPagesBatch(C.byref(self.desc), C.byref(R.bkPagesBatchArgs(seqs, n_new, parent, table, lens, pos, slot, mask, ok, count, n, T, mask_words))))
 
     def commit(self, seqs: int, n: int, *, T: int, parent: int, token: int, target: int, n_new: int = 0, path: int = 0, n_path: int = 0, next: int = 0,
-               ok: int = 0, history: int = 0, hist_len: int = 0, history_ld: int = 0) -> None:
-        """Of every drafted tree the path that agrees with target stays, the rest of its rows are given up (bkPagesCommit)."""
+               ok: int = 0, history: int = 0, hist_len: int = 0, history_ld: int = 0, values: bool = False) -> None:
+        """Of every drafted tree the path that agrees with target stays, the rest of its rows are given up (bkPagesCommit).  values: the targets' logits lie behind
+        them, and one of -inf is no target."""
         _check(cu().bkPagesCommit(C.byref(self.desc), C.byref(R.bkPagesCommitArgs(seqs, n_new, parent, token, target, path, n_path, next, ok, history, hist_len,
-                                                                                   n, T, history_ld))))
+                                                                                   n, T, history_ld, int(values)))))

@@ -98,7 +98,7 @@ class bkLogitsArgs(C.Structure):
 
 class bkPagesCommitArgs(C.Structure):
     _fields_ = [(n, C.c_uint64) for n in ("seqs", "n_new", "parent", "token", "target", "path", "n_path", "next", "ok", "history", "hist_len")] + \
-               [(n, C.c_int32) for n in ("n", "T", "history_ld", "reserved")]
+               [(n, C.c_int32) for n in ("n", "T", "history_ld", "values")]
 
 
 class bkLoraSeg(C.Structure):

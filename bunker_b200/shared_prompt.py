@@ -168,16 +168,17 @@ class SharedPrompt:
         self.nodes = T
         return self._layer(x, T * self.n, self.n, T, 1, self.b_count.ptr, [a for _ in range(T) for a in adapters], self.prompt_rows if share and new[0] else 0, tree=True)
 
-    def keep(self, token: np.ndarray, target: int) -> tuple[np.ndarray, np.ndarray]:
+    def keep(self, token: np.ndarray, target: int, values: bool = False) -> tuple[np.ndarray, np.ndarray]:
         """Of the trees of ``draft``, whose tokens are token int [T][requests], the paths that agree with target (device int32 [T * requests], the model's token after each
-        node) stay.  Waits for the answer: (how many nodes of each request stayed, the token that follows them); 0 and -1 for requests without nodes."""
+        node) stay.  values: the logits of those tokens lie behind them (f32 [T * requests]), and one of -inf is no token.  Waits for the answer: (how many nodes of each request stayed, the
+        token that follows them, -1 where there is none); 0 and -1 for requests without nodes."""
         if not self.nodes:
             raise RuntimeError("no drafted trees")
         token = np.ascontiguousarray(token, np.int32)
         if token.shape != (self.nodes, self.n):
             raise ValueError(f"tokens {token.shape} of {self.nodes} nodes for {self.n} requests")
         self.pool.commit(self._list("seqs", np.arange(1, self.n + 1)), self.n, T=self.nodes, n_new=self.b_count.ptr, parent=self.lists["parent"].ptr,
-                         token=self._list("token", token.reshape(-1)), target=target, path=self.path.ptr, n_path=self.n_path.ptr, next=self.next.ptr)
+                         token=self._list("token", token.reshape(-1)), target=target, path=self.path.ptr, n_path=self.n_path.ptr, next=self.next.ptr, values=values)
         self.nodes = 0
         return self.n_path.download(np.int32, (self.n,)), self.next.download(np.int32, (self.n,))
 

@@ -372,12 +372,12 @@ export function adjustLogits(a: AdjustLogits): void {
 /** What the model agrees with stays (bkPagesCommitArgs, 104 bytes): the longest path of every drafted tree. */
 export interface PagesCommit {
   seqs: bigint; nNew?: bigint; parent: bigint; token: bigint; target: bigint; path?: bigint; nPath?: bigint; next?: bigint; ok?: bigint; history?: bigint; histLen?: bigint;
-  n: number; T: number; historyLd?: number;
+  n: number; T: number; historyLd?: number; values?: boolean;
 }
 export function pagesCommit(pool: Buffer, a: PagesCommit): void {
   const b = Buffer.alloc(104);
   [a.seqs, a.nNew, a.parent, a.token, a.target, a.path, a.nPath, a.next, a.ok, a.history, a.histLen].forEach((v, i) => b.writeBigUInt64LE(v ?? 0n, 8 * i));
-  [a.n, a.T, a.historyLd ?? 0].forEach((v, i) => b.writeInt32LE(v, 88 + 4 * i));
+  [a.n, a.T, a.historyLd ?? 0, a.values ? 1 : 0].forEach((v, i) => b.writeInt32LE(v, 88 + 4 * i));
   check(cu().bkPagesCommit(pool, b), "bkPagesCommit");
 }
 

@@ -386,7 +386,9 @@ BK_API uint64_t bkTreeAttnScratchBytes(int32_t B, int32_t T, int32_t Hq, int32_t
  * n = how often v stands in the request's history behind its prompt, plus how often on the row's path (whose tokens the history does not hold yet):
  *   x = logits[v];   if v stands in the history or on the path:  x = x > 0 ? x / repetition : x * repetition,  x -= frequency * n + presence * [n > 0];
  *   x += bias of v (a token that a request names several times gets the sum, in the list's order);   x = -inf where the row's mask does not allow v.
- * A logit that nothing names or hides is neither read nor written.  NaN stays NaN where it is allowed. */
+ * A logit that nothing names or hides is neither read nor written.  NaN stays NaN where it is allowed.
+ * A row whose mask allows no token is -inf throughout.  bkArgmax and bkSample still name one of its tokens (bkArgmax token 0), with val -inf: that val says that
+ * there is none, and bkPagesCommit with `values` takes it so. */
 #define BK_LOGITS_MAX_BIAS 1024
 typedef struct bkLogitsArgs {
   uint64_t logits;
@@ -409,7 +411,9 @@ typedef struct bkLogitsArgs {
 BK_API int32_t bkAdjustLogits(const bkLogitsArgs* args);
 
 /* What the model agrees with stays.  target int32 [T][n] is the model's token after each node, token int32 [T][n] the node's own.  From node 0 the path
- * goes on to the lowest child whose token is the target of the node before, as long as there is one.  The rows of the path move up
+ * goes on to the lowest child whose token is the target of the node before, as long as there is one.  A target below 0 is no token: no child's is the same, and next
+ * says it.  With values = 1 the logits of the targets (bkArgmax's or bkSample's val) lie right behind them, f32 [T][n]; a target whose logit is -inf counts as -1 (a row
+ * whose grammar allows nothing).  The rows of the path move up
  * behind the rows before the tree, in all planes; the others are given up, with the pages that only they had.
  *   path int32 [T][n]: nodes of the path, -1 behind it (0 = not wanted); n_path int32 [n]; next int32 [n]: the target of the last (a token without a row yet)
  *   history int32 [n_seqs][history_ld], hist_len int32 [n_seqs] (0 = none): the tokens of the path are appended, node 0's first.  A history is then what has rows; next
@@ -419,10 +423,11 @@ BK_API int32_t bkAdjustLogits(const bkLogitsArgs* args);
  * in 1..T, the sequence has fewer rows, a page that holds rows of its tree is shared (or none of the pool's), or its history has no room (or a length below 0). */
 typedef struct bkPagesCommitArgs {
   uint64_t seqs, n_new;  /* int32 [n]; n_new 0 = T of each */
-  uint64_t parent, token, target;
+  uint64_t parent, token, target; /* values = 1: target is [T][n] tokens, then [T][n] logits */
   uint64_t path, n_path, next, ok;
   uint64_t history, hist_len;
-  int32_t n, T, history_ld, reserved; /* T 1..1024 */
+  int32_t n, T, history_ld;           /* T 1..1024 */
+  int32_t values;                     /* 0 or 1 */
 } bkPagesCommitArgs;
 BK_API int32_t bkPagesCommit(const bkPages* pool, const bkPagesCommitArgs* args);
 

@@ -1,0 +1,122 @@
+"""Drafted trees where they can go wrong: grammars that allow nothing, results that lie over inputs, calls without counts or without new rows, trees and drafts of many nodes, and the
+attention against bounds that a single hidden or extra node does not stay inside.  Expectations and helpers are those of test_gpu_trees.py.
+"""
+import ctypes as C
+import math
+
+import numpy as np
+import pytest
+
+from bunker_b200 import ops
+from bunker_b200 import runtime as R
+from tests.test_gpu_serving import bf16, i32, rnd, val
+from tests.test_gpu_trees import Draft, Logits, TreeCase, words
+from tests.util import dev
+
+pytestmark = pytest.mark.gpu
+
+
+# ---- grammars that allow nothing, or next to nothing ----------------------------------
+
+@pytest.mark.parametrize("V", [37, 5000, 151936])
+@pytest.mark.parametrize("how", ["argmax", "sample"])
+def test_a_grammar_that_allows_nothing_ends_the_path(bk, V, how):
+    """Rows of -inf: the selection says so by its val, and commit, which is given the vals, keeps no child of such a node although its token is the one that the selection named."""
+    n, T = 4, 5
+    rng = np.random.default_rng(V)
+    c = Logits(V, n, T, V, history=20, n_masks=3)
+    allowed = np.zeros((3, V), bool)
+    allowed[1, rng.permutation(V)[:3]] = True
+    allowed[2] = True
+    c.allowed = words(allowed, c.W)
+    c.allowed[:, -1] = 0xFFFFFFFF                      # (bits behind the vocabulary)
+    c.mask_id = i32(*[(0, -1, 1, 2)[(t + i) % 4 if i else (1, 1, 0, 1, 1)[t]] for t in range(T) for i in range(n)])
+    dead = (c.mask_id == 0).reshape(T, n)
+    got = c.check()
+    assert np.isneginf(got.reshape(T, n, V)[dead]).all() and dead.any(0).any()
+    chosen, a = R.DeviceBuffer(8 * T * n), c.args()
+    ops.adjust_logits(a)
+    if how == "argmax":
+        scratch = R.DeviceBuffer.zeros(ops.argmax_scratch_bytes(T * n))
+        ops.argmax(a.logits, V, T * n, chosen.ptr, chosen.ptr + 4 * T * n, scratch.ptr)
+    else:
+        ops.sample(a.logits, V, T * n, chosen.ptr, chosen.ptr + 4 * T * n, temperature=1.3, top_k=40, seed=3)
+    assert R.cuSync() == 0, R.last_error()
+    idx, logit = chosen.download(np.int32, (2, T, n))[0], chosen.download(np.float32, (2, T, n))[1]
+    assert np.array_equal(np.isneginf(logit), dead) and (idx >= 0).all() and (idx < V).all()
+    p = Draft(rng, n_pages=24, seqs=n)
+    order = list(rng.permutation(24))
+    for s in range(n):
+        p.own(s, 20 + 3 * s, order)
+    p.grown(rng, T, [T] * n)
+    p.parent[:] = np.arange(-1, T - 1)[:, None]
+    p.token[1:] = idx[:-1]                             # every node is what the selection named after its parent
+    pool = p.upload()
+    d = {k: dev(x) for k, x in (("seqs", np.arange(n, dtype=np.int32)), ("parent", p.parent), ("token", p.token))}
+    o = {k: R.DeviceBuffer.from_numpy(np.full(size, 77, np.int32)) for k, size in (("path", T * n), ("n_path", n), ("next", n), ("ok", n))}
+    pool.commit(n=n, T=T, target=chosen.ptr, values=True, **{k: b.ptr for k, b in {**d, **o}.items()})
+    p.target = np.where(dead, -1, idx)
+    want = p.commit(np.arange(n))
+    p.check()
+    for (name, b), w in zip(o.items(), want):
+        assert np.array_equal(b.download(np.int32, w.shape), w), name
+    first = np.where(dead.any(0), dead.argmax(0), T - 1)
+    assert np.array_equal(want[1], first + 1) and np.array_equal(want[2] == -1, dead.any(0))
+
+
+def test_a_target_below_zero_is_no_token(bk):
+    """Also where a node's own token is below zero."""
+    rng = np.random.default_rng(1)
+    p = Draft(rng, seqs=2)
+    p.own(0, 20, [3, 4])
+    p.grown(rng, 4, [4])
+    p.parent[:, 0], p.token[:, 0], p.target[:, 0] = [-1, 0, 0, 1], [5, -1, 8, 9], [-1, 9, 3, 2]
+    pool = p.upload()
+    d = {k: dev(x) for k, x in (("seqs", i32(0)), ("parent", p.parent), ("token", p.token), ("target", p.target))}
+    o = {k: R.DeviceBuffer.from_numpy(np.full(4, 77, np.int32)) for k in ("path", "n_path", "next", "ok")}
+    pool.commit(n=1, T=4, **{k: b.ptr for k, b in {**d, **o}.items()})
+    assert R.cuSync() == 0, R.last_error()
+    got = {k: b.download(np.int32, (4,)).tolist() for k, b in o.items()}
+    assert got == {"path": [0, -1, -1, -1], "n_path": [1, 77, 77, 77], "next": [-1, 77, 77, 77], "ok": [1, 77, 77, 77]}
+    assert p.d["lens"].download(np.int32, (2,)).tolist() == [17, 0]
+    a = R.bkPagesCommitArgs(seqs=d["seqs"].ptr, parent=d["parent"].ptr, token=d["token"].ptr, target=d["target"].ptr, n=1, T=4, values=2)
+    assert R.cu().bkPagesCommit(C.byref(pool.desc), C.byref(a)) == R.BK_ERR_ARG and "values" in R.last_error()
+
+
+@pytest.mark.parametrize("V,few", [(33, 1), (33, 7), (9000, 1), (9000, 5), (151936, 3), (151936, 39)])
+@pytest.mark.parametrize("top_k", [1, 2, 40, 64])
+def test_a_sample_of_fewer_tokens_than_it_may_look_at(bk, V, few, top_k):
+    """A mask that leaves fewer tokens than top_k: only those are ever chosen, whatever the temperature and nucleus."""
+    B, rng = 3, np.random.default_rng(V + few)
+    c = Logits(few, B, 1, V, n_masks=1, history=9)
+    allowed = np.zeros((1, V), bool)
+    allowed[0, rng.permutation(V)[:few]] = True
+    c.allowed, c.mask_id = words(allowed, c.W), i32(0, 0, 0)
+    a = c.args()
+    ops.adjust_logits(a)
+    idx, v = R.DeviceBuffer(4 * B), R.DeviceBuffer(4 * B)
+    seen = set()
+    for step in range(40):
+        ops.sample(a.logits, V, B, idx.ptr, v.ptr, temperature=(0.0, 0.3, 1.0, 50.0)[step % 4], top_k=top_k, top_p=(1.0, 0.9)[step % 2], seed=11, step_add=step)
+        got = idx.download(np.int32, (B,))
+        assert allowed[0, got].all() and np.isfinite(v.download(np.float32, (B,))).all()
+        seen |= set(got.tolist())
+    assert few == 1 or top_k == 1 or len(seen) > 1
+
+
+def test_the_layer_ends_a_path_where_nothing_is_allowed(bk):
+    from bunker_b200 import shared_prompt as S
+    from bunker_b200.model import CONFIG_TINY as cfg
+    w, lora = S.random_layer(cfg, seed=5)
+    s = S.SharedPrompt(cfg, w, lora, 2, 64, 8)
+    x = dev(rnd(np.random.default_rng(1), 64, cfg.hidden))
+    s.prompt(x.ptr, 20)
+    assert s.fork([0, 1]).all()
+    chain = np.array([[-1, -1], [0, 0], [1, 1]], np.int32)
+    token = np.array([[4, 4], [0, 0], [6, 6]], np.int32)
+    target, logit = np.array([[0, 0], [6, 6], [2, 3]], np.int32), np.array([[1.5, -np.inf], [0.0, 1.0], [-2.0, 1.0]], np.float32)
+    for values, kept_want, next_want in ((False, [3, 3], [2, 3]), (True, [3, 1], [2, -1])):
+        s.draft(x.ptr, chain, [-1, -1])
+        d = dev(np.concatenate([target.view(np.uint32), logit.view(np.uint32)]))
+        kept, after = s.keep(token, d.ptr, values=values)
+        assert kept.tolist() == kept_want and after.tolist() == next_want
