@@ -549,6 +549,20 @@ int32_t check_list(const char* what, int32_t n, uint64_t a, uint64_t b) {
   return BK_OK;
 }
 
+// bytes of device memory, none where at is 0
+struct Span {
+  uint64_t at, bytes;
+};
+bool overlap(const Span& a, const Span& b) { return a.at && b.at && a.at < b.at + b.bytes && b.at < a.at + a.bytes; }
+// whether they are part of what a pool holds: its lists and pages (not what lies between planes)
+bool in_pool(const bkPages& pool, const Pool& p, const Span& a) {
+  if (overlap(a, {pool.lens, 4ull * p.n_seqs}) || overlap(a, {pool.table, 4ull * p.n_seqs * p.max_pages}) || overlap(a, {pool.ref, 4ull * p.n_pages})) return true;
+  const unsigned long long plane = p.n_pages * p.page_bytes;
+  for (int i = 0; i < p.n_planes; i++)
+    if (overlap(a, {pool.base + i * p.plane_bytes, plane})) return true;
+  return false;
+}
+
 // CTAs for `items` warps' worth of copying, at most eight an SM
 int copy_ctas(long long items) { return (int)std::max<long long>(1, std::min<long long>((items + kCopyThreads / 32 - 1) / (kCopyThreads / 32), 8ll * bk_ctx().sm_count)); }
 
@@ -679,12 +693,21 @@ int32_t bkPagesCommit(const bkPages* pool, const bkPagesCommitArgs* args) {
   BK_ARG(a.T >= 1 && a.T <= kMaxNodes, "bkPagesCommit: T=%d (1 to %d)", a.T, kMaxNodes);
   BK_ARG(a.n == 0 || (a.parent && a.token && a.target), "bkPagesCommit: parent, token and target must be non-null int32 arrays");
   BK_ARG(((a.n_new | a.parent | a.token | a.target | a.path | a.n_path | a.next | a.ok | a.history | a.hist_len) & 3) == 0, "bkPagesCommit: all arrays are of int32");
-  for (const uint64_t result : {a.path, a.n_path, a.next, a.ok})   // (a cluster's CTAs read while the first writes)
-    BK_ARG(result == 0 || (result != a.seqs && result != a.n_new && result != a.parent && result != a.token && result != a.target),
-           "bkPagesCommit: path, n_path, next and ok must lie apart from what the call reads");
   BK_ARG(a.values == 0 || a.values == 1, "bkPagesCommit: values=%d (0 or 1)", a.values);
   BK_ARG((a.history != 0) == (a.hist_len != 0) && (!a.history || a.history_ld > 0), "bkPagesCommit: history and hist_len go together (history_ld=%d)", a.history_ld);
   if (a.n == 0) return BK_OK;
+  // a cluster's CTAs, and those of other sequences, read while the first writes
+  const uint64_t list = 4ull * a.n, nodes = list * a.T;
+  const Span read[] = {{a.seqs, list}, {a.n_new, list}, {a.parent, nodes}, {a.token, nodes}, {a.target, nodes * (1 + a.values)}};
+  const Span histories[] = {{a.history, 4ull * p.n_seqs * a.history_ld}, {a.hist_len, 4ull * p.n_seqs}};
+  auto apart = [&](const Span& w) {
+    for (const Span& r : read)
+      if (overlap(w, r)) return false;
+    return !in_pool(*pool, p, w);
+  };
+  for (const Span& w : {Span{a.path, nodes}, Span{a.n_path, list}, Span{a.next, list}, Span{a.ok, list}})
+    BK_ARG(apart(w) && !overlap(w, histories[0]) && !overlap(w, histories[1]), "bkPagesCommit: path, n_path, next and ok must lie apart from what the call reads");
+  BK_ARG(apart(histories[0]) && apart(histories[1]) && !overlap(histories[0], histories[1]), "bkPagesCommit: history and hist_len must lie apart from the other arrays");
   const CommitParams c = {bk_ptr<int>(a.seqs), bk_ptr<int>(a.n_new), bk_ptr<int>(a.parent), bk_ptr<int>(a.token), bk_ptr<int>(a.target), bk_ptr<int>(a.path), bk_ptr<int>(a.n_path),
                           bk_ptr<int>(a.next), bk_ptr<int>(a.ok), bk_ptr<int>(a.history), bk_ptr<int>(a.hist_len), a.n, a.T, a.history_ld, a.values};
   // CTAs a sequence: as many as its warps have runs of rows for, at most 8 (a cluster) and four an SM

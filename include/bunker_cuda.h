@@ -418,7 +418,7 @@ BK_API int32_t bkAdjustLogits(const bkLogitsArgs* args);
  *   path int32 [T][n]: nodes of the path, -1 behind it (0 = not wanted); n_path int32 [n]; next int32 [n]: the target of the last (a token without a row yet)
  *   history int32 [n_seqs][history_ld], hist_len int32 [n_seqs] (0 = none): the tokens of the path are appended, node 0's first.  A history is then what has rows; next
  *   comes with the next tree, as its node 0 (and bkAdjustLogits counts it with the path, not twice)
- * path, n_path, next and ok lie apart from what the call reads.
+ * path, n_path, next and ok lie apart from what the call reads (the histories and the pool among it), and the histories from the rest of it.
  * ok[i] (0 to skip): 1, or 0 where nothing is changed, n_path is 0, next and path are -1: the entry names no sequence or one named before, n_new[i] is not
  * in 1..T, the sequence has fewer rows, a page that holds rows of its tree is shared (or none of the pool's), or its history has no room (or a length below 0). */
 typedef struct bkPagesCommitArgs {

@@ -120,3 +120,50 @@ def test_the_layer_ends_a_path_where_nothing_is_allowed(bk):
         d = dev(np.concatenate([target.view(np.uint32), logit.view(np.uint32)]))
         kept, after = s.keep(token, d.ptr, values=values)
         assert kept.tolist() == kept_want and after.tolist() == next_want
+
+
+# ---- results that lie over what a call reads --------------------------------------------
+
+def test_commit_refuses_results_over_its_inputs(bk):
+    """Ranges, not addresses alone: lists, trees, histories, and the pool's own tables, counts, lengths and pages."""
+    rng = np.random.default_rng(5)
+    p = Draft(rng, planes=2, seqs=3)
+    p.own(0, 20, [3, 4])
+    p.own(1, 30, [5, 6])
+    n, T = 2, 4
+    p.grown(rng, T, [T] * n)
+    pool = p.upload()
+    every = R.DeviceBuffer.from_numpy(np.full(512, 1, np.int32))
+    size = dict(seqs=n, n_new=n, parent=n * T, token=n * T, target=2 * n * T, path=n * T, n_path=n, next=n, ok=n, history=3 * 9, hist_len=3)
+    at, place = {}, every.ptr
+    for k, m in size.items():
+        at[k], place = place, place + 4 * m
+    lib = R.cu()
+
+    def call(**change):
+        a = R.bkPagesCommitArgs(**{**at, **dict(n=n, T=T, history_ld=9, values=1), **change})
+        return lib.bkPagesCommit(C.byref(pool.desc), C.byref(a))
+
+    data = p.d["data"].ptr
+    pools = [(p.d["lens"].ptr, 12), (p.d["table"].ptr, p.table.nbytes), (p.d["ref"].ptr, p.ref.nbytes), (data, p.data.nbytes // 2), (data + p.data.nbytes // 2, p.data.nbytes // 2)]
+    for w in ("path", "n_path", "next", "ok", "history", "hist_len"):
+        reads = [k for k in ("seqs", "n_new", "parent", "token", "target", "history", "hist_len") if k != w and not (w == "hist_len" and k == "history")]
+        for lo, length in [(at[k], 4 * size[k]) for k in reads] + pools:
+            for place in (lo, lo + length - 4, lo - 4 * size[w] + 4):
+                assert call(**{w: place}) == R.BK_ERR_ARG and "apart" in R.last_error(), (w, R.last_error())
+    p.check("nothing changed")
+    assert np.array_equal(every.download(np.int32, (512,)), np.full(512, 1, np.int32))
+    # side by side, as they lie here, they are apart
+    R.cuHtoD(at["seqs"], i32(0, 1))
+    R.cuHtoD(at["n_new"], i32(T, T))
+    for k, x in (("parent", p.parent), ("token", p.token), ("target", p.target)):
+        R.cuHtoD(at[k], x)
+    R.cuHtoD(at["hist_len"], i32(0, 2, 0))
+    history, hist_len = np.full((3, 9), 1, np.int32), i32(0, 2, 0)
+    assert call() == 0
+    want = p.commit(i32(0, 1), history, hist_len)
+    p.check()
+    got = every.download(np.int32, (512,))
+    for k, w in (("path", want[0]), ("n_path", want[1]), ("next", want[2]), ("ok", want[3]), ("history", history), ("hist_len", hist_len)):
+        first = (at[k] - every.ptr) // 4
+        assert np.array_equal(got[first:first + w.size], w.reshape(-1)), k
