@@ -674,6 +674,15 @@ int32_t bkPagesBatch(const bkPages* pool, const bkPagesBatchArgs* args) {
   BK_ARG(!a.mask || a.mask_words >= (a.T + 31) / 32, "bkPagesBatch: mask_words=%d for %d nodes", a.mask_words, a.T);
   BK_ARG(!a.slot || (long long)p.n_pages * p.page_rows < (1ll << 31), "bkPagesBatch: %d pages of %d rows: a slot has 31 bits", p.n_pages, p.page_rows);
   if (a.n == 0) return BK_OK;
+  // a sequence's CTAs read while the first writes
+  const uint64_t list = 4ull * a.n, nodes = list * a.T;
+  const Span read[] = {{a.seqs, list}, {a.parent, nodes}, {a.n_new, list}, {a.ok, list}};
+  const Span write[] = {{a.count, list}, {a.table, list * p.max_pages}, {a.lens, list}, {a.pos, nodes}, {a.slot, nodes}, {a.mask, a.mask ? nodes * a.mask_words : 0}};
+  for (int i = 0; i < 6; i++) {
+    bool apart = !in_pool(*pool, p, write[i]);
+    for (int j = 0; j < 4; j++) apart = apart && (!overlap(write[i], read[j]) || (i == 0 && j >= 2 && write[i].at == read[j].at));
+    BK_ARG(apart, "bkPagesBatch: results must lie apart from what the call reads (count alone may be the array of n_new or ok)");
+  }
   const BatchParams b = {bk_ptr<int>(a.seqs), bk_ptr<int>(a.n_new), bk_ptr<int>(a.parent), bk_ptr<int>(a.ok), bk_ptr<int>(a.table), bk_ptr<int>(a.lens), bk_ptr<int>(a.pos),
                          bk_ptr<int>(a.slot), bk_ptr<int>(a.count), bk_ptr<uint32_t>(a.mask), a.n, a.T, a.mask_words};
   // CTAs a sequence: 1,024 entries of its table each, no more than fill the GPU twice

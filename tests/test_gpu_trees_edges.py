@@ -167,3 +167,48 @@ def test_commit_refuses_results_over_its_inputs(bk):
     for k, w in (("path", want[0]), ("n_path", want[1]), ("next", want[2]), ("ok", want[3]), ("history", history), ("hist_len", hist_len)):
         first = (at[k] - every.ptr) // 4
         assert np.array_equal(got[first:first + w.size], w.reshape(-1)), k
+
+
+def test_batch_refuses_results_over_its_inputs(bk):
+    """lens in the place of the pool's own lens, for one, would be written by a sequence's first CTA while the others read it."""
+    rng = np.random.default_rng(6)
+    p = Draft(rng, planes=2, seqs=3)
+    p.own(0, 20, [3, 4])
+    p.own(1, 30, [5, 6])
+    n, T, W = 3, 4, 2
+    pool = p.upload()
+    every = R.DeviceBuffer.from_numpy(np.full(512, 1, np.int32))
+    size = dict(seqs=n, n_new=n, parent=n * T, ok=n, table=n * p.max_pages, lens=n, pos=n * T, slot=n * T, mask=n * T * W, count=n)
+    at, place = {}, every.ptr
+    for k, m in size.items():
+        at[k], place = place, place + 4 * m
+    lib = R.cu()
+
+    def call(**change):
+        a = R.bkPagesBatchArgs(**{**at, **dict(n=n, T=T, mask_words=W), **change})
+        return lib.bkPagesBatch(C.byref(pool.desc), C.byref(a))
+
+    pools = [(p.d["lens"].ptr, 12), (p.d["table"].ptr, p.table.nbytes), (p.d["ref"].ptr, p.ref.nbytes), (p.d["data"].ptr, p.data.nbytes)]
+    for w in ("table", "lens", "pos", "slot", "mask", "count"):
+        for k, lo, length in [(k, at[k], 4 * size[k]) for k in ("seqs", "n_new", "parent", "ok")] + [("pool", *x) for x in pools]:
+            for place in (lo, lo + length - 4, lo - 4 * size[w] + 4):
+                if w == "count" and k in ("n_new", "ok") and place == lo:
+                    continue                                    # (these may be the same)
+                assert call(**{w: place}) == R.BK_ERR_ARG and "apart" in R.last_error(), (w, k, R.last_error())
+    p.check("nothing changed")
+    assert np.array_equal(every.download(np.int32, (512,)), np.full(512, 1, np.int32))
+    assert call(count=at["n_new"], lens=at["n_new"]) == R.BK_ERR_ARG and "apart" in R.last_error()
+    # side by side, as they lie here, they are apart; so are count and what it comes from where they are one array
+    for one in ("count", "n_new", "ok"):
+        R.cuHtoD(every.ptr, np.full(512, 1, np.int32))
+        R.cuHtoD(at["seqs"], i32(0, 2, 1))
+        R.cuHtoD(at["n_new"], i32(T, T, 2))
+        assert call(count=at[one], parent=0) == 0
+        assert R.cuSync() == 0
+        got = every.download(np.int32, (512,))
+        part = {k: got[(at[k] - every.ptr) // 4:][:m] for k, m in size.items()}
+        assert part[one].tolist() == [T, 0, 2] and part["lens"].tolist() == [20, 0, 30]
+        assert part["pos"].reshape(T, n).T.tolist() == [[16, 17, 18, 19], [-1] * 4, [28, 29, -1, -1]]
+    p.check("unchanged")
+    b = R.bkPagesBatchArgs(seqs=at["seqs"], n=n, T=T, n_new=at["n_new"], ok=at["n_new"], count=at["n_new"])      # all three
+    assert lib.bkPagesBatch(C.byref(pool.desc), C.byref(b)) == 0 and R.cuSync() == 0
