@@ -224,7 +224,7 @@ def main() -> None:
     cfg = CONFIG_TINY
     w, lora = random_layer(cfg)
     half = max(1, (a.steps - 2) // 2)
-    nodes = max(1, min(a.draft, SharedPrompt.CHUNK // a.requests))
+    nodes = max(1, min(a.draft, SharedPrompt.CHUNK // max(1, a.requests)))
     rows = a.prompt + 2 * (1 + half) + nodes * (1 + half) + 1    # (both ways of reading the prompt and trees, each with a step ahead of the timed ones, and one at the end)
     layer = SharedPrompt(cfg, w, lora, a.requests, rows, n_pages=-(-a.prompt // 16) + a.requests * (-(-rows // 16) - a.prompt // 16))
     rng = synth.rng_for(1, 72)
