@@ -212,3 +212,65 @@ def test_batch_refuses_results_over_its_inputs(bk):
     p.check("unchanged")
     b = R.bkPagesBatchArgs(seqs=at["seqs"], n=n, T=T, n_new=at["n_new"], ok=at["n_new"], count=at["n_new"])      # all three
     assert lib.bkPagesBatch(C.byref(pool.desc), C.byref(b)) == 0 and R.cuSync() == 0
+
+
+# ---- attention: what a single hidden or extra node moves ---------------------------------
+
+def row_bound(w, v, o, d, gate=1.0):
+    """What a row's result o gate [HD], o = w v, may be off by: 16 bits of probabilities (2^-13 of the largest |v|, see test_gpu_trees.py), scores that are off by up to d, 2^-20 of it
+    for the sigmoid and its product, and one rounding of what all that gives (2^-8 of it).  Weights w_j f_j with 1 / e^d <= f_j <= e^d give
+    o + sum w_j (f_j - 1) (v_j - o) / sum w_j f_j, for sum w_j (v_j - o) is 0: at most (e^d - 1) e^d sum w_j |v_j - o| from o."""
+    before = gate * (2.0 ** -13 * np.abs(v).max() + math.expm1(d) * math.exp(d) * (w @ np.abs(v - o))) + 2.0 ** -20 * np.abs(o * gate)
+    return 2.0 ** -8 * np.abs(o * gate) + (1 + 2.0 ** -8) * before
+
+
+def check_rows(c, **change):
+    """As TreeCase.check, but with the keys that the call left in the pages, and with values of a query that lie so near the border of two bf16 values that the call may have taken either:
+    a score is off by what those make of it, and no more.  A value of q is x / sqrt(mean x^2 + eps) (1 + w), in f32: the sum of squares is off by 14 roundings of 2^-24, half of it after the
+    root, which has 4 more, and 3 products; then the rotation's products and sum, 3 of its terms' size, which the pair's length bounds: 2^-19 of the length in all."""
+    bits = c.run(c.tree_args(**change))
+    got = val(bits)
+    want, kp, vp = c.want()
+    k = c.keep["kp"].download(np.uint16, c.kp.shape)
+    assert np.array_equal(c.keep["vp"].download(np.uint16, c.vp.shape), vp)
+    changed = kp != c.kp
+    assert np.array_equal(k[~changed], kp[~changed])
+    assert (np.abs(val(k[changed]) - val(kp[changed])) <= 2.0 ** -7 * np.abs(val(kp[changed])) + 2.0 ** -16).all()
+    assert not bits[c.nothing_seen()].any()
+    at, G, r = c.positions(), c.Hq // c.Hkv, c.rot
+    for b in range(c.B):
+        n, base = c.n_base(b)
+        for t in range(n):
+            e, j = t * c.B + b, np.concatenate([np.arange(base), base + np.nonzero(c.sees[t, b, :n])[0]])
+            if at[t, b] < 0 or not len(j):
+                continue
+            K, V = (val(x[c.table[b, j // c.rows], :, j % c.rows]) for x in (k, vp))
+            q, off = val(c.q[e]), np.zeros((c.Hq, c.HD))
+            if c.fused:
+                y = c.turned(c.q[e], c.qw, c.pos[t, b])
+                size = np.abs(y)
+                size[:, :r] = size[:, r:2 * r] = np.hypot(y[:, :r], y[:, r:2 * r])
+                q = val(bf16(y))
+                off = np.abs(val(bf16(y + 2.0 ** -19 * size)) - val(bf16(y - 2.0 ** -19 * size)))
+            gate = 1 / (1 + np.exp(-val(c.g[e]))) if c.g is not None else np.ones((c.Hq, c.HD))
+            for h in range(c.Hq):
+                Kh, Vh = K[:, h // G], V[:, h // G]
+                s = Kh @ q[h] * float(c.scale)
+                w = np.exp(s - s.max())
+                w /= w.sum()
+                o = w @ Vh
+                d = float(c.scale) * (np.abs(Kh) @ off[h]).max()
+                tol = row_bound(w, Vh, o, d, gate[h])
+                bad = np.abs(got[e, h] - o * gate[h]) > tol
+                assert not bad.any(), (b, t, h, np.abs(got[e, h] - o * gate[h])[bad][:4], tol[bad][:4], d)
+
+
+@pytest.mark.parametrize("fused", [True, False])
+@pytest.mark.parametrize("B,T,prefix,own,new,Hq,Hkv,HD,rows", [
+    (1, 8, 0, [8], None, 4, 1, 128, 16), (1, 32, 0, [65], None, 4, 1, 128, 16), (1, 32, 0, [33], None, 8, 1, 256, 32), (4, 12, 150, [12, 40, 77, 13], [12, 5, 1, 12], 16, 2, 256, 64),
+    (2, 40, 0, [140, 41], [40, 33], 8, 2, 256, 16), (1, 64, 0, [128], None, 6, 1, 128, 16), (3, 9, 70, [9, 50, 20], [9, 4, 9], 4, 1, 128, 16), (2, 33, 64, [70, 34], [33, 20], 24, 4, 128, 32),
+    (20, 5, 40, [5 + i for i in range(20)], [5 - i % 3 for i in range(20)], 8, 1, 256, 16)])
+@pytest.mark.parametrize("tree", ["tree", "any"])
+def test_no_node_is_hidden_or_shown_that_is_not(bk, fused, B, T, prefix, own, new, Hq, Hkv, HD, rows, tree):
+    """Up to 230 keys a row: a bit that is wrong in one row is outside these bounds (the CPU's tests say how surely), with ready queries and with the fused norm."""
+    check_rows(TreeCase(T + Hq + HD, B, T, prefix, own, tree=tree, new=new, Hq=Hq, Hkv=Hkv, HD=HD, rows=rows, fused=fused))
