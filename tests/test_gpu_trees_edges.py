@@ -274,3 +274,48 @@ def check_rows(c, **change):
 def test_no_node_is_hidden_or_shown_that_is_not(bk, fused, B, T, prefix, own, new, Hq, Hkv, HD, rows, tree):
     """Up to 230 keys a row: a bit that is wrong in one row is outside these bounds (the CPU's tests say how surely), with ready queries and with the fused norm."""
     check_rows(TreeCase(T + Hq + HD, B, T, prefix, own, tree=tree, new=new, Hq=Hq, Hkv=Hkv, HD=HD, rows=rows, fused=fused))
+
+
+# ---- attention: forms of the call ---------------------------------------------------------
+
+@pytest.mark.parametrize("HD,prefix", [(128, 0), (128, 70), (256, 48)])
+def test_trees_whose_rows_are_in_the_pages_already(bk, HD, prefix):
+    """k, v and slot 0: nothing is stored, the same results to the bit."""
+    c = TreeCase(HD + prefix, 3, 9, prefix, [9, 50, 20], new=[9, 4, 9], Hq=8, Hkv=2, HD=HD, fused=False)
+    first = c.run(c.tree_args())
+    _, c.kp, c.vp = c.want()
+    a = c.tree_args(pos=0, slot=0)
+    a.attn.k = a.attn.v = 0
+    assert np.array_equal(c.run(a), first)
+    assert np.array_equal(c.keep["kp"].download(np.uint16, c.kp.shape), c.kp) and np.array_equal(c.keep["vp"].download(np.uint16, c.vp.shape), c.vp)
+
+
+@pytest.mark.parametrize("fused", [True, False])
+@pytest.mark.parametrize("B,T,own", [(1, 1, [1]), (3, 7, [7, 60, 8]), (5, 33, [40, 33, 32, 90, 34])])
+def test_trees_of_all_nodes_without_counts(bk, fused, B, T, own):
+    """n_new 0: T of each; a sequence with fewer rows has none."""
+    c = TreeCase(T, B, T, 0, own, new=[T] * B, Hq=4, Hkv=2, HD=128, fused=fused)
+    first = c.run(c.tree_args())
+    c = TreeCase(T, B, T, 0, own, new=[T] * B, Hq=4, Hkv=2, HD=128, fused=fused)
+    a = c.tree_args()
+    a.attn.n_new = 0
+    assert np.array_equal(c.run(a), first)
+    c.check()
+
+
+@pytest.mark.parametrize("B,T,prefix,own,new,Hq,Hkv,HD,tree", [
+    (1, 300, 0, [300], None, 2, 1, 128, "any"), (2, 600, 100, [611, 320], [600, 311], 2, 2, 128, "tree"), (1, 1024, 0, [1200], None, 4, 1, 128, "tree"), (1, 513, 40, [513], None, 16, 1, 256, "tree"),
+    (3, 257, 0, [257, 300, 200], [257, 256, 129], 3, 1, 256, "any")])
+def test_trees_of_many_nodes(bk, B, T, prefix, own, new, Hq, Hkv, HD, tree):
+    TreeCase(T, B, T, prefix, own, tree=tree, new=new, Hq=Hq, Hkv=Hkv, HD=HD, fused=T % 2 == 0).check(1)
+
+
+# ---- logits of many nodes -------------------------------------------------------------------
+
+@pytest.mark.parametrize("B,T,V,history,n_bias,n_masks", [(1, 513, 300, 0, 0, 0), (1, 1024, 700, 50, 9, 3), (2, 600, 1500, 300, 0, 2), (1, 1000, 9000, 4000, 1024, 0), (3, 512, 33, 7, 2, 2)])
+def test_logits_of_trees_of_many_nodes(bk, B, T, V, history, n_bias, n_masks):
+    """Above 512 nodes a thread has more than one drafted token; tokens of the whole vocabulary, and of a few."""
+    c = Logits(T + V, B, T, V, history=history, n_bias=n_bias, n_masks=n_masks, tree=True)
+    c.check()
+    c.draft = np.random.default_rng(T).integers(-1, V + 1, T * B).astype(np.int32)
+    c.check()
