@@ -348,11 +348,13 @@ extern "C" int32_t bkAdjustLogits(const bkLogitsArgs* args) {
                     bk_ptr<int>(a.bias_n), bk_ptr<uint32_t>(a.allowed), bk_ptr<int>(a.mask_id), a.B, a.T, a.V, a.n_seqs ? a.n_seqs : a.B, a.history_ld, a.bias_ld, a.path_words,
                     a.n_masks, a.allowed_words, 0, 0, 0, 0, 0, 0, a.ld ? a.ld : a.V};
   if (!a.bias_token) p.bias_ld = 0;
-  // Who names: slices of at most 8,192 words (48 KB with the list; 512 rows behind 16,000 tokens 117 us, with twice as many words 118), shorter while that leaves SMs without a
-  // CTA, to 1,024; then rows apart, until each SM has two (111 us; with four 117, none apart 159), but no
-  // fewer rows than half the slices, each of which counts the whole history (4 requests, 10 rows behind 6,000 tokens, 32 slices: 13.8 us with four rows a CTA, 10.1 with ten).  Where such a slice has more than 4,096 words and the request's tokens fit a table,
-  // fewer CTAs with a table each (64 requests, 5,000 tokens of 151,936: 25 us with slices of words, 15 with four tables; one request, 700 tokens: 4.6 with 128 slices of
-  // words, 5.2 with as many tables).
+  // (Figures: 151,936 logits, 148 SMs.)  Who names: slices of at most 8,192 words (48 KB with the list; 512 rows behind 16,000 tokens 111 us, with half as many words 116, with twice as many
+  // 112; 4 requests, 10 rows, 9,000 tokens 11.7, 11.3 and 14.2), shorter while that leaves SMs without a CTA, to 1,024; then rows apart, until each SM has two (one request of 100 rows behind
+  // 30,000 tokens 35 us, none apart 74; 512 rows, which are not taken apart so, 111, until each SM has four 116), but no fewer rows than half the slices, each of which counts the whole history (4 requests,
+  // 10 rows, 9,000 tokens, 32 slices: 11.7 us with ten rows a CTA, 14.6 with four; 100 rows behind 30,000 34.7 and 41.5; against it one request of 32 rows behind 16,000, 15.9 and 12.6).
+  // Where such a slice has more than 4,096 words and the request's tokens fit a table, fewer CTAs with a table each (64 requests, 5,000 tokens: 15.4 us with four tables, 46 with slices of
+  // words; against it 4 requests, 10 rows, 6,000 tokens, 12.4 and 9.0; below 4,096 words 4 requests, 2,000 tokens: 4.8 us with slices of 2,560 words, 5.7 with tables).  A request's tokens are
+  // what its arrays hold (history_ld, bias_ld, T): its lengths are on the device.
   // Who hides: four CTAs an SM, no more than have 4,096 tokens each.
   const long long sms = bk_ctx().sm_count;
   const int blocks = (a.V + kBlock - 1) / kBlock;

@@ -349,11 +349,14 @@ BK_DEVINL void plan_jobs(const Params<false>& p, const Layout& L, uint8_t* scrat
 // equal width but for one tile.  Teams of one width are jobs on a line of their own, which is cut into equal pieces for the line's share of the CTAs; shares are the
 // smallest longest piece.  (32 sequences of up to 16,384 rows and 64 nodes, 24 heads on 4, with the merge that the calls had then: teams of one 578 us, of up to two 543, three 520, four 527,
 // six 539; 16 behind 8,192 common rows, 16 on 2: 77, 69, 63, 63, 61.)  Only row tiles and tokens that are there have a place; with all of T for each sequence, half of
-// them there, the first took 704 us on one line.  It takes 449 to 469 now, about 300 of them for the tiles; in a loop the power limit sets the clock.
+// them there, the first took 704 us on one line.  It takes 450 to 480 now in a loop, where the power limit sets the clock (984 W, 1,395 MHz); one call at
+// a time, at 1,965 MHz, 410: queries and plan 29, tiles 329, merge 37 (each alone), the rest between them.
 constexpr int kTeam = 4;
 // What a job's start and end cost, in steps: its queries and masks, the tile at its end whose rows are not seen by all, and the partial result, 4,500 cycles for 128 rows of 256.
 // (In us, at 3, 4, 5, 6 steps.  HD 256: one sequence of 16,384 rows and 64 nodes, 24 heads on 4: 82, 70, 65, 65; the same with 188: 151, 157, 130, 131; 16 behind 8,192 common rows,
-// 16 nodes, 16 on 2: 45.6, 44.2, 44.2, 44.2; 64 of 2,000 and one, 24 on 4: 58.8, 59.1, 59.9, 60.0.  HD 128, 4 of up to 4,300 and 100, 24 on 4: 60.9, 61.7, 64.1, 64.7, and 67.6 at 9.)
+// 16 nodes, 16 on 2: 45.6, 44.2, 44.2, 44.2; 64 of 2,000 and one, 24 on 4: 58.8, 59.1, 59.9, 60.0.
+// HD 128, at 2, 3, 4, 5 steps, 24 on 4: 4 of up to 4,300 and 100: 61.2, 60.4, 61.6, 64.2; 64 of 2,000 and one 46.4, 44.2, 44.5, 45.1; 64 of 4 behind 1,000 31.5, 31.9, 33.0, 33.6; 32 of 32 and up to 500
+// 49.8, 49.7, 48.5, 48.4; 16 of up to 8,192 and 64 110, 109, 109, 109; 16 behind 8,192 common rows, 16 nodes, 16 on 2 40.1, 37.0, 37.0, 37.6.)
 __host__ __device__ constexpr int tree_overhead(int HD) { return HD == 256 ? 5 : 3; }
 // Team job i: {start on its line, job of its first row tile, end of its keys, slot of its first row tile's partial result for team 0}; the slots of a team job's pieces
 // are kTeam-wide steps: slot + w * team + rank, which no two pieces share since i + team grows from piece to piece of a line.  jobs[j] = {.., .., first slot, number and
@@ -1532,7 +1535,8 @@ __global__ void __launch_bounds__(256 * kSlices) paged_merge_kernel(const Params
 
 
 // The same for trees.  A thread has kQuads times 4 dims of one head, 64 apart; a CTA 64 kQuads dims of the group's heads, from kSlices slices of pieces.  Many rows have few
-// pieces each: one slice and all dims, so that the chain of loads (place, lists of pieces, sums and results) is there once a row and KV head.  Few rows may have a piece of
+// pieces each: one slice and half of the dims, so that the chain of loads (place, lists of pieces, sums and results) is there twice a row and KV head (all dims a CTA, 2,048 tokens of 32
+// sequences, 24 heads on 4: with HD 256 84 us a call for 82, with HD 128 66 to 70 for 71 to 73).  Few rows may have a piece of
 // every CTA: more slices (2,048 tokens, half of them there, 24 heads on 4: 76 us with 64 dims a CTA and every list read anew, so 35; one token, 16 heads on 2, 8,192 rows: 17.5 us
 // with four slices, so 12; caches cold).
 template <int HD, int kSlices, int kQuads>

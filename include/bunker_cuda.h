@@ -388,7 +388,9 @@ BK_API uint64_t bkTreeAttnScratchBytes(int32_t B, int32_t T, int32_t Hq, int32_t
  *   x += bias of v (a token that a request names several times gets the sum, in the list's order);   x = -inf where the row's mask does not allow v.
  * A logit that nothing names or hides is neither read nor written.  NaN stays NaN where it is allowed.
  * A row whose mask allows no token is -inf throughout.  bkArgmax and bkSample still name one of its tokens (bkArgmax token 0), with val -inf: that val says that
- * there is none, and bkPagesCommit with `values` takes it so. */
+ * there is none, and bkPagesCommit with `values` takes it so.
+ * x / repetition is x times 1 / repetition, rounded (repetition 2^-126 to 2^126).  How the work is shared out goes by history_ld, bias_ld and T, since lengths are on
+ * the device: a history_ld near the lengths in use is fastest. */
 #define BK_LOGITS_MAX_BIAS 1024
 typedef struct bkLogitsArgs {
   uint64_t logits;
